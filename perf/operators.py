@@ -255,35 +255,35 @@ def _plain(state):
 # the framework's calls
 # ---------------------------------------------------------------------------
 def _own(state):
-  from mesh_amd import moe_hip
+  from mesh_amd import fp8_hip
   case = state["case"]
   kind = case["kind"]
 
   def operand(name, n):
-    return moe_hip.Fp8Blocks(state[name][0], state[name][1], n)
+    return fp8_hip.Fp8Blocks(state[name][0], state[name][1], n)
 
   if kind == "quantize":
-    rows, columns = moe_hip.quantize_fp8(
+    rows, columns = fp8_hip.quantize(
         state["x"], rows=True, columns=True,
         relu_mask=state["mask"] if case["masked"] else None)
-    return moe_hip.dequantize_fp8(rows), moe_hip.dequantize_fp8(columns)
+    return fp8_hip.dequantize(rows), fp8_hip.dequantize(columns)
   if kind in ("norm", "mlp"):
-    total, y = moe_hip.residual_rms_norm_fp8(
+    total, y = fp8_hip.residual_rms_norm(
         state["x"], state["residual"], state["scale"],
         row_mask=state["mask"] if case["masked"] else None)
     if kind == "norm":
-      return total, moe_hip.dequantize_fp8(y)
-    h = moe_hip.dense_fp8(y, operand("wi", case["width"]), "relu", eight_bit=True)
-    return total, moe_hip.dense_fp8(h, operand("wo", case["columns"]))
+      return total, fp8_hip.dequantize(y)
+    h = fp8_hip.dense(y, operand("wi", case["width"]), "relu", eight_bit=True)
+    return total, fp8_hip.dense(h, operand("wo", case["columns"]))
   if kind == "product":
     out = state["out"]
     if isinstance(out, tuple):
       out = operand("out", case["columns"])
-    y = moe_hip.expert_linear_fp8(
+    y = fp8_hip.expert_linear(
         operand("a", case["width"]), operand("w", case["width"]), case["activation"],
         eight_bit=case["eight_bit"], row_count=state["count"], out=out)
-    return moe_hip.dequantize_fp8(y) if case["eight_bit"] else y
-  return moe_hip.expert_linear_fp8_backward(
+    return fp8_hip.dequantize(y) if case["eight_bit"] else y
+  return fp8_hip.expert_linear_backward(
       operand("a_columns", case["rows"]), state["dy"], operand("w_rows", case["columns"]),
       relu_mask=state["mask"] if case["masked"] else None, row_count=state["count"],
       da=state["da"])
