@@ -1,0 +1,318 @@
+"""ctypes binding of the 8-bit operands of libmesh_moe_hip.so (declared in
+include/mesh_moe_fp8.h): dense layers and experts on e4m3 numbers with a scale for each
+block of 128, the passes that make such operands, and the RMS norm that ends in one.
+
+An operand is an Fp8Blocks.  The calls follow those of moe_hip, whose bf16 forms they
+are: GPU tensors that are contiguous, checked on the host; launched on the current
+stream; nothing kept between calls, so that each can be recorded into a HIP graph.  All
+tensors of a call have to lie on the current device.
+
+A dense layer in training (w [K, N] bf16, x [rows, K], dy [rows, N]):
+
+  w_rows, w_columns = quantize(w.unsqueeze(0), rows=True, columns=True)  # per update
+  a, a_columns = quantize(x.unsqueeze(0), rows=True, columns=True)
+  y = expert_linear(a, w_columns)
+  dx, dw = expert_linear_backward(a_columns, dy.unsqueeze(0), w_rows)
+"""
+
+import ctypes
+
+import torch
+
+from mesh_amd import moe_hip
+from mesh_amd.moe_hip import MoeHipError
+
+ABI_VERSION = 1
+BLOCK = 128
+
+_vp = ctypes.c_void_p
+_int = ctypes.c_int
+_size = ctypes.c_size_t
+_SIGNATURES = {
+    "mesh_moe_fp8_abi_version": (_int, []),
+    "mesh_moe_fp8_quantize": (_int, [_vp] * 7 + [_int] * 4 + [_vp]),
+    "mesh_moe_fp8_dequantize": (_int, [
+        _vp, _vp, _vp, ctypes.c_int64, _int, _int, _vp]),
+    "mesh_moe_fp8_residual_rms_norm": (_int, [_vp] * 8 + [
+        ctypes.c_int64, _int, ctypes.c_double, _int, _vp]),
+    "mesh_moe_fp8_expert_linear_workspace_bytes": (_size, [_int] * 5),
+    "mesh_moe_fp8_expert_linear": (_int, [_vp] * 7 + [_int] * 5 + [
+        _vp, _size, _vp]),
+    "mesh_moe_fp8_expert_linear_backward_workspace_bytes": (_size, [_int] * 5),
+    "mesh_moe_fp8_expert_linear_backward": (_int, [_vp] * 9 + [_int] * 5 + [
+        _vp, _size, _vp]),
+}
+EXPORTS = sorted(_SIGNATURES)
+
+_lib = None
+
+
+def load_library():
+  """The library with the entry points of this module declared."""
+  global _lib
+  if _lib is None:
+    lib = moe_hip.load_library()
+    for name, (restype, argtypes) in _SIGNATURES.items():
+      fn = getattr(lib, name)  # AttributeError if a symbol is missing
+      fn.restype = restype
+      fn.argtypes = argtypes
+    version = lib.mesh_moe_fp8_abi_version()
+    if version != ABI_VERSION:
+      raise MoeHipError("8-bit ABI version %d, expected %d" % (version, ABI_VERSION))
+    _lib = lib
+  return _lib
+
+
+def row_bytes(n):
+  """Bytes of a row of n values: whole blocks."""
+  return (n + BLOCK - 1) // BLOCK * BLOCK
+
+
+def scale_bytes(n):
+  """Scale bytes of a row of n values: a byte per block, whole groups of four."""
+  return ((n + BLOCK - 1) // BLOCK + 3) // 4 * 4
+
+
+class Fp8Blocks(object):
+  """An 8-bit operand: values [..., rows, row_bytes(n)] of torch.float8_e4m3fn, scales
+  [..., rows, scale_bytes(n)] of torch.uint8; value i of a row stands for values[i] *
+  2^(scales[i // 128] - 127).  The values from n on are zeros."""
+
+  __slots__ = ("values", "scales", "n")
+
+  def __init__(self, values, scales, n):
+    n = int(n)
+    if (values.dtype != torch.float8_e4m3fn or scales.dtype != torch.uint8 or n < 1 or
+        values.dim() < 1 or values.shape[-1] != row_bytes(n) or
+        tuple(scales.shape) != tuple(values.shape[:-1]) + (scale_bytes(n),)):
+      raise ValueError(
+          "values %s of %s and scales %s of %s are not rows of %d 8-bit values"
+          % (tuple(values.shape), values.dtype, tuple(scales.shape), scales.dtype, n))
+    self.values = values
+    self.scales = scales
+    self.n = n
+
+  @property
+  def shape(self):
+    """Of the tensor that the operand stands for."""
+    return tuple(self.values.shape[:-1]) + (self.n,)
+
+  @classmethod
+  def empty(cls, shape, device):
+    """An operand for a tensor of `shape`, not filled in."""
+    rows, n = tuple(shape[:-1]), shape[-1]
+    return cls(torch.empty(rows + (row_bytes(n),), dtype=torch.float8_e4m3fn,
+                           device=device),
+               torch.empty(rows + (scale_bytes(n),), dtype=torch.uint8, device=device),
+               n)
+
+  def reshape(self, *rows):
+    """The same rows under other leading dimensions."""
+    return Fp8Blocks(self.values.reshape(rows + self.values.shape[-1:]),
+                     self.scales.reshape(rows + self.scales.shape[-1:]), self.n)
+
+  def __repr__(self):
+    return "Fp8Blocks%s" % (self.shape,)
+
+
+def _dev(t, name, dtype=None, shape=None):
+  at = moe_hip._dev(t, name, dtype, shape)  # pylint: disable=protected-access
+  if t.device.index != moe_hip.current_device():
+    raise MoeHipError("%s lies on %s, the current device is %d"
+                      % (name, t.device, moe_hip.current_device()))
+  return at
+
+
+def _operand(q, name, shape=None):
+  """Pointers to an operand's values and scales."""
+  if not isinstance(q, Fp8Blocks):
+    raise MoeHipError("%s must be an Fp8Blocks" % name)
+  if shape is not None and q.shape != tuple(shape):
+    raise MoeHipError("%s: shape %s, expected %s" % (name, q.shape, tuple(shape)))
+  return _dev(q.values, name + ".values"), _dev(q.scales, name + ".scales")
+
+
+def _counts(row_count, e):
+  return (None if row_count is None
+          else _dev(row_count, "row_count", torch.int32, (e,)))
+
+
+def _workspace(nbytes, like):
+  return torch.empty((nbytes,), dtype=torch.uint8, device=like.device)
+
+
+def _activation(name):
+  if name not in moe_hip.ACTIVATIONS:
+    raise ValueError("unsupported activation %r" % (name,))
+  return moe_hip.ACTIVATIONS[name]
+
+
+_stage = moe_hip._stage    # pylint: disable=protected-access
+_check = moe_hip._check    # pylint: disable=protected-access
+_stream = moe_hip._stream  # pylint: disable=protected-access
+
+
+def quantize(x, rows=True, columns=False, relu_mask=None, row_count=None):
+  """x [E, R, K] (or [R, K]) as 8-bit operands, in one pass over it: its rows
+  [E, R, K], for products over K, its columns [E, K, R], for products over R, or both.
+  relu_mask (shape and dtype of x): elements whose mask is not positive count as 0.
+  row_count [E] int32: rows of an expert from its count on count as zeros.
+  -> the one operand asked for, or (rows, columns)
+
+  The columns of a weight [E, K, N] are what expert_linear multiplies by (as
+  moe_hip.pack_weights lays out a bf16 one), its rows what expert_linear_backward
+  needs."""
+  lib = load_library()
+  if not (rows or columns):
+    raise ValueError("neither rows nor columns are wanted")
+  if x.dim() not in (2, 3):
+    raise ValueError("x %s, expected [E, R, K] or [R, K]" % (tuple(x.shape),))
+  sizes = tuple(x.shape)
+  e, r, k = (1,) * (3 - x.dim()) + sizes
+  code = moe_hip.dtype_code(x.dtype)
+  by_row = Fp8Blocks.empty(sizes, x.device) if rows else None
+  by_column = (Fp8Blocks.empty(sizes[:-2] + (k, r), x.device)
+               if columns else None)
+  xp = _dev(x, "x")
+  mp = None if relu_mask is None else _dev(relu_mask, "relu_mask", x.dtype, sizes)
+  cp = _counts(row_count, e)
+  if x.numel():
+    with _stage("fp8_quantize"):
+      _check(lib.mesh_moe_fp8_quantize(
+          xp, mp, cp, *(_operand(by_row, "rows") if rows else (None, None)),
+          *(_operand(by_column, "columns") if columns else (None, None)), e, r, k,
+          code, _stream()), "fp8_quantize")
+  return (by_row, by_column) if rows and columns else by_row if rows else by_column
+
+
+def dequantize(q, dtype=torch.bfloat16):
+  """The tensor that an operand stands for, exact in bfloat16 and float32."""
+  lib = load_library()
+  code = moe_hip.dtype_code(dtype)
+  y = torch.empty(q.shape, dtype=dtype, device=q.values.device)
+  values, scales = _operand(q, "q")
+  if y.numel():
+    with _stage("fp8_dequantize"):
+      _check(lib.mesh_moe_fp8_dequantize(values, scales, y.data_ptr(),
+                                         y.numel() // q.n, q.n, code, _stream()),
+             "fp8_dequantize")
+  return y
+
+
+def residual_rms_norm(x, residual, scale, epsilon=1e-6, row_mask=None,
+                      want_norm=False):
+  """rms_norm(x + residual) * row_mask as an 8-bit operand: x, residual (or None) [...,
+  M], scale [M], row_mask [...] (or None) -> (x + residual or x itself, Fp8Blocks [...,
+  M]).  want_norm: also the result in x's dtype, as a third one (what a training step
+  quantizes the columns of)."""
+  lib = load_library()
+  m = x.shape[-1]
+  shape = tuple(x.shape)
+  code = moe_hip.dtype_code(x.dtype)
+  xp, sp = _dev(x, "x"), _dev(scale, "scale", x.dtype, (m,))
+  rp = None if residual is None else _dev(residual, "residual", x.dtype, shape)
+  mp = None if row_mask is None else _dev(row_mask, "row_mask", x.dtype, shape[:-1])
+  total = x if residual is None else torch.empty_like(x)
+  norm = torch.empty_like(x) if want_norm else None
+  y = Fp8Blocks.empty(shape, x.device)
+  if x.numel():
+    with _stage("rms_norm"):
+      _check(lib.mesh_moe_fp8_residual_rms_norm(
+          xp, rp, sp, mp, None if residual is None else total.data_ptr(),
+          None if norm is None else norm.data_ptr(), *_operand(y, "y"),
+          x.numel() // m, m, float(epsilon), code, _stream()), "fp8_residual_rms_norm")
+  return (total, y, norm) if want_norm else (total, y)
+
+
+def expert_linear(a, w, activation="linear", eight_bit=False, row_count=None, out=None):
+  """a [E, R, K] and w [E, N, K], 8-bit operands over K -> act(a[e] . w[e]^T) [E, R, N],
+  in bfloat16, or (eight_bit) as an 8-bit operand over N.  row_count [E] int32: only the
+  first rows of an expert, as many as its count, are multiplied, the others of `out` stay
+  as they were (without an `out` they are unspecified)."""
+  lib = load_library()
+  ap, asp = _operand(a, "a")
+  wp, wsp = _operand(w, "w")
+  if len(a.shape) != 3 or len(w.shape) != 3:
+    raise MoeHipError("a %s, w %s: expected [E, R, K] and [E, N, K]"
+                      % (a.shape, w.shape))
+  e, r, k = a.shape
+  n = w.shape[1]
+  if w.shape != (e, n, k):
+    raise MoeHipError("w: shape %s, expected %s" % (w.shape, (e, n, k)))
+  act = _activation(activation)
+  cp = _counts(row_count, e)
+  if eight_bit:
+    if out is None:
+      out = Fp8Blocks.empty((e, r, n), a.values.device)
+    yp, ysp = _operand(out, "out", (e, r, n))
+  else:
+    if out is None:
+      out = torch.empty((e, r, n), dtype=torch.bfloat16, device=a.values.device)
+    yp, ysp = _dev(out, "out", torch.bfloat16, (e, r, n)), None
+  if e * r * n == 0:
+    return out
+  ws_bytes = lib.mesh_moe_fp8_expert_linear_workspace_bytes(e, r, k, n, int(eight_bit))
+  ws = _workspace(ws_bytes, a.values) if ws_bytes else None
+  with _stage("fp8_linear"):
+    _check(lib.mesh_moe_fp8_expert_linear(
+        ap, asp, wp, wsp, cp, yp, ysp, e, r, k, n, act,
+        None if ws is None else ws.data_ptr(), ws_bytes, _stream()),
+           "fp8_expert_linear")
+  return out
+
+
+def dense(x, w, activation=None, eight_bit=False):
+  """x [..., K] times a kernel [1, N, K], 8-bit operands over K -> act(x . w^T) [..., N],
+  in bfloat16, or (eight_bit) as an 8-bit operand (mtf.layers.dense without bias)."""
+  if not isinstance(x, Fp8Blocks):
+    raise MoeHipError("x must be an Fp8Blocks")
+  lead = x.shape[:-1]
+  rows = 1
+  for size in lead:
+    rows *= size
+  y = expert_linear(x.reshape(1, rows), w, activation, eight_bit)
+  return y.reshape(*lead) if eight_bit else y.reshape(lead + (w.shape[1],))
+
+
+def expert_linear_backward(a_columns, dy, w_rows=None, relu_mask=None, row_count=None,
+                           da=None):
+  """The gradients of expert_linear: a_columns [E, K, R] (the columns of a), dy [E, R, N]
+  in bfloat16 or float32, w_rows [E, K, N] (the rows of w [E, K, N]; None: da is not
+  wanted) -> (da [E, R, K] or None, dw [E, K, N]), both bfloat16.  dy becomes an 8-bit
+  operand along N for da and along R for dw.  relu_mask [E, R, N]: the output of a
+  product with a ReLU, behind which dy counts as 0 where it is not positive.  row_count
+  as given to expert_linear: rows of dy behind it count as zeros, those of `da` stay as
+  they were (rows of a behind it are zeros in a_columns, or finite)."""
+  lib = load_library()
+  if dy.dim() != 3:
+    raise MoeHipError("dy %s, expected [E, R, N]" % (tuple(dy.shape),))
+  e, r, n = dy.shape
+  if not isinstance(a_columns, Fp8Blocks) or len(a_columns.shape) != 3:
+    raise MoeHipError("a_columns must be an Fp8Blocks [E, K, R]")
+  k = a_columns.shape[1]
+  code = moe_hip.dtype_code(dy.dtype)
+  ap, asp = _operand(a_columns, "a_columns", (e, k, r))
+  yp = _dev(dy, "dy")
+  mp = (None if relu_mask is None
+        else _dev(relu_mask, "relu_mask", dy.dtype, (e, r, n)))
+  cp = _counts(row_count, e)
+  wp = wsp = None
+  if w_rows is not None:
+    wp, wsp = _operand(w_rows, "w_rows", (e, k, n))
+    if da is None:
+      da = torch.empty((e, r, k), dtype=torch.bfloat16, device=dy.device)
+  elif da is not None:
+    raise MoeHipError("da needs w_rows")
+  dap = None if da is None else _dev(da, "da", torch.bfloat16, (e, r, k))
+  if dy.numel() == 0 or k == 0:
+    dw = torch.zeros((e, k, n), dtype=torch.bfloat16, device=dy.device)
+    return (None if da is None else da.zero_() if r and n == 0 else da), dw
+  dw = torch.empty((e, k, n), dtype=torch.bfloat16, device=dy.device)
+  ws_bytes = lib.mesh_moe_fp8_expert_linear_backward_workspace_bytes(
+      e, r, k, n, int(da is not None))
+  ws = _workspace(ws_bytes, dy)
+  with _stage("fp8_linear_backward"):
+    _check(lib.mesh_moe_fp8_expert_linear_backward(
+        ap, asp, yp, mp, cp, wp, wsp, dap, dw.data_ptr(), e, r, k, n, code,
+        ws.data_ptr(), ws_bytes, _stream()), "fp8_expert_linear_backward")
+  return da, dw

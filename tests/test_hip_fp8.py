@@ -1,0 +1,592 @@
+"""The 8-bit operators on the GPU against float64 (tests/fp8_reference.py).
+
+Tolerances.  Operands: the exponent is settled by comparisons and values are rounded to
+nearest, so that both are equal bit for bit.  Results that become operands: half a step of
+e4m3 (2^-4 relative, or 2^-10 of the block's unit below its normal numbers), the unit
+being the smallest that holds the block's largest value up to float32 rounding.  bfloat16
+results: half a step (2^-8) plus what the matrix instructions drop.  They keep the sum of
+a group of 8 products to 2^-14 of the largest one at least, so at most 8 * 2^-14 of the
+sum of the products' magnitudes over 8, 2^-14 of it on the whole; 2^-13 with the float32
+additions behind."""
+
+import numpy as np
+import pytest
+import torch
+
+from tests import fp8_reference as F
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"bf16": torch.bfloat16, "f32": torch.float32}
+
+
+@pytest.fixture(scope="module")
+def hip():
+  from mesh_amd import fp8_hip
+  fp8_hip.load_library()
+  return fp8_hip
+
+
+def _f64(t):
+  return t.detach().double().cpu().numpy()
+
+
+def _tensor(rng, shape, dtype, spread=2.0):
+  x = rng.standard_normal(shape) * np.exp(spread * rng.standard_normal(shape[-1:]))
+  return torch.from_numpy(x.astype(np.float32)).to(TYPES[dtype]).cuda()
+
+
+def _assert_operand(q, want):
+  """q holds the codes and scale bytes of the 8-bit form of `want` [..., n]."""
+  n = want.shape[-1]
+  codes, scales = F.quantize(want.reshape(-1, n))
+  got = q.values.view(torch.uint8).cpu().numpy().reshape(codes.shape)
+  got_scales = q.scales.cpu().numpy().reshape(codes.shape[0], -1)
+  np.testing.assert_array_equal(got_scales[:, :scales.shape[1]], scales)
+  # (either NaN is one)
+  np.testing.assert_array_equal(np.where(got == 0xff, 0x7f, got), codes)
+
+
+def _assert_rounded(q, want, slack=2.0 ** -18):
+  """q stands for `want` up to a rounding to e4m3."""
+  n = want.shape[-1]
+  want = want.reshape(-1, n)
+  got = F.operand_value(q).reshape(-1, n)
+  blocks = (n + 127) // 128
+  scales = q.scales.cpu().numpy().reshape(want.shape[0], -1)[:, :blocks]
+  unit = 2.0 ** (scales.astype(np.float64) - 127)
+  full = np.zeros((want.shape[0], blocks * 128))
+  full[:, :n] = np.abs(want)
+  top = full.reshape(-1, blocks, 128).max(-1)
+  assert (top <= 448 * unit * (1 + slack)).all()
+  smaller = (unit > 2.0 ** -117) & (top <= 224 * unit * (1 - slack))
+  assert not smaller.any()
+  unit = np.repeat(unit, 128, axis=-1)[:, :n]
+  step = np.maximum(np.abs(want) * 2.0 ** -4, unit * 2.0 ** -10)
+  assert (np.abs(got - want) <= step * (1 + 2.0 ** -8) + np.abs(want) * slack).all()
+  codes = q.values.view(torch.uint8).cpu().numpy().reshape(want.shape[0], -1)
+  assert (codes[:, n:] == 0).all()
+
+
+def _assert_product(got, want, magnitudes):
+  error = np.abs(_f64(got) - want)
+  assert (error <= np.abs(want) * 2.0 ** -8 + magnitudes * 2.0 ** -13).all()
+
+
+# --- operands ---------------------------------------------------------------
+SHAPES = [(1, 1, 1), (1, 1, 128), (1, 128, 1), (2, 129, 127), (3, 5, 1000),
+          (1, 300, 264), (2, 64, 513), (1, 700, 1032), (5, 130, 8)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_quantize(hip, shape, dtype):
+  rng = np.random.default_rng(sum(shape))
+  x = _tensor(rng, shape, dtype)
+  rows, columns = hip.quantize(x, rows=True, columns=True)
+  _assert_operand(rows, _f64(x))
+  _assert_operand(columns, _f64(x).transpose(0, 2, 1))
+  only = hip.quantize(x)
+  assert torch.equal(only.values.view(torch.uint8), rows.values.view(torch.uint8))
+  only = hip.quantize(x, rows=False, columns=True)
+  assert torch.equal(only.values.view(torch.uint8), columns.values.view(torch.uint8))
+  flat = hip.quantize(x[0], rows=False, columns=True)
+  assert flat.shape == (shape[2], shape[1])
+  assert torch.equal(flat.values.view(torch.uint8),
+                     columns.values[0].view(torch.uint8))
+
+
+def test_quantize_of_many_tiles(hip):
+  """Blocks of the grid in the order that keeps an XCD's tiles together."""
+  rng = np.random.default_rng(0)
+  x = _tensor(rng, (1, 2055, 5000), "bf16")
+  rows, columns = hip.quantize(x, rows=True, columns=True)
+  _assert_operand(rows, _f64(x))
+  _assert_operand(columns, _f64(x).transpose(0, 2, 1))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_quantize_of_borders(hip, dtype):
+  """Ties, values next to a unit's limit, zeros, the smallest and the largest numbers,
+  infinities and NaN."""
+  x = np.zeros((40, 128), np.float32)
+  for i in range(20):
+    x[i] = np.linspace(-17, 17, 128) * 2.0 ** (7 * i - 70)
+    x[i, 0] = [448, 449, 447, 450, 452, 224, 225, 1, 1.75, 1.7578125][i % 10] * 2.0 ** (
+        7 * i - 70)
+  x[20, 5] = 1e-45
+  x[21] = np.float32(2.0 ** -126) * np.linspace(-1, 1, 128)
+  x[22] = np.float32(3.3e38) * np.linspace(-1, 1, 128)
+  x[23, 1], x[24, 2], x[25, 3] = np.inf, -np.inf, np.nan
+  x[26, 1:3] = 448, 0.5 * 2.0 ** -9          # a tie with zero
+  x[27, 1:4] = 448, 1.5 * 2.0 ** -9, 2.5 * 2.0 ** -9
+  x[28] = -0.0
+  x[29, :2] = 2.0 ** -109 * 1.75, 2.0 ** -126
+  x[30, :2] = 2.0 ** -120, 2.0 ** -127
+  t = torch.from_numpy(x).to(TYPES[dtype]).cuda()
+  for rows, want in ((hip.quantize(t), _f64(t)),
+                     (hip.quantize(t.t().contiguous(), rows=False, columns=True),
+                      _f64(t))):
+    _assert_operand(rows, want)
+    for to in (torch.bfloat16, torch.float32):
+      # (numbers from 248 * 2^120 on round to 2^128, which neither type has: there the
+      # 8-bit value is read as an infinity)
+      want = F.operand_value(rows)
+      want = np.where(np.abs(want) == 2.0 ** 128, np.copysign(np.inf, want), want)
+      np.testing.assert_array_equal(_f64(hip.dequantize(rows, to)), want)
+
+
+@pytest.mark.parametrize("shape", [(3, 140, 200), (2, 70, 131)])
+def test_quantize_masks_and_counts(hip, shape):
+  """What is masked or behind the count does not reach the operands, whatever it is."""
+  rng = np.random.default_rng(7)
+  x = _tensor(rng, shape, "bf16")
+  mask = torch.from_numpy(np.maximum(rng.standard_normal(shape), 0)).to(x).contiguous()
+  mask[0, 3, 5], mask[1, 2, 2], mask[0, 0, 0] = float("nan"), -1, -float("inf")
+  x = torch.where(mask > 0, x, torch.full_like(x, float("inf")))
+  count = torch.tensor([0, shape[1] + 9, 129][:shape[0]], dtype=torch.int32).cuda()
+  x[2:, 129:] = float("nan")
+  want = np.where(_f64(mask) > 0, _f64(x), 0)
+  for e, c in enumerate(count.tolist()):
+    want[e, c:] = 0
+  rows, columns = hip.quantize(x, rows=True, columns=True, relu_mask=mask,
+                               row_count=count)
+  _assert_operand(rows, want)
+  _assert_operand(columns, want.transpose(0, 2, 1))
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (7, 130), (300, 1024), (2, 3, 77)])
+def test_dequantize(hip, shape):
+  q = F.random_operand(np.random.default_rng(1), shape, 3.0)
+  for dtype in (torch.bfloat16, torch.float32):
+    y = hip.dequantize(q, dtype)
+    assert y.dtype == dtype and tuple(y.shape) == shape
+    np.testing.assert_array_equal(_f64(y), F.operand_value(q))
+
+
+# --- the norm ---------------------------------------------------------------
+def _norm_64(total, scale, mask, epsilon):
+  t = _f64(total)
+  y = t / np.sqrt((t * t).mean(-1, keepdims=True) + epsilon) * _f64(scale)
+  return y if mask is None else np.where(_f64(mask)[..., None] != 0, y, 0) * np.where(
+      _f64(mask) != 0, _f64(mask), 0)[..., None]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,m", [(1, 1), (5, 100), (3, 128), (33, 1024), (2, 1025),
+                                    (7, 2048), (3, 4096), (4, 4099), (2, 8192),
+                                    (3, 9000), (1, 16385), (2, 20000)])
+def test_residual_rms_norm(hip, rows, m, dtype):
+  rng = np.random.default_rng(m + rows)
+  x, residual = (_tensor(rng, (rows, m), dtype, 1.0) for _ in range(2))
+  scale = (1 + 0.2 * torch.randn(m, generator=torch.Generator().manual_seed(m))).to(
+      x).contiguous()
+  mask = torch.tensor([1.0, 0.0, 0.5, 1.0])[torch.arange(rows) % 4].to(x)
+  want_sum = (x.float() + residual.float()).to(x.dtype)
+  total, y, norm = hip.residual_rms_norm(x, residual, scale, want_norm=True)
+  assert torch.equal(total, want_sum)
+  want = _norm_64(total, scale, None, 1e-6)
+  _assert_rounded(y, want)
+  eps = 2.0 ** -8 if dtype == "bf16" else 2.0 ** -19
+  assert (np.abs(_f64(norm) - want) <= eps * np.abs(want) * (1 + 2.0 ** -8)).all()
+  total, y = hip.residual_rms_norm(x, residual, scale, 1e-3, row_mask=mask)
+  assert torch.equal(total, want_sum)
+  _assert_rounded(y, _norm_64(total, scale, mask, 1e-3))
+  total, y = hip.residual_rms_norm(x, None, scale)
+  assert total is x
+  _assert_rounded(y, _norm_64(x, scale, None, 1e-6))
+
+
+def test_residual_rms_norm_of_odd_rows(hip):
+  """Zeros, rows that are masked out with an infinity in them, rows with one, more
+  leading dimensions, operands that do not start on 16 bytes."""
+  rng = np.random.default_rng(0)
+  x = _tensor(rng, (2, 3, 640), "bf16", 1.0)
+  x[0, 0] = 0
+  x[0, 1, 7], x[1, 0, 600] = float("inf"), float("nan")
+  scale = torch.ones(640, dtype=torch.bfloat16, device="cuda")
+  mask = torch.ones(2, 3, dtype=torch.bfloat16, device="cuda")
+  mask[0, 1] = 0
+  total, y = hip.residual_rms_norm(x, torch.zeros_like(x), scale, row_mask=mask)
+  got = F.operand_value(y)
+  assert y.shape == (2, 3, 640) and total.shape == (2, 3, 640)
+  assert (got[0, :2] == 0).all() and np.isnan(got[1, 0]).all()
+  for at in ((0, 2), (1, 1), (1, 2)):
+    assert np.isfinite(got[at]).all() and np.abs(got[at]).max() > 0.5
+  flat = _tensor(rng, (5 * 640 + 3,), "bf16", 1.0)
+  odd = flat[3:].view(5, 640)
+  assert odd.data_ptr() % 16
+  total, y = hip.residual_rms_norm(odd, odd, scale)
+  again = hip.residual_rms_norm(odd.clone(), odd.clone(), scale)
+  assert torch.equal(total, again[0])
+  assert torch.equal(y.values.view(torch.uint8), again[1].values.view(torch.uint8))
+
+
+# --- products ---------------------------------------------------------------
+def _act(y, activation):
+  if activation == "relu":
+    return np.maximum(y, 0)
+  if activation == "gelu":
+    return y * 0.5 * (1 + np.tanh(0.7978845608028654 * (y + 0.044715 * y ** 3)))
+  if activation == "sigmoid":
+    return 1 / (1 + np.exp(-y))
+  if activation == "swish":
+    return y / (1 + np.exp(-y))
+  return np.tanh(y) if activation == "tanh" else y
+
+
+# rows from one to several tiles, reductions of one block and of many, odd columns
+PRODUCTS = [(1, 1, 1, 1), (1, 1, 128, 32), (1, 1, 4096, 1000), (1, 3, 300, 17),
+            (2, 33, 130, 129), (1, 64, 1024, 256), (5, 40, 256, 64), (1, 65, 640, 385),
+            (1, 129, 2000, 130), (3, 200, 384, 300), (1, 257, 512, 513),
+            (2, 300, 1100, 256), (1, 1000, 256, 1024), (4, 520, 896, 640),
+            (1, 2050, 384, 1537), (1, 512, 4224, 512), (64, 6, 512, 256),
+            (1, 8, 1024, 4096), (1, 1100, 128, 8), (1, 384, 129, 4000)]
+
+
+@pytest.mark.parametrize("e,r,k,n", PRODUCTS)
+def test_expert_linear(hip, e, r, k, n):
+  rng = np.random.default_rng(e + r + k + n)
+  a = F.random_operand(rng, (e, r, k), 1.0)
+  w = F.random_operand(rng, (e, n, k), k ** -0.5)
+  av, wv = F.operand_value(a), F.operand_value(w).transpose(0, 2, 1)
+  want, magnitudes = av @ wv, np.abs(av) @ np.abs(wv)
+  _assert_product(hip.expert_linear(a, w), want, magnitudes)
+  for activation in ("relu", "gelu"):
+    # (their slopes are at most 1.13)
+    _assert_product(hip.expert_linear(a, w, activation), _act(want, activation),
+                    1.13 * magnitudes)
+  q = hip.expert_linear(a, w, "relu", eight_bit=True)
+  y = hip.dequantize(hip.quantize(torch.from_numpy(
+      np.maximum(want, 0)).float().cuda()), torch.float32)
+  # the 8-bit result against the 8-bit form of the exact one: the same but where the
+  # sums' error crosses a rounding border, there a step apart
+  got, ref = F.operand_value(q), _f64(y)
+  assert np.abs(got - np.maximum(want, 0)).max() <= (
+      2.0 ** -4 * np.abs(want).max() + 2.0 ** -13 * magnitudes.max())
+  assert (got == ref).mean() > 0.98
+  codes = q.values.view(torch.uint8).cpu().numpy()
+  assert (codes[..., n:] == 0).all()
+
+
+@pytest.mark.parametrize("activation", [None, "linear", "sigmoid", "tanh", "swish"])
+@pytest.mark.parametrize("r", [2, 300])
+def test_activations(hip, activation, r):
+  rng = np.random.default_rng(3)
+  a, w = F.random_operand(rng, (1, r, 256), 1.0), F.random_operand(rng, (1, 264, 256),
+                                                                  0.06)
+  av, wv = F.operand_value(a), F.operand_value(w).transpose(0, 2, 1)
+  _assert_product(hip.expert_linear(a, w, activation), _act(av @ wv, activation),
+                  1.13 * (np.abs(av) @ np.abs(wv)))
+
+
+@pytest.mark.parametrize("eight_bit", [False, True])
+@pytest.mark.parametrize("r,n", [(6, 200), (70, 128), (300, 256), (600, 392)])
+def test_row_counts(hip, r, n, eight_bit):
+  """Rows behind an expert's count are left as they were; infinities in them go
+  nowhere."""
+  rng = np.random.default_rng(r)
+  e, k = 5, 320
+  a, w = F.random_operand(rng, (e, r, k), 1.0), F.random_operand(rng, (e, n, k), 0.05)
+  count = [0, 1, r // 2 + 1, r, r + 100]
+  for i, c in enumerate(count):
+    a.values[i, c:].view(torch.uint8).fill_(0x7f)
+  counts = torch.tensor(count, dtype=torch.int32, device="cuda")
+  whole = hip.expert_linear(a, w, "relu", eight_bit)
+  if eight_bit:
+    out = hip.Fp8Blocks.empty((e, r, n), "cuda")
+    out.values.view(torch.uint8).fill_(0x55)
+    out.scales.fill_(99)
+  else:
+    out = torch.full((e, r, n), 7.0, dtype=torch.bfloat16, device="cuda")
+  got = hip.expert_linear(a, w, "relu", eight_bit, row_count=counts, out=out)
+  assert got is out
+  for i, c in enumerate(count):
+    if eight_bit:
+      assert torch.equal(got.values[i, :c].view(torch.uint8),
+                         whole.values[i, :c].view(torch.uint8))
+      assert (got.values[i, c:].view(torch.uint8) == 0x55).all()
+      assert (got.scales[i, c:] == 99).all()
+    else:
+      assert torch.equal(got[i, :c], whole[i, :c]) and (got[i, c:] == 7).all()
+  counts.fill_(-3)
+  hip.expert_linear(a, w, "relu", eight_bit, row_count=counts, out=out)
+  assert ((got.values[0].view(torch.uint8) == 0x55) if eight_bit else got[0] == 7).all()
+
+
+@pytest.mark.parametrize("r", [1, 40, 300])
+def test_infinities_stay_in_their_rows(hip, r):
+  """A block that is NaN makes its row of the result NaN, and no other one."""
+  rng = np.random.default_rng(r)
+  x = _tensor(rng, (1, r, 300), "bf16", 0.5)
+  x[0, r // 2, 200] = float("inf")
+  w = F.random_operand(rng, (1, 256, 300), 0.05)
+  y = hip.expert_linear(hip.quantize(x), w)
+  bad = torch.isnan(y[0]).all(-1)
+  assert bad[r // 2] and bad.sum() == 1 and torch.isnan(y).sum() == 256
+  q = hip.expert_linear(hip.quantize(x), w, eight_bit=True)
+  assert np.isnan(F.operand_value(q)[0, r // 2]).all()
+  assert np.isnan(F.operand_value(q)).sum() == 256
+
+
+def test_scales_of_all_sizes(hip):
+  """Every unit an operand can have, on both sides."""
+  rng = np.random.default_rng(0)
+  a, w = F.random_operand(rng, (1, 235, 512), 1.0), F.random_operand(rng, (1, 16, 512),
+                                                                    1.0)
+  a.scales[0, :, :] = torch.arange(10, 245, dtype=torch.uint8, device="cuda")[:, None]
+  w.scales.fill_(120)
+  w.scales[..., 1] = 130
+  av, wv = F.operand_value(a), F.operand_value(w).transpose(0, 2, 1)
+  want, magnitudes = (av @ wv)[0], (np.abs(av) @ np.abs(wv))[0]
+  got = _f64(hip.expert_linear(a, w))[0]
+  # (where neither the results nor their parts leave float32's normal numbers)
+  inside = (magnitudes < 2.0 ** 126) & (np.arange(235)[:, None] > 25)
+  error = np.abs(got - want)
+  assert inside.any(-1).sum() > 180
+  assert (error <= np.abs(want) * 2.0 ** -8 + magnitudes * 2.0 ** -13)[inside].all()
+
+
+def test_dense(hip):
+  rng = np.random.default_rng(5)
+  x, w = F.random_operand(rng, (3, 5, 384), 1.0), F.random_operand(rng, (1, 250, 384),
+                                                                  0.05)
+  flat = hip.expert_linear(x.reshape(1, 15), w, "relu")
+  y = hip.dense(x, w, "relu")
+  assert tuple(y.shape) == (3, 5, 250) and torch.equal(y.view(1, 15, 250), flat)
+  q = hip.dense(x, w, "relu", eight_bit=True)
+  assert q.shape == (3, 5, 250)
+
+
+def test_refusals(hip):
+  rng = np.random.default_rng(5)
+  a, w = F.random_operand(rng, (2, 4, 256), 1.0), F.random_operand(rng, (2, 8, 256), 1.0)
+  Error = hip.MoeHipError
+  other = F.random_operand(rng, (2, 8, 255), 1.0)
+  bf16 = torch.zeros(2, 4, 8, dtype=torch.bfloat16, device="cuda")
+  count = torch.zeros(2, dtype=torch.int32, device="cuda")
+  strided = hip.Fp8Blocks(a.values.transpose(0, 1), a.scales.transpose(0, 1), 256)
+  for call in (
+      lambda: hip.expert_linear(a, other), lambda: hip.expert_linear(a, w.reshape(16)),
+      lambda: hip.expert_linear(strided, w),
+      lambda: hip.expert_linear(a, w, out=bf16.float()),
+      lambda: hip.expert_linear(a, w, out=bf16[..., :7]),
+      lambda: hip.expert_linear(a, w, eight_bit=True, out=bf16),
+      lambda: hip.expert_linear(a, w, row_count=count.long()),
+      lambda: hip.expert_linear(a, w, row_count=count[:1]),
+      lambda: hip.dense(a, w),
+      lambda: hip.quantize(bf16.transpose(1, 2)),
+      lambda: hip.quantize(bf16, relu_mask=bf16.float()),
+      lambda: hip.residual_rms_norm(bf16, None, torch.ones(8, device="cuda")),
+      lambda: hip.residual_rms_norm(bf16, bf16[:1], bf16[0, 0]),
+      lambda: hip.expert_linear_backward(a, bf16),
+      lambda: hip.expert_linear_backward(w, bf16, da=bf16)):
+    with pytest.raises(Error):
+      call()
+  with pytest.raises(ValueError):
+    hip.expert_linear(a, w, "softplus")
+
+
+def test_tensors_without_elements(hip):
+  empty = torch.empty(0, 256, dtype=torch.bfloat16, device="cuda")
+  q = hip.quantize(empty)
+  assert q.shape == (0, 256) and hip.dequantize(q).shape == (0, 256)
+  total, y = hip.residual_rms_norm(empty, empty, torch.ones_like(empty[:1].sum(0)))
+  assert y.shape == (0, 256) and total.shape == (0, 256)
+  w = F.random_operand(np.random.default_rng(0), (1, 8, 256), 1.0)
+  assert hip.dense(q, w).shape == (0, 8)
+
+
+# --- gradients --------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("e,r,k,n", [(1, 1, 8, 16), (2, 70, 200, 136), (1, 300, 256, 520),
+                                     (3, 130, 129, 33), (1, 1385, 256, 512)])
+def test_expert_linear_backward(hip, e, r, k, n, dtype):
+  rng = np.random.default_rng(e + r + k + n)
+  a_columns = F.random_operand(rng, (e, k, r), 1.0)
+  w_rows = F.random_operand(rng, (e, k, n), 0.05)
+  dy = _tensor(rng, (e, r, n), dtype, 0.5)
+  mask = torch.from_numpy(np.maximum(rng.standard_normal((e, r, n)), 0)).to(dy)
+  count = torch.tensor([r, r // 2, 0][:e], dtype=torch.int32, device="cuda")
+  for masked in (False, True):
+    kept = _f64(dy)
+    if masked:
+      kept = np.where(_f64(mask) > 0, kept, 0)
+      for i, c in enumerate(count.tolist()):
+        kept[i, c:] = 0
+    by_row = F.value(*F.quantize(kept.reshape(-1, n)))[:, :n].reshape(e, r, n)
+    turned = kept.transpose(0, 2, 1).reshape(-1, r)
+    by_column = F.value(*F.quantize(turned))[:, :r].reshape(e, n, r)
+    wv, av = F.operand_value(w_rows).transpose(0, 2, 1), F.operand_value(a_columns)
+    da0 = torch.full((e, r, k), 3.0, dtype=torch.bfloat16, device="cuda")
+    da, dw = hip.expert_linear_backward(
+        a_columns, dy, w_rows, relu_mask=mask if masked else None,
+        row_count=count if masked else None, da=da0 if masked else None)
+    _assert_product(dw, av @ by_column.transpose(0, 2, 1),
+                    np.abs(av) @ np.abs(by_column).transpose(0, 2, 1))
+    want, magnitudes = by_row @ wv, np.abs(by_row) @ np.abs(wv)
+    if masked:
+      for i, c in enumerate(count.tolist()):
+        want[i, c:], magnitudes[i, c:] = 3.0, 0
+    _assert_product(da, want, magnitudes)
+    none, dw2 = hip.expert_linear_backward(
+        a_columns, dy, relu_mask=mask if masked else None,
+        row_count=count if masked else None)
+    assert none is None and torch.equal(dw, dw2)
+
+
+def test_gradient_against_differences(hip):
+  """The gradient of sum(y * g) in w and x against differences of the product itself,
+  on numbers that e4m3 holds (all blocks have the unit 2^-2 or less, so that nothing is
+  rounded before the sums)."""
+  rng = np.random.default_rng(2)
+  r, k, n = 130, 40, 24
+
+  def small(*shape):       # multiples of 1/8 up to 1: e4m3 numbers
+    return torch.from_numpy(rng.integers(-8, 9, shape) / 8.0).to(
+        torch.bfloat16).cuda()
+  x, w, g = small(1, r, k), small(1, k, n), small(1, r, n)
+
+  def product(x, w):
+    y = hip.expert_linear(hip.quantize(x), hip.quantize(w, rows=False, columns=True))
+    return _f64(y)
+  # y itself is rounded to bf16: its parts are multiples of 1/64 below 40, differences
+  # of single elements are at most 2 * 1/8, and sums of those over a row need few bits
+  _, a_columns = hip.quantize(x, rows=True, columns=True)
+  dx, dw = hip.expert_linear_backward(a_columns, g, hip.quantize(w))
+  gd, base = _f64(g), product(x * 0, w * 0)
+  assert (base == 0).all()
+  for _ in range(20):
+    i, j, l = rng.integers(r), rng.integers(k), rng.integers(n)
+    one = torch.zeros_like(x)
+    one[0, i, j] = 1
+    want = (product(one, w) * gd).sum()
+    assert abs(_f64(dx)[0, i, j] - want) <= 2.0 ** -8 * abs(want) + 2.0 ** -13 * 40
+    one = torch.zeros_like(w)
+    one[0, j, l] = 1
+    want = (product(x, one) * gd).sum()
+    assert abs(_f64(dw)[0, j, l] - want) <= 2.0 ** -8 * abs(want) + 2.0 ** -13 * r
+
+
+# --- together ---------------------------------------------------------------
+def _mlp(hip, x, residual, scale, wi, wo):
+  total, y = hip.residual_rms_norm(x, residual, scale)
+  h = hip.dense(y, wi, "relu", eight_bit=True)
+  return total, hip.dense(h, wo)
+
+
+def _mlp_inputs(rng, rows, m, f):
+  return (_tensor(rng, (rows, m), "bf16", 0.5), _tensor(rng, (rows, m), "bf16", 0.5),
+          torch.ones(m, dtype=torch.bfloat16, device="cuda"),
+          F.random_operand(rng, (1, f, m), m ** -0.5),
+          F.random_operand(rng, (1, m, f), f ** -0.5))
+
+
+@pytest.mark.parametrize("rows,m,f", [(1, 256, 1024), (40, 384, 1000), (700, 512, 2048)])
+def test_dense_block(hip, rows, m, f):
+  """Norm, wi, wo as a serving program runs them, against float64 with 8-bit roundings.
+  A value on the other side of a rounding border moves by a step, 2^-3 of it; at the
+  sums' 2^-13 error about one in 2^9 does, so the results differ by far less than the
+  2^-4 that rounding itself costs in the root mean square."""
+  x, residual, scale, wi, wo = _mlp_inputs(np.random.default_rng(rows), rows, m, f)
+  total, y = _mlp(hip, x, residual, scale, wi, wo)
+  a = F.value(*F.quantize(_norm_64(total, scale, None, 1e-6)))[:, :m]
+  h = np.maximum(a @ F.operand_value(wi)[0].T, 0)
+  h = F.value(*F.quantize(h))[:, :f]
+  want = h @ F.operand_value(wo)[0].T
+  error = np.sqrt(np.square(_f64(y) - want).mean() / np.square(want).mean())
+  assert error < 2.0 ** -7
+
+
+def test_training_step(hip):
+  """A dense block's gradients as a training program makes them: dw of both layers and
+  dx, against the same products in float64 without any 8-bit rounding."""
+  rng = np.random.default_rng(9)
+  r, m, f = 260, 192, 328
+  x = _tensor(rng, (1, r, m), "bf16", 0.3)
+  wi = torch.from_numpy(rng.standard_normal((1, m, f)) * m ** -0.5).to(x)
+  wo = torch.from_numpy(rng.standard_normal((1, f, m)) * f ** -0.5).to(x)
+  dy = _tensor(rng, (1, r, m), "bf16", 0.3)
+  a, a_columns = hip.quantize(x, rows=True, columns=True)
+  wi_rows, wi_columns = hip.quantize(wi, rows=True, columns=True)
+  wo_rows, wo_columns = hip.quantize(wo, rows=True, columns=True)
+  h = hip.expert_linear(a, wi_columns, "relu")
+  hq, h_columns = hip.quantize(h, rows=True, columns=True)
+  y = hip.expert_linear(hq, wo_columns)
+  dh, dwo = hip.expert_linear_backward(h_columns, dy, wo_rows)
+  dx, dwi = hip.expert_linear_backward(a_columns, dh, wi_rows, relu_mask=h)
+
+  def near(got, want):
+    assert np.sqrt(np.square(_f64(got) - want).mean() /
+                   np.square(want).mean()) < 2.0 ** -3.5
+  # (against the products without any rounding to 8 bits: two operands of a root mean
+  # square error of at most 2^-4 / sqrt(3) each, and as much from what they came from)
+  hx = np.maximum(_f64(x[0]) @ _f64(wi[0]), 0)
+  near(y[0], hx @ _f64(wo[0]))
+  dhx = _f64(dy[0]) @ _f64(wo[0]).T
+  near(dh[0], dhx)
+  near(dwo[0], hx.T @ _f64(dy[0]))
+  # (the mask is the h that the step has: units near 0 are on the other side of it)
+  dhx = dhx * (_f64(h[0]) > 0)
+  near(dx[0], dhx @ _f64(wi[0]).T)
+  near(dwi[0], _f64(x[0]).T @ dhx)
+
+
+@pytest.mark.parametrize("rows", [1, 300])
+def test_captured(hip, rows):
+  """The block recorded into a graph, replayed with new inputs and work between the
+  replays; two graphs and an eager call do not meet."""
+  rng = np.random.default_rng(rows)
+  inputs = [_mlp_inputs(rng, rows, 256, 640) for _ in range(2)]
+  eager = [_mlp(hip, *i) for i in inputs]
+  torch.cuda.synchronize()
+  graphs = []
+  for i in inputs:
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+      outs = _mlp(hip, *i)
+    graphs.append((graph, outs))
+  for _ in range(3):
+    for (graph, outs), want in zip(graphs, eager):
+      for t in outs:
+        t.fill_(-1)
+      graph.replay()
+      again = _mlp(hip, *inputs[0])
+      torch.cuda.synchronize()
+      assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+      assert torch.equal(again[1], eager[0][1])
+
+
+def test_captured_gradients(hip):
+  rng = np.random.default_rng(4)
+  a_columns = F.random_operand(rng, (2, 256, 300), 1.0)
+  w_rows = F.random_operand(rng, (2, 256, 520), 0.05)
+  dy = _tensor(rng, (2, 300, 520), "bf16", 0.5)
+  want = hip.expert_linear_backward(a_columns, dy, w_rows)
+  torch.cuda.synchronize()
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    got = hip.expert_linear_backward(a_columns, dy, w_rows)
+  for _ in range(3):
+    for t in got:
+      t.fill_(-1)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_two_streams(hip):
+  """Calls on two streams at once give what they give one after the other."""
+  rng = np.random.default_rng(11)
+  inputs = [_mlp_inputs(rng, 200 + 100 * i, 512, 1024) for i in range(2)]
+  want = [_mlp(hip, *i) for i in inputs]
+  torch.cuda.synchronize()
+  streams = [torch.cuda.Stream() for _ in range(2)]
+  for _ in range(3):
+    got = []
+    for stream, i in zip(streams, inputs):
+      with torch.cuda.stream(stream):
+        got.append(_mlp(hip, *i))
+    torch.cuda.synchronize()
+    for (total, y), (total0, y0) in zip(got, want):
+      assert torch.equal(total, total0) and torch.equal(y, y0)
