@@ -186,6 +186,13 @@ __device__ __forceinline__ void load_to_lds(const uint8_t* from, int bytes, uint
       (lds_void_t*)to, 16, at, 0, 0, 0);
 }
 
+// 16 bytes per lane, at `at` of the `bytes` at `base`; what lies behind is dropped
+__device__ __forceinline__ void store_line(u32x4_t v, uint8_t* base, int bytes,
+                                           uint32_t at) {
+  __builtin_amdgcn_raw_buffer_store_b128(
+      v, __builtin_amdgcn_make_buffer_rsrc(base, 0, max(bytes, 0), 0x00027000), at, 0, 0);
+}
+
 // two 16-byte chunks of a row
 __device__ __forceinline__ i32x8_t fp8_fragment(const unsigned char* lo,
                                                 const unsigned char* hi) {
@@ -212,8 +219,8 @@ __device__ __forceinline__ void lds_write_b64(uint32_t at, u32x2_t v) {
 }
 
 // EIGHT: the result is an 8-bit operand; ACT: an activation that is neither linear nor
-// relu.
-template <bool EIGHT, bool ACT>
+// relu; WHOLE: rows of a bf16 result are whole pieces of 16 bytes that lie on 16 bytes.
+template <bool EIGHT, bool ACT, bool WHOLE>
 __global__ __launch_bounds__(TileCfg::THREADS) void fp8_tile_kernel(GemmArgs g,
                                                                     TileGrid grid) {
   using Cfg = TileCfg;
@@ -376,9 +383,14 @@ __global__ __launch_bounds__(TileCfg::THREADS) void fp8_tile_kernel(GemmArgs g,
   };
 
   // One K tile; lk: the one that the loads fetch; NA: the wavefront's pieces of 32 rows
-  // that hold rows of the tile.
-  auto k_tile = [&](auto na_tag, int lk) FP8_INLINE {
+  // that hold rows of the tile; LAST: of its tile (whose successor's fragments are read
+  // when the result is out of the registers); stores_out: what follows the token loads
+  // of the K tile that the barrier waits for, besides the four weight loads, may still
+  // be out too.
+  constexpr int STORES = EIGHT ? 4 : 8;           // of 16 bytes per lane and piece
+  auto k_tile = [&](auto na_tag, auto last_tag, int lk, bool stores_out) FP8_INLINE {
     constexpr int NA = decltype(na_tag)::value;
+    constexpr bool LAST = decltype(last_tag)::value;
     const int wnext = wslot == 2 ? 0 : wslot + 1, wload = wnext == 2 ? 0 : wnext + 1;
     const int anext = aslot ^ 1;
 #pragma unroll
@@ -393,30 +405,43 @@ __global__ __launch_bounds__(TileCfg::THREADS) void fp8_tile_kernel(GemmArgs g,
       };
       Source from = s == 0 ? w_source(lk) : a_source(lk);
       const int into = s == 0 ? Cfg::W_BASE + wload * Cfg::SLOT : aslot * Cfg::SLOT;
-      auto rd_a = [&](int i) { if (i < NA) fa[to][i] = read_a(at, as, to, i); };
-      auto rd_w = [&](int j) { if (NA > 0) fw[j] = read_w(at, ws, to, j); };
+      constexpr bool READ[2] = {NA > 0, NA > 0 && !LAST};
+      auto rd_a = [&](int i) { if (READ[s] && i < NA) fa[to][i] = read_a(at, as, to, i); };
+      auto rd_w = [&](int j) { if (READ[s]) fw[j] = read_w(at, ws, to, j); };
+      // (the weight loads have half a K tile more than the token loads, which go first)
+      auto ld = [&](int j, bool here) { if (here) load(from, j, into); };
       fence();
+      if (s == 1) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ld(j, true);
+        fence();
+      }
       rd_a(0);
       mfma(0); fence();
       rd_a(1);
       mfma(1); fence();
       rd_w(0);
-      load(from, 0, into);
+      ld(0, s == 0);
       mfma(2); fence();
       mfma(3); fence();
       rd_w(1);
-      load(from, 1, into);
+      ld(1, s == 0);
       mfma(4); fence();
       mfma(5); fence();
       rd_w(2);
-      load(from, 2, into);
+      ld(2, s == 0);
       mfma(6); fence();
       mfma(7); fence();
       rd_w(3);
-      load(from, 3, into);
+      ld(3, s == 0);
       fence();
       if (s == 0) {
-        __builtin_amdgcn_s_waitcnt(4 | (7 << 4) | (0 << 8));    // vmcnt 4, lgkmcnt 0
+        // lgkmcnt 0 and vmcnt 4, or with the stores of the tile before
+        constexpr int OUT = 4 + STORES * NA;
+        if (stores_out)
+          __builtin_amdgcn_s_waitcnt((OUT & 15) | (OUT >> 4) << 14 | (7 << 4));
+        else
+          __builtin_amdgcn_s_waitcnt(4 | (7 << 4));
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
@@ -429,7 +454,8 @@ __global__ __launch_bounds__(TileCfg::THREADS) void fp8_tile_kernel(GemmArgs g,
   // The result of a tile.  A pass turns 32 rows of 128 bytes round: 64 columns of bf16, or
   // a block of 128 in 8 bits.  Lane l writes 8-byte units of row l % 32 and reads 16
   // bytes of the rows 8 n + l / 8; unit u of a row lies at u ^ 2 (row % 8) ^ (row / 8 %
-  // 2).
+  // 2).  The stores of whole lines go through a buffer that ends with the tile's rows, so
+  // that they leave in any case and the next tile's first wait can count on them.
   auto write_out = [&](const Tile& t, auto na_tag) FP8_INLINE {
     constexpr int NA = decltype(na_tag)::value;
     const int wfree = wslot == 0 ? 2 : wslot - 1;       // of the last K tile
@@ -441,7 +467,6 @@ __global__ __launch_bounds__(TileCfg::THREADS) void fp8_tile_kernel(GemmArgs g,
     const int get_row = lane >> 3, get_chunk = lane & 7;
     const uint32_t get_at = stage + get_row * 128 + ((get_chunk ^ get_row) * 16);
     const int col0 = t.col0 + 128 * wn;
-    const bool whole = EIGHT || (g.N % 8 == 0 && (uintptr_t)g.y % 16 == 0);
     const int64_t first = (int64_t)t.e * g.R + t.row0;
     const int64_t np = fp8_row_bytes(g.N), ns = fp8_scale_bytes(g.N);
     u32x4_t line[4];
@@ -449,7 +474,19 @@ __global__ __launch_bounds__(TileCfg::THREADS) void fp8_tile_kernel(GemmArgs g,
       u32x4_t v = line[n];
       return n & 1 ? __builtin_shufflevector(v, v, 2, 3, 0, 1) : v;
     };
-    if (col0 >= g.N) return;
+    const int row_bytes = EIGHT ? (int)np : 2 * g.N;
+    // lines from column `col` (in bytes) of the piece's rows
+    auto store_lines = [&](int piece, int col) FP8_INLINE {
+      const int rows = t.valid - piece;
+      uint8_t* const base = (uint8_t*)g.y + (first + piece) * row_bytes + col;
+      const uint32_t at = col + 16 * get_chunk < row_bytes
+                              ? (uint32_t)(get_row * row_bytes + 16 * get_chunk)
+                              : 0x80000000u;      // (past every buffer)
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        store_line(chunk_of(n), base + (int64_t)8 * n * row_bytes,
+                   max(min(rows - 8 * n, 8), 0) * row_bytes - col, at);
+    };
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
       const int piece = 128 * i + 32 * wm;
@@ -496,16 +533,10 @@ __global__ __launch_bounds__(TileCfg::THREADS) void fp8_tile_kernel(GemmArgs g,
             const int unit = 2 * (2 * j + (q >> 3));    // + fc, which put_at has
             lds_write_b64(put_at ^ (unit * 8), u32x2_t{w[0], w[1]});
           }
-        if (fc == 0 && piece + fr < t.valid)
+        if (fc == 0 && piece + fr < t.valid && col0 < g.N)
           g.y_scales[(first + piece + fr) * ns + col0 / FP8_BLOCK] = (uint8_t)s.byte;
         lds_read_lines(line, get_at);
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const int row = piece + 8 * n + get_row;
-          if (row < t.valid)
-            *reinterpret_cast<u32x4_t*>((uint8_t*)g.y + (first + row) * np + col0 +
-                                        16 * get_chunk) = chunk_of(n);
-        }
+        store_lines(piece, col0);
       } else {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -519,17 +550,11 @@ __global__ __launch_bounds__(TileCfg::THREADS) void fp8_tile_kernel(GemmArgs g,
                                     f32x2_to_bf16x2(v[j][q + 2], v[j][q + 3])});
             }
           lds_read_lines(line, get_at);
-          bf16_t* const to = (bf16_t*)g.y + (first + piece) * g.N + col0 + 64 * h;
-          if (whole) {
-            const int col = 8 * get_chunk;
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              const int row = 8 * n + get_row;
-              if (piece + row < t.valid && col0 + 64 * h + col < g.N)
-                *reinterpret_cast<u32x4_t*>(to + (int64_t)row * g.N + col) = chunk_of(n);
-            }
+          if constexpr (WHOLE) {
+            store_lines(piece, 2 * (col0 + 64 * h));
           } else if (col0 + 64 * h + lane < g.N) {
             // rows that do not start on 16 bytes: a column per lane
+            bf16_t* const to = (bf16_t*)g.y + (first + piece) * g.N + col0 + 64 * h;
             const int rows = min(32, t.valid - piece);
 #pragma unroll 1
             for (int row = 0; row < rows; ++row) {
@@ -561,15 +586,17 @@ __global__ __launch_bounds__(TileCfg::THREADS) void fp8_tile_kernel(GemmArgs g,
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  first_fragments(0, 0);
+  bool stores_out = false;
   for (;;) {
     Tile after = {0, 0, 0, 0};
     auto tile_pass = [&](auto na_tag) FP8_INLINE {
+      constexpr int NA = decltype(na_tag)::value;
+      if constexpr (NA > 0) first_fragments(aslot, wslot);
 #pragma unroll
-      for (int i = 0; i < decltype(na_tag)::value; ++i)
+      for (int i = 0; i < NA; ++i)
 #pragma unroll
         for (int j = 0; j < Cfg::TN; ++j) acc[i][j] = f32x16_t{};
-      for (int kt = 0; kt < nk; ++kt) {
+      auto next_scales = [&](int kt) FP8_INLINE {
         if ((kt & 3) == 0) {
 #pragma unroll
           for (int i = 0; i < Cfg::TM; ++i) sa[i] = sa_next[i];
@@ -582,23 +609,29 @@ __global__ __launch_bounds__(TileCfg::THREADS) void fp8_tile_kernel(GemmArgs g,
 #pragma unroll
           for (int j = 0; j < Cfg::TN; ++j) sw[j] >>= 8;
         }
+      };
+      for (int kt = 0; kt < nk - 1; ++kt) {
+        next_scales(kt);
         if (kt == nk - 2) {
           // the last two K tiles load the next tile's first two (without a next one,
           // this one's again, which nobody reads)
           after = tile_at(number(++round));
           set_loads(after.valid != 0 ? after : t);
         }
-        if (kt == nk - 1 && after.valid != 0) load_scales(after, 0);
-        k_tile(na_tag, kt + 2 < nk ? kt + 2 : kt + 2 - nk);
+        k_tile(na_tag, std::false_type{}, kt == nk - 2 ? 0 : kt + 2, stores_out);
+        stores_out = false;
       }
+      next_scales(nk - 1);
+      if (after.valid != 0) load_scales(after, 0);
+      k_tile(na_tag, std::true_type{}, 1, false);
       write_out(t, na_tag);
+      stores_out = (EIGHT || WHOLE) && NA > 0;
     };
     const int pieces = t.valid > 128 + 32 * wm ? 2 : t.valid > 32 * wm ? 1 : 0;
     if (pieces == 2) tile_pass(std::integral_constant<int, 2>{});
     else if (pieces == 1) tile_pass(std::integral_constant<int, 1>{});
     else tile_pass(std::integral_constant<int, 0>{});
     if (after.valid == 0) break;
-    if (pieces < 2) first_fragments(aslot, wslot);
     t = after;
   }
   // no direct load may outlive the block
@@ -607,11 +640,12 @@ __global__ __launch_bounds__(TileCfg::THREADS) void fp8_tile_kernel(GemmArgs g,
 #undef FP8_INLINE
 
 // bytes of scratch one product needs
-static bool tiles_apply(int R, int K) {
-  return R > 64 && K > FP8_BLOCK && K <= 1 << 22;
+// (a tile's operand rows and 8 rows of its result are addressed in 31 bits)
+static bool tiles_apply(int R, int K, int N) {
+  return R > 64 && K > FP8_BLOCK && K <= 1 << 22 && N <= 1 << 26;
 }
 static size_t product_workspace(int E, int R, int K, int N, bool eight_bit) {
-  return eight_bit && !tiles_apply(R, K) ? (size_t)E * R * N * sizeof(float) : 0;
+  return eight_bit && !tiles_apply(R, K, N) ? (size_t)E * R * N * sizeof(float) : 0;
 }
 
 template <bool EIGHT>
@@ -628,8 +662,13 @@ static int run_tiles(const GemmArgs& g, hipStream_t st) {
   const int cus = compute_units();
   if (cus == 0) return MESH_MOE_E_HIP;
   const int most = cus / 8 * 8, want = (grid.tiles + 7) / 8 * 8;
-  auto kernel = g.activation == MESH_MOE_ACT_LINEAR || g.activation == MESH_MOE_ACT_RELU
-                    ? fp8_tile_kernel<EIGHT, false> : fp8_tile_kernel<EIGHT, true>;
+  const bool act =
+      g.activation != MESH_MOE_ACT_LINEAR && g.activation != MESH_MOE_ACT_RELU;
+  const bool whole = EIGHT || (g.N % 8 == 0 && (uintptr_t)g.y % 16 == 0);
+  auto kernel = whole ? act ? fp8_tile_kernel<EIGHT, true, true>
+                            : fp8_tile_kernel<EIGHT, false, true>
+                : act ? fp8_tile_kernel<EIGHT, true, EIGHT>
+                      : fp8_tile_kernel<EIGHT, false, EIGHT>;
   MOE_ALLOW_LDS(kernel, TileCfg::LDS_BYTES);
   kernel<<<(unsigned)(want < most ? want : most), TileCfg::THREADS,
                            TileCfg::LDS_BYTES, st>>>(g, grid);
@@ -638,7 +677,7 @@ static int run_tiles(const GemmArgs& g, hipStream_t st) {
 }
 
 static int run_product(const GemmArgs& g, void* workspace, hipStream_t st) {
-  if (tiles_apply(g.R, g.K))
+  if (tiles_apply(g.R, g.K, g.N))
     return g.y_scales ? run_tiles<true>(g, st) : run_tiles<false>(g, st);
   const dim3 grid((g.N + 31) / 32, (g.R + 31) / 32, g.E);
   MOE_REQUIRE(grid.y <= 65535 && grid.z <= 65535, MESH_MOE_E_UNSUPPORTED,
