@@ -383,16 +383,16 @@ __global__ __launch_bounds__(TileCfg::THREADS) void fp8_tile_kernel(GemmArgs g,
   };
 
   // One K tile; lk: the one that the loads fetch; NA: the wavefront's pieces of 32 rows
-  // that hold rows of the tile; LAST: of its tile (whose successor's fragments are read
-  // when the result is out of the registers); stores_out: what follows the token loads
-  // of the K tile that the barrier waits for, besides the four weight loads, may still
-  // be out too.
+  // that hold rows of the tile; FIRST: the sums begin; LAST: the next tile's fragments
+  // are read when the result is out of the registers.  No branches inside: the compiler
+  // would move matrix instructions past them, behind the barrier.
   constexpr int STORES = EIGHT ? 4 : 8;           // of 16 bytes per lane and piece
-  auto k_tile = [&](auto na_tag, auto last_tag, int lk, bool stores_out) FP8_INLINE {
+  auto k_tile = [&](auto na_tag, auto first_tag, auto last_tag, int lk) FP8_INLINE {
     constexpr int NA = decltype(na_tag)::value;
-    constexpr bool LAST = decltype(last_tag)::value;
+    constexpr bool FIRST = decltype(first_tag)::value, LAST = decltype(last_tag)::value;
     const int wnext = wslot == 2 ? 0 : wslot + 1, wload = wnext == 2 ? 0 : wnext + 1;
     const int anext = aslot ^ 1;
+    const f32x16_t none = {};
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int at = frag_again();
@@ -401,7 +401,8 @@ __global__ __launch_bounds__(TileCfg::THREADS) void fp8_tile_kernel(GemmArgs g,
       auto mfma = [&](int m) {
         const int j = m >> 1, i = m & 1;
         if (i >= NA) return;
-        acc[i][j] = fp8_mfma(fw[j], fa[s][i], acc[i][j], sw[j], sa[i]);
+        acc[i][j] = fp8_mfma(fw[j], fa[s][i], FIRST && s == 0 ? none : acc[i][j], sw[j],
+                             sa[i]);
       };
       Source from = s == 0 ? w_source(lk) : a_source(lk);
       const int into = s == 0 ? Cfg::W_BASE + wload * Cfg::SLOT : aslot * Cfg::SLOT;
@@ -436,12 +437,11 @@ __global__ __launch_bounds__(TileCfg::THREADS) void fp8_tile_kernel(GemmArgs g,
       ld(3, s == 0);
       fence();
       if (s == 0) {
-        // lgkmcnt 0 and vmcnt 4, or with the stores of the tile before
-        constexpr int OUT = 4 + STORES * NA;
-        if (stores_out)
-          __builtin_amdgcn_s_waitcnt((OUT & 15) | (OUT >> 4) << 14 | (7 << 4));
-        else
-          __builtin_amdgcn_s_waitcnt(4 | (7 << 4));
+        // lgkmcnt 0, and vmcnt: besides the weight loads of step 0 the first K tile leaves
+        // out as many of the last tile's stores as every wavefront has at least (see the
+        // end of a tile)
+        constexpr int OUT = FIRST ? 4 + STORES : 4;
+        __builtin_amdgcn_s_waitcnt((OUT & 15) | (OUT >> 4) << 14 | (7 << 4));
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
@@ -582,20 +582,14 @@ __global__ __launch_bounds__(TileCfg::THREADS) void fp8_tile_kernel(GemmArgs g,
 #pragma unroll
     for (int j = 0; j < 4; ++j) load(ws, j, Cfg::W_BASE + k * Cfg::SLOT);
   }
-  __builtin_amdgcn_s_waitcnt(8 | (7 << 4) | (15 << 8));         // vmcnt 8
+  __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));             // vmcnt 0
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  bool stores_out = false;
   for (;;) {
     Tile after = {0, 0, 0, 0};
     auto tile_pass = [&](auto na_tag) FP8_INLINE {
       constexpr int NA = decltype(na_tag)::value;
-      if constexpr (NA > 0) first_fragments(aslot, wslot);
-#pragma unroll
-      for (int i = 0; i < NA; ++i)
-#pragma unroll
-        for (int j = 0; j < Cfg::TN; ++j) acc[i][j] = f32x16_t{};
       auto next_scales = [&](int kt) FP8_INLINE {
         if ((kt & 3) == 0) {
 #pragma unroll
@@ -610,22 +604,28 @@ __global__ __launch_bounds__(TileCfg::THREADS) void fp8_tile_kernel(GemmArgs g,
           for (int j = 0; j < Cfg::TN; ++j) sw[j] >>= 8;
         }
       };
-      for (int kt = 0; kt < nk - 1; ++kt) {
+      // the last two K tiles load the next tile's first two (without a next one, this
+      // one's again, which nobody reads)
+      auto advance = [&]() FP8_INLINE {
+        after = tile_at(number(++round));
+        set_loads(after.valid != 0 ? after : t);
+      };
+      if constexpr (NA > 0) first_fragments(aslot, wslot);
+      next_scales(0);
+      if (nk == 2) advance();
+      k_tile(na_tag, std::true_type{}, std::false_type{}, nk == 2 ? 0 : 2);
+      for (int kt = 1; kt < nk - 1; ++kt) {
         next_scales(kt);
-        if (kt == nk - 2) {
-          // the last two K tiles load the next tile's first two (without a next one,
-          // this one's again, which nobody reads)
-          after = tile_at(number(++round));
-          set_loads(after.valid != 0 ? after : t);
-        }
-        k_tile(na_tag, std::false_type{}, kt == nk - 2 ? 0 : kt + 2, stores_out);
-        stores_out = false;
+        if (kt == nk - 2) advance();
+        k_tile(na_tag, std::false_type{}, std::false_type{}, kt == nk - 2 ? 0 : kt + 2);
       }
       next_scales(nk - 1);
       if (after.valid != 0) load_scales(after, 0);
-      k_tile(na_tag, std::true_type{}, 1, false);
+      k_tile(na_tag, std::false_type{}, std::true_type{}, 1);
       write_out(t, na_tag);
-      stores_out = (EIGHT || WHOLE) && NA > 0;
+      // The next first K tile's barrier takes it that STORES stores at least came after
+      // the loads that it waits for, or that they have landed.
+      if constexpr (NA == 0 || !WHOLE) __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));
     };
     const int pieces = t.valid > 128 + 32 * wm ? 2 : t.valid > 32 * wm ? 1 : 0;
     if (pieces == 2) tile_pass(std::integral_constant<int, 2>{});
