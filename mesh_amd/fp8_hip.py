@@ -78,7 +78,7 @@ class Fp8Blocks(object):
   [..., rows, scale_bytes(n)] of torch.uint8; value i of a row stands for values[i] *
   2^(scales[i // 128] - 127).  The values from n on are zeros."""
 
-  __slots__ = ("values", "scales", "n")
+  __slots__ = ("_values", "_scales", "_shape")
 
   def __init__(self, values, scales, n):
     n = int(n)
@@ -88,38 +88,69 @@ class Fp8Blocks(object):
       raise ValueError(
           "values %s of %s and scales %s of %s are not rows of %d 8-bit values"
           % (tuple(values.shape), values.dtype, tuple(scales.shape), scales.dtype, n))
-    self.values = values
-    self.scales = scales
-    self.n = n
+    self._set(values, scales, tuple(values.shape[:-1]) + (n,))
+
+  def _set(self, values, scales, shape):
+    self._values = values
+    self._scales = scales
+    self._shape = shape
+    return self
+
+  @property
+  def values(self):
+    return self._values
+
+  @property
+  def scales(self):
+    return self._scales
+
+  @property
+  def n(self):
+    return self._shape[-1]
 
   @property
   def shape(self):
     """Of the tensor that the operand stands for."""
-    return tuple(self.values.shape[:-1]) + (self.n,)
+    return self._shape
 
   @classmethod
   def empty(cls, shape, device):
     """An operand for a tensor of `shape`, not filled in."""
-    rows, n = tuple(shape[:-1]), shape[-1]
-    return cls(torch.empty(rows + (row_bytes(n),), dtype=torch.float8_e4m3fn,
-                           device=device),
-               torch.empty(rows + (scale_bytes(n),), dtype=torch.uint8, device=device),
-               n)
+    shape = tuple(shape)
+    rows, n = shape[:-1], shape[-1]
+    if n < 1:
+      raise ValueError("rows without values: shape %s" % (shape,))
+    # (what __init__ checks holds by construction)
+    return cls.__new__(cls)._set(  # pylint: disable=protected-access
+        _empty(rows + (row_bytes(n),), dtype=torch.float8_e4m3fn, device=device),
+        _empty(rows + (scale_bytes(n),), dtype=torch.uint8, device=device), shape)
 
   def reshape(self, *rows):
     """The same rows under other leading dimensions."""
-    return Fp8Blocks(self.values.reshape(rows + self.values.shape[-1:]),
-                     self.scales.reshape(rows + self.scales.shape[-1:]), self.n)
+    values = self._values.reshape(rows + self._values.shape[-1:])
+    scales = self._scales.reshape(rows + self._scales.shape[-1:])
+    return Fp8Blocks.__new__(Fp8Blocks)._set(
+        values, scales, tuple(values.shape[:-1]) + self._shape[-1:])
 
   def __repr__(self):
     return "Fp8Blocks%s" % (self.shape,)
 
 
+_empty = torch.empty
+_Tensor = torch.Tensor
+_current_device = moe_hip.current_device
+
+
 def _dev(t, name, dtype=None, shape=None):
+  # (one expression for what passes: the checks cost as much as a small kernel)
+  if (isinstance(t, _Tensor) and t.is_cuda and t.get_device() == _current_device() and
+      t.is_contiguous() and (dtype is None or t.dtype is dtype) and
+      (shape is None or t.shape == shape)):
+    return t.data_ptr()
   at = moe_hip._dev(t, name, dtype, shape)  # pylint: disable=protected-access
-  if t.device.index != moe_hip.current_device():
+  if t.get_device() != _current_device():
     raise MoeHipError("%s lies on %s, the current device is %d"
-                      % (name, t.device, moe_hip.current_device()))
+                      % (name, t.device, _current_device()))
   return at
 
 
@@ -127,9 +158,21 @@ def _operand(q, name, shape=None):
   """Pointers to an operand's values and scales."""
   if not isinstance(q, Fp8Blocks):
     raise MoeHipError("%s must be an Fp8Blocks" % name)
-  if shape is not None and q.shape != tuple(shape):
-    raise MoeHipError("%s: shape %s, expected %s" % (name, q.shape, tuple(shape)))
-  return _dev(q.values, name + ".values"), _dev(q.scales, name + ".scales")
+  if shape is not None and q.shape != shape:
+    raise MoeHipError("%s: shape %s, expected %s" % (name, q.shape, shape))
+  values, scales = q._values, q._scales  # pylint: disable=protected-access
+  if (values.is_cuda and scales.is_cuda and
+      values.get_device() == scales.get_device() == _current_device() and
+      values.is_contiguous() and scales.is_contiguous()):
+    return values.data_ptr(), scales.data_ptr()
+  return _dev(values, name + ".values"), _dev(scales, name + ".scales")
+
+
+def _pointers(q):
+  """Of an operand that was made here."""
+  if q is None:
+    return None, None
+  return q._values.data_ptr(), q._scales.data_ptr()  # pylint: disable=protected-access
 
 
 def _counts(row_count, e):
@@ -138,7 +181,7 @@ def _counts(row_count, e):
 
 
 def _workspace(nbytes, like):
-  return torch.empty((nbytes,), dtype=torch.uint8, device=like.device)
+  return _empty((nbytes,), dtype=torch.uint8, device=like.device)
 
 
 def _activation(name):
@@ -179,9 +222,8 @@ def quantize(x, rows=True, columns=False, relu_mask=None, row_count=None):
   if x.numel():
     with _stage("fp8_quantize"):
       _check(lib.mesh_moe_fp8_quantize(
-          xp, mp, cp, *(_operand(by_row, "rows") if rows else (None, None)),
-          *(_operand(by_column, "columns") if columns else (None, None)), e, r, k,
-          code, _stream()), "fp8_quantize")
+          xp, mp, cp, *_pointers(by_row), *_pointers(by_column), e, r, k, code,
+          _stream()), "fp8_quantize")
   return (by_row, by_column) if rows and columns else by_row if rows else by_column
 
 
@@ -189,7 +231,7 @@ def dequantize(q, dtype=torch.bfloat16):
   """The tensor that an operand stands for, exact in bfloat16 and float32."""
   lib = load_library()
   code = moe_hip.dtype_code(dtype)
-  y = torch.empty(q.shape, dtype=dtype, device=q.values.device)
+  y = _empty(q.shape, dtype=dtype, device=q.values.device)
   values, scales = _operand(q, "q")
   if y.numel():
     with _stage("fp8_dequantize"):
@@ -219,36 +261,32 @@ def residual_rms_norm(x, residual, scale, epsilon=1e-6, row_mask=None,
     with _stage("rms_norm"):
       _check(lib.mesh_moe_fp8_residual_rms_norm(
           xp, rp, sp, mp, None if residual is None else total.data_ptr(),
-          None if norm is None else norm.data_ptr(), *_operand(y, "y"),
+          None if norm is None else norm.data_ptr(), *_pointers(y),
           x.numel() // m, m, float(epsilon), code, _stream()), "fp8_residual_rms_norm")
   return (total, y, norm) if want_norm else (total, y)
 
 
-def expert_linear(a, w, activation="linear", eight_bit=False, row_count=None, out=None):
-  """a [E, R, K] and w [E, N, K], 8-bit operands over K -> act(a[e] . w[e]^T) [E, R, N],
-  in bfloat16, or (eight_bit) as an 8-bit operand over N.  row_count [E] int32: only the
-  first rows of an expert, as many as its count, are multiplied, the others of `out` stay
-  as they were (without an `out` they are unspecified)."""
+def _linear(a, w, sizes, shape, activation, eight_bit, row_count, out):
+  """expert_linear with sizes (e, r, k, n); `shape`: of the result."""
   lib = load_library()
+  e, r, k, n = sizes
   ap, asp = _operand(a, "a")
-  wp, wsp = _operand(w, "w")
-  if len(a.shape) != 3 or len(w.shape) != 3:
-    raise MoeHipError("a %s, w %s: expected [E, R, K] and [E, N, K]"
-                      % (a.shape, w.shape))
-  e, r, k = a.shape
-  n = w.shape[1]
-  if w.shape != (e, n, k):
-    raise MoeHipError("w: shape %s, expected %s" % (w.shape, (e, n, k)))
+  wp, wsp = _operand(w, "w", (e, n, k))
   act = _activation(activation)
   cp = _counts(row_count, e)
   if eight_bit:
     if out is None:
-      out = Fp8Blocks.empty((e, r, n), a.values.device)
-    yp, ysp = _operand(out, "out", (e, r, n))
+      out = Fp8Blocks.empty(shape, a.values.device)
+      yp, ysp = _pointers(out)
+    else:
+      yp, ysp = _operand(out, "out", shape)
   else:
     if out is None:
-      out = torch.empty((e, r, n), dtype=torch.bfloat16, device=a.values.device)
-    yp, ysp = _dev(out, "out", torch.bfloat16, (e, r, n)), None
+      out = _empty(shape, dtype=torch.bfloat16, device=a.values.device)
+      yp = out.data_ptr()
+    else:
+      yp = _dev(out, "out", torch.bfloat16, shape)
+    ysp = None
   if e * r * n == 0:
     return out
   ws_bytes = lib.mesh_moe_fp8_expert_linear_workspace_bytes(e, r, k, n, int(eight_bit))
@@ -261,17 +299,33 @@ def expert_linear(a, w, activation="linear", eight_bit=False, row_count=None, ou
   return out
 
 
+def expert_linear(a, w, activation="linear", eight_bit=False, row_count=None, out=None):
+  """a [E, R, K] and w [E, N, K], 8-bit operands over K -> act(a[e] . w[e]^T) [E, R, N],
+  in bfloat16, or (eight_bit) as an 8-bit operand over N.  row_count [E] int32: only the
+  first rows of an expert, as many as its count, are multiplied, the others of `out` stay
+  as they were (without an `out` they are unspecified)."""
+  if not isinstance(a, Fp8Blocks) or not isinstance(w, Fp8Blocks):
+    raise MoeHipError("a and w must be Fp8Blocks")
+  if len(a.shape) != 3 or len(w.shape) != 3:
+    raise MoeHipError("a %s, w %s: expected [E, R, K] and [E, N, K]"
+                      % (a.shape, w.shape))
+  e, r, k = a.shape
+  n = w.shape[1]
+  return _linear(a, w, (e, r, k, n), (e, r, n), activation, eight_bit, row_count, out)
+
+
 def dense(x, w, activation=None, eight_bit=False):
   """x [..., K] times a kernel [1, N, K], 8-bit operands over K -> act(x . w^T) [..., N],
   in bfloat16, or (eight_bit) as an 8-bit operand (mtf.layers.dense without bias)."""
-  if not isinstance(x, Fp8Blocks):
-    raise MoeHipError("x must be an Fp8Blocks")
-  lead = x.shape[:-1]
+  if not isinstance(x, Fp8Blocks) or not isinstance(w, Fp8Blocks):
+    raise MoeHipError("x and w must be Fp8Blocks")
+  if len(w.shape) != 3:
+    raise MoeHipError("w %s: expected [1, N, K]" % (w.shape,))
+  lead, k, n = x.shape[:-1], x.shape[-1], w.shape[1]
   rows = 1
   for size in lead:
     rows *= size
-  y = expert_linear(x.reshape(1, rows), w, activation, eight_bit)
-  return y.reshape(*lead) if eight_bit else y.reshape(lead + (w.shape[1],))
+  return _linear(x, w, (1, rows, k, n), lead + (n,), activation, eight_bit, None, None)
 
 
 def expert_linear_backward(a_columns, dy, w_rows=None, relu_mask=None, row_count=None,
@@ -300,14 +354,14 @@ def expert_linear_backward(a_columns, dy, w_rows=None, relu_mask=None, row_count
   if w_rows is not None:
     wp, wsp = _operand(w_rows, "w_rows", (e, k, n))
     if da is None:
-      da = torch.empty((e, r, k), dtype=torch.bfloat16, device=dy.device)
+      da = _empty((e, r, k), dtype=torch.bfloat16, device=dy.device)
   elif da is not None:
     raise MoeHipError("da needs w_rows")
   dap = None if da is None else _dev(da, "da", torch.bfloat16, (e, r, k))
   if dy.numel() == 0 or k == 0:
     dw = torch.zeros((e, k, n), dtype=torch.bfloat16, device=dy.device)
     return (None if da is None else da.zero_() if r and n == 0 else da), dw
-  dw = torch.empty((e, k, n), dtype=torch.bfloat16, device=dy.device)
+  dw = _empty((e, k, n), dtype=torch.bfloat16, device=dy.device)
   ws_bytes = lib.mesh_moe_fp8_expert_linear_backward_workspace_bytes(
       e, r, k, n, int(da is not None))
   ws = _workspace(ws_bytes, dy)
