@@ -58,6 +58,8 @@ struct GemmArgs {
   void* y;                  // bf16, float32 or e4m3, see the kernels
   uint8_t* y_scales;
   int E, R, K, N, activation;
+  // values of expert e's rows that are not zeros, or null: a kernel may leave the others out
+  const int32_t* k_count;
 };
 
 // ---------------------------------------------------------------------------
@@ -362,6 +364,10 @@ __device__ __forceinline__ Tile find_tile(const GemmArgs& g, const TileGrid& gri
   t.col0 = __builtin_amdgcn_readfirstlane(tn * BN);
   t.e = __builtin_amdgcn_readfirstlane(t.e);
   t.valid = __builtin_amdgcn_readfirstlane(min(BM, t.valid - t.row0));
+  if constexpr (!PARTS)
+    if (g.k_count != nullptr)       // (two K tiles at least)
+      t.nk = max(min((live_rows(g.k_count, t.e, g.K) + FP8_BLOCK - 1) / FP8_BLOCK, k_tiles),
+                 2);
   return t;
 }
 // number of the block's tile of round `round`
@@ -720,7 +726,7 @@ __global__ __launch_bounds__(BigCfg::THREADS) void fp8_tile256_kernel(GemmArgs g
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   for (;;) {
-    Tile after = {0, 0, 0, 0};
+    Tile after = {};
     auto tile_pass = [&](auto na_tag) FP8_INLINE {
       constexpr int NA = decltype(na_tag)::value;
       auto next_scales = [&](int kt) FP8_INLINE {
@@ -729,7 +735,7 @@ __global__ __launch_bounds__(BigCfg::THREADS) void fp8_tile256_kernel(GemmArgs g
           for (int i = 0; i < Cfg::TM; ++i) sa[i] = sa_next[i];
 #pragma unroll
           for (int j = 0; j < Cfg::TN; ++j) sw[j] = sw_next[j];
-          if (kt + 4 < nk) load_scales(t, kt / 4 + 1);
+          if (kt + 4 < t.nk) load_scales(t, kt / 4 + 1);
         } else {
 #pragma unroll
           for (int i = 0; i < Cfg::TM; ++i) sa[i] >>= 8;
@@ -745,14 +751,14 @@ __global__ __launch_bounds__(BigCfg::THREADS) void fp8_tile256_kernel(GemmArgs g
       };
       if constexpr (NA > 0) first_fragments(aslot, wslot);
       next_scales(0);
-      if (nk == 2) advance();
-      k_tile(na_tag, std::true_type{}, std::false_type{}, nk == 2 ? 0 : 2);
-      for (int kt = 1; kt < nk - 1; ++kt) {
+      if (t.nk == 2) advance();
+      k_tile(na_tag, std::true_type{}, std::false_type{}, t.nk == 2 ? 0 : 2);
+      for (int kt = 1; kt < t.nk - 1; ++kt) {
         next_scales(kt);
-        if (kt == nk - 2) advance();
-        k_tile(na_tag, std::false_type{}, std::false_type{}, kt == nk - 2 ? 0 : kt + 2);
+        if (kt == t.nk - 2) advance();
+        k_tile(na_tag, std::false_type{}, std::false_type{}, kt == t.nk - 2 ? 0 : kt + 2);
       }
-      next_scales(nk - 1);
+      next_scales(t.nk - 1);
       if (after.valid != 0) load_scales(after, 0);
       k_tile(na_tag, std::false_type{}, std::true_type{}, 1);
       write_out(t, na_tag);
@@ -1539,7 +1545,7 @@ extern "C" int mesh_moe_fp8_expert_linear(const void* a_values, const uint8_t* a
               "fp8_expert_linear: workspace too small (%zu of %zu)", workspace_bytes,
               need);
   const GemmArgs g = {(const uint8_t*)a_values, a_scales, (const uint8_t*)w_values,
-                      w_scales, row_count, y, y_scales, E, R, K, N, activation};
+                      w_scales, row_count, y, y_scales, E, R, K, N, activation, nullptr};
   return run_product(g, workspace, (hipStream_t)stream);
 }
 
@@ -1610,11 +1616,11 @@ extern "C" int mesh_moe_fp8_expert_linear_backward(
   if (rc != 0) return rc;
   const GemmArgs weights = {(const uint8_t*)a_column_values, a_column_scales,
                             ws + p.columns, ws + p.column_scales, nullptr, dw, nullptr,
-                            E, K, R, N, MESH_MOE_ACT_LINEAR};
+                            E, K, R, N, MESH_MOE_ACT_LINEAR, row_count};
   rc = run_product(weights, ws + p.products, st);
   if (rc != 0 || da == nullptr) return rc;
   const GemmArgs input = {rows, ws + p.row_scales, (const uint8_t*)w_row_values,
                           w_row_scales, row_count, da, nullptr, E, R, N, K,
-                          MESH_MOE_ACT_LINEAR};
+                          MESH_MOE_ACT_LINEAR, nullptr};
   return run_product(input, ws + p.products, st);
 }

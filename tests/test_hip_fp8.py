@@ -269,6 +269,86 @@ def test_expert_linear(hip, e, r, k, n):
   assert (codes[..., n:] == 0).all()
 
 
+# sizes that fill the GPU with tiles of each kind, some more than once, with rows that
+# are and are not whole pieces of 16 bytes, and ones that split the reduction
+MANY = [(16, 1100, 300, 1030), (8, 2000, 400, 1032), (40, 300, 384, 520),
+        (64, 200, 256, 1000), (16, 300, 256, 1030), (32, 260, 256, 1032),
+        (4, 500, 3100, 300), (1, 200, 2300, 640), (1, 1000, 8192, 520),
+        (1, 40, 4096, 300), (32, 24, 1024, 1030), (1, 24, 11080, 1500)]
+
+
+def _random(hip, shape, std, seed):
+  """A random operand and its value in float64, on the GPU."""
+  gen = torch.Generator(device="cuda").manual_seed(seed)
+  x = torch.randn(shape, generator=gen, device="cuda") * std
+  q = hip.quantize(x * torch.exp(0.5 * torch.randn(shape[-1:], generator=gen,
+                                                   device="cuda")))
+  return q, hip.dequantize(q, torch.float32).double()
+
+
+def _near(got, want, magnitudes):
+  return ((got.double() - want).abs() <= want.abs() * 2.0 ** -8 +
+          magnitudes * 2.0 ** -13).all()
+
+
+@pytest.mark.parametrize("e,r,k,n", MANY)
+def test_expert_linear_of_many_tiles(hip, e, r, k, n):
+  a, av = _random(hip, (e, r, k), 1.0, 1)
+  w, wv = _random(hip, (e, n, k), k ** -0.5, 2)
+  wt = wv.transpose(1, 2).contiguous()
+  want, magnitudes = av @ wt, av.abs() @ wt.abs()
+  assert _near(hip.expert_linear(a, w), want, magnitudes)
+  act = torch.nn.functional.gelu(want, approximate="tanh")
+  assert _near(hip.expert_linear(a, w, "gelu"), act, 1.13 * magnitudes)
+  count = torch.randint(0, r + 1, (e,), dtype=torch.int32, device="cuda")
+  count[0], count[e // 2] = r // 2 + 1, 0 if e > 1 else 1
+  live = torch.arange(r, device="cuda") < count.unsqueeze(1)
+  out = torch.full((e, r, n), 7.0, dtype=torch.bfloat16, device="cuda")
+  hip.expert_linear(a, w, row_count=count, out=out)
+  assert (out[~live] == 7).all() and _near(out[live], want[live], magnitudes[live])
+  for activation, exact in (("relu", want.clamp_min(0)), ("gelu", act)):
+    exact = hip.dequantize(hip.quantize(exact.float()), torch.float32)
+    for counts in (None, count):
+      q = hip.Fp8Blocks.empty((e, r, n), "cuda")
+      q.values.view(torch.uint8).fill_(0x55)
+      q.scales.fill_(99)
+      hip.expert_linear(a, w, activation, True, row_count=counts, out=q)
+      codes, got = q.values.view(torch.uint8), hip.dequantize(q, torch.float32)
+      rows = torch.ones_like(live) if counts is None else live
+      assert (codes[~rows] == 0x55).all() and (q.scales[~rows] == 99).all()
+      assert (codes[rows][:, n:] == 0).all()
+      # (a step apart where the sums' error crosses a rounding border, see above)
+      assert (got[rows] == exact[rows]).double().mean() > 0.98
+      assert (got[rows] - exact[rows]).abs().max() <= (
+          2.0 ** -4 * exact.abs().max() + 2.0 ** -13 * 1.13 * magnitudes.max())
+
+
+@pytest.mark.parametrize("e,r,k,n", [(40, 384, 300, 520), (16, 384, 300, 1030),
+                                     (24, 900, 300, 1030), (6, 700, 1300, 256),
+                                     (2, 1000, 520, 1024)])
+def test_gradients_of_counted_rows(hip, e, r, k, n):
+  """Experts with none, one, a block, a block and one, and all of their rows."""
+  count = torch.tensor([(0, 1, 128, 129, r, r - 1, 257)[i % 7] for i in range(e)],
+                       dtype=torch.int32, device="cuda")
+  live = (torch.arange(r, device="cuda") < count.unsqueeze(1)).unsqueeze(2)
+  gen = torch.Generator(device="cuda").manual_seed(3)
+  dy = torch.randn((e, r, n), generator=gen, device="cuda").bfloat16()
+  x = torch.randn((e, r, k), generator=gen, device="cuda") * live
+  a_columns = hip.quantize(x, rows=False, columns=True)
+  w_rows, wv = _random(hip, (e, k, n), 0.05, 4)
+  da = torch.full((e, r, k), 3.0, dtype=torch.bfloat16, device="cuda")
+  hip.expert_linear_backward(a_columns, dy, w_rows, row_count=count, da=da)
+  _, dw = hip.expert_linear_backward(a_columns, dy, row_count=count)
+  by_row, by_column = hip.quantize((dy * live).contiguous(), rows=True, columns=True)
+  by_row, by_column, av = (hip.dequantize(q, torch.float32).double()
+                           for q in (by_row, by_column, a_columns))
+  wt, yt = wv.transpose(1, 2).contiguous(), by_column.transpose(1, 2).contiguous()
+  want, magnitudes = by_row @ wt, by_row.abs() @ wt.abs()
+  dead = ~live.squeeze(2)
+  assert (da[dead] == 3).all() and _near(da[~dead], want[~dead], magnitudes[~dead])
+  assert _near(dw, av @ yt, av.abs() @ yt.abs())
+
+
 @pytest.mark.parametrize("activation", [None, "linear", "sigmoid", "tanh", "swish"])
 @pytest.mark.parametrize("r", [2, 300])
 def test_activations(hip, activation, r):
