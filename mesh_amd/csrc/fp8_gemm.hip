@@ -249,11 +249,14 @@ __device__ __forceinline__ void load_to_lds(const uint8_t* from, int bytes, uint
       (lds_void_t*)to, 16, at, skip, 0, 0);
 }
 
-// 16 bytes per lane, at `at` of the `bytes` at `base`; what lies behind is dropped
+// 16 bytes per lane, at `at` of the `bytes` at `base`; what lies behind is dropped.  Past
+// the caches (the last argument, nt), which the operands need: weight gradients of 32
+// experts 4096 x 640 -> 1024 take 90 us instead of 110, 64 experts' 705 rows 1024 -> 4096
+// 197 instead of 204.
 __device__ __forceinline__ void store_line(u32x4_t v, uint8_t* base, int bytes,
                                            uint32_t at) {
   __builtin_amdgcn_raw_buffer_store_b128(
-      v, __builtin_amdgcn_make_buffer_rsrc(base, 0, max(bytes, 0), 0x00027000), at, 0, 0);
+      v, __builtin_amdgcn_make_buffer_rsrc(base, 0, max(bytes, 0), 0x00027000), at, 0, 2);
 }
 
 __device__ __forceinline__ f32x16_t fp8_mfma(i32x8_t w, i32x8_t a, f32x16_t c,
