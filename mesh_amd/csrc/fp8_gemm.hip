@@ -66,13 +66,34 @@ struct GemmArgs {
 // Few rows: 16 TM rows per block, and 16 columns with the reduction dealt out over the 8
 // wavefronts, whose sums meet in LDS (CW = 1), or 8 times 16 columns of a wavefront each
 // (CW = 8: for a reduction of one block of 128, and what the tile kernels cannot address).
-// Bound by the weights, which are read once, straight from memory into the matrix
-// instructions' registers (v_mfma_scale_f32_16x16x128_f8f6f4): four blocks of 128 of a
-// row are requested before the first is multiplied.  One row 4096 -> 16384 takes 14.1 us,
-// 4.7 TB/s (16.0 us with requests for 32 bytes of each row instead of 64).
+// Bound by the weights, which are read once, straight from memory into registers: four
+// blocks of 128 of a row are requested before the first is multiplied.  One row 4096 ->
+// 16384 takes 14.4 us, 4.7 TB/s (16.0 us with requests for 32 bytes of each row instead of
+// 64).  That leaves time to multiply in bfloat16, which holds an e4m3 number times its
+// unit, so that the sums are float32 ones; the instructions for 8 bits lose bits below
+// 2^-14 of the largest of 8 products.
 // TO: bf16_t, float (rows of fp8_row_bytes(N), without the activation: fp8_parts_kernel
 // goes on from there) or uint8_t (an 8-bit operand; CW is 8: a block of 128 columns).
 // ---------------------------------------------------------------------------
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+// the unit that a scale byte stands for, 255 being NaN
+__device__ __forceinline__ float fp8_unit(uint8_t byte) {
+  return __uint_as_float(byte == 255 ? 0x7fc00000u : (uint32_t)byte << 23);
+}
+// 8 numbers times their unit, exact: 2^-9 times the least unit, 2^-117, is normal
+__device__ __forceinline__ bf16x8_t fp8_widen(int lo, int hi, float unit) {
+  bf16x2_t v[4];
+  v[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, unit, false);
+  v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, unit, true);
+  v[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, unit, false);
+  v[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, unit, true);
+  const bf16x4_t a = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3);
+  const bf16x4_t b = __builtin_shufflevector(v[2], v[3], 0, 1, 2, 3);
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
 template <int TM, int CW, typename TO>
 __global__ __launch_bounds__(512) void fp8_few_rows_kernel(GemmArgs g, int tiles_m,
                                                            int tiles_n) {
@@ -114,7 +135,7 @@ __global__ __launch_bounds__(512) void fp8_few_rows_kernel(GemmArgs g, int tiles
   auto step = [&](auto n_tag, int b) __attribute__((always_inline)) {
     constexpr int N = decltype(n_tag)::value;
     i32x8_t vw[N], va[N][TM];
-    uint32_t sw[N], sa[N][TM];
+    uint8_t sw[N], sa[N][TM];
 #pragma unroll
     for (int u = 0; u < N; ++u) {
       vw[u] = fragment(w + (int64_t)(b + u) * FP8_BLOCK);
@@ -127,11 +148,20 @@ __global__ __launch_bounds__(512) void fp8_few_rows_kernel(GemmArgs g, int tiles
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int u = 0; u < N; ++u)
+    for (int u = 0; u < N; ++u) {
+      const float fw = fp8_unit(sw[u]);
+      float fa[TM];
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
-        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-            vw[u], va[u][i], acc[i], 0, 0, 0, (int)sw[u], 0, (int)sa[u][i]);
+      for (int i = 0; i < TM; ++i) fa[i] = fp8_unit(sa[u][i]);
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        const bf16x8_t w8 = fp8_widen(vw[u][2 * m], vw[u][2 * m + 1], fw);
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              w8, fp8_widen(va[u][i][2 * m], va[u][i][2 * m + 1], fa[i]), acc[i], 0, 0, 0);
+      }
+    }
   };
   // (runs of whole groups of U where there are that many)
   const int blocks = (int)(kp / FP8_BLOCK);
@@ -397,7 +427,8 @@ __device__ __forceinline__ int tile_number(int round) {
 //   step 1   reads the fragments of tile t + 1's step 0; token loads of tile t + 2,
 //            into the slot that the barrier freed
 // Blocks are persistent, one per CU, and the K tiles of a block's tiles follow each other:
-// the loads of a tile's last two K tiles are the first of the next.  Needs two K tiles.
+// the loads of a tile's last two K tiles are the first of the next.  (An only K tile is
+// followed by one of zeros: 16384 rows 128 -> 4096 take 28 us, 150 with few-rows blocks.)
 // Block b runs on XCD b % 8; the blocks of an XCD hold consecutive tiles, numbered in
 // bands of 8 row tiles, so that 32 of them share 8 + 4 operand panels in its L2.
 //
@@ -428,7 +459,10 @@ __global__ __launch_bounds__(BigCfg::THREADS) void fp8_tile256_kernel(GemmArgs g
   const int wm = wave >> 1, wn = wave & 1;
   const int fr = lane & 31, fc = lane >> 5;
   const int64_t kp = fp8_row_bytes(g.K), ks = fp8_scale_bytes(g.K);
-  const int nk = (int)(kp / FP8_BLOCK);
+  // (an only K tile is followed by one of zeros, with scales that are no NaN)
+  const bool single = kp == FP8_BLOCK;
+  const int nk = single ? 2 : (int)(kp / FP8_BLOCK);
+  const uint32_t scale_mask = single ? 0xffu : ~0u;
 
   // (What is computed from the lane index outside the K loop is computed from a copy
   // that the compiler cannot see through: made once it would be live across the K loop,
@@ -463,11 +497,11 @@ __global__ __launch_bounds__(BigCfg::THREADS) void fp8_tile256_kernel(GemmArgs g
     w_bytes = min(Cfg::BN, g.N - t.col0) * (int)kp;
   };
   auto load_a = [&](int kt, int j, int slot) FP8_INLINE {
-    load_to_lds(a_base, a_bytes, load_at[j], kt * FP8_BLOCK,
+    load_to_lds(a_base, single && kt == 1 ? 0 : a_bytes, load_at[j], kt * FP8_BLOCK,
                 smem + slot * Cfg::SLOT + (wave + 8 * j) * 1024);
   };
   auto load_w = [&](int kt, int j, int slot) FP8_INLINE {
-    load_to_lds(w_base, w_bytes, load_at[j], kt * FP8_BLOCK,
+    load_to_lds(w_base, single && kt == 1 ? 0 : w_bytes, load_at[j], kt * FP8_BLOCK,
                 smem + Cfg::W_BASE + slot * Cfg::SLOT + (wave + 8 * j) * 1024);
   };
 
@@ -735,9 +769,9 @@ __global__ __launch_bounds__(BigCfg::THREADS) void fp8_tile256_kernel(GemmArgs g
       auto next_scales = [&](int kt) FP8_INLINE {
         if ((kt & 3) == 0) {
 #pragma unroll
-          for (int i = 0; i < Cfg::TM; ++i) sa[i] = sa_next[i];
+          for (int i = 0; i < Cfg::TM; ++i) sa[i] = sa_next[i] & scale_mask;
 #pragma unroll
-          for (int j = 0; j < Cfg::TN; ++j) sw[j] = sw_next[j];
+          for (int j = 0; j < Cfg::TN; ++j) sw[j] = sw_next[j] & scale_mask;
           if (kt + 4 < t.nk) load_scales(t, kt / 4 + 1);
         } else {
 #pragma unroll
@@ -833,7 +867,10 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(GemmArgs g, TileGrid g
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave;
   const int64_t kp = fp8_row_bytes(g.K), ks = fp8_scale_bytes(g.K);
-  const int k_tiles = (int)(kp / FP8_BLOCK);
+  // (an only K tile is followed by one of zeros, with scales that are no NaN)
+  const bool single = kp == FP8_BLOCK;
+  const int k_tiles = single ? 2 : (int)(kp / FP8_BLOCK);
+  const uint32_t scale_mask = single ? 0xffu : ~0u;
 
   // (What is computed from the lane index outside the K loop is computed from a copy
   // that the compiler cannot see through: made once it would be live across the K loop.)
@@ -948,14 +985,17 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(GemmArgs g, TileGrid g
     // the K tiles that are loaded: of this tile, or the next one
     auto a_source = [&](int p) {
       const bool mine = p < t.nk;
-      return Source{mine ? here.a : next.a, mine ? here.a_bytes : next.a_bytes,
-                    (mine ? p : p - t.nk) * FP8_BLOCK, aslot * Cfg::A_SLOT};
+      const int at = mine ? p : p - t.nk;
+      return Source{mine ? here.a : next.a,
+                    single && at == 1 ? 0 : mine ? here.a_bytes : next.a_bytes,
+                    at * FP8_BLOCK, aslot * Cfg::A_SLOT};
     };
     auto w_source = [&](int p, int slot) {
       const bool mine = p < t.nk;
-      return Source{mine ? here.w : next.w, mine ? here.w_bytes : next.w_bytes,
-                    (mine ? p : p - t.nk) * FP8_BLOCK,
-                    Cfg::W_BASE + slot * Cfg::W_SLOT};
+      const int at = mine ? p : p - t.nk;
+      return Source{mine ? here.w : next.w,
+                    single && at == 1 ? 0 : mine ? here.w_bytes : next.w_bytes,
+                    at * FP8_BLOCK, Cfg::W_BASE + slot * Cfg::W_SLOT};
     };
     const Fragments w_now = w_fragments(wslot);
     Fragments w_then = {0, 0}, a_then = {0, 0};
@@ -1184,8 +1224,10 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(GemmArgs g, TileGrid g
   load_scales(t, 0);
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const Source as = {here.a, here.a_bytes, k * FP8_BLOCK, k * Cfg::A_SLOT};
-    const Source ws = {here.w, here.w_bytes, k * FP8_BLOCK, Cfg::W_BASE + k * Cfg::W_SLOT};
+    const bool zeros = single && k == 1;
+    const Source as = {here.a, zeros ? 0 : here.a_bytes, k * FP8_BLOCK, k * Cfg::A_SLOT};
+    const Source ws = {here.w, zeros ? 0 : here.w_bytes, k * FP8_BLOCK,
+                       Cfg::W_BASE + k * Cfg::W_SLOT};
 #pragma unroll
     for (int n = 0; n < A_LOADS; ++n) load(as, n);
 #pragma unroll
@@ -1206,9 +1248,9 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(GemmArgs g, TileGrid g
 #pragma unroll
       for (int j = 0; j < 3; ++j) fw[j] = read_w(w_first, j);
 #pragma unroll
-      for (int i = 0; i < TM; ++i) sa[i] = sa_next[i];
+      for (int i = 0; i < TM; ++i) sa[i] = sa_next[i] & scale_mask;
 #pragma unroll
-      for (int j = 0; j < TN; ++j) sw[j] = sw_next[j];
+      for (int j = 0; j < TN; ++j) sw[j] = sw_next[j] & scale_mask;
       // (without a next tile its loads fetch this one again, which nobody reads)
       after = tile_at(++round);
       next = operands(after.valid != 0 ? after : t);
@@ -1324,10 +1366,10 @@ struct Plan {
 
 static Plan plan_product(int E, int R, int K, int N, bool eight_bit, bool counted) {
   Plan p;
-  // (a tile's operand rows and 8 rows of its result are addressed in 31 bits; an only
-  // block of 128 has nothing to be overlapped with)
-  if (K <= FP8_BLOCK || K > 1 << 22 || N > 1 << 26) return p;
-  const int nk = (int)(fp8_row_bytes(K) / FP8_BLOCK);
+  // (a tile's operand rows and 8 rows of its result are addressed in 31 bits)
+  if (K > 1 << 22 || N > 1 << 26) return p;
+  const bool single = K <= FP8_BLOCK;
+  const int nk = single ? 2 : (int)(fp8_row_bytes(K) / FP8_BLOCK);
   const int64_t np = fp8_row_bytes(N);
   const double weights = (double)E * N * nk * FP8_BLOCK / 1e6;        // MB
   auto over = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
@@ -1339,7 +1381,12 @@ static Plan plan_product(int E, int R, int K, int N, bool eight_bit, bool counte
       p.split = split;
     }
   };
-  if (R <= 128) {
+  if (single) {
+    // nothing to deal out over wavefronts, nor to be overlapped with
+    const int rows = R <= 16 ? 16 : R <= 32 ? 32 : 64;
+    const int64_t blocks = over(N, 128) * over(R, rows) * E;
+    offer(ONE_BLOCK, 1, 3.2 + over(blocks, 256) * (rows == 16 ? 1.0 : rows == 32 ? 1.6 : 4.2));
+  } else if (R <= 128) {
     // a wavefront's run is nk / 8 blocks: bound by the weights, by the blocks' own reads,
     // or by the time to memory
     const bool one = R <= 16;

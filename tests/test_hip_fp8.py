@@ -241,7 +241,8 @@ PRODUCTS = [(1, 1, 1, 1), (1, 1, 128, 32), (1, 1, 4096, 1000), (1, 3, 300, 17),
             (1, 129, 2000, 130), (3, 200, 384, 300), (1, 257, 512, 513),
             (2, 300, 1100, 256), (1, 1000, 256, 1024), (4, 520, 896, 640),
             (1, 2050, 384, 1537), (1, 512, 4224, 512), (64, 6, 512, 256),
-            (1, 8, 1024, 4096), (1, 1100, 128, 8), (1, 384, 129, 4000)]
+            (1, 8, 1024, 4096), (1, 1100, 128, 8), (1, 384, 129, 4000),
+            (1, 700, 128, 520), (3, 400, 65, 1000)]
 
 
 @pytest.mark.parametrize("e,r,k,n", PRODUCTS)
@@ -274,7 +275,8 @@ def test_expert_linear(hip, e, r, k, n):
 MANY = [(16, 1100, 300, 1030), (8, 2000, 400, 1032), (40, 300, 384, 520),
         (64, 200, 256, 1000), (16, 300, 256, 1030), (32, 260, 256, 1032),
         (4, 500, 3100, 300), (1, 200, 2300, 640), (1, 1000, 8192, 520),
-        (1, 40, 4096, 300), (32, 24, 1024, 1030), (1, 24, 11080, 1500)]
+        (1, 40, 4096, 300), (32, 24, 1024, 1030), (1, 24, 11080, 1500),
+        (16, 1100, 128, 1030), (16, 300, 100, 1032), (64, 60, 77, 520)]
 
 
 def _random(hip, shape, std, seed):
@@ -325,7 +327,8 @@ def test_expert_linear_of_many_tiles(hip, e, r, k, n):
 
 @pytest.mark.parametrize("e,r,k,n", [(40, 384, 300, 520), (16, 384, 300, 1030),
                                      (24, 900, 300, 1030), (6, 700, 1300, 256),
-                                     (2, 1000, 520, 1024)])
+                                     (2, 1000, 520, 1024), (24, 100, 600, 1030),
+                                     (8, 128, 300, 100)])
 def test_gradients_of_counted_rows(hip, e, r, k, n):
   """Experts with none, one, a block, a block and one, and all of their rows."""
   count = torch.tensor([(0, 1, 128, 129, r, r - 1, 257)[i % 7] for i in range(e)],
