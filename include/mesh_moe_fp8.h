@@ -24,6 +24,8 @@
  * bfloat16 too.  Below -117 it would not be; values under 2^-127 become zeros or
  * multiples of 2^-126 instead.  A block with an infinity or a NaN is NaN as a whole
  * (scale byte 127).
+ * Products take scale bytes from 10 (which is -117) on, 255 making a block NaN; blocks
+ * with a byte below, which no call here makes, they may count as zeros.
  *
  * The reference has no 8-bit arithmetic; the calls are forms of what it does in
  * float32 or bfloat16, which is named at each.

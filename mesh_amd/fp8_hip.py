@@ -24,6 +24,7 @@ from mesh_amd.moe_hip import MoeHipError
 
 ABI_VERSION = 1
 BLOCK = 128
+_E4M3 = torch.float8_e4m3fn
 
 _vp = ctypes.c_void_p
 _int = ctypes.c_int
@@ -82,13 +83,15 @@ class Fp8Blocks(object):
 
   def __init__(self, values, scales, n):
     n = int(n)
-    if (values.dtype != torch.float8_e4m3fn or scales.dtype != torch.uint8 or n < 1 or
-        values.dim() < 1 or values.shape[-1] != row_bytes(n) or
-        tuple(scales.shape) != tuple(values.shape[:-1]) + (scale_bytes(n),)):
+    shape = values.shape
+    lead = tuple(shape[:-1])
+    if (values.dtype is not _E4M3 or scales.dtype is not torch.uint8 or n < 1 or
+        not shape or shape[-1] != row_bytes(n) or
+        scales.shape != lead + (scale_bytes(n),)):
       raise ValueError(
           "values %s of %s and scales %s of %s are not rows of %d 8-bit values"
-          % (tuple(values.shape), values.dtype, tuple(scales.shape), scales.dtype, n))
-    self._set(values, scales, tuple(values.shape[:-1]) + (n,))
+          % (tuple(shape), values.dtype, tuple(scales.shape), scales.dtype, n))
+    self._set(values, scales, lead + (n,))
 
   def _set(self, values, scales, shape):
     self._values = values

@@ -412,6 +412,19 @@ def test_infinities_stay_in_their_rows(hip, r):
   assert np.isnan(F.operand_value(q)).sum() == 256
 
 
+@pytest.mark.parametrize("r", [1, 40, 300])
+def test_scale_byte_of_nan(hip, r):
+  rng = np.random.default_rng(r)
+  a = F.random_operand(rng, (1, r, 640), 1.0)
+  w = F.random_operand(rng, (1, 200, 640), 0.05)
+  want = hip.expert_linear(a, w)
+  a.scales[0, r // 2, 4], w.scales[0, 77, 0] = 255, 255
+  got = hip.expert_linear(a, w)
+  nan = torch.zeros_like(got, dtype=torch.bool)
+  nan[0, r // 2], nan[0, :, 77] = True, True
+  assert got[nan].isnan().all() and torch.equal(got[~nan], want[~nan])
+
+
 def test_scales_of_all_sizes(hip):
   """Every unit an operand can have, on both sides."""
   rng = np.random.default_rng(0)
