@@ -135,6 +135,14 @@ class Fp8Blocks(object):
     return Fp8Blocks.__new__(Fp8Blocks)._set(
         values, scales, tuple(values.shape[:-1]) + self._shape[-1:])
 
+  def copy_(self, other):
+    """Takes the contents of an operand of the same shape."""
+    if other.shape != self._shape:
+      raise ValueError("shape %s, expected %s" % (other.shape, self._shape))
+    self._values.view(torch.uint8).copy_(other.values.view(torch.uint8))
+    self._scales.copy_(other.scales)
+    return self
+
   def __repr__(self):
     return "Fp8Blocks%s" % (self.shape,)
 

@@ -10,6 +10,7 @@ return their input (placement_mesh_impl.py:291-292, :376-377).
 
 import torch
 
+from mesh_amd import fp8_hip
 from mesh_amd import moe_hip
 from mesh_amd import ops as mtf
 
@@ -165,6 +166,8 @@ class HipMeshImpl(mtf.MeshImpl):
       for (kind, dtype), t in self._derived.items():
         if kind == "act":
           t.copy_(self._slice)
+        elif kind == "eight_bit":
+          t.copy_(self._as_eight_bit(dtype))
         else:
           s = self._slice
           moe_hip.pack_weights(s.reshape(-1, s.shape[-2], s.shape[-1]), dtype,
@@ -188,6 +191,20 @@ class HipMeshImpl(mtf.MeshImpl):
         s = self._slice
         k, n = s.shape[-2], s.shape[-1]
         self._derived[key] = moe_hip.pack_weights(s.reshape(-1, k, n), dtype)
+      return self._derived[key]
+
+    def _as_eight_bit(self, which):
+      kernels = self._slice.reshape(-1, *self._slice.shape[-2:])
+      with torch.cuda.device(kernels.device):
+        return fp8_hip.quantize(kernels, rows=which == "rows",
+                                columns=which == "columns")
+
+    def eight_bit(self, which):
+      """[..., K, N] slice as an 8-bit operand of fp8_hip: its "columns" [E, N, K], what
+      products multiply by, or its "rows" [E, K, N], what their input gradients do."""
+      key = ("eight_bit", which)
+      if key not in self._derived:
+        self._derived[key] = self._as_eight_bit(which)
       return self._derived[key]
 
     @staticmethod

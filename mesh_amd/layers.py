@@ -198,11 +198,15 @@ class DenseOperation(mtf.Operation):
   """y = activation(x . kernel) over the last dim of x: the einsum (+ relu) of
   mtf.layers.dense without bias (mesh_tensorflow/layers.py:112-160) as one
   operation on the matrix cores.  The kernel is read from the variable's
-  K-contiguous packed copy."""
+  K-contiguous packed copy.  eight_bit: the product and its gradients multiply 8-bit
+  operands (fp8_hip): x and the kernel with a scale for each block of 128 along the
+  dimension that is summed over, the kernel's quantized when it changes."""
 
-  def __init__(self, x, kernel, new_dims, activation, name=None):
+  def __init__(self, x, kernel, new_dims, activation, name=None, eight_bit=False):
     super(DenseOperation, self).__init__([x, kernel], name=name or "dense")
     self._activation = activation
+    self.eight_bit = eight_bit
+    self._handed_over = (0, False)
     shape = mtf.Shape(x.shape.dims[:-1] + list(new_dims))
     self._outputs = [mtf.Tensor(self, shape, x.dtype)]
     self.siblings = None       # a SharedInput
@@ -231,10 +235,47 @@ class DenseOperation(mtf.Operation):
       lowering.done_ahead.add(op)
     return True
 
+  def _hands_over(self):
+    """Whether nothing but the next 8-bit product reads the result, which then leaves
+    as its operand."""
+    operations, y = self.graph.operations, self.outputs[0]
+    if self._handed_over[0] != len(operations):
+      readers = [op for op in operations if y in op.inputs]
+      self._handed_over = (len(operations), len(readers) == 1 and
+                           isinstance(readers[0], DenseOperation) and
+                           readers[0].eight_bit)
+    return self._handed_over[1]
+
+  def _lower_eight_bit(self, lowering):
+    from mesh_amd import fp8_hip
+    (x, kernel), y = self.inputs, self.outputs[0]
+    mesh_impl = lowering.mesh_impl(self)
+    w = lowering.variables[kernel.operation].eight_bit("columns")
+    act = self._activation
+    sizes = y.shape.to_integer_list
+    operand = lowering.run_values.pop(x, None)
+    if operand is None:
+      operand = mesh_impl.slicewise(
+          lambda xs: fp8_hip.quantize(xs.contiguous().reshape(-1, xs.shape[-1])),
+          lowering.tensors[x]).tensor_list[0]
+    if not self._hands_over():
+      lowering.set_tensor_lowering(y, mesh_impl.slicewise(
+          lambda: fp8_hip.dense(operand, w, act).reshape(sizes)))
+      return
+    hidden = lowering.run_values[y] = mesh_impl.slicewise(
+        lambda: fp8_hip.dense(operand, w, act, eight_bit=True)).tensor_list[0]
+    # (whoever else asks for the tensor sees the values that are multiplied)
+    lowering.set_tensor_lowering(y, mesh_impl.LazyLaidOutTensor(
+        lambda: mesh_impl.slicewise(
+            lambda: fp8_hip.dequantize(hidden).reshape(sizes)), sizes))
+
   def lower(self, lowering):
     from mesh_amd import moe_hip
     if self in lowering.done_ahead or (
         self.siblings is not None and self._lower_siblings(lowering)):
+      return
+    if self.eight_bit:
+      self._lower_eight_bit(lowering)
       return
     x, kernel = self.inputs
     mesh_impl = lowering.mesh_impl(self)
@@ -271,8 +312,9 @@ class DenseGradOperation(mtf.Operation):
     producer_x = x.operation
     consumers = [op for op in x.graph.operations
                  if x in op.inputs and not isinstance(op, DenseGradOperation)]
+    # (The gradients of 8-bit operands mask dy while they quantize it instead.)
     self._masks_dx = (
-        isinstance(producer_x, DenseOperation)
+        not forward.eight_bit and isinstance(producer_x, DenseOperation)
         and producer_x._activation == "relu"      # pylint: disable=protected-access
         and x is producer_x.outputs[0]
         and consumers == [forward]
@@ -345,8 +387,31 @@ class DenseGradOperation(mtf.Operation):
     else:
       lowering.set_tensor_lowering(self._dx, value)
 
+  def _lower_eight_bit(self, lowering):
+    from mesh_amd import fp8_hip
+    dy, x, kernel, y = self.inputs
+    k, n = kernel.shape.to_integer_list
+    w_rows = lowering.variables[kernel.operation].eight_bit("rows")
+    relu = self._relu and not self._dy_is_masked
+    dtype = kernel.dtype
+
+    def fn(dy, x, y):
+      a_columns = fp8_hip.quantize(x.contiguous().reshape(1, -1, k), rows=False,
+                                   columns=True)
+      dx, dw = fp8_hip.expert_linear_backward(
+          a_columns, dy.contiguous().reshape(1, -1, n), w_rows,
+          relu_mask=y.contiguous().reshape(1, -1, n) if relu else None)
+      return dx.reshape(x.shape), dw.reshape(k, n).to(dtype)
+    dx, dw = lowering.mesh_impl(self).slicewise(
+        fn, *[lowering.tensors[t] for t in (dy, x, y)])
+    self._set_dx(lowering, dx)
+    lowering.set_tensor_lowering(self._dw, dw)
+
   def lower(self, lowering):
     from mesh_amd import moe_hip
+    if self._forward.eight_bit:
+      self._lower_eight_bit(lowering)
+      return
     mesh_impl = lowering.mesh_impl(self)
     made = self._made_ahead(lowering)
     last = self._forward.siblings and self.sums_up_in(self._forward.siblings.layers)
@@ -397,11 +462,12 @@ def _activation_name(activation):
 def dense(x, new_dims, reduced_dims=None, expert_dims=None, use_bias=True,
           activation=None, master_dtype=mtf.float32, slice_dtype=mtf.float32,
           variable_dtype=None, kernel_initializer=None, kernel_weights=None,
-          name=None):
+          name=None, eight_bit=False):
   """mtf.layers.dense (mesh_tensorflow/layers.py:112-160) for the case the
   transformer layers use: no bias, no expert dims, the reduced dims being the
   trailing dims of x; activation None / "linear" / relu.  The variable is
-  `<name>/kernel` with shape reduced_dims + new_dims."""
+  `<name>/kernel` with shape reduced_dims + new_dims.  eight_bit (x in bfloat16):
+  the product and its gradients on 8-bit operands, see DenseOperation."""
   if isinstance(new_dims, mtf.Dimension) or not isinstance(new_dims,
                                                            (list, tuple)):
     new_dims = [new_dims]
@@ -421,10 +487,14 @@ def dense(x, new_dims, reduced_dims=None, expert_dims=None, use_bias=True,
   if x.shape.dims[-1] != reduced_dims[0]:
     raise NotImplementedError("the reduced dim must be the last dim of x")
   act = _activation_name(activation)
+  if eight_bit and x.dtype != torch.bfloat16:
+    raise ValueError("dense on 8-bit operands takes and gives bfloat16, not %s"
+                     % (x.dtype,))
   w = get_dense_kernel_weights(x, new_dims, reduced_dims, [],
                                kernel_initializer, name, variable_dtype,
                                master_dtype, slice_dtype)
-  return DenseOperation(x, w, new_dims, act, name=name).outputs[0]
+  return DenseOperation(x, w, new_dims, act, name=name,
+                        eight_bit=eight_bit).outputs[0]
 
 
 def dense_product(x, reduced_dims, new_dims, activation_functions=None,

@@ -11,10 +11,12 @@ from mesh_amd.transformer import transformer
 class DenseReluDense(transformer.TransformerLayer):
   """Two dense layers with an activation on the hidden layer
   (transformer_layers.py:36-76): variables wi/kernel [d_model, d_ff] and
-  wo/kernel [d_ff, d_model]."""
+  wo/kernel [d_ff, d_model].  eight_bit (activations in bfloat16): both layers and
+  their gradients multiply 8-bit operands, the variables staying as they are."""
 
   def __init__(self, hidden_size=4096, dropout_rate=0.0, activation="relu",
-               use_bias=False):
+               use_bias=False, eight_bit=False):
+    self.eight_bit = eight_bit
     self.hidden_size = hidden_size
     self.dropout_rate = dropout_rate
     self.activation = activation
@@ -29,14 +31,14 @@ class DenseReluDense(transformer.TransformerLayer):
     h = mtf_layers.dense_product(
         x, reduced_dims=x.shape.dims[-1:], new_dims=hidden_channels,
         activation_functions=self.activation, use_bias=self.use_bias,
-        variable_dtype=context.variable_dtype, name="wi")
+        variable_dtype=context.variable_dtype, name="wi", eight_bit=self.eight_bit)
     if context.train and self.dropout_rate != 0.0:   # transformer_layers.py:67-69
       h = mtf.dropout(h, context.train, keep_prob=1.0 - self.dropout_rate,
                       noise_shape=h.shape - context.length_dim)
     y = mtf_layers.dense(
         h, io_channels, use_bias=self.use_bias, activation=None,
         variable_dtype=context.variable_dtype, reduced_dims=h.shape.dims[-1:],
-        name="wo")
+        name="wo", eight_bit=self.eight_bit)
     return y
 
 

@@ -201,3 +201,25 @@ def test_linear_backward_refusals(lib):
   _refused(lib, with_(_15=need - 1), -1, "workspace")
   assert lib.mesh_moe_fp8_expert_linear_backward_workspace_bytes(1, 0, 128, 64, 1) == 0
   assert ctypes.sizeof(ctypes.c_size_t) == 8
+
+
+def test_layers_on_8_bit_operands():
+  """The same variables and shapes as without, and float32 activations are refused."""
+  from mesh_amd import layers as mtf_layers
+  from mesh_amd import ops as mtf
+
+  def build(eight_bit, dtype):
+    graph = mtf.Graph()
+    mesh = mtf.Mesh(graph, "mesh")
+    dims = [mtf.Dimension("batch", 2), mtf.Dimension("d_model", 64)]
+    x = mtf.import_tf_tensor(mesh, torch.zeros(2, 64, dtype=dtype), mtf.Shape(dims))
+    y = mtf_layers.dense(
+        x, mtf.Dimension("d_ff", 96), use_bias=False, activation="relu", name="wi",
+        variable_dtype=mtf.VariableDType(torch.float32, torch.float32, dtype),
+        eight_bit=eight_bit)
+    grads = mtf.gradients([y], [x] + [v.outputs[0] for v in graph.trainable_variables])
+    return ([(v.name, str(v.shape)) for v in graph.all_variables], str(y.shape), y.dtype,
+            [(str(g.shape), g.dtype) for g in grads])
+  assert build(True, torch.bfloat16) == build(False, torch.bfloat16)
+  with pytest.raises(ValueError, match="bfloat16"):
+    build(True, torch.float32)

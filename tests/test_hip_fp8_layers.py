@@ -1,0 +1,180 @@
+"""Dense layers on 8-bit operands in graphs: the same numbers, bit for bit, as the calls of
+fp8_hip that they stand for (tests/test_hip_fp8.py tests those), in eager runs, gradients
+and captured steps, before and after an assignment."""
+
+import pytest
+import torch
+
+import mesh_amd as mtf
+from mesh_amd import layers as mtf_layers
+from mesh_amd.transformer import transformer
+from mesh_amd.transformer import transformer_layers
+
+pytestmark = pytest.mark.gpu
+
+BF16 = torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def hip():
+  from mesh_amd import fp8_hip
+  fp8_hip.load_library()
+  return fp8_hip
+
+
+def _normal(seed, sizes, std=1.0):
+  gen = torch.Generator().manual_seed(seed)
+  return torch.randn(sizes, generator=gen) * std
+
+
+def _graph(b, l, m, f, seed=0, dtype=BF16, master=torch.float32):
+  """x -> wi (relu) -> h -> wo -> y, with the variables' values."""
+  graph = mtf.Graph()
+  mesh = mtf.Mesh(graph, "mesh")
+  dims = [mtf.Dimension("batch", b), mtf.Dimension("length", l),
+          mtf.Dimension("d_model", m)]
+  x = mtf.import_tf_tensor(mesh, _normal(seed, (b, l, m)).to(dtype), mtf.Shape(dims))
+  kind = dict(use_bias=False, eight_bit=True,
+              variable_dtype=mtf.VariableDType(master, master, dtype))
+  h = mtf_layers.dense(x, mtf.Dimension("d_ff", f), activation="relu", name="wi", **kind)
+  y = mtf_layers.dense(h, dims[-1], name="wo", **kind)
+  values = {"wi/kernel": _normal(seed + 1, (m, f), m ** -0.5),
+            "wo/kernel": _normal(seed + 2, (f, m), f ** -0.5)}
+  return graph, mesh, x, h, y, values
+
+
+def _lower(graph, mesh, values):
+  return mtf.Lowering(graph, {mesh: mtf.HipMeshImpl()}, initial_values=values)
+
+
+def _columns(hip, w):
+  return hip.quantize(w.cuda().unsqueeze(0), rows=False, columns=True)
+
+
+def _forward(hip, x, values):
+  a = hip.quantize(x.cuda().reshape(-1, x.shape[-1]))
+  h = hip.dense(a, _columns(hip, values["wi/kernel"]), "relu", eight_bit=True)
+  y = hip.dense(h, _columns(hip, values["wo/kernel"]))
+  return hip.dequantize(h).reshape(x.shape[:-1] + (-1,)), y.reshape(x.shape)
+
+
+SIZES = [(1, 1, 128, 512), (2, 5, 200, 333), (3, 100, 256, 1024)]
+
+
+@pytest.mark.parametrize("sizes", SIZES)
+@pytest.mark.parametrize("master", [torch.float32, BF16])
+def test_forward_and_assignment(hip, sizes, master):
+  graph, mesh, x, h, y, values = _graph(*sizes, master=master)
+  values = {k: v.to(master) for k, v in values.items()}
+  lowering = _lower(graph, mesh, values)
+  given = lowering.export_to_tf_tensor(x)
+  for step in range(3):
+    want_h, want_y = _forward(hip, given, values)
+    assert torch.equal(lowering.export_to_tf_tensor(y), want_y)
+    assert torch.equal(lowering.export_to_tf_tensor(h), want_h)
+    values = {k: v * 1.5 - 0.01 for k, v in values.items()}
+    for var, laid_out in lowering.variables.items():
+      laid_out.assign(values[var.name])
+    given = _normal(10 + step, sizes[:3]).to(BF16)
+    lowering.run({x: given})
+
+
+@pytest.mark.parametrize("sizes", SIZES)
+def test_gradients(hip, sizes):
+  graph, mesh, x, h, y, values = _graph(*sizes)
+  dy = mtf.import_tf_tensor(mesh, _normal(7, sizes[:3]).to(BF16), y.shape)
+  variables = [v.outputs[0] for v in graph.trainable_variables]
+  grads = mtf.gradients([y], [x] + variables, [dy])
+  lowering = _lower(graph, mesh, values)
+  b, l, m, f = sizes
+  for step in range(2):
+    xs, dys = (lowering.export_to_tf_tensor(t) for t in (x, dy))
+    wi, wo = (values[k].cuda().unsqueeze(0) for k in ("wi/kernel", "wo/kernel"))
+    wi_rows, wi_columns = hip.quantize(wi, rows=True, columns=True)
+    wo_rows, wo_columns = hip.quantize(wo, rows=True, columns=True)
+    a, a_columns = hip.quantize(xs.reshape(1, -1, m), rows=True, columns=True)
+    hs = hip.expert_linear(a, wi_columns, "relu")
+    hq, h_columns = hip.quantize(hs, rows=True, columns=True)
+    ys = hip.expert_linear(hq, wo_columns)
+    dh, dwo = hip.expert_linear_backward(h_columns, dys.reshape(1, -1, m), wo_rows)
+    dx, dwi = hip.expert_linear_backward(a_columns, dh, wi_rows, relu_mask=hs)
+    for tensor, want in [(h, hs), (y, ys), (grads[0], dx), (grads[1], dwi),
+                         (grads[2], dwo)]:
+      got = lowering.export_to_tf_tensor(tensor)
+      assert torch.equal(got.reshape(-1), want.reshape(-1).to(got.dtype))
+    values = {k: v * 0.5 + 0.02 for k, v in values.items()}
+    for var, laid_out in lowering.variables.items():
+      laid_out.assign(values[var.name])
+    lowering.run({x: _normal(20 + step, sizes[:3]).to(BF16)})
+
+
+def test_hidden_tensor_that_is_read_twice(hip):
+  """Another reader of the hidden tensor: it is a bfloat16 tensor then."""
+  graph, mesh, x, h, y, values = _graph(2, 40, 256, 512)
+  twice = mtf_layers.dense(h, mtf.Dimension("d_out", 64), use_bias=False, name="w2",
+                           variable_dtype=mtf.VariableDType(torch.float32, torch.float32,
+                                                            BF16))
+  values["w2/kernel"] = _normal(5, (512, 64), 0.05)
+  lowering = _lower(graph, mesh, values)
+  a = hip.quantize(lowering.export_to_tf_tensor(x).reshape(-1, 256))
+  hs = hip.dense(a, _columns(hip, values["wi/kernel"]), "relu")
+  assert torch.equal(lowering.export_to_tf_tensor(h).reshape(80, 512), hs)
+  ys = hip.dense(hip.quantize(hs), _columns(hip, values["wo/kernel"]))
+  assert torch.equal(lowering.export_to_tf_tensor(y).reshape(80, 256), ys)
+  assert lowering.export_to_tf_tensor(twice).shape == (2, 40, 64)
+
+
+@pytest.mark.parametrize("with_gradients", [False, True])
+def test_captured_step(hip, with_gradients):
+  sizes = (2, 33, 256, 640)
+  graph, mesh, x, h, y, values = _graph(*sizes)
+  outputs = [y]
+  if with_gradients:
+    dy = mtf.import_tf_tensor(mesh, _normal(7, sizes[:3]).to(BF16), y.shape)
+    variables = [v.outputs[0] for v in graph.trainable_variables]
+    outputs += mtf.gradients([y], [x] + variables, [dy])
+  lowering = _lower(graph, mesh, values)
+  step = lowering.capture()
+  other = _lower(graph, mesh, values)
+  for i in range(3):
+    given = _normal(30 + i, sizes[:3]).to(BF16)
+    step.replay({x: given})
+    got = [lowering.export_to_tf_tensor(t).clone() for t in outputs]
+    other.run({x: given})
+    for t, value in zip(outputs, got):
+      assert torch.equal(value, other.export_to_tf_tensor(t))
+    values = {k: v * 0.9 + 0.01 for k, v in values.items()}
+    for low in (lowering, other):
+      for var, laid_out in low.variables.items():
+        laid_out.assign(values[var.name])
+
+
+def test_layer_stack(hip):
+  """DenseReluDense in a stack with and without 8-bit operands.  Two operands of a root
+  mean square error of at most 2^-4 / sqrt(3) each, in two layers one behind the other,
+  half of whose result the residual is."""
+  del hip
+  b, l, m, f = 2, 70, 256, 1024
+  results = []
+  for eight_bit in (False, True):
+    graph = mtf.Graph()
+    mesh = mtf.Mesh(graph, "mesh")
+    dims = [mtf.Dimension("batch", b), mtf.Dimension("length", l),
+            mtf.Dimension("d_model", m)]
+    x = mtf.import_tf_tensor(mesh, _normal(1, (b, l, m)).to(BF16), mtf.Shape(dims))
+    stack = transformer.make_layer_stack(
+        [(transformer_layers.DenseReluDense, dict(hidden_size=f, eight_bit=eight_bit))],
+        num_layers=2)
+    model = transformer.Unitransformer(stack, d_model=m, name="encoder")
+    y, _ = model.call_layers(
+        x, mtf.VariableDType(torch.float32, torch.float32, BF16), mode="eval")
+    values = {}
+    for i, v in enumerate(graph.all_variables):
+      sizes = v.shape.to_integer_list
+      values[v.name] = (torch.ones(sizes) if len(sizes) == 1
+                        else _normal(50 + i, sizes, sizes[0] ** -0.5))
+    lowering = _lower(graph, mesh, values)
+    results.append(lowering.export_to_tf_tensor(y).double())
+  exact, got = results
+  error = ((got - exact).square().mean() / exact.square().mean()).sqrt()
+  assert 0 < error < 2.0 ** -3.5
