@@ -58,10 +58,12 @@ __device__ __forceinline__ uint32_t max16(uint32_t v) {
   return max(v, dpp<0x140>(v));   // row_mirror
 }
 
-// fp8.hip, for the calls that end in an 8-bit operand (arguments checked by them)
+// fp8.hip, for the gradients, which make operands of dy (arguments checked by them).
+// only_counted: rows from an expert's count on are left out, but for the columns' first
+// two blocks.
 int fp8_quantize(const void* x, const void* relu_mask, const int32_t* row_count,
                  void* row_values, uint8_t* row_scales, void* column_values,
                  uint8_t* column_scales, int E, int R, int K, int dtype,
-                 bool skip_uncounted, hipStream_t st);
+                 bool only_counted, hipStream_t st);
 
 }  // namespace mesh_moe

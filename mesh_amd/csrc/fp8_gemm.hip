@@ -1661,8 +1661,14 @@ extern "C" int mesh_moe_fp8_expert_linear_backward(
   hipStream_t st = (hipStream_t)stream;
   uint8_t* ws = (uint8_t*)workspace;
   uint8_t* rows = da ? ws + p.rows : nullptr;
+  // (tiles read the blocks of rows that an expert has, other kinds and parts all of them;
+  // for half of 32 x 640 rows x 1024 the pass takes 26 us instead of 28)
+  const Plan dw_plan = plan_product(E, K, R, N, false, false);
+  const bool only_counted = row_count != nullptr && dw_plan.kind >= TILES_64 &&
+                            dw_plan.split == 1;
   int rc = fp8_quantize(dy, relu_mask, row_count, rows, da ? ws + p.row_scales : nullptr,
-                        ws + p.columns, ws + p.column_scales, E, R, N, dtype, false, st);
+                        ws + p.columns, ws + p.column_scales, E, R, N, dtype,
+                        only_counted, st);
   if (rc != 0) return rc;
   const GemmArgs weights = {(const uint8_t*)a_column_values, a_column_scales,
                             ws + p.columns, ws + p.column_scales, nullptr, dw, nullptr,
