@@ -628,6 +628,46 @@ def test_training_step(hip):
   near(dwi[0], _f64(x[0]).T @ dhx)
 
 
+def test_beyond_2_to_the_31_elements(hip):
+  """Operands, results and norms of more than 2^31 elements: their first and last rows
+  are what the calls make of those alone."""
+  rows, k, n = 140032, 16384, 256
+  gen = torch.Generator(device="cuda").manual_seed(5)
+  x = torch.empty((rows, k), dtype=torch.bfloat16, device="cuda")
+  for at in range(0, rows, 8192):
+    x[at:at + 8192] = torch.randn((min(8192, rows - at), k), generator=gen, device="cuda")
+  ends = (slice(0, 128), slice(rows - 128, rows))
+  q, columns = hip.quantize(x, rows=True, columns=True)
+  w, wv = _random(hip, (1, n, k), 0.01, 6)
+  y = hip.dense(q, w)
+  back = hip.dequantize(q)
+  total, norm = hip.residual_rms_norm(x, x, x[7].contiguous())
+  assert y.shape == (rows, n) and columns.shape == (k, rows)
+  wt = wv[0].t().contiguous()
+  for sl in ends:
+    part = x[sl].contiguous()
+    r, c = hip.quantize(part, rows=True, columns=True)
+    assert torch.equal(q.values[sl].view(torch.uint8), r.values.view(torch.uint8))
+    assert torch.equal(q.scales[sl], r.scales)
+    assert torch.equal(columns.values[:, sl].view(torch.uint8),
+                       c.values.view(torch.uint8))
+    assert torch.equal(back[sl], hip.dequantize(r))
+    a = back[sl].double()
+    assert _near(y[sl], a @ wt, a.abs() @ wt.abs())
+    t, m = hip.residual_rms_norm(part, part, x[7].contiguous())
+    assert torch.equal(total[sl], t)
+    assert torch.equal(norm.values[sl].view(torch.uint8), m.values.view(torch.uint8))
+  del total, norm, back, columns, x
+  wide, _ = _random(hip, (1, 17000, 256), 0.05, 8)       # a result of 2.4e9 elements
+  a, av = _random(hip, (1, rows, 256), 1.0, 9)
+  y = hip.expert_linear(a, wide)[0]
+  wt = hip.dequantize(wide, torch.float32)[0].double().t().contiguous()
+  for sl in ends:
+    assert _near(y[sl], av[0, sl] @ wt, av[0, sl].abs() @ wt.abs())
+  dw_rows = hip.quantize(y[None, -300:].contiguous(), rows=False, columns=True)
+  assert dw_rows.shape == (1, 17000, 300)
+
+
 @pytest.mark.parametrize("rows", [1, 300])
 def test_captured(hip, rows):
   """The block recorded into a graph, replayed with new inputs and work between the
