@@ -438,6 +438,9 @@ __device__ __forceinline__ int tile_number(int round) {
 // A result is turned round in the weight slot that the last K tile has left, 32 rows of
 // 128 bytes at a time, each wavefront in the kilobytes that its own loads fill
 // afterwards (so no barrier), and leaves in whole 128-byte lines.
+//
+// 8192^3 takes 430 us, 2560 TFLOP/s, 1.6 us per K tile; with zeros for operands 349 us:
+// the difference is what the socket's power limit takes.  16384 rows 1024 -> 4096 66 us (49).
 // ---------------------------------------------------------------------------
 struct BigCfg {
   static constexpr int BM = 256, BN = 256, THREADS = 512, WAVES = 8;
@@ -842,6 +845,10 @@ __global__ __launch_bounds__(BigCfg::THREADS) void fp8_tile256_kernel(GemmArgs g
 // four are requested more than a K tile ahead.  A result is turned round in the weight
 // slot that the last K tile has left, each wavefront in the kilobytes that its own loads
 // fill afterwards (so no barrier), and leaves in whole lines.
+//
+// 1024 rows 11080 -> 4096 (256 tiles of 128 x 128, one per CU) take 51 us, 0.58 us per K
+// tile, and two blocks on a CU 1.0 together: bound by what the L2s give, 27 bytes per
+// clock and CU.
 // ---------------------------------------------------------------------------
 // TM: 2 or 1
 template <int TM_>
