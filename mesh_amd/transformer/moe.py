@@ -19,6 +19,7 @@ expert_selection router, and a mesh with more than one device.
 
 import torch
 
+from mesh_amd import fp8_hip
 from mesh_amd import layers as mtf_layers
 from mesh_amd import moe_hip
 from mesh_amd import ops as mtf
@@ -453,7 +454,7 @@ class MoEV1Operation(mtf.Operation):
 
   def __init__(self, inputs, w_gate, wi, wo, importance, output_dim, capacity,
                gating, activation, k_wo=None, hidden_keep_prob=None,
-               name="moe_v1"):
+               eight_bit=False, name="moe_v1"):
     """With k_wo (moe_use_experts_attention, moe.py:514-522) `wo` is the "q_wo"
     kernel, the operation has a second output projection of the same hidden
     tensor and its outputs are (q, loss, k).
@@ -461,7 +462,9 @@ class MoEV1Operation(mtf.Operation):
     `wi` and `activation` may be lists of the same length: the hidden tensor
     is then the product of act_i(expert_in . wi_i) (moe.py:469-475).
     hidden_keep_prob: keep probability of the dropout on the hidden tensor
-    (moe.py:477-479), None for none."""
+    (moe.py:477-479), None for none.
+    eight_bit: the experts' products and their gradients multiply 8-bit operands
+    (fp8_hip); one bfloat16 layer wi, one wo, no hidden dropout."""
     wis = list(wi) if isinstance(wi, (list, tuple)) else [wi]
     acts = (list(activation) if isinstance(activation, (list, tuple))
             else [activation])
@@ -484,6 +487,12 @@ class MoEV1Operation(mtf.Operation):
     self._more_wi = wis[1:]
     self._more_activations = acts[1:]
     self._hidden_keep_prob = hidden_keep_prob
+    self._eight_bit = eight_bit
+    if eight_bit and (inputs.dtype != torch.bfloat16 or len(wis) > 1 or
+                      k_wo is not None or hidden_keep_prob is not None):
+      raise NotImplementedError(
+          "experts on 8-bit operands are bfloat16 layers wi and wo without a product of "
+          "activations, a second projection or dropout on the hidden tensor")
     # experts that are not one ReLU / linear layer: the backward pass needs the
     # pre-activation of every factor
     self._general_hidden = bool(self._more_wi) or (
@@ -501,6 +510,9 @@ class MoEV1Operation(mtf.Operation):
     """Gradients w.r.t. (inputs, gate kernel, wi, wo[, importance][, k_wo])
     from those of (outputs, loss[, second outputs]); importance carries
     none."""
+    if self._eight_bit and self._general_hidden:
+      raise NotImplementedError("gradient of experts on 8-bit operands with activation %r"
+                                % (self._activation,))
     self._save_for_backward = True
     self._num_grad_ops = getattr(self, "_num_grad_ops", 0) + 1
     d_out, d_loss = grad_ys[:2]
@@ -524,6 +536,7 @@ class MoEV1Operation(mtf.Operation):
     if (type(gating) is not _GatingSpec or gating.policy == "random" or
         self._save_for_backward or self._k_wo is not None or self._more_wi or
         self._hidden_keep_prob is not None or self.scaled_loss is None or
+        self._eight_bit or
         moe_hip.timing()):
       return False
     o, g, s, _ = x.shape.to_integer_list
@@ -550,11 +563,26 @@ class MoEV1Operation(mtf.Operation):
     lowering.operations[self] = {}
     return True
 
+  def _eight_bit_experts(self, lowering):
+    """expert_in [E, R, M] -> (y [E, R, N], the hidden tensor where a gradient reads
+    it)."""
+    wi, wo = [lowering.variables[t.operation].eight_bit("columns")
+              for t in self.inputs[2:4]]
+    keep = self._save_for_backward
+
+    def fn(expert_in):
+      h = fp8_hip.expert_linear(fp8_hip.quantize(expert_in), wi, self._activation,
+                                eight_bit=not keep)
+      return (fp8_hip.expert_linear(fp8_hip.quantize(h) if keep else h, wo),
+              h if keep else None)
+    return fn
+
   def lower(self, lowering):
     x, w_gate, wi, wo = self.inputs[:4]
     dt = x.dtype
-    wi_p = _packed(lowering, wi, dt)
-    wo_p = _packed(lowering, wo, dt)
+    experts = self._eight_bit_experts(lowering) if self._eight_bit else None
+    wi_p = None if experts else _packed(lowering, wi, dt)
+    wo_p = None if experts else _packed(lowering, wo, dt)
     wg_p = _packed(lowering, w_gate, dt)               # [1, E, M]
     if self._lower_whole(lowering, x, w_gate, (wg_p, wi_p, wo_p)):
       return
@@ -596,7 +624,7 @@ class MoEV1Operation(mtf.Operation):
       expert_in = h = None
       # one relu / linear / ... layer per expert, with or without the hidden
       # dropout: what the compacted calls take
-      one_layer = not more_wi_p and not keep_pre
+      one_layer = not more_wi_p and not keep_pre and experts is None
       single_choice = (not by_slot and kwo_p is None and one_layer and
                        self._gating.router != "top_2")
       compact_forward = single_choice or (
@@ -640,7 +668,7 @@ class MoEV1Operation(mtf.Operation):
         if compact is not None:
           y, row_offsets = compact
       if (y is None and not (save or by_slot or kwo_p is not None) and
-          plain_hidden):
+          plain_hidden and experts is None):
         # nobody reads expert_in afterwards: fold the dispatch into the first
         # expert GEMM where the library can
         y = moe_hip.dispatched_expert_ffn(xg, r, wi_p, wo_p,
@@ -649,7 +677,9 @@ class MoEV1Operation(mtf.Operation):
         expert_in = (moe_hip.slot_dispatch(xg, r) if by_slot
                      else moe_hip.dispatch(xg, r))
         expert_in = expert_in.reshape(e_, groups * c_, m_)
-      if y is None and plain_hidden:
+      if experts is not None:
+        y, h = experts(expert_in)
+      elif y is None and plain_hidden:
         h = None
         if save or kwo_p is not None:
           h = torch.empty((e_, groups * c_, wi_p.shape[1]), dtype=dt,
@@ -820,6 +850,16 @@ class MoEV1GradOperation(mtf.Operation):
             fwd._activation, dh_scale=sv["hidden_noise"],
             keep_prob=fwd._hidden_keep_prob)
         dkwo, dwis = None, [dwi]
+      elif fwd._eight_bit:
+        a_columns, h_columns = [
+            fp8_hip.quantize(t.reshape(e_, groups * c_, -1), rows=False, columns=True)
+            for t in (sv["expert_in"], sv["h"])]
+        dh, dwo = fp8_hip.expert_linear_backward(
+            h_columns, dy.reshape(e_, groups * c_, n_), wo_s)
+        dxe, dwi = fp8_hip.expert_linear_backward(
+            a_columns, dh, wi_s,
+            relu_mask=sv["h"] if fwd._activation == "relu" else None)
+        dkwo, dwis = None, [dwi]
       elif fwd._general_hidden:
         dys, wos = [dy.reshape(e_, groups * c_, n_)], [wo_s]
         if has_k:
@@ -903,7 +943,9 @@ class MoEV1GradOperation(mtf.Operation):
       return res + tuple(dwis[1:])
 
     ins = self.inputs
-    args = [lowering.tensors[ins[i]] for i in (2, 3, 4, 5)]
+    args = [lowering.variables[ins[i].operation].eight_bit("rows")
+            if fwd._eight_bit and i < 4 else lowering.tensors[ins[i]]
+            for i in (2, 3, 4, 5)]
     args += [lowering.tensors[t] for t in ins[6:]]
     outs = mesh_impl.slicewise(fn, *args)
     _release_saved(lowering.operations[fwd])
@@ -927,7 +969,8 @@ def transformer_moe_layer_v1(
       moe_gating, moe_dropout_rate, moe_use_experts_attention, moe_loss_coef,
       moe_use_second_place_loss, moe_second_policy_train/eval,
       moe_second_threshold_train/eval; for switch gating
-      moe_switch_policy_train/eval and moe_z_loss)
+      moe_switch_policy_train/eval and moe_z_loss; moe_eight_bit, which the reference
+      does not have: the experts multiply 8-bit operands)
     train: a boolean
     variable_dtype: a mtf.VariableDType
     layout: optional - an input to mtf.convert_to_layout_rules
@@ -998,6 +1041,9 @@ def transformer_moe_layer_v1(
     gating = _GatingSpec(hparams, train, num_microbatches)
     router_name = "top_2_gating"                        # moe.py:1314
   act_names = _activation_names(activation)
+  eight_bit = getattr(hparams, "moe_eight_bit", False)
+  if eight_bit and hparams.moe_use_experts_attention:
+    raise NotImplementedError("experts attention on 8-bit operands")
 
   # variables, named and shaped as the reference's dense layers create them
   w_gate = mtf_layers.get_dense_kernel_weights(
@@ -1030,7 +1076,7 @@ def transformer_moe_layer_v1(
 
   output, loss = MoEV1Operation(
       inputs, w_gate, wi, wo, nonpadding, output_dim, expert_capacity, gating,
-      act_names, hidden_keep_prob=hidden_keep_prob).outputs
+      act_names, hidden_keep_prob=hidden_keep_prob, eight_bit=eight_bit).outputs
   output = mtf.reshape(output, batch_and_length_dims + [output_dim])
   return output, _scaled_loss(loss, hparams.moe_loss_coef)
 
@@ -1262,6 +1308,8 @@ def transformer_moe_layer_v2(
     inputs = mtf.reshape(
         inputs, [mtf.Dimension("outer_batch", 1)] + inputs.shape.dims)
 
+  if getattr(hparams, "moe_eight_bit", False):
+    raise NotImplementedError("hierarchical experts on 8-bit operands")
   assert len(hparams.moe_num_experts) == 2
   a0, b1, l, m = inputs.shape.dims
   hidden_dim = mtf.Dimension("expert_hidden", hparams.moe_hidden_size)
@@ -1404,6 +1452,15 @@ class MoE1D(transformer.TransformerLayer):
       else:
         y = mtf.reshape(y, x_shape)
     return y
+
+
+class EightBitMoE1D(MoE1D):
+  """MoE1D whose experts multiply 8-bit operands, forward and backward (moe_eight_bit of
+  transformer_moe_layer_v1): the same arguments and variables."""
+
+  def __init__(self, *args, **kwargs):
+    super(EightBitMoE1D, self).__init__(*args, **kwargs)
+    self._hparams.moe_eight_bit = True
 
 
 class MoE2D(transformer.TransformerLayer):

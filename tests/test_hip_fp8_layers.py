@@ -7,6 +7,7 @@ import torch
 
 import mesh_amd as mtf
 from mesh_amd import layers as mtf_layers
+from mesh_amd.transformer import moe
 from mesh_amd.transformer import transformer
 from mesh_amd.transformer import transformer_layers
 
@@ -178,3 +179,127 @@ def test_layer_stack(hip):
   exact, got = results
   error = ((got - exact).square().mean() / exact.square().mean()).sqrt()
   assert 0 < error < 2.0 ** -3.5
+
+
+def _moe(b, l, m, f, e, gating="top_2", activation="relu", eight_bit=True, grads=False):
+  graph = mtf.Graph()
+  mesh = mtf.Mesh(graph, "mesh")
+  dims = [mtf.Dimension("batch", b), mtf.Dimension("length", l),
+          mtf.Dimension("d_model", m)]
+  x = mtf.import_tf_tensor(mesh, _normal(1, (b, l, m)).to(BF16), mtf.Shape(dims))
+  hparams = moe.HParams()
+  moe.set_default_moe_hparams(hparams)
+  for name, value in (("moe_gating", gating), ("moe_num_experts", e),
+                      ("moe_hidden_size", f), ("moe_group_size", 64),
+                      ("moe_min_expert_capacity", 4), ("moe_dropout_rate", 0.0),
+                      ("moe_use_experts_attention", False), ("moe_z_loss", None),
+                      ("moe_second_policy_train", "all"),
+                      ("moe_second_policy_eval", "all"),
+                      ("moe_switch_policy_train", "argmax"),
+                      ("moe_switch_policy_eval", "argmax"), ("moe_switch_dropout", 0.0),
+                      ("moe_switch_temperature", 1.0), ("moe_switch_jitter", 0.0),
+                      ("moe_ntlb_top_k", 2), ("moe_eight_bit", eight_bit)):
+    setattr(hparams, name, value)
+  nonpadding = None
+  if gating == "expert_selection":
+    nonpadding = mtf.import_tf_tensor(mesh, torch.ones((b, l), dtype=BF16),
+                                      mtf.Shape(dims[:2]))
+  y, loss = moe.transformer_moe_layer_v1(
+      x, dims[-1], hparams, grads, mtf.VariableDType(torch.float32, torch.float32, BF16),
+      nonpadding=nonpadding, activation=activation)
+  outputs = [y]
+  if grads:
+    dy = mtf.import_tf_tensor(mesh, _normal(2, (b, l, m)).to(BF16), y.shape)
+    outputs += mtf.gradients(
+        [y, loss], [x] + [v.outputs[0] for v in graph.trainable_variables], [dy, None])
+  values = {}
+  for i, v in enumerate(graph.all_variables):
+    sizes = v.shape.to_integer_list
+    values[v.name] = _normal(60 + i, sizes, sizes[-2] ** -0.5)
+  return _lower(graph, mesh, values), x, outputs, values
+
+
+def _error(got, exact):
+  got, exact = got.double(), exact.double()
+  return float(((got - exact).square().mean() / exact.square().mean()).sqrt())
+
+
+@pytest.mark.parametrize("gating", ["top_2", "switch", "expert_selection"])
+@pytest.mark.parametrize("activation", ["relu", "gelu"])
+def test_experts(hip, gating, activation):
+  """The layer against the one in bfloat16: the same routing, and two products whose
+  operands are off by at most 2^-4 / sqrt(3) each in the root mean square."""
+  del hip
+  sizes = (2, 128, 256, 640, 8)
+  lowering, x, (y,), _ = _moe(*sizes, gating=gating, activation=activation)
+  plain, _, (exact,), _ = _moe(*sizes, gating=gating, activation=activation,
+                               eight_bit=False)
+  got, want = lowering.export_to_tf_tensor(y), plain.export_to_tf_tensor(exact)
+  assert 0 < _error(got, want) < 2.0 ** -3.5
+  # (tokens without a slot; single elements may be 0 in one of them)
+  assert torch.equal((got == 0).all(-1), (want == 0).all(-1))
+  step = lowering.capture()
+  given = _normal(9, sizes[:3]).to(BF16)
+  lowering.run({x: given})
+  eager = lowering.export_to_tf_tensor(y).clone()
+  for _ in range(3):
+    step.replay({x: given})
+    assert torch.equal(lowering.export_to_tf_tensor(y), eager)
+
+
+@pytest.mark.parametrize("gating", ["top_2", "switch"])
+def test_gradients_of_experts(hip, gating):
+  """dx, dwi and dwo against those of the bfloat16 layer; the router's gradient reads the
+  experts' outputs, which are as far apart as the products make them.  (Where the two
+  hidden tensors differ in sign the masks do: 2^-2.5 instead of 2^-3.5.)"""
+  del hip
+  sizes = (2, 128, 256, 640, 8)
+  lowering, x, got, values = _moe(*sizes, gating=gating, grads=True)
+  plain, _, exact, _ = _moe(*sizes, gating=gating, grads=True, eight_bit=False)
+  assert len(got) == len(exact) == 5
+  for a, b in zip(got, exact):
+    assert a.shape.to_integer_list == b.shape.to_integer_list and a.dtype == b.dtype
+    assert 0 < _error(lowering.export_to_tf_tensor(a),
+                      plain.export_to_tf_tensor(b)) < 2.0 ** -2.5
+  for low in (lowering, plain):
+    for var, laid_out in low.variables.items():
+      laid_out.assign(values[var.name] * 0.8)
+    low.run()
+  for a, b in zip(got, exact):
+    assert 0 < _error(lowering.export_to_tf_tensor(a),
+                      plain.export_to_tf_tensor(b)) < 2.0 ** -2.5
+
+
+def test_experts_refusals(hip):
+  del hip
+  with pytest.raises(NotImplementedError, match="8-bit"):
+    _moe(1, 64, 64, 64, 4, activation=["relu", "linear"])
+  with pytest.raises(NotImplementedError, match="8-bit"):
+    _moe(1, 64, 64, 64, 4, activation="gelu", grads=True)
+
+
+def test_moe_layer_in_a_stack(hip):
+  del hip
+  results = []
+  for layer in (moe.MoE1D, moe.EightBitMoE1D):
+    graph = mtf.Graph()
+    mesh = mtf.Mesh(graph, "mesh")
+    dims = [mtf.Dimension("batch", 2), mtf.Dimension("length", 96),
+            mtf.Dimension("d_model", 128)]
+    x = mtf.import_tf_tensor(mesh, _normal(1, (2, 96, 128)).to(BF16), mtf.Shape(dims))
+    stack = transformer.make_layer_stack(
+        [(layer, dict(num_experts=4, hidden_size=384, group_size=64,
+                      second_policy_eval="all"))], num_layers=1)
+    model = transformer.Unitransformer(stack, d_model=128, name="encoder")
+    y, losses = model.call_layers(
+        x, mtf.VariableDType(torch.float32, torch.float32, BF16), mode="eval")
+    values = {}
+    for i, v in enumerate(graph.all_variables):
+      sizes = v.shape.to_integer_list
+      values[v.name] = (torch.ones(sizes) if len(sizes) == 1
+                        else _normal(70 + i, sizes, sizes[-2] ** -0.5))
+    lowering = _lower(graph, mesh, values)
+    results.append((lowering.export_to_tf_tensor(y),
+                    [float(lowering.export_to_tf_tensor(t)) for t in losses]))
+  assert results[0][1] == results[1][1]
+  assert 0 < _error(results[1][0], results[0][0]) < 2.0 ** -3.5
