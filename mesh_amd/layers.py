@@ -207,6 +207,7 @@ class DenseOperation(mtf.Operation):
     self._activation = activation
     self.eight_bit = eight_bit
     self._handed_over = (0, False)
+    self._num_grad_ops = 0
     shape = mtf.Shape(x.shape.dims[:-1] + list(new_dims))
     self._outputs = [mtf.Tensor(self, shape, x.dtype)]
     self.siblings = None       # a SharedInput
@@ -255,9 +256,16 @@ class DenseOperation(mtf.Operation):
     sizes = y.shape.to_integer_list
     operand = lowering.run_values.pop(x, None)
     if operand is None:
-      operand = mesh_impl.slicewise(
-          lambda xs: fp8_hip.quantize(xs.contiguous().reshape(-1, xs.shape[-1])),
-          lowering.tensors[x]).tensor_list[0]
+      # (with a gradient to follow, the columns that it reads in the same pass)
+      made = mesh_impl.slicewise(
+          lambda xs: fp8_hip.quantize(xs.contiguous().reshape(-1, xs.shape[-1]),
+                                      columns=self._num_grad_ops > 0),
+          lowering.tensors[x])
+      if self._num_grad_ops:
+        operand, columns = [t.tensor_list[0] for t in made]
+        lowering.run_values[self] = [columns, self._num_grad_ops]
+      else:
+        operand = made.tensor_list[0]
     if not self._hands_over():
       lowering.set_tensor_lowering(y, mesh_impl.slicewise(
           lambda: fp8_hip.dense(operand, w, act).reshape(sizes)))
@@ -287,7 +295,15 @@ class DenseOperation(mtf.Operation):
     lowering.set_tensor_lowering(
         self.outputs[0], mesh_impl.slicewise(fn, lowering.tensors[x]))
 
+  def take_columns(self, lowering):
+    """The columns of x that the forward product left for its gradients, the last of
+    which drops them."""
+    kept = lowering.run_values[self]
+    kept[1] -= 1
+    return kept[0] if kept[1] else lowering.run_values.pop(self)[0]
+
   def gradient(self, grad_ys):
+    self._num_grad_ops += 1
     return list(DenseGradOperation(self, grad_ys[0]).outputs)
 
 
@@ -391,19 +407,18 @@ class DenseGradOperation(mtf.Operation):
     from mesh_amd import fp8_hip
     dy, x, kernel, y = self.inputs
     k, n = kernel.shape.to_integer_list
+    a_columns = self._forward.take_columns(lowering).reshape(1, k)
     w_rows = lowering.variables[kernel.operation].eight_bit("rows")
     relu = self._relu and not self._dy_is_masked
-    dtype = kernel.dtype
+    dtype, x_sizes = kernel.dtype, x.shape.to_integer_list
 
-    def fn(dy, x, y):
-      a_columns = fp8_hip.quantize(x.contiguous().reshape(1, -1, k), rows=False,
-                                   columns=True)
+    def fn(dy, y):
       dx, dw = fp8_hip.expert_linear_backward(
           a_columns, dy.contiguous().reshape(1, -1, n), w_rows,
           relu_mask=y.contiguous().reshape(1, -1, n) if relu else None)
-      return dx.reshape(x.shape), dw.reshape(k, n).to(dtype)
+      return dx.reshape(x_sizes), dw.reshape(k, n).to(dtype)
     dx, dw = lowering.mesh_impl(self).slicewise(
-        fn, *[lowering.tensors[t] for t in (dy, x, y)])
+        fn, *[lowering.tensors[t] for t in (dy, y)])
     self._set_dx(lowering, dx)
     lowering.set_tensor_lowering(self._dw, dw)
 

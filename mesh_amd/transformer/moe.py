@@ -564,17 +564,21 @@ class MoEV1Operation(mtf.Operation):
     return True
 
   def _eight_bit_experts(self, lowering):
-    """expert_in [E, R, M] -> (y [E, R, N], the hidden tensor where a gradient reads
-    it)."""
+    """expert_in [E, R, M] -> (y [E, R, N], what a gradient reads: the hidden tensor and
+    the columns of the input and of the hidden tensor)."""
     wi, wo = [lowering.variables[t.operation].eight_bit("columns")
               for t in self.inputs[2:4]]
     keep = self._save_for_backward
 
     def fn(expert_in):
-      h = fp8_hip.expert_linear(fp8_hip.quantize(expert_in), wi, self._activation,
-                                eight_bit=not keep)
-      return (fp8_hip.expert_linear(fp8_hip.quantize(h) if keep else h, wo),
-              h if keep else None)
+      if not keep:
+        h = fp8_hip.expert_linear(fp8_hip.quantize(expert_in), wi, self._activation,
+                                  eight_bit=True)
+        return fp8_hip.expert_linear(h, wo), ()
+      a, a_columns = fp8_hip.quantize(expert_in, columns=True)
+      h = fp8_hip.expert_linear(a, wi, self._activation)
+      hq, h_columns = fp8_hip.quantize(h, columns=True)
+      return fp8_hip.expert_linear(hq, wo), (h, a_columns, h_columns)
     return fn
 
   def lower(self, lowering):
@@ -678,7 +682,11 @@ class MoEV1Operation(mtf.Operation):
                      else moe_hip.dispatch(xg, r))
         expert_in = expert_in.reshape(e_, groups * c_, m_)
       if experts is not None:
-        y, h = experts(expert_in)
+        y, kept = experts(expert_in)
+        expert_in = None
+        if save:
+          h = kept[0]
+          saved.update(columns=kept[1:])
       elif y is None and plain_hidden:
         h = None
         if save or kwo_p is not None:
@@ -851,9 +859,7 @@ class MoEV1GradOperation(mtf.Operation):
             keep_prob=fwd._hidden_keep_prob)
         dkwo, dwis = None, [dwi]
       elif fwd._eight_bit:
-        a_columns, h_columns = [
-            fp8_hip.quantize(t.reshape(e_, groups * c_, -1), rows=False, columns=True)
-            for t in (sv["expert_in"], sv["h"])]
+        a_columns, h_columns = sv["columns"]
         dh, dwo = fp8_hip.expert_linear_backward(
             h_columns, dy.reshape(e_, groups * c_, n_), wo_s)
         dxe, dwi = fp8_hip.expert_linear_backward(
