@@ -403,6 +403,14 @@ def _packed(lowering, kernel_tensor, dtype):
   return lowering.variables[kernel_tensor.operation].packed(dtype)
 
 
+def _compact_rows(r):
+  """Where the occupied slots of a Routing go at the front of every expert's rows:
+  (row_offsets [E, G], rows per expert [E])."""
+  used = r.fill.t()
+  ends = torch.cumsum(used, 1, dtype=torch.int32)
+  return (ends - used).contiguous(), ends[:, -1].contiguous()
+
+
 def _release_saved(saved):
   """Called by a gradient operation when it has run: the activations the
   forward operation kept for it (several GiB at the largest benchmark layer)
@@ -564,21 +572,23 @@ class MoEV1Operation(mtf.Operation):
     return True
 
   def _eight_bit_experts(self, lowering):
-    """expert_in [E, R, M] -> (y [E, R, N], what a gradient reads: the hidden tensor and
-    the columns of the input and of the hidden tensor)."""
+    """expert_in [E, R, M], rows per expert [E] (or None) -> (y [E, R, N], what a
+    gradient reads: the hidden tensor and the columns of the input and of the hidden
+    tensor)."""
     wi, wo = [lowering.variables[t.operation].eight_bit("columns")
               for t in self.inputs[2:4]]
     keep = self._save_for_backward
 
-    def fn(expert_in):
+    def fn(expert_in, count):
+      counted = {"row_count": count}
       if not keep:
-        h = fp8_hip.expert_linear(fp8_hip.quantize(expert_in), wi, self._activation,
-                                  eight_bit=True)
-        return fp8_hip.expert_linear(h, wo), ()
-      a, a_columns = fp8_hip.quantize(expert_in, columns=True)
-      h = fp8_hip.expert_linear(a, wi, self._activation)
-      hq, h_columns = fp8_hip.quantize(h, columns=True)
-      return fp8_hip.expert_linear(hq, wo), (h, a_columns, h_columns)
+        a = fp8_hip.quantize(expert_in, **counted)
+        h = fp8_hip.expert_linear(a, wi, self._activation, eight_bit=True, **counted)
+        return fp8_hip.expert_linear(h, wo, **counted), ()
+      a, a_columns = fp8_hip.quantize(expert_in, columns=True, **counted)
+      h = fp8_hip.expert_linear(a, wi, self._activation, **counted)
+      hq, h_columns = fp8_hip.quantize(h, columns=True, **counted)
+      return fp8_hip.expert_linear(hq, wo, **counted), (h, a_columns, h_columns)
     return fn
 
   def lower(self, lowering):
@@ -677,16 +687,20 @@ class MoEV1Operation(mtf.Operation):
         # expert GEMM where the library can
         y = moe_hip.dispatched_expert_ffn(xg, r, wi_p, wo_p,
                                           self._activation)
+      count = None
+      if experts is not None and not by_slot and (
+          self._gating.router != "top_2" or moe_hip.top2_compacts(groups, c_)):
+        row_offsets, count = _compact_rows(r)
       if y is None:
         expert_in = (moe_hip.slot_dispatch(xg, r) if by_slot
-                     else moe_hip.dispatch(xg, r))
+                     else moe_hip.dispatch(xg, r, row_offsets=row_offsets))
         expert_in = expert_in.reshape(e_, groups * c_, m_)
       if experts is not None:
-        y, kept = experts(expert_in)
+        y, kept = experts(expert_in, count)
         expert_in = None
         if save:
           h = kept[0]
-          saved.update(columns=kept[1:])
+          saved.update(columns=kept[1:], row_count=count)
       elif y is None and plain_hidden:
         h = None
         if save or kwo_p is not None:
@@ -851,20 +865,21 @@ class MoEV1GradOperation(mtf.Operation):
       dy, dgate = combine_backward(
           dout_s.reshape(groups, s_, n_).contiguous(),
           sv["y"].reshape(e_, groups, c_, n_), r, **compact)
-      if row_offsets is not None:
+      if fwd._eight_bit:
+        a_columns, h_columns = sv["columns"]
+        count = sv["row_count"]
+        dh, dwo = fp8_hip.expert_linear_backward(
+            h_columns, dy.reshape(e_, groups * c_, n_), wo_s, row_count=count)
+        dxe, dwi = fp8_hip.expert_linear_backward(
+            a_columns, dh, wi_s,
+            relu_mask=sv["h"] if fwd._activation == "relu" else None, row_count=count)
+        dkwo, dwis = None, [dwi]
+      elif row_offsets is not None:
         dxe, dwi, dwo = moe_hip.compact_expert_ffn_backward(
             sv["expert_in"].reshape(e_, groups * c_, m_), sv["h"],
             dy.reshape(e_, groups * c_, n_), wi_s, wo_s, r, row_offsets,
             fwd._activation, dh_scale=sv["hidden_noise"],
             keep_prob=fwd._hidden_keep_prob)
-        dkwo, dwis = None, [dwi]
-      elif fwd._eight_bit:
-        a_columns, h_columns = sv["columns"]
-        dh, dwo = fp8_hip.expert_linear_backward(
-            h_columns, dy.reshape(e_, groups * c_, n_), wo_s)
-        dxe, dwi = fp8_hip.expert_linear_backward(
-            a_columns, dh, wi_s,
-            relu_mask=sv["h"] if fwd._activation == "relu" else None)
         dkwo, dwis = None, [dwi]
       elif fwd._general_hidden:
         dys, wos = [dy.reshape(e_, groups * c_, n_)], [wo_s]

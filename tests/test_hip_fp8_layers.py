@@ -224,7 +224,7 @@ def _error(got, exact):
   return float(((got - exact).square().mean() / exact.square().mean()).sqrt())
 
 
-@pytest.mark.parametrize("gating", ["top_2", "switch", "expert_selection"])
+@pytest.mark.parametrize("gating", ["top_2", "switch", "ntlb", "expert_selection"])
 @pytest.mark.parametrize("activation", ["relu", "gelu"])
 def test_experts(hip, gating, activation):
   """The layer against the one in bfloat16: the same routing, and two products whose
@@ -242,12 +242,17 @@ def test_experts(hip, gating, activation):
   given = _normal(9, sizes[:3]).to(BF16)
   lowering.run({x: given})
   eager = lowering.export_to_tf_tensor(y).clone()
-  for _ in range(3):
-    step.replay({x: given})
-    assert torch.equal(lowering.export_to_tf_tensor(y), eager)
+  for i in range(4):
+    other = _normal(10 + i, sizes[:3]).to(BF16)
+    step.replay({x: other})
+    replayed = lowering.export_to_tf_tensor(y).clone()
+    lowering.run({x: other})
+    assert torch.equal(replayed, lowering.export_to_tf_tensor(y))
+  step.replay({x: given})
+  assert torch.equal(lowering.export_to_tf_tensor(y), eager)
 
 
-@pytest.mark.parametrize("gating", ["top_2", "switch"])
+@pytest.mark.parametrize("gating", ["top_2", "switch", "ntlb"])
 def test_gradients_of_experts(hip, gating):
   """dx, dwi and dwo against those of the bfloat16 layer; the router's gradient reads the
   experts' outputs, which are as far apart as the products make them.  (Where the two
