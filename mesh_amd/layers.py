@@ -194,6 +194,12 @@ def _rows_of(lowering, tensor):
   return lowering.tensors[tensor].to_laid_out_tensor().tensor_list[0]
 
 
+def only_eight_bit_dense_reads(tensor):
+  readers = [op for op in tensor.graph.operations if tensor in op.inputs]
+  return (len(readers) == 1 and isinstance(readers[0], DenseOperation) and
+          readers[0].eight_bit)
+
+
 class DenseOperation(mtf.Operation):
   """y = activation(x . kernel) over the last dim of x: the einsum (+ relu) of
   mtf.layers.dense without bias (mesh_tensorflow/layers.py:112-160) as one
@@ -239,12 +245,9 @@ class DenseOperation(mtf.Operation):
   def _hands_over(self):
     """Whether nothing but the next 8-bit product reads the result, which then leaves
     as its operand."""
-    operations, y = self.graph.operations, self.outputs[0]
-    if self._handed_over[0] != len(operations):
-      readers = [op for op in operations if y in op.inputs]
-      self._handed_over = (len(operations), len(readers) == 1 and
-                           isinstance(readers[0], DenseOperation) and
-                           readers[0].eight_bit)
+    count = len(self.graph.operations)
+    if self._handed_over[0] != count:
+      self._handed_over = (count, only_eight_bit_dense_reads(self.outputs[0]))
     return self._handed_over[1]
 
   def _lower_eight_bit(self, lowering):

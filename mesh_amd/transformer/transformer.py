@@ -179,11 +179,58 @@ class RmsNormOperation(mtf.Operation):
                        % (scale.shape, x.shape))
     self._epsilon = float(epsilon)
     self._outputs = [mtf.Tensor(self, x.shape, x.dtype)]
+    self._handed_over = (0, False)
     self.mask = None         # the MaskPaddingOperation of the result
     residual = x.operation
     if (isinstance(residual, ResidualAddOperation) and residual.norm is None and
         (isinstance(scale.operation, mtf.Variable) or _is_ahead(scale, residual))):
       residual.norm = self
+
+  def _hands_over(self):
+    """Whether nothing but an 8-bit dense layer reads the (masked) norm, which then
+    leaves as its operand."""
+    count, mask, y = len(self.graph.operations), self.mask, self.outputs[0]
+    if self._handed_over[0] != count:
+      over = mtf_layers.only_eight_bit_dense_reads(y if mask is None
+                                                   else mask.outputs[0])
+      if mask is not None:
+        over = over and [mask] == [op for op in self.graph.operations if y in op.inputs]
+      self._handed_over = (count, over)
+    return self._handed_over[1]
+
+  def _lower_to_eight_bits(self, lowering, residual):
+    """lower_with() into the operand of an 8-bit dense layer."""
+    from mesh_amd import fp8_hip
+    x, scale = self.inputs
+    mask, eps = self.mask, self._epsilon
+    if scale not in lowering.tensors or not self._hands_over():
+      return False
+    ins = residual.inputs if residual is not None else [x]
+    rows = [_slice_of(lowering, t).contiguous() for t in ins]
+    w = _slice_of(lowering, scale).contiguous()
+    if w.dtype != rows[0].dtype or rows[0].numel() == 0:
+      return False
+    row_mask = None if mask is None else _slice_of(lowering, mask.inputs[1]).contiguous()
+    mesh_impl = lowering.mesh_impl(self)
+    total, operand = [t.tensor_list[0] for t in mesh_impl.slicewise(
+        lambda: fp8_hip.residual_rms_norm(
+            rows[0], rows[1] if residual is not None else None, w, eps, row_mask))]
+    # (whoever else asks for the tensors sees the values that are multiplied, or the
+    # norm without its mask)
+    y = self.outputs[0] if mask is None else mask.outputs[0]
+    lowering.run_values[y] = operand
+    sizes = y.shape.to_integer_list
+    lowering.set_tensor_lowering(y, mesh_impl.LazyLaidOutTensor(
+        lambda: mesh_impl.slicewise(lambda: fp8_hip.dequantize(operand)), sizes))
+    if mask is not None:
+      laid_out = mesh_impl.LaidOutTensor
+      lowering.set_tensor_lowering(self.outputs[0], mesh_impl.LazyLaidOutTensor(
+          lambda: self._alone(mesh_impl, laid_out([total]), laid_out([w])), sizes))
+      lowering.done_ahead.add(mask)
+    if residual is not None:
+      lowering.set_tensor_lowering(x, mesh_impl.LaidOutTensor([total]))
+      lowering.done_ahead.add(self)
+    return True
 
   def lower_with(self, lowering, residual):
     """Makes this norm, the residual sum in front of it (`residual`, or None: the
@@ -192,6 +239,8 @@ class RmsNormOperation(mtf.Operation):
     from mesh_amd import moe_hip
     x, scale = self.inputs
     mask = self.mask
+    if self._lower_to_eight_bits(lowering, residual):
+      return True
     if scale not in lowering.tensors or (residual is None and mask is None):
       return False
     ins = residual.inputs if residual is not None else [x]

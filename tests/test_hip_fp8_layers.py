@@ -150,11 +150,13 @@ def test_captured_step(hip, with_gradients):
         laid_out.assign(values[var.name])
 
 
-def test_layer_stack(hip):
+@pytest.mark.parametrize("padded", [False, True])
+def test_layer_stack(hip, padded):
   """DenseReluDense in a stack with and without 8-bit operands.  Two operands of a root
   mean square error of at most 2^-4 / sqrt(3) each, in two layers one behind the other,
-  half of whose result the residual is."""
-  del hip
+  half of whose result the residual is.  Norms leave as operands: nothing is quantized
+  on the way."""
+  from mesh_amd import moe_hip
   b, l, m, f = 2, 70, 256, 1024
   results = []
   for eight_bit in (False, True):
@@ -167,15 +169,44 @@ def test_layer_stack(hip):
         [(transformer_layers.DenseReluDense, dict(hidden_size=f, eight_bit=eight_bit))],
         num_layers=2)
     model = transformer.Unitransformer(stack, d_model=m, name="encoder")
+    ids = None
+    if padded:
+      ids = torch.ones((b, l), dtype=torch.int32)
+      ids[:, 50:] = 0
+      ids = mtf.import_tf_tensor(mesh, ids, mtf.Shape(dims[:2]))
     y, _ = model.call_layers(
-        x, mtf.VariableDType(torch.float32, torch.float32, BF16), mode="eval")
+        x, mtf.VariableDType(torch.float32, torch.float32, BF16), mode="eval",
+        sequence_id=ids)
     values = {}
     for i, v in enumerate(graph.all_variables):
       sizes = v.shape.to_integer_list
-      values[v.name] = (torch.ones(sizes) if len(sizes) == 1
+      values[v.name] = (1 + 0.1 * _normal(40 + i, sizes) if len(sizes) == 1
                         else _normal(50 + i, sizes, sizes[0] ** -0.5))
     lowering = _lower(graph, mesh, values)
-    results.append(lowering.export_to_tf_tensor(y).double())
+    first = lowering.export_to_tf_tensor(y).clone()
+    with moe_hip.StageTimer() as timer:
+      lowering.run()
+    assert ("fp8_linear" in timer.totals()) == eight_bit
+    assert "fp8_quantize" not in timer.totals()
+    assert torch.equal(lowering.export_to_tf_tensor(y), first)
+    if eight_bit:
+      # the first layer by hand
+      norm = [op for op in graph.operations
+              if isinstance(op, transformer.RmsNormOperation)][0]
+      mask = None
+      if padded:
+        mask = torch.zeros((b, l), dtype=BF16, device="cuda")
+        mask[:, :50] = 1
+      given = lowering.export_to_tf_tensor(norm.inputs[0])
+      scale = lowering.export_to_tf_tensor(norm.inputs[1])
+      _, want = hip.residual_rms_norm(given, None, scale, row_mask=mask)
+      reader = norm.mask or norm
+      assert torch.equal(lowering.export_to_tf_tensor(reader.outputs[0]),
+                         hip.dequantize(want))
+      if padded:
+        assert torch.equal(lowering.export_to_tf_tensor(norm.outputs[0]),
+                           moe_hip.rms_norm(given, scale, 1e-6))
+    results.append(first.double())
   exact, got = results
   error = ((got - exact).square().mean() / exact.square().mean()).sqrt()
   assert 0 < error < 2.0 ** -3.5
