@@ -276,7 +276,9 @@ MANY = [(16, 1100, 300, 1030), (8, 2000, 400, 1032), (40, 300, 384, 520),
         (64, 200, 256, 1000), (16, 300, 256, 1030), (32, 260, 256, 1032),
         (4, 500, 3100, 300), (1, 200, 2300, 640), (1, 1000, 8192, 520),
         (1, 40, 4096, 300), (32, 24, 1024, 1030), (1, 24, 11080, 1500),
-        (16, 1100, 128, 1030), (16, 300, 100, 1032), (64, 60, 77, 520)]
+        (16, 1100, 128, 1030), (16, 300, 100, 1032), (64, 60, 77, 520),
+        (16, 1100, 4200, 1030), (8, 1100, 8192, 2056), (8, 1100, 8200, 1030),
+        (16, 600, 8300, 1032)]
 
 
 def _random(hip, shape, std, seed):
@@ -328,7 +330,8 @@ def test_expert_linear_of_many_tiles(hip, e, r, k, n):
 @pytest.mark.parametrize("e,r,k,n", [(40, 384, 300, 520), (16, 384, 300, 1030),
                                      (24, 900, 300, 1030), (6, 700, 1300, 256),
                                      (2, 1000, 520, 1024), (24, 100, 600, 1030),
-                                     (8, 128, 300, 100)])
+                                     (8, 128, 300, 100), (16, 4400, 600, 1030),
+                                     (8, 8200, 1100, 1030)])
 def test_gradients_of_counted_rows(hip, e, r, k, n):
   """Experts with none, one, a block, a block and one, and all of their rows."""
   count = torch.tensor([(0, 1, 128, 129, r, r - 1, 257)[i % 7] for i in range(e)],
