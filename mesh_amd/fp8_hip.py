@@ -135,14 +135,6 @@ class Fp8Blocks(object):
     return Fp8Blocks.__new__(Fp8Blocks)._set(
         values, scales, tuple(values.shape[:-1]) + self._shape[-1:])
 
-  def copy_(self, other):
-    """Takes the contents of an operand of the same shape."""
-    if other.shape != self._shape:
-      raise ValueError("shape %s, expected %s" % (other.shape, self._shape))
-    self._values.view(torch.uint8).copy_(other.values.view(torch.uint8))
-    self._scales.copy_(other.scales)
-    return self
-
   def __repr__(self):
     return "Fp8Blocks%s" % (self.shape,)
 
@@ -206,11 +198,12 @@ _check = moe_hip._check    # pylint: disable=protected-access
 _stream = moe_hip._stream  # pylint: disable=protected-access
 
 
-def quantize(x, rows=True, columns=False, relu_mask=None, row_count=None):
+def quantize(x, rows=True, columns=False, relu_mask=None, row_count=None, out=None):
   """x [E, R, K] (or [R, K]) as 8-bit operands, in one pass over it: its rows
   [E, R, K], for products over K, its columns [E, K, R], for products over R, or both.
   relu_mask (shape and dtype of x): elements whose mask is not positive count as 0.
-  row_count [E] int32: rows of an expert from its count on count as zeros.
+  row_count [E] int32: rows of an expert from its count on count as zeros.  out: the
+  operand, or the pair, to write to instead of new ones.
   -> the one operand asked for, or (rows, columns)
 
   The columns of a weight [E, K, N] are what expert_linear multiplies by (as
@@ -224,17 +217,26 @@ def quantize(x, rows=True, columns=False, relu_mask=None, row_count=None):
   sizes = tuple(x.shape)
   e, r, k = (1,) * (3 - x.dim()) + sizes
   code = moe_hip.dtype_code(x.dtype)
-  by_row = Fp8Blocks.empty(sizes, x.device) if rows else None
-  by_column = (Fp8Blocks.empty(sizes[:-2] + (k, r), x.device)
-               if columns else None)
+  turned = sizes[:-2] + (k, r)
+  by_row = by_column = None
+  if out is None:
+    if rows:
+      by_row = Fp8Blocks.empty(sizes, x.device)
+    if columns:
+      by_column = Fp8Blocks.empty(turned, x.device)
+    outs = _pointers(by_row) + _pointers(by_column)
+  else:
+    by_row, by_column = (out if rows and columns else (out, None) if rows
+                         else (None, out))
+    outs = ((_operand(by_row, "rows", sizes) if rows else (None, None)) +
+            (_operand(by_column, "columns", turned) if columns else (None, None)))
   xp = _dev(x, "x")
   mp = None if relu_mask is None else _dev(relu_mask, "relu_mask", x.dtype, sizes)
   cp = _counts(row_count, e)
   if x.numel():
     with _stage("fp8_quantize"):
       _check(lib.mesh_moe_fp8_quantize(
-          xp, mp, cp, *_pointers(by_row), *_pointers(by_column), e, r, k, code,
-          _stream()), "fp8_quantize")
+          xp, mp, cp, *outs, e, r, k, code, _stream()), "fp8_quantize")
   return (by_row, by_column) if rows and columns else by_row if rows else by_column
 
 

@@ -166,12 +166,14 @@ class HipMeshImpl(mtf.MeshImpl):
       for (kind, dtype), t in self._derived.items():
         if kind == "act":
           t.copy_(self._slice)
-        elif kind == "eight_bit":
-          t.copy_(self._as_eight_bit(dtype))
-        else:
+        elif kind == "packed":
           s = self._slice
           moe_hip.pack_weights(s.reshape(-1, s.shape[-2], s.shape[-1]), dtype,
                                out=t)
+      made = [self._derived.get(("eight_bit", which)) for which in ("rows", "columns")]
+      if any(made):
+        self._as_eight_bit(*[q is not None for q in made],
+                           out=made if all(made) else made[0] or made[1])
 
     def activation_tensor(self):
       """Slice cast to the activation dtype (Variable.lower,
@@ -193,18 +195,17 @@ class HipMeshImpl(mtf.MeshImpl):
         self._derived[key] = moe_hip.pack_weights(s.reshape(-1, k, n), dtype)
       return self._derived[key]
 
-    def _as_eight_bit(self, which):
+    def _as_eight_bit(self, rows, columns, out=None):
       kernels = self._slice.reshape(-1, *self._slice.shape[-2:])
       with torch.cuda.device(kernels.device):
-        return fp8_hip.quantize(kernels, rows=which == "rows",
-                                columns=which == "columns")
+        return fp8_hip.quantize(kernels, rows, columns, out=out)
 
     def eight_bit(self, which):
       """[..., K, N] slice as an 8-bit operand of fp8_hip: its "columns" [E, N, K], what
       products multiply by, or its "rows" [E, K, N], what their input gradients do."""
       key = ("eight_bit", which)
       if key not in self._derived:
-        self._derived[key] = self._as_eight_bit(which)
+        self._derived[key] = self._as_eight_bit(which == "rows", which == "columns")
       return self._derived[key]
 
     @staticmethod

@@ -96,6 +96,27 @@ def test_quantize(hip, shape, dtype):
                      columns.values[0].view(torch.uint8))
 
 
+def test_quantize_into_given_operands(hip):
+  rng = np.random.default_rng(4)
+  x = _tensor(rng, (2, 70, 300), "bf16")
+  want = hip.quantize(x, rows=True, columns=True)
+  out = hip.Fp8Blocks.empty((2, 70, 300), "cuda"), hip.Fp8Blocks.empty((2, 300, 70), "cuda")
+  for rows, columns, given in ((True, True, out), (True, False, out[0]),
+                               (False, True, out[1])):
+    for q in out:
+      q.values.view(torch.uint8).fill_(0x55)
+    got = hip.quantize(x, rows, columns, out=given)
+    for g, o, w in zip(got if rows and columns else (got,),
+                       out if rows and columns else (given,),
+                       want if rows and columns else want[:1] if rows else want[1:]):
+      assert g is o
+      assert torch.equal(hip.dequantize(g, torch.float32), hip.dequantize(w, torch.float32))
+  for rows, columns, given in ((True, False, out[1]), (False, True, out[0]),
+                               (True, True, out[::-1])):
+    with pytest.raises(hip.MoeHipError, match="shape"):
+      hip.quantize(x, rows, columns, out=given)
+
+
 def test_quantize_of_many_tiles(hip):
   """Blocks of the grid in the order that keeps an XCD's tiles together."""
   rng = np.random.default_rng(0)
