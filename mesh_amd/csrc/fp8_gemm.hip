@@ -1084,7 +1084,8 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(GemmArgs g, TileGrid g
   // The result of a tile: 32 rows at a time are turned round and leave 16 bytes per lane.
   // Lane l has row l % 16 and the columns 16 j + 4 (l / 16) .. of a piece.  The stores of
   // whole lines go through a buffer that ends with the tile's rows, so that they leave in
-  // any case and the next tile's first wait can count on them.
+  // any case and the next tile's first wait can count on them.  (Rows that are not there
+  // count as none before they are multiplied: up to -59 times a row passes 32 bits.)
   auto write_out = [&](const Tile& t, auto na_tag) FP8_INLINE {
     constexpr int NA = decltype(na_tag)::value;
     const int wfree = wslot == 0 ? 2 : wslot - 1;       // of the last K tile
@@ -1166,7 +1167,7 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(GemmArgs g, TileGrid g
           if (p >= NA) continue;
           store_line(line[n],
                      (uint8_t*)g.y + (first + row_of(p) + 8 * (n & 1)) * row_bytes + col0,
-                     col0 < g.N ? min(left, 8) * row_bytes - col0 : 0, at);
+                     col0 < g.N ? max(min(left, 8), 0) * row_bytes - col0 : 0, at);
         }
       } else {
         // Rows of 256 bytes, 4 to a kilobyte; the 8 bytes of unit u (4 columns) of row r
@@ -1199,7 +1200,7 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(GemmArgs g, TileGrid g
 #pragma unroll
           for (int n = 0; n < 4; ++n)
             store_line(line[n], (uint8_t*)g.y + (row + 4 * n) * row_bytes + 2 * col0,
-                       min(rows - 4 * n, 4) * row_bytes - 2 * col0, at);
+                       max(min(rows - 4 * n, 4), 0) * row_bytes - 2 * col0, at);
         } else {
           // rows that do not start on 16 bytes: a column per lane
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");

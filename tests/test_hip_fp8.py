@@ -692,6 +692,40 @@ def test_beyond_2_to_the_31_elements(hip):
   assert dw_rows.shape == (1, 17000, 300)
 
 
+@pytest.mark.parametrize("eight_bit,n", [(False, 20070400), (True, 40140800)])
+def test_wide_results_stay_in_their_rows(hip, eight_bit, n):
+  """One row whose bytes times the rows that a tile could hold pass 32 bits: the other
+  rows of the buffer that the result is the first row of stay as they were."""
+  period, k, rows = 1024, 256, 128
+  a, av = _random(hip, (1, 1, k), 1.0, 1)
+  w, wv = _random(hip, (1, period, k), k ** -0.5, 2)
+  wide = hip.Fp8Blocks(
+      w.values.view(torch.uint8).repeat(1, n // period, 1).view(torch.float8_e4m3fn),
+      w.scales.repeat(1, n // period, 1), k)
+  if eight_bit:
+    buffer = torch.full((rows, n), 0x55, dtype=torch.uint8, device="cuda")
+    scales = torch.full((rows, hip.scale_bytes(n)), 99, dtype=torch.uint8, device="cuda")
+    out = hip.Fp8Blocks(buffer[None, :1].view(torch.float8_e4m3fn), scales[None, :1], n)
+    hip.expert_linear(a, wide, eight_bit=True, out=out)
+    assert (scales[1:] == 99).all()
+    y = hip.dequantize(out, torch.float32)
+  else:
+    buffer = torch.full((rows, n), 0x5555, dtype=torch.int16, device="cuda")
+    y = hip.expert_linear(a, wide, out=buffer[None, :1].view(torch.bfloat16))
+  assert (buffer[1:] == buffer[1, 0]).all() and buffer[1, 0] % 256 == 0x55
+  y = y.view(-1, period)
+  assert torch.equal(y, y[:1].expand_as(y))
+  wt = wv[0].t().contiguous()
+  want, magnitudes = av[0] @ wt, av[0].abs() @ wt.abs()
+  if eight_bit:
+    # (half a step of e4m3, or of its least numbers under the block's unit)
+    top = want.abs().view(-1, 128).amax(-1, keepdim=True).expand(-1, 128).reshape(1, -1)
+    assert ((y[:1].double() - want).abs() <= want.abs() * 2.0 ** -4 + top * 2.0 ** -17 +
+            magnitudes * 2.0 ** -13 * (1 + 2.0 ** -4)).all()
+  else:
+    assert _near(y[:1], want, magnitudes)
+
+
 @pytest.mark.parametrize("rows", [1, 300])
 def test_captured(hip, rows):
   """The block recorded into a graph, replayed with new inputs and work between the
