@@ -17,25 +17,29 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 // The activations as the products apply them to their float32 sums; NaN stays NaN.  All
-// but relu are (n0 + n1 v) / (1 + exp(v (k1 + k3 v^2))) + off with constants of the
+// but relu are (n0 or v) / (1 + exp(v (k1 + k3 v^2))) + off with constants of the
 // activation: 0.5 (1 + tanh u) = 1 / (1 + exp(-2 u)), tanh v = 2 / (1 + exp(-2 v)) - 1,
-// the latter by its series where the difference would lose bits.  The hardware's
-// exponential and reciprocal are off by 2^-21 or so (relative, for arguments that
-// matter), far below the rounding of the result.
+// the latter by its series where the difference would lose bits.  v^2 is kept finite and
+// the numerator chosen: 0 times an infinity would be NaN, where only gelu has a k3 and
+// sigmoid and tanh no v.  (gelu and swish of -infinity are NaN, as an infinity divided by
+// one is.)  The hardware's exponential and reciprocal are off by 2^-21 or so (relative,
+// for arguments that matter; results below 2^-119 may become zeros), far below the
+// rounding of the result.
 struct Fp8Act {
-  float n0, n1, k1, k3, off, near;
+  float n0, k1, k3, off, near;
+  bool times_v;
   __device__ __forceinline__ explicit Fp8Act(int act) {
     const bool tanh = act == MESH_MOE_ACT_TANH, gelu = act == MESH_MOE_ACT_GELU;
-    n0 = tanh ? 2.f : act == MESH_MOE_ACT_SIGMOID ? 1.f : 0.f;
-    n1 = gelu || act == MESH_MOE_ACT_SWISH ? 1.f : 0.f;
+    n0 = tanh ? 2.f : 1.f;
+    times_v = gelu || act == MESH_MOE_ACT_SWISH;
     k1 = gelu ? -1.5957691216057308f : tanh ? -2.f : -1.f;
     k3 = gelu ? -1.5957691216057308f * 0.044715f : 0.f;
     off = tanh ? -1.f : 0.f;
     near = tanh ? 4e-4f : 0.f;
   }
   __device__ __forceinline__ float operator()(float v) const {
-    const float v2 = v * v;
-    const float y = (n0 + n1 * v) *
+    const float v2 = fminf(v * v, 3e38f);
+    const float y = (times_v ? v : n0) *
                         __builtin_amdgcn_rcpf(1.f + __expf(v * (k1 + k3 * v2))) + off;
     const float series = v - v * v2 * 0.33333334f;
     return v2 < near ? series : y;

@@ -387,6 +387,55 @@ def test_activations(hip, activation, r):
                   1.13 * (np.abs(av) @ np.abs(wv)))
 
 
+# of the few rows' kernel, of the one for one block, of 64-row tiles with and without a
+# split reduction, of 128- and 256-row tiles
+@pytest.mark.parametrize("e,r,k,n", [(30, 16, 256, 40), (480, 1, 64, 200),
+                                     (1, 480, 256, 40), (1, 480, 4096, 200),
+                                     (1, 480, 512, 16384), (8, 60, 512, 40000)])
+@pytest.mark.parametrize("activation", ["relu", "gelu", "sigmoid", "tanh", "swish"])
+def test_activations_of_all_magnitudes(hip, activation, e, r, k, n):
+  """Sums from 2^-110 to 2^127, of either sign, and infinite ones: every row has one
+  value, which every column takes as it is.  The sums are exact here; results are off by
+  half a step, by 2^-13 from the exponential, and by 2^-118 where they are next to
+  nothing."""
+  p = np.arange(480) // 2 - 110
+  codes, scales = np.zeros((480, hip.row_bytes(k)), np.uint8), np.full(
+      (480, hip.scale_bytes(k)), 127, np.uint8)
+  # 1.5 in e4m3 is 0x3c; units go up to 2^120
+  codes[:, 0] = 0x3c + 8 * np.clip(p - 120, 0, 7) + 128 * (np.arange(480) % 2)
+  codes[:, 1] = np.where(p > 127, codes[:, 0], 0)         # twice 1.5 * 2^127
+  scales[:, 0] = np.minimum(p, 120) + 127
+  v = F.value(codes, scales)[:, :2].sum(-1, keepdims=True)
+  v = np.where(np.abs(v) < 2.0 ** 128, v, np.copysign(np.inf, v))
+  assert np.isinf(v).sum() == 4
+  a = hip.Fp8Blocks(
+      torch.from_numpy(codes).view(torch.float8_e4m3fn).cuda().reshape(e, r, -1),
+      torch.from_numpy(scales).cuda().reshape(e, r, -1), k)
+  w = hip.Fp8Blocks.empty((e, n, k), "cuda")
+  w.values.view(torch.uint8).zero_()
+  w.values.view(torch.uint8)[..., :2] = 0x38              # 1.0
+  w.scales.fill_(127)
+  with np.errstate(all="ignore"):
+    want = _act(v, activation)                            # [480, 1]
+  ends = np.isfinite(want[:, 0])
+  got = hip.expert_linear(a, w, activation).reshape(480, n)
+  assert torch.equal(got.isnan(), got[:, :1].isnan().expand_as(got))
+  assert torch.equal(got.nan_to_num(0.5), got[:, :1].nan_to_num(0.5).expand_as(got))
+  got = _f64(got[:, :1])
+  np.testing.assert_array_equal(got[~ends], want[~ends])
+  assert (np.abs(got[ends] - want[ends]) <= np.abs(want[ends]) * (2.0 ** -8 + 2.0 ** -13) +
+          2.0 ** -118).all()
+  q = hip.expert_linear(a, w, activation, eight_bit=True).reshape(480)
+  # (columns are alike: the first block, rows with an infinity being NaN)
+  first = [t.view(torch.uint8)[:, :m] for t, m in ((q.values, 128), (q.scales, 4))]
+  def rows(which):
+    values, scales = (t[torch.from_numpy(which).cuda()] for t in first)
+    return hip.Fp8Blocks(values.view(torch.float8_e4m3fn), scales, min(n, 128))
+  assert np.isnan(F.operand_value(rows(~ends))).all()
+  finite = rows(ends)
+  _assert_rounded(finite, np.broadcast_to(want[ends], finite.shape), 2.0 ** -12)
+
+
 @pytest.mark.parametrize("eight_bit", [False, True])
 @pytest.mark.parametrize("r,n", [(6, 200), (70, 128), (300, 256), (600, 392)])
 def test_row_counts(hip, r, n, eight_bit):
