@@ -29,10 +29,11 @@ __device__ __forceinline__ void store_piece(T* at, uint4 v) {
 
 // 8 neighbouring values of a row from column `at` on, zeros from `end` on.  ALIGNED:
 // every row's pieces of 16 bytes lie on 16 bytes, and `end` is a multiple of 8.  ONCE:
-// nothing reads them again.
+// nothing reads them again.  (`at` goes up to 2^31 - 8, so nothing is added to it before
+// it is known to be below `end`.)
 template <typename T, bool ALIGNED, bool ONCE = true>
 __device__ __forceinline__ void load8(const T* row, int at, int end, float (&v)[8]) {
-  if (ALIGNED ? at < end : at + 8 <= end) {
+  if (ALIGNED ? at < end : at <= end - 8) {
     if constexpr (sizeof(T) == 2) {
       unpack16(load_piece<T, ONCE>(row + at), v, T());
     } else {
@@ -55,7 +56,7 @@ __device__ __forceinline__ void load8(const T* row, int at, int end, float (&v)[
 
 template <typename T, bool ALIGNED>
 __device__ __forceinline__ void store8(T* row, int at, int end, const float (&v)[8]) {
-  if (ALIGNED ? at < end : at + 8 <= end) {
+  if (ALIGNED ? at < end : at <= end - 8) {
     if constexpr (sizeof(T) == 2) {
       store_piece(row + at, pack16(v, T()));
     } else {

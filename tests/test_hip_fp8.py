@@ -243,6 +243,22 @@ def test_residual_rms_norm_of_odd_rows(hip):
   assert torch.equal(y.values.view(torch.uint8), again[1].values.view(torch.uint8))
 
 
+def test_residual_rms_norm_of_the_widest_row(hip):
+  """A row whose last step's columns reach 2^31: what lies behind it is not read.  Every
+  sum is 1 and the norm of ones is one, whose code is 256 under the unit 2^-8."""
+  m = 0x7ffffefd
+  x, residual = (torch.full((m + 300,), 0.5, dtype=torch.bfloat16, device="cuda")
+                 for _ in range(2))
+  x[m:], residual[m:] = float("nan"), float("nan")
+  scale = torch.ones(m, dtype=torch.bfloat16, device="cuda")
+  total, y = hip.residual_rms_norm(x[:m].view(1, m), residual[:m].view(1, m), scale, 0.0)
+  assert (total == 1).all()
+  del x, residual, scale, total
+  codes = y.values.view(torch.uint8)[0]
+  assert (codes[:m] == 0x78).all() and (codes[m:] == 0).all()
+  assert (y.scales[0, :hip.row_bytes(m) // 128] == 127 - 8).all()
+
+
 # --- products ---------------------------------------------------------------
 def _act(y, activation):
   if activation == "relu":
