@@ -26,6 +26,8 @@
  * (scale byte 127).
  * Products take scale bytes from 10 (which is -117) on, 255 making a block NaN; blocks
  * with a byte below, which no call here makes, they may count as zeros.
+ * What a launch of 2^32 threads cannot cover (8 million tiles of few rows, 16 million
+ * tiles of 128 x 128 to quantize) is refused, MESH_MOE_E_UNSUPPORTED.
  *
  * The reference has no 8-bit arithmetic; the calls are forms of what it does in
  * float32 or bfloat16, which is named at each.
@@ -40,7 +42,7 @@ extern "C" {
 #endif
 
 /* (counted up with every change of a declaration, and of what a call accepts) */
-#define MESH_MOE_FP8_ABI_VERSION 1
+#define MESH_MOE_FP8_ABI_VERSION 2
 
 int mesh_moe_fp8_abi_version(void);
 

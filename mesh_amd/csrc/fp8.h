@@ -8,6 +8,7 @@ namespace mesh_moe {
 
 constexpr int FP8_BLOCK = 128;    // values that share a scale
 constexpr int FP8_UNIT = 127;     // the scale byte of 2^0
+constexpr int64_t MAX_THREADS = 0xffffffffLL;   // of a launch, in one dimension
 
 // bytes of a row of K values, and of its scales
 __host__ __device__ __forceinline__ int64_t fp8_row_bytes(int K) {

@@ -2,6 +2,9 @@
 // (The products are in fp8_gemm.hip.)
 #include "fp8.h"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace mesh_moe {
 
 // Pieces of 16 bytes that lie on a T: the hardware takes any address.  (Rows and columns
@@ -222,11 +225,13 @@ static int run_quantize(const T* x, const T* relu_mask, const int32_t* row_count
   o.tiles_k = (int)(((int64_t)K + QT - 1) / QT);
   o.groups_k = (o.tiles_k + 3) / 4;
   o.groups = (int64_t)((o.tiles_r + 3) / 4) * o.groups_k;
+  // (in multiples of 128 the limit is one, too; divided, not to pass 64 bits)
+  constexpr int64_t most = MAX_THREADS / 256 / 128 * 128;
+  MOE_REQUIRE(o.groups <= most / 16 / E, MESH_MOE_E_UNSUPPORTED,
+              "fp8_quantize: too many tiles (E=%d R=%d K=%d)", E, R, K);
   int64_t blocks = o.groups * E * 16;
   o.by_xcd = blocks >= 1024;
   if (o.by_xcd) blocks = (blocks + 127) / 128 * 128;
-  MOE_REQUIRE(blocks <= 0x7fffffffLL, MESH_MOE_E_UNSUPPORTED,
-              "fp8_quantize: too many tiles (E=%d R=%d K=%d)", E, R, K);
   const bool aligned =
       K % 8 == 0 && ((uintptr_t)x | (uintptr_t)relu_mask) % 16 == 0;
   auto kernel = aligned ? fp8_quantize_kernel<T, true> : fp8_quantize_kernel<T, false>;
@@ -446,22 +451,48 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void fp8_rms_norm_kernel(
   }
 }
 
+// rows `row` .. row + rows - 1 of a norm
+template <typename T>
+static NormArgs norm_rows(const NormArgs& a, int64_t row, int64_t rows) {
+  NormArgs p = a;
+  auto skip = [&](auto& at, int64_t bytes) {
+    if (at != nullptr) at = (std::remove_reference_t<decltype(at)>)((uint8_t*)at + bytes);
+  };
+  const int64_t line = row * a.M * (int64_t)sizeof(T);
+  skip(p.x, line);
+  skip(p.residual, line);
+  skip(p.sum, line);
+  skip(p.norm, line);
+  skip(p.row_mask, row * (int64_t)sizeof(T));
+  skip(p.values, row * fp8_row_bytes(a.M));
+  skip(p.scales, row * fp8_scale_bytes(a.M));
+  p.rows = rows;
+  return p;
+}
+
 template <typename T, bool ALIGNED>
 static void launch_norm(const NormArgs& a, hipStream_t st) {
   const int64_t mp = fp8_row_bytes(a.M);
-  const unsigned quarter = (unsigned)((a.rows + 3) / 4), whole = (unsigned)a.rows;
+  // (a launch has MAX_THREADS threads at most: 67 million rows of one wavefront)
+  auto launch = [&](auto kernel, int threads, int per_block) {
+    const int64_t most = MAX_THREADS / threads * per_block;
+    for (int64_t row = 0; row < a.rows; row += most) {
+      const NormArgs p = norm_rows<T>(a, row, std::min(most, a.rows - row));
+      kernel<<<(unsigned)((p.rows + per_block - 1) / per_block), threads, 0, st>>>(p);
+    }
+  };
   if (mp <= 1024)
-    fp8_rms_norm_kernel<T, 1, 2, ALIGNED, false><<<quarter, 256, 0, st>>>(a);
+    launch(fp8_rms_norm_kernel<T, 1, 2, ALIGNED, false>, 256, 4);
   else if (mp <= 2048)
-    fp8_rms_norm_kernel<T, 1, 4, ALIGNED, false><<<quarter, 256, 0, st>>>(a);
+    launch(fp8_rms_norm_kernel<T, 1, 4, ALIGNED, false>, 256, 4);
   else if (mp <= 4096)
-    fp8_rms_norm_kernel<T, 4, 2, ALIGNED, false><<<whole, 256, 0, st>>>(a);
+    launch(fp8_rms_norm_kernel<T, 4, 2, ALIGNED, false>, 256, 1);
   else if (mp <= 8192)
-    fp8_rms_norm_kernel<T, 4, 4, ALIGNED, false><<<whole, 256, 0, st>>>(a);
+    launch(fp8_rms_norm_kernel<T, 4, 4, ALIGNED, false>, 256, 1);
   else if (mp <= 16384)
-    fp8_rms_norm_kernel<T, 8, 4, ALIGNED, false><<<whole, 512, 0, st>>>(a);
+    launch(fp8_rms_norm_kernel<T, 8, 4, ALIGNED, false>, 512, 1);
   else
-    fp8_rms_norm_kernel<T, 4, 1, ALIGNED, true><<<whole, 256, 0, st>>>(a);
+    launch(fp8_rms_norm_kernel<T, 4, 1, ALIGNED, true>, 256, 1);
 }
 
 template <typename T>

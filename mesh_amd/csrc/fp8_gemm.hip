@@ -1494,7 +1494,7 @@ static int launch_tiles(const GemmArgs& g, int split, hipStream_t st) {
 static int add_parts(const GemmArgs& g, const float* parts, int split, hipStream_t st) {
   const int64_t threads = (int64_t)g.E * g.R * (fp8_row_bytes(g.N) / 8);
   const int64_t blocks = (threads + 255) / 256;
-  MOE_REQUIRE(blocks <= 0x7fffffff, MESH_MOE_E_UNSUPPORTED,
+  MOE_REQUIRE(blocks <= MAX_THREADS / 256, MESH_MOE_E_UNSUPPORTED,
               "fp8_expert_linear: too many elements (E=%d R=%d N=%d)", g.E, g.R, g.N);
   if (g.y_scales)
     fp8_parts_kernel<true><<<(unsigned)blocks, 256, 0, st>>>(parts, g, split);
@@ -1522,7 +1522,7 @@ template <int TM, int CW, typename TO>
 static int launch_few_rows(const GemmArgs& g, hipStream_t st) {
   const int64_t tiles_m = ((int64_t)g.R + 16 * TM - 1) / (16 * TM);
   const int64_t tiles_n = ((int64_t)g.N + 16 * CW - 1) / (16 * CW);
-  MOE_REQUIRE(tiles_m * tiles_n <= 1 << 30 && tiles_m * tiles_n * g.E <= 1 << 30,
+  MOE_REQUIRE(tiles_m * tiles_n <= MAX_THREADS / 512 / g.E,
               MESH_MOE_E_UNSUPPORTED, "fp8_expert_linear: too many tiles (E=%d R=%d N=%d)",
               g.E, g.R, g.N);
   fp8_few_rows_kernel<TM, CW, TO>

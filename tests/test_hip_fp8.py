@@ -243,6 +243,29 @@ def test_residual_rms_norm_of_odd_rows(hip):
   assert torch.equal(y.values.view(torch.uint8), again[1].values.view(torch.uint8))
 
 
+@pytest.mark.parametrize("rows,m", [(67108860 + 7, 1), (16777215 + 5, 2049)])
+def test_residual_rms_norm_of_more_rows_than_a_launch_has(hip, rows, m):
+  """Rows around the first launch's end are what the call makes of those alone."""
+  at = torch.arange(rows, device="cuda")
+  mask = (at % 5 != 0).bfloat16()
+  x = ((at % 7).bfloat16() + 1)[:, None].expand(rows, m).contiguous()
+  del at
+  residual = -0.5 * x if m == 1 else None
+  scale = torch.linspace(0.5, 2, m, device="cuda").bfloat16()
+  total, y, *norm = hip.residual_rms_norm(x, residual, scale, row_mask=mask,
+                                          want_norm=m == 1)
+  edge = rows - (7 if m == 1 else 5)
+  for sl in (slice(0, 9), slice(edge - 9, edge + 1), slice(edge, rows)):
+    part = (x[sl].contiguous(), None if residual is None else residual[sl].contiguous())
+    t, q, *n = hip.residual_rms_norm(*part, scale, row_mask=mask[sl].contiguous(),
+                                     want_norm=m == 1)
+    assert torch.equal(total[sl], t)
+    assert torch.equal(y.values[sl].view(torch.uint8), q.values.view(torch.uint8))
+    assert torch.equal(y.scales[sl], q.scales)
+    for whole, alone in zip(norm, n):
+      assert torch.equal(whole[sl], alone)
+
+
 def test_residual_rms_norm_of_the_widest_row(hip):
   """A row whose last step's columns reach 2^31: what lies behind it is not read.  Every
   sum is 1 and the norm of ones is one, whose code is 256 under the unit 2^-8."""
