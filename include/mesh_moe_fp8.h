@@ -69,8 +69,9 @@ int mesh_moe_fp8_quantize(const void* x, const void* relu_mask,
 
 /*
  * What an operand stands for: y[r, i] = values[r, i] * 2^(scales[r, i / 128] - 127),
- * i < K.  Exact in both types (but for 2^128, which float32 values from 248 * 2^120 on
- * round to: an infinity here).
+ * i < K; NaN where the scale byte is 255.  Exact in float32, and from scale byte 3 on in
+ * bfloat16, below it rounded to it (but for numbers from 2^128 on, which float32 values
+ * from 248 * 2^120 on round to: infinities here).
  *   values [rows,KP], scales [rows,KS]; y [rows,K] dtype
  */
 int mesh_moe_fp8_dequantize(const void* values, const uint8_t* scales, void* y,

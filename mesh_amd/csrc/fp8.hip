@@ -291,7 +291,10 @@ __global__ __launch_bounds__(256) void fp8_dequantize_kernel(
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
       if (row[u] >= rows) continue;
-      const float f = __uint_as_float(unit[u] << 23);
+      // (2^-127 is not a normal number)
+      const float f = __uint_as_float(unit[u] == 255   ? 0x7fc00000u
+                                      : unit[u] == 0 ? 0x00400000u
+                                                     : unit[u] << 23);
       float v[V];
 #pragma unroll
       for (int j = 0; j < V / 4; ++j) {

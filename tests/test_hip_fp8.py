@@ -185,6 +185,23 @@ def test_dequantize(hip, shape):
     np.testing.assert_array_equal(_f64(y), F.operand_value(q))
 
 
+def test_dequantize_every_scale_byte(hip):
+  """Every code under every scale byte, 255 being NaN; numbers that are not normal are
+  kept, in bfloat16 to its last bit, 2^-133."""
+  codes = torch.arange(256, dtype=torch.uint8).repeat(256, 1)
+  scales = torch.arange(256, dtype=torch.uint8)[:, None].repeat(1, 4)
+  q = hip.Fp8Blocks(codes.view(torch.float8_e4m3fn).cuda(), scales.cuda(), 256)
+  want = F.value(codes.numpy(), scales.numpy())
+  want[255] = np.nan
+  want = np.where(np.abs(want) >= 2.0 ** 128, np.copysign(np.inf, want), want)
+  np.testing.assert_array_equal(_f64(hip.dequantize(q, torch.float32)), want)
+  with np.errstate(invalid="ignore"):
+    rounded = np.where(np.abs(want) < 2.0 ** -126,
+                       np.round(want * 2.0 ** 133) * 2.0 ** -133, want)
+  assert (rounded[3:255] == want[3:255])[~np.isnan(want[3:255])].all()
+  np.testing.assert_array_equal(_f64(hip.dequantize(q)), rounded)
+
+
 # --- the norm ---------------------------------------------------------------
 def _norm_64(total, scale, mask, epsilon):
   t = _f64(total)
