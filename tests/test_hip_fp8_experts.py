@@ -198,10 +198,12 @@ CASES = [("top_2", (4, 64, 256, 384, 64, 64, 64.0)),
          ("top_2", (3, 50, 200, 333, 6, 50, 1.25)),
          ("switch", (2, 128, 256, 640, 8, 64, 1.25)),
          ("switch", (3, 50, 131, 333, 6, 50, 2.0)),
-         ("ntlb", (2, 128, 200, 257, 8, 64, 1.25))]
+         ("ntlb", (2, 128, 200, 257, 8, 64, 1.25)),
+         ("expert_selection", (2, 128, 256, 640, 8, 64, 1.25)),
+         ("expert_selection", (3, 50, 131, 333, 6, 50, 2.0))]
 
 
-@pytest.mark.parametrize("grads", [False])
+@pytest.mark.parametrize("grads", [False, True])
 @pytest.mark.parametrize("activation", ["relu", "linear"])
 @pytest.mark.parametrize("gating,sizes", CASES)
 def test_experts_bit_for_bit(hip, gating, sizes, activation, grads):
@@ -220,3 +222,19 @@ def test_experts_bit_for_bit(hip, gating, sizes, activation, grads):
     laid_out.assign(laid_out.master * 0.75)
   layer.lowering.run({layer.x: layer.tokens(5)})
   layer.check(hip)
+
+
+@pytest.mark.parametrize("gating,sizes", CASES[1:4] + CASES[6:7] + CASES[9:10])
+def test_recorded_training_step(hip, gating, sizes):
+  """Replays with other tokens and weights, eager work between them."""
+  layer = _Layer(gating, "relu", *sizes, grads=True)
+  step = layer.lowering.capture()
+  for i in range(3):
+    step.replay({layer.x: layer.tokens(10 + i)})
+    layer.check(hip)
+    replayed = [layer.get(t).clone() for t in layer.outputs]
+    layer.lowering.run({layer.x: layer.tokens(10 + i)})
+    for tensor, value in zip(layer.outputs, replayed):
+      assert torch.equal(layer.get(tensor), value)
+    for var, laid_out in layer.lowering.variables.items():
+      laid_out.assign(laid_out.master * 0.9)
