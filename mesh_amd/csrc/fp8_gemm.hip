@@ -74,8 +74,8 @@ struct GemmArgs {
 // blocks of 128 of a row are requested before the first is multiplied.  One row 4096 ->
 // 16384 takes 14.4 us, 4.7 TB/s (16.0 us with requests for 32 bytes of each row instead of
 // 64).  That leaves time to multiply in bfloat16, which holds an e4m3 number times its
-// unit, so that the sums are float32 ones; the instructions for 8 bits lose bits below
-// 2^-14 of the largest of 8 products.
+// unit, so that the sums are float32 ones; the instructions for 8 bits cut 8 neighbouring
+// products off below 2^-13 of the largest one's power of two.
 // TO: bf16_t, float (rows of fp8_row_bytes(N), without the activation: fp8_parts_kernel
 // goes on from there) or uint8_t (an 8-bit operand; CW is 8: a block of 128 columns).
 // ---------------------------------------------------------------------------
@@ -1572,6 +1572,14 @@ using namespace mesh_moe;
 static bool fp8_sizes(int E, int R, int K, int N) {
   return E >= 1 && R >= 1 && K >= 1 && N >= 1 && R <= 0x7fffff00 && K <= 0x7fffff00 &&
          N <= 0x7fffff00;
+}
+
+extern "C" int mesh_moe_fp8_expert_linear_exact(int E, int R, int K, int N,
+                                                int eight_bit, int counted) {
+  if (!fp8_sizes(E, R, K, N)) return 0;
+  const ProductKind kind =
+      plan_product(E, R, K, N, eight_bit != 0, counted != 0).kind;
+  return kind == ONE_BLOCK || kind == FEW_ROWS ? 1 : 0;
 }
 
 extern "C" size_t mesh_moe_fp8_expert_linear_workspace_bytes(int E, int R, int K, int N,

@@ -36,6 +36,7 @@ _SIGNATURES = {
         _vp, _vp, _vp, ctypes.c_int64, _int, _int, _vp]),
     "mesh_moe_fp8_residual_rms_norm": (_int, [_vp] * 8 + [
         ctypes.c_int64, _int, ctypes.c_double, _int, _vp]),
+    "mesh_moe_fp8_expert_linear_exact": (_int, [_int] * 6),
     "mesh_moe_fp8_expert_linear_workspace_bytes": (_size, [_int] * 5),
     "mesh_moe_fp8_expert_linear": (_int, [_vp] * 7 + [_int] * 5 + [
         _vp, _size, _vp]),
@@ -325,6 +326,16 @@ def expert_linear(a, w, activation="linear", eight_bit=False, row_count=None, ou
   e, r, k = a.shape
   n = w.shape[1]
   return _linear(a, w, (e, r, k, n), (e, r, n), activation, eight_bit, row_count, out)
+
+
+def multiplies_exactly(e, r, k, n, eight_bit=False, counted=False):
+  """Whether expert_linear (counted: with row_count) of these sizes multiplies exactly and
+  adds up in float32.  Otherwise sums lose up to 2^-10 of their products' magnitudes (about
+  2^-14 of themselves with normally distributed operands): the matrix instructions for 8
+  bits cut the products of 8 neighbouring values off below 2^-13 of the largest.  The faster
+  way is taken, so one row's bits may depend on what is beside it."""
+  return load_library().mesh_moe_fp8_expert_linear_exact(
+      e, r, k, n, int(eight_bit), int(counted)) == 1
 
 
 def dense(x, w, activation=None, eight_bit=False):

@@ -229,3 +229,20 @@ def test_layers_on_8_bit_operands():
   assert build(True, torch.bfloat16) == build(False, torch.bfloat16)
   with pytest.raises(ValueError, match="bfloat16"):
     build(True, torch.float32)
+
+
+def test_sizes_that_are_multiplied_exactly(lib):
+  """Few rows at most; none of the sizes that a call refuses."""
+  del lib
+  assert fp8_hip.multiplies_exactly(1, 1, 4096, 16384)
+  assert fp8_hip.multiplies_exactly(1, 16, 100, 1000, eight_bit=True, counted=True)
+  assert not fp8_hip.multiplies_exactly(64, 6, 4096, 1024)
+  for eight_bit in (False, True):
+    for counted in (False, True):
+      for e in (1, 8, 64):
+        for k in (1, 128, 129, 1024, 16384):
+          for n in (1, 200, 4096, 65536):
+            for r in (129, 500, 8192):
+              assert not fp8_hip.multiplies_exactly(e, r, k, n, eight_bit, counted)
+  for sizes in ((0, 1, 1, 1), (1, 0, 1, 1), (1, 1, 0, 1), (1, 1, 1, 0)):
+    assert not fp8_hip.multiplies_exactly(*sizes)

@@ -432,6 +432,34 @@ def test_gradients_of_counted_rows(hip, e, r, k, n):
   assert _near(dw, av @ yt, av.abs() @ yt.abs())
 
 
+@pytest.mark.parametrize("e,r,k,n", [(1, 1, 4096, 1000), (1, 16, 1024, 4096),
+                                     (2, 100, 700, 130), (30, 16, 100, 40),
+                                     (3, 200, 384, 300), (8, 1100, 256, 520)])
+def test_products_that_are_exact(hip, e, r, k, n):
+  """Seven products of 2^-15 beside each of 1 or -1, which cancel out: the instructions
+  for 8 bits lose them.  Where the call says that products are exact, so are these sums
+  (multiples of 2^-15 below 2^9 in any order), and the result is the nearest bfloat16.
+  Elsewhere seven products of eight lose 2^-13 of the largest at most, so sums less than
+  2^-10 of their products' magnitudes."""
+  x = torch.full((e, r, k), 2.0 ** -7, device="cuda")
+  w = torch.full((e, n, k), 2.0 ** -8, device="cuda")
+  x[..., ::16], x[..., 8::16], w[..., ::8] = 1.0, -1.0, 1.0
+  x *= (torch.arange(r, device="cuda")[:, None] % 3 - 1.0)      # rows of -1, 0, 1 of it
+  a, b = hip.quantize(x), hip.quantize(w)
+  assert torch.equal(hip.dequantize(a, torch.float32), x)
+  wt = w.double().transpose(1, 2).contiguous()
+  want, magnitudes = x.double() @ wt, x.double().abs() @ wt
+  for counts in (None, torch.full((e,), r, dtype=torch.int32, device="cuda")):
+    exact = hip.multiplies_exactly(e, r, k, n, counted=counts is not None)
+    assert exact == (r <= 100)
+    got = hip.expert_linear(a, b, row_count=counts)
+    if exact:
+      assert torch.equal(got, want.to(torch.bfloat16))
+    else:
+      assert ((got.double() - want).abs() <= want.abs() * 2.0 ** -8 +
+              magnitudes * 2.0 ** -10).all()
+
+
 @pytest.mark.parametrize("activation", [None, "linear", "sigmoid", "tanh", "swish"])
 @pytest.mark.parametrize("r", [2, 300])
 def test_activations(hip, activation, r):
