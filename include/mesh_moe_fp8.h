@@ -42,7 +42,7 @@ extern "C" {
 #endif
 
 /* (counted up with every change of a declaration, and of what a call accepts) */
-#define MESH_MOE_FP8_ABI_VERSION 2
+#define MESH_MOE_FP8_ABI_VERSION 3
 
 int mesh_moe_fp8_abi_version(void);
 

@@ -22,7 +22,7 @@ import torch
 from mesh_amd import moe_hip
 from mesh_amd.moe_hip import MoeHipError
 
-ABI_VERSION = 2
+ABI_VERSION = 3
 BLOCK = 128
 _E4M3 = torch.float8_e4m3fn
 
