@@ -238,3 +238,18 @@ def test_recorded_training_step(hip, gating, sizes):
       assert torch.equal(layer.get(tensor), value)
     for var, laid_out in layer.lowering.variables.items():
       laid_out.assign(laid_out.master * 0.9)
+
+
+@pytest.mark.parametrize("gating,sizes", CASES[:1] + CASES[3:5] + CASES[6:7])
+def test_forward_with_and_without_gradients(hip, gating, sizes):
+  """With a gradient to follow the hidden tensor is rounded to bfloat16 before it is to 8
+  bits.  That moves a value by 2^-9 of it at most, so with a probability of at most 2 *
+  2^-9 / 2^-4 over a border to the next one, a step of at most 2^-3 of it away: 2^-2 *
+  2^-3 in the root mean square."""
+  del hip
+  outs = []
+  for grads in (False, True):
+    layer = _Layer(gating, "linear", *sizes, grads=grads)
+    outs.append(layer.get(layer.outputs[0]).double())
+  error = ((outs[1] - outs[0]).square().mean() / outs[0].square().mean()).sqrt()
+  assert 0 < error < 2.0 ** -5

@@ -339,3 +339,39 @@ def test_moe_layer_in_a_stack(hip):
                     [float(lowering.export_to_tf_tensor(t)) for t in losses]))
   assert results[0][1] == results[1][1]
   assert 0 < _error(results[1][0], results[0][0]) < 2.0 ** -3.5
+
+
+def test_forward_with_and_without_gradients(hip):
+  """With a gradient to follow, a norm and a hidden tensor are rounded to bfloat16 before
+  they are to 8 bits, the norm in each of its three steps.  A rounding moves a value by
+  2^-9 of it at most, so with a probability of at most 2 * 2^-9 / 2^-4 over a border to
+  the next 8-bit one, 2^-3 of it away at most: 2^-2 * 2^-3 in the root mean square behind
+  the hidden tensor, sqrt(3) times that behind the norm."""
+  del hip
+  results = []
+  for grads in (False, True):
+    graph = mtf.Graph()
+    mesh = mtf.Mesh(graph, "mesh")
+    dims = [mtf.Dimension("batch", 2), mtf.Dimension("length", 70),
+            mtf.Dimension("d_model", 256)]
+    x = mtf.import_tf_tensor(mesh, _normal(1, (2, 70, 256)).to(BF16), mtf.Shape(dims))
+    with mtf.variable_scope("norm"):
+      scale = mtf.get_variable(
+          mesh, "scale", mtf.Shape(dims[-1:]),
+          dtype=mtf.VariableDType(torch.float32, torch.float32, BF16))
+    norm = transformer.RmsNormOperation(x, scale, 1e-6).outputs[0]
+    kind = dict(use_bias=False, eight_bit=True,
+                variable_dtype=mtf.VariableDType(torch.float32, torch.float32, BF16))
+    h = mtf_layers.dense(norm, mtf.Dimension("d_ff", 1024), name="wi", **kind)
+    y = mtf_layers.dense(h, dims[-1], name="wo", **kind)
+    if grads:
+      mtf.gradients([y], [v.outputs[0] for v in graph.trainable_variables],
+                    [mtf.import_tf_tensor(mesh, _normal(2, (2, 70, 256)).to(BF16),
+                                          y.shape)])
+    values = {"norm/scale": 1 + 0.1 * _normal(3, (256,)),
+              "wi/kernel": _normal(4, (256, 1024), 1.0 / 16),
+              "wo/kernel": _normal(5, (1024, 256), 1.0 / 32)}
+    lowering = _lower(graph, mesh, values)
+    lowering.run()
+    results.append(lowering.export_to_tf_tensor(y))
+  assert 0 < _error(results[1], results[0]) < (1 + 3 ** 0.5) * 2.0 ** -5
