@@ -260,7 +260,8 @@ def residual_rms_norm(x, residual, scale, epsilon=1e-6, row_mask=None,
   """rms_norm(x + residual) * row_mask as an 8-bit operand: x, residual (or None) [...,
   M], scale [M], row_mask [...] (or None) -> (x + residual or x itself, Fp8Blocks [...,
   M]).  want_norm: also the result in x's dtype, as a third one (what a training step
-  quantizes the columns of)."""
+  quantizes the columns of; for programs without a graph: a graph with gradients makes the
+  norm in bfloat16 and quantizes that, rows and columns, in one pass)."""
   lib = load_library()
   m = x.shape[-1]
   shape = tuple(x.shape)

@@ -206,7 +206,10 @@ class DenseOperation(mtf.Operation):
   operation on the matrix cores.  The kernel is read from the variable's
   K-contiguous packed copy.  eight_bit: the product and its gradients multiply 8-bit
   operands (fp8_hip): x and the kernel with a scale for each block of 128 along the
-  dimension that is summed over, the kernel's quantized when it changes."""
+  dimension that is summed over, the kernel's quantized when it changes.  Where nothing
+  but an 8-bit layer reads a norm or a hidden tensor it is rounded once, to 8 bits; where
+  a gradient reads it too it is a bfloat16 tensor first, so that the same weights may give
+  a value one 8-bit step apart with and without gradients in the graph."""
 
   def __init__(self, x, kernel, new_dims, activation, name=None, eight_bit=False):
     super(DenseOperation, self).__init__([x, kernel], name=name or "dense")

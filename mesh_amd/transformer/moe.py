@@ -472,7 +472,8 @@ class MoEV1Operation(mtf.Operation):
     hidden_keep_prob: keep probability of the dropout on the hidden tensor
     (moe.py:477-479), None for none.
     eight_bit: the experts' products and their gradients multiply 8-bit operands
-    (fp8_hip); one bfloat16 layer wi, one wo, no hidden dropout."""
+    (fp8_hip); one bfloat16 layer wi, one wo, no hidden dropout.  Without a gradient in the
+    graph the hidden tensor is rounded once, to 8 bits, with one to bfloat16 before."""
     wis = list(wi) if isinstance(wi, (list, tuple)) else [wi]
     acts = (list(activation) if isinstance(activation, (list, tuple))
             else [activation])
