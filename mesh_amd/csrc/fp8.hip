@@ -86,9 +86,9 @@ __device__ __forceinline__ void store8(T* row, int at, int end, const float (&v)
 // column so that the lanes of a write spread over all banks.
 //
 // Bound by memory: the tensor is read once, whichever forms are wanted.  Both forms of
-// 65536 x 4096 in bf16 take 211 us, 5.1 TB/s (254 with 144 registers and three blocks per
-// CU instead of 94 and five), the rows alone 143; pieces that do not lie on 16 bytes need
-// the registers.
+// 65536 x 4096 in bf16 take 204 to 231 us, 5.3 to 4.7 TB/s (254 with 144 registers and
+// three blocks per CU instead of 94 and five), the rows alone 143; pieces that do not lie
+// on 16 bytes need the registers.
 // ---------------------------------------------------------------------------
 constexpr int QT = FP8_BLOCK;     // a tile's rows and columns
 
@@ -335,7 +335,7 @@ static void run_dequantize(const uint8_t* values, const uint8_t* scales, T* y,
 // from the sum that the same threads wrote.  The mean's sum, the root and the product
 // are float32; the residual sum is rounded to the tensors' type first, being one.
 //
-// Bound by memory: 32000 x 4096 in bf16 with a residual 150 us, 6.1 TB/s.  At most 32
+// Bound by memory: 32000 x 4096 in bf16 with a residual 140 us, 6.5 TB/s.  At most 32
 // values of a lane's row are in registers: 4000 rows of 16384 take 85 us on 8
 // wavefronts, 118 on 4 with 64 values each; 30000 rows of 2048 take 78 us on one
 // wavefront with 32, 82 on 4 with 8 (whose barrier the others wait at).

@@ -488,7 +488,10 @@ def dense(x, new_dims, reduced_dims=None, expert_dims=None, use_bias=True,
   transformer layers use: no bias, no expert dims, the reduced dims being the
   trailing dims of x; activation None / "linear" / relu.  The variable is
   `<name>/kernel` with shape reduced_dims + new_dims.  eight_bit (x in bfloat16):
-  the product and its gradients on 8-bit operands, see DenseOperation."""
+  the product and its gradients on 8-bit operands, see DenseOperation.  It pays where the
+  product or the stream of its weights takes the time (64 tokens 4096 -> 16384 -> 4096 57
+  us instead of 116), not for a few tokens through a small layer (8 tokens 1024 -> 4096 ->
+  1024 51 us instead of 26 eager, 21 instead of 19 recorded)."""
   if isinstance(new_dims, mtf.Dimension) or not isinstance(new_dims,
                                                            (list, tuple)):
     new_dims = [new_dims]
