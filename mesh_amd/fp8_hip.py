@@ -179,6 +179,16 @@ def _pointers(q):
   return q._values.data_ptr(), q._scales.data_ptr()  # pylint: disable=protected-access
 
 
+# (a larger argument of a C call would lose its upper bits)
+_INT_MAX = 0x7fffffff
+
+
+def _ints(*sizes):
+  """Refuses sizes that the library's calls cannot be given."""
+  if max(sizes) > _INT_MAX:
+    raise MoeHipError("a size of %s is beyond 2^31 - 1" % (sizes,))
+
+
 def _counts(row_count, e):
   return (None if row_count is None
           else _dev(row_count, "row_count", torch.int32, (e,)))
@@ -217,6 +227,7 @@ def quantize(x, rows=True, columns=False, relu_mask=None, row_count=None, out=No
     raise ValueError("x %s, expected [E, R, K] or [R, K]" % (tuple(x.shape),))
   sizes = tuple(x.shape)
   e, r, k = (1,) * (3 - x.dim()) + sizes
+  _ints(e, r, k)
   code = moe_hip.dtype_code(x.dtype)
   turned = sizes[:-2] + (k, r)
   by_row = by_column = None
@@ -245,6 +256,7 @@ def dequantize(q, dtype=torch.bfloat16):
   """The tensor that an operand stands for, exact in bfloat16 and float32."""
   lib = load_library()
   code = moe_hip.dtype_code(dtype)
+  _ints(q.n)
   y = _empty(q.shape, dtype=dtype, device=q.values.device)
   values, scales = _operand(q, "q")
   if y.numel():
@@ -266,6 +278,7 @@ def residual_rms_norm(x, residual, scale, epsilon=1e-6, row_mask=None,
   m = x.shape[-1]
   shape = tuple(x.shape)
   code = moe_hip.dtype_code(x.dtype)
+  _ints(m)
   xp, sp = _dev(x, "x"), _dev(scale, "scale", x.dtype, (m,))
   rp = None if residual is None else _dev(residual, "residual", x.dtype, shape)
   mp = None if row_mask is None else _dev(row_mask, "row_mask", x.dtype, shape[:-1])
@@ -285,6 +298,7 @@ def _linear(a, w, sizes, shape, activation, eight_bit, row_count, out):
   """expert_linear with sizes (e, r, k, n); `shape`: of the result."""
   lib = load_library()
   e, r, k, n = sizes
+  _ints(e, r, k, n)
   ap, asp = _operand(a, "a")
   wp, wsp = _operand(w, "w", (e, n, k))
   act = _activation(activation)
@@ -335,6 +349,7 @@ def multiplies_exactly(e, r, k, n, eight_bit=False, counted=False):
   2^-14 of themselves with normally distributed operands): the matrix instructions for 8
   bits cut the products of 8 neighbouring values off below 2^-13 of the largest.  The faster
   way is taken, so one row's bits may depend on what is beside it."""
+  _ints(e, r, k, n)
   return load_library().mesh_moe_fp8_expert_linear_exact(
       e, r, k, n, int(eight_bit), int(counted)) == 1
 
@@ -369,6 +384,7 @@ def expert_linear_backward(a_columns, dy, w_rows=None, relu_mask=None, row_count
   if not isinstance(a_columns, Fp8Blocks) or len(a_columns.shape) != 3:
     raise MoeHipError("a_columns must be an Fp8Blocks [E, K, R]")
   k = a_columns.shape[1]
+  _ints(e, r, k, n)
   code = moe_hip.dtype_code(dy.dtype)
   ap, asp = _operand(a_columns, "a_columns", (e, k, r))
   yp = _dev(dy, "dy")

@@ -246,3 +246,31 @@ def test_sizes_that_are_multiplied_exactly(lib):
               assert not fp8_hip.multiplies_exactly(e, r, k, n, eight_bit, counted)
   for sizes in ((0, 1, 1, 1), (1, 0, 1, 1), (1, 1, 0, 1), (1, 1, 1, 0)):
     assert not fp8_hip.multiplies_exactly(*sizes)
+
+
+def test_sizes_beyond_an_int_are_refused(lib):
+  """2^32 + 8 would be 8 in a C int: the first 8 values of a row alone."""
+  del lib
+  many = 2 ** 32 + 128
+  one = torch.zeros(1, dtype=torch.bfloat16)
+  byte = torch.zeros(1, dtype=torch.uint8)
+
+  def operand(*shape):
+    n = shape[-1]
+    return fp8_hip.Fp8Blocks(
+        byte.view(torch.float8_e4m3fn).expand(shape[:-1] + (fp8_hip.row_bytes(n),)),
+        byte.expand(shape[:-1] + (fp8_hip.scale_bytes(n),)), n)
+  for call in (
+      lambda: fp8_hip.quantize(one.expand(1, many)),
+      lambda: fp8_hip.quantize(one.expand(many, 4), rows=False, columns=True),
+      lambda: fp8_hip.quantize(one.expand(many, 4, 4)),
+      lambda: fp8_hip.dequantize(operand(1, many)),
+      lambda: fp8_hip.residual_rms_norm(one.expand(1, many), None, one.expand(many)),
+      lambda: fp8_hip.expert_linear(operand(1, 4, many), operand(1, 4, many)),
+      lambda: fp8_hip.expert_linear(operand(1, 4, 128), operand(1, many, 128)),
+      lambda: fp8_hip.dense(operand(2 ** 16, 2 ** 16, 128), operand(1, 4, 128)),
+      lambda: fp8_hip.expert_linear_backward(operand(1, many, 4), one.expand(1, 4, 4)),
+      lambda: fp8_hip.expert_linear_backward(operand(1, 4, 4), one.expand(1, 4, many)),
+      lambda: fp8_hip.multiplies_exactly(1, 1, 1, many)):
+    with pytest.raises(moe_hip.MoeHipError, match="2\\^31"):
+      call()
