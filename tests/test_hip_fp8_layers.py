@@ -375,3 +375,72 @@ def test_forward_with_and_without_gradients(hip):
     lowering.run()
     results.append(lowering.export_to_tf_tensor(y))
   assert 0 < _error(results[1], results[0]) < (1 + 3 ** 0.5) * 2.0 ** -5
+
+
+@pytest.mark.parametrize("padded", [False, True])
+def test_training_a_layer_stack(hip, padded):
+  """DenseReluDense layers with norms, residual sums, a padding mask and gradients: every
+  8-bit layer and its gradients are what the calls make of the tensors that reach them,
+  in an eager step and in recorded ones."""
+  b, l, m, f = 2, 70, 256, 1024
+  graph = mtf.Graph()
+  mesh = mtf.Mesh(graph, "mesh")
+  dims = [mtf.Dimension("batch", b), mtf.Dimension("length", l),
+          mtf.Dimension("d_model", m)]
+  x = mtf.import_tf_tensor(mesh, _normal(1, (b, l, m)).to(BF16), mtf.Shape(dims))
+  stack = transformer.make_layer_stack(
+      [(transformer_layers.DenseReluDense, dict(hidden_size=f, eight_bit=True))],
+      num_layers=2)
+  model = transformer.Unitransformer(stack, d_model=m, name="encoder")
+  ids = None
+  if padded:
+    ids = torch.ones((b, l), dtype=torch.int32)
+    ids[:, 50:] = 0
+    ids = mtf.import_tf_tensor(mesh, ids, mtf.Shape(dims[:2]))
+  y, _ = model.call_layers(
+      x, mtf.VariableDType(torch.float32, torch.float32, BF16), mode="train",
+      sequence_id=ids)
+  dy = mtf.import_tf_tensor(mesh, _normal(2, (b, l, m)).to(BF16), y.shape)
+  grads = mtf.gradients([y], [x] + [v.outputs[0] for v in graph.trainable_variables],
+                        [dy])
+  values = {}
+  for i, v in enumerate(graph.all_variables):
+    sizes = v.shape.to_integer_list
+    values[v.name] = (1 + 0.1 * _normal(40 + i, sizes) if len(sizes) == 1
+                      else _normal(50 + i, sizes, sizes[0] ** -0.5))
+  lowering = _lower(graph, mesh, values)
+  layers = [op for op in graph.operations if isinstance(op, mtf_layers.DenseOperation)]
+  backward = [op for op in graph.operations
+              if isinstance(op, mtf_layers.DenseGradOperation)]
+  assert len(layers) == len(backward) == 4 and all(op.eight_bit for op in layers)
+
+  def check():
+    got = lowering.export_to_tf_tensor
+    for op in layers:
+      xs = got(op.inputs[0])
+      a, a_columns = hip.quantize(xs.reshape(1, -1, xs.shape[-1]), columns=True)
+      w = hip.quantize(lowering.variables[op.inputs[1].operation].master.unsqueeze(0),
+                       columns=True)
+      want = hip.expert_linear(a, w[1], op._activation)
+      ys = got(op.outputs[0])
+      assert torch.equal(ys, want.reshape(ys.shape))
+      back = [g for g in backward if g.inputs[1] is op.inputs[0]]
+      assert len(back) == 1
+      dx, dw = hip.expert_linear_backward(
+          a_columns, got(back[0].inputs[0]).reshape(want.shape), w[0],
+          relu_mask=want if op._activation == "relu" else None)
+      for tensor, value in zip(back[0].outputs, (dx, dw)):
+        value = value.to(tensor.dtype)
+        assert torch.equal(got(tensor).reshape(-1), value.reshape(-1))
+    return [got(t).clone() for t in [y] + grads]
+  lowering.run()
+  first = check()
+  assert all(torch.isfinite(t).all() for t in first)
+  step = lowering.capture()
+  for i in range(3):
+    given = _normal(3 + i, (b, l, m)).to(BF16)
+    step.replay({x: given})
+    replayed = check()
+    lowering.run({x: given, dy: lowering.export_to_tf_tensor(dy)})
+    for t, value in zip([y] + grads, replayed):
+      assert torch.equal(lowering.export_to_tf_tensor(t), value)
