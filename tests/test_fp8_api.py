@@ -127,9 +127,6 @@ def test_quantize_refusals(lib):
   for change in (dict(_3=AT + 8), dict(_5=AT + 4), dict(_0=AT + 1)):
     _refused(lib, with_(**change), -2, "16 bytes")
   _refused(lib, with_(_7=1 << 20, _8=1 << 20, _9=1 << 20), -2, "tiles")
-  # more than 2^32 threads; a number of tiles that passes 64 bits
-  _refused(lib, with_(_7=1 << 20, _8=1, _9=1), -2, "tiles")
-  _refused(lib, with_(_7=1 << 19, _8=0x7fffff00, _9=0x7fffff00), -2, "tiles")
 
 
 def test_dequantize_and_norm_refusals(lib):
@@ -180,9 +177,6 @@ def test_linear_refusals(lib):
     _refused(lib, with_(_6=AT, _13=need - 1), -1, "workspace")
     _refused(lib, with_(_6=AT, _12=None, _13=need), -1, "workspace")
   assert lib.mesh_moe_fp8_expert_linear_workspace_bytes(0, 4, 128, 64, 1) == 0
-  # more than 2^32 threads
-  for n, eight_bit in ((0x7fffff00, AT), (0x7fffff00, None), (1 << 30, None)):
-    _refused(lib, with_(_6=eight_bit, _10=n), -2, "too many tiles")
 
 
 def test_linear_backward_refusals(lib):
@@ -274,3 +268,14 @@ def test_sizes_beyond_an_int_are_refused(lib):
       lambda: fp8_hip.multiplies_exactly(1, 1, 1, many)):
     with pytest.raises(moe_hip.MoeHipError, match="2\\^31"):
       call()
+
+
+def test_more_than_a_launch_has_is_refused(lib):
+  """2^32 threads; a number of tiles that passes 64 bits."""
+  for e, r, k in ((1 << 20, 1, 1), (1 << 19, 0x7fffff00, 0x7fffff00)):
+    _refused(lib, lib.mesh_moe_fp8_quantize(AT, None, None, AT, AT, AT, AT, e, r, k, 1,
+                                            None), -2, "tiles")
+  for n, scales in ((0x7fffff00, AT), (0x7fffff00, None), (1 << 30, None)):
+    _refused(lib, lib.mesh_moe_fp8_expert_linear(
+        AT, AT, AT, AT, None, AT, scales, 1, 4, 128, n, 1, AT, 1 << 40, None),
+             -2, "too many tiles")
