@@ -281,6 +281,8 @@ def test_residual_rms_norm_of_more_rows_than_a_launch_has(hip, rows, m):
     assert torch.equal(y.scales[sl], q.scales)
     for whole, alone in zip(norm, n):
       assert torch.equal(whole[sl], alone)
+  del x, y, total, residual, norm
+  torch.cuda.empty_cache()                     # (up to 105 GB)
 
 
 def test_residual_rms_norm_of_the_widest_row(hip):
@@ -853,10 +855,11 @@ def test_wide_results_stay_in_their_rows(hip, eight_bit, n):
   if eight_bit:
     # (half a step of e4m3, or of its least numbers under the block's unit)
     top = want.abs().view(-1, 128).amax(-1, keepdim=True).expand(-1, 128).reshape(1, -1)
-    assert ((y[:1].double() - want).abs() <= want.abs() * 2.0 ** -4 + top * 2.0 ** -17 +
-            magnitudes * 2.0 ** -13 * (1 + 2.0 ** -4)).all()
+    half = want.abs() * 2.0 ** -4 + top * 2.0 ** -17
   else:
-    assert _near(y[:1], want, magnitudes)
+    half = want.abs() * 2.0 ** -8
+  # (7 products of 8 are cut off by up to 2^-13 of the largest: less than 2^-10 of all)
+  assert ((y[:1].double() - want).abs() <= half + magnitudes * 2.0 ** -10).all()
 
 
 @pytest.mark.parametrize("rows", [1, 300])
