@@ -7,74 +7,6 @@
 
 namespace mesh_moe {
 
-// Pieces of 16 bytes that lie on a T: the hardware takes any address.  (Rows and columns
-// of 9000 x 2050 in bf16 take 29 us with them, 53 with a load per value, and 26 at 2048
-// columns, where pieces lie on 16 bytes; the norm of 32000 x 2050 124, 267 and 83.)
-template <typename T> struct PieceOf;
-template <> struct PieceOf<bf16_t> {
-  typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2)));
-};
-template <> struct PieceOf<float> {
-  typedef uint32_t type __attribute__((ext_vector_type(4), aligned(4)));
-};
-template <typename T, bool ONCE>
-__device__ __forceinline__ uint4 load_piece(const T* at) {
-  typedef typename PieceOf<T>::type piece_t;
-  const piece_t* p = reinterpret_cast<const piece_t*>(at);
-  const piece_t v = ONCE ? __builtin_nontemporal_load(p) : *p;
-  return make_uint4(v[0], v[1], v[2], v[3]);
-}
-template <typename T>
-__device__ __forceinline__ void store_piece(T* at, uint4 v) {
-  typedef typename PieceOf<T>::type piece_t;
-  __builtin_nontemporal_store(piece_t{v.x, v.y, v.z, v.w}, reinterpret_cast<piece_t*>(at));
-}
-
-// 8 neighbouring values of a row from column `at` on, zeros from `end` on.  ALIGNED:
-// every row's pieces of 16 bytes lie on 16 bytes, and `end` is a multiple of 8.  ONCE:
-// nothing reads them again.  (`at` goes up to 2^31 - 8, so nothing is added to it before
-// it is known to be below `end`.)
-template <typename T, bool ALIGNED, bool ONCE = true>
-__device__ __forceinline__ void load8(const T* row, int at, int end, float (&v)[8]) {
-  if (ALIGNED ? at < end : at <= end - 8) {
-    if constexpr (sizeof(T) == 2) {
-      unpack16(load_piece<T, ONCE>(row + at), v, T());
-    } else {
-      float lo[4], hi[4];
-      unpack16(load_piece<T, ONCE>(row + at), lo, T());
-      unpack16(load_piece<T, ONCE>(row + at + 4), hi, T());
-#pragma unroll
-      for (int j = 0; j < 4; ++j) { v[j] = lo[j]; v[4 + j] = hi[j]; }
-    }
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = 0.f;
-  if constexpr (!ALIGNED)
-    if (at < end)
-#pragma unroll
-      for (int j = 0; j < 7; ++j)
-        if (at + j < end) v[j] = load_f32<T>(row + at + j);
-}
-
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ void store8(T* row, int at, int end, const float (&v)[8]) {
-  if (ALIGNED ? at < end : at <= end - 8) {
-    if constexpr (sizeof(T) == 2) {
-      store_piece(row + at, pack16(v, T()));
-    } else {
-      const float lo[4] = {v[0], v[1], v[2], v[3]}, hi[4] = {v[4], v[5], v[6], v[7]};
-      store_piece(row + at, pack16(lo, T()));
-      store_piece(row + at + 4, pack16(hi, T()));
-    }
-    return;
-  }
-  if constexpr (!ALIGNED)
-#pragma unroll
-    for (int j = 0; j < 7; ++j)
-      if (at + j < end) store_f32<T>(row + at + j, v[j]);
-}
-
 // ---------------------------------------------------------------------------
 // Quantizing.  A block of 256 threads has a tile of 128 rows x 128 columns in
 // registers, 8 rows x 8 columns a thread: thread t the columns 8 (t % 16) .. and the

@@ -1,0 +1,162 @@
+"""The paged cache's interface on the CPU: exported symbols, what a cache is made of, and
+what is refused before a launch."""
+
+import os
+import re
+
+import pytest
+import torch
+
+from mesh_amd import cache_hip
+from mesh_amd import moe_hip
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+E4M3 = torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module")
+def lib():
+  if not os.path.exists(moe_hip.LIB_PATH):
+    from mesh_amd.csrc import build
+    build.build_library(verbose=False)
+  return cache_hip.load_library()
+
+
+def test_library_exports_every_declared_symbol(lib):
+  header = open(os.path.join(ROOT, "include", "mesh_moe_cache.h")).read()
+  code = re.sub(r"/\*.*?\*/", " ", header, flags=re.DOTALL)
+  declared = set(re.findall(r"\b(mesh_moe_cache_[a-z0-9_]+)\s*\(", code))
+  assert declared == set(cache_hip.EXPORTS)
+  for name in declared:
+    assert getattr(lib, name) is not None
+  version = re.search(r"MESH_MOE_CACHE_ABI_VERSION (\d+)", header).group(1)
+  assert lib.mesh_moe_cache_abi_version() == cache_hip.ABI_VERSION == int(version)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, E4M3])
+@pytest.mark.parametrize("shared", [False, True])
+def test_empty_cache(dtype, shared):
+  c = cache_hip.PagedCache.empty(5, 16, 3, 200, dtype, "cpu", shared_kv=shared)
+  assert (c.pages, c.page_size, c.heads, c.d_kv) == (5, 16, 3, 200)
+  assert c.k_pages.shape == (5, 3, 16, 200) and c.dtype == dtype
+  assert c.eight_bit == (dtype == E4M3) and c.shared_kv == shared
+  assert (c.v_pages is None) == shared
+  if c.eight_bit:
+    assert c.k_scales.shape == (5, 3, 16, 2) and c.k_scales.dtype == torch.uint8
+    assert (c.v_scales is None) == shared
+  else:
+    assert c.k_scales is None and c.v_scales is None
+  assert "page_size=16" in repr(c)
+
+
+def test_pages_that_are_no_cache():
+  def pages(*shape, dtype=torch.bfloat16):
+    return torch.empty(shape, dtype=dtype)
+  k8, s8 = pages(4, 2, 8, 32, dtype=E4M3), pages(4, 2, 8, 1, dtype=torch.uint8)
+  for args in ((pages(4, 8, 32), None), (pages(4, 2, 8, 32), pages(4, 2, 8, 16)),
+               (pages(4, 2, 8, 32), pages(4, 2, 8, 32, dtype=torch.float32)),
+               (pages(0, 2, 8, 32), None), (pages(4, 2, 8, 32), None, s8),
+               (k8, k8), (k8, k8, s8), (k8, k8, s8, s8[:1]), (k8, None, s8, s8),
+               (k8, k8, s8, s8.to(torch.int8)), (pages(4, 2, 12, 32), None)):
+    with pytest.raises(ValueError):
+      cache_hip.PagedCache(*args)
+  with pytest.raises(moe_hip.MoeHipError, match="dtype"):
+    cache_hip.PagedCache(pages(4, 2, 8, 32, dtype=torch.float16))
+
+
+def test_cpu_tensors_are_refused(lib):
+  del lib
+  cache = cache_hip.PagedCache.empty(4, 8, 2, 32, device="cpu")
+  x = torch.zeros(3, 64, dtype=torch.bfloat16)
+  table = torch.zeros(3, 2, dtype=torch.int32)
+  at = torch.zeros(3, dtype=torch.int32)
+  for call in (lambda: cache_hip.write(cache, x, x, table, at),
+               lambda: cache_hip.read(cache, table, at, 4),
+               lambda: cache_hip.attention(x, cache, table, at)):
+    with pytest.raises(moe_hip.MoeHipError, match="GPU tensor"):
+      call()
+  with pytest.raises(moe_hip.MoeHipError, match="PagedCache"):
+    cache_hip.write(x, x, x, table, at)
+
+
+# addresses that are never read: every call below is refused before a launch
+AT = 1 << 20
+
+
+def _refused(lib, rc, code, words):
+  assert rc == code
+  text = lib.mesh_moe_last_error().decode()
+  assert words in text, text
+
+
+def _changed(call, ok):
+  def with_(**changes):
+    args = list(ok)
+    for at, v in changes.items():
+      args[int(at[1:])] = v
+    return call(*args)
+  return with_
+
+
+def test_write_refusals(lib):
+  # k v table position count k_pages v_pages k_scales v_scales B T HK D N S P dtype
+  with_ = _changed(lib.mesh_moe_cache_write,
+                   [AT] * 4 + [None] + [AT] * 4 + [2, 3, 4, 64, 5, 16, 6, 1, None])
+  for change in (dict(_0=None), dict(_2=None), dict(_3=None), dict(_5=None)):
+    _refused(lib, with_(**change), -1, "null")
+  for change in (dict(_1=None), dict(_6=None)):
+    _refused(lib, with_(**change), -1, "go together")
+  for change in (dict(_7=None), dict(_8=None), dict(_1=None, _6=None)):
+    _refused(lib, with_(**change), -1, "scales")
+  for at in range(9, 16):
+    _refused(lib, with_(**{"_%d" % at: 0}), -1, "sizes")
+  _refused(lib, with_(_16=2), -1, "dtype")
+  _refused(lib, with_(_14=24), -2, "power of two")
+  _refused(lib, with_(_12=257), -2, "256")
+  _refused(lib, with_(_11=65537), -2, "65536")
+  _refused(lib, with_(_14=1 << 16, _15=1 << 15), -2, "2^30")
+
+
+def test_read_refusals(lib):
+  # k_pages v_pages k_scales v_scales table position count k v B T HK D N S P dtype
+  with_ = _changed(lib.mesh_moe_cache_read,
+                   [AT] * 6 + [None] + [AT] * 2 + [2, 3, 4, 64, 5, 16, 6, 0, None])
+  for change in (dict(_0=None), dict(_4=None), dict(_5=None), dict(_7=None)):
+    _refused(lib, with_(**change), -1, "null")
+  for change in (dict(_1=None), dict(_8=None)):
+    _refused(lib, with_(**change), -1, "go together")
+  for change in (dict(_2=None), dict(_3=None)):
+    _refused(lib, with_(**change), -1, "scales")
+  for at in range(9, 16):
+    _refused(lib, with_(**{"_%d" % at: -1}), -1, "sizes")
+  _refused(lib, with_(_16=2), -1, "dtype")
+  _refused(lib, with_(_14=3), -2, "power of two")
+
+
+def test_attention_refusals(lib):
+  # q k_new v_new k_pages v_pages k_scales v_scales table position rel_values rel_bucket
+  # num_buckets reach out B H HK D N S P dtype workspace bytes
+  with_ = _changed(lib.mesh_moe_cache_attention,
+                   [AT] * 9 + [None, None, 0, 0, AT, 2, 8, 4, 64, 5, 16, 6, 1, AT,
+                               1 << 40, None])
+  for change in (dict(_0=None), dict(_3=None), dict(_7=None), dict(_8=None),
+                 dict(_13=None)):
+    _refused(lib, with_(**change), -1, "null")
+  for change in (dict(_1=None), dict(_2=None), dict(_4=None, _6=None)):
+    _refused(lib, with_(**change), -1, "go together")
+  for change in (dict(_5=None), dict(_6=None)):
+    _refused(lib, with_(**change), -1, "scales")
+  for change in (dict(_9=AT), dict(_10=AT), dict(_9=AT, _10=AT, _11=4),
+                 dict(_9=AT, _10=AT, _12=4)):
+    _refused(lib, with_(**change), -1, "go together")
+  for at in (14, 16, 17, 18, 19, 20):
+    _refused(lib, with_(**{"_%d" % at: 0}), -1, "sizes")
+  for heads in (0, 6):
+    _refused(lib, with_(_15=heads), -1, "query heads")
+  _refused(lib, with_(_21=5), -1, "dtype")
+  _refused(lib, with_(_17=260), -2, "256")
+  _refused(lib, with_(_14=1 << 30), -2, "more than a launch")
+  need = lib.mesh_moe_cache_attention_workspace_bytes(2, 8, 4, 64, 16, 1 << 20)
+  if need:
+    _refused(lib, with_(_20=1 << 20, _23=need - 1), -1, "workspace")
+    _refused(lib, with_(_20=1 << 20, _22=None), -1, "workspace")
