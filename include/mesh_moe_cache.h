@@ -92,7 +92,7 @@ int mesh_moe_cache_read(const void* k_pages, const void* v_pages,
  *   workspace: mesh_moe_cache_attention_workspace_bytes bytes, which may be 0
  */
 size_t mesh_moe_cache_attention_workspace_bytes(int B, int H, int HK, int D, int S,
-                                                int P);
+                                                int P, int dtype, int eight_bit);
 int mesh_moe_cache_attention(const void* q, const void* k_new, const void* v_new,
                              void* k_pages, void* v_pages, uint8_t* k_scales,
                              uint8_t* v_scales, const int32_t* table,

@@ -36,7 +36,7 @@ _SIGNATURES = {
     "mesh_moe_cache_abi_version": (_int, []),
     "mesh_moe_cache_write": (_int, [_vp] * 9 + [_int] * 8 + [_vp]),
     "mesh_moe_cache_read": (_int, [_vp] * 9 + [_int] * 8 + [_vp]),
-    "mesh_moe_cache_attention_workspace_bytes": (_size, [_int] * 6),
+    "mesh_moe_cache_attention_workspace_bytes": (_size, [_int] * 8),
     "mesh_moe_cache_attention": (_int, [_vp] * 11 + [_int] * 2 + [_vp] + [_int] * 8 + [
         _vp, _size, _vp]),
 }
@@ -267,7 +267,8 @@ def attention(q, cache, table, position, k_new=None, v_new=None, relative_bias=N
   if not (b and columns):
     return torch.zeros_like(q)
   out = _empty(shape, dtype=dtype, device=q.device)
-  ws_bytes = lib.mesh_moe_cache_attention_workspace_bytes(b, h, heads, d, s, columns)
+  ws_bytes = lib.mesh_moe_cache_attention_workspace_bytes(
+      b, h, heads, d, s, columns, code, int(cache._k_scales is not None))  # pylint: disable=protected-access
   ws = _empty((ws_bytes,), dtype=torch.uint8, device=q.device) if ws_bytes else None
   with _stage("cache_attention"):
     _check(lib.mesh_moe_cache_attention(

@@ -4,8 +4,11 @@
 #include "fp8.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace mesh_moe {
+
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int MAX_WIDTH = 256;                  // D
 constexpr int MAX_HEADS = 1 << 16;              // HK
@@ -117,7 +120,6 @@ __global__ __launch_bounds__(256) void cache_read_kernel(
     RowsOf r, const void* __restrict__ k_pages, const void* __restrict__ v_pages,
     const uint8_t* __restrict__ k_scales, const uint8_t* __restrict__ v_scales,
     T* __restrict__ k, T* __restrict__ v) {
-  typedef float f32x2_t __attribute__((ext_vector_type(2)));
   const bool is_v = blockIdx.y != 0;
   T* y = is_v ? v : k;
   const uint8_t* values = static_cast<const uint8_t*>(is_v ? v_pages : k_pages);
@@ -283,6 +285,581 @@ __global__ __launch_bounds__(256) void cache_attention_kernel(Attention a) {
 }
 
 // ---------------------------------------------------------------------------
+// The same on the matrix cores, for rows of 16 values and more.
+//
+// The query heads that share a key / value head are a tile of 16 columns (a group has
+// several where it is larger, empty columns where it is smaller), 16 positions the tile's
+// rows: logits^T [position][head] = K . q^T, out^T [value][head] = V^T . w^T.  The first
+// product leaves lane 16 j + c with the logits of head c for positions 4 j .. 4 j + 3,
+// which is where the second one wants the weights of its reduction index, so that nothing
+// but two steps of a maximum crosses lanes.  Keys and values go from memory to registers in
+// the forms that the products take:
+//   keys    lane 16 j + c the pieces j, j + 4, .. of 16 bytes of position c (reductions
+//           take the pieces in whatever order the queries have them, too)
+//   values  lane 16 j + c the values of chunk c of positions 4 j .. 4 j + 3, so that 16
+//           lanes read a whole row; pairs of positions are put together (bfloat16) by
+//           v_perm, and a lane's results are neighbours in the output
+// Bound by the memory: a position costs 2 D values of traffic for 4 D operations a head,
+// and the products of 16 columns take a twentieth of the matrix cores' time.  Four
+// wavefronts take turns with groups of NS x 16 positions, without barriers; what they have
+// in flight at once is what hides the memory's latency.
+//
+// Positions are dealt out in chunks of one length for all sequences, so many that the chip
+// is full, by what the sequences' lengths turn out to be on the device (chunk_of); a
+// chunk's triple goes to the workspace where its sequence has several, and
+// cache_attention_join_kernel puts them together.
+// ---------------------------------------------------------------------------
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+template <int BYTES> struct Words;                 // of any address
+template <> struct Words<4> { typedef uint32_t type __attribute__((aligned(1))); };
+template <> struct Words<8> {
+  typedef uint32_t type __attribute__((ext_vector_type(2), aligned(1)));
+};
+template <> struct Words<16> {
+  typedef uint32_t type __attribute__((ext_vector_type(4), aligned(1)));
+};
+// two 8-bit values of a word, times their unit, in bfloat16 (exact)
+template <bool HIGH>
+__device__ __forceinline__ uint32_t widened(uint32_t word, float unit) {
+  return __builtin_bit_cast(
+      uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, unit, HIGH));
+}
+
+template <int BYTES>
+__device__ __forceinline__ void load_words(const uint8_t* at, uint32_t* to) {
+  typedef typename Words<BYTES>::type words_t;
+  const words_t v = *reinterpret_cast<const words_t*>(at);
+  if constexpr (BYTES == 4) {
+    to[0] = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < BYTES / 4; ++i) to[i] = v[i];
+  }
+}
+
+constexpr int HEADS = 16;                          // columns of a tile
+
+template <typename T, bool EIGHT, int DP>
+struct TileOf {
+  static constexpr int SIZE = EIGHT ? 1 : (int)sizeof(T);      // of a value in a page
+  static constexpr int KV = 16 / SIZE;                         // values of a key's piece
+  static constexpr int KC = DP / (4 * KV);                     // a lane's pieces of a key
+  static constexpr int VD = DP / 16;                           // a lane's values of a row,
+  static constexpr int VB = VD * SIZE < 16 ? VD * SIZE : 16;   // in pieces of VB bytes
+  static constexpr int VP = VD * SIZE / VB;
+  static constexpr int VE = VB / SIZE;                         // values of a piece
+  static constexpr bool WIDE = sizeof(T) == 4;                 // float32 products
+  // groups of 16 positions that a wavefront has in registers at once
+  static constexpr int NS = WIDE ? (EIGHT ? (DP == 256 ? 1 : 2) : (DP == 64 ? 2 : 1))
+                                 : (EIGHT ? (DP == 256 ? 2 : 4) : (DP == 64 ? 4 : 2));
+  static constexpr int GRAIN = 4 * 16 * NS;                    // positions of four wavefronts
+};
+
+// The chunks of all sequences, numbered sequence by sequence, in each unit (key / value
+// head and tile of its query heads) by unit.
+struct Chunks {
+  int units;                      // of a sequence
+  int grain;                      // a chunk's positions are a multiple
+  int target;                     // chunks that fill the chip
+};
+struct Chunk {
+  int b, unit, index, count;      // chunk `index` of `count` of a unit
+  int length;                     // of a chunk
+};
+
+__device__ __forceinline__ int chunk_count(int seen, int length) {
+  return max((int)(((int64_t)seen + length - 1) / length), 1);
+}
+
+// The positions of a chunk: all sequences' positions over `target` chunks.
+__device__ __forceinline__ int chunk_length(const Attention& a, const Chunks& c) {
+  const int lane = threadIdx.x & 63;
+  int64_t all = 0;
+  for (int b = lane; b < a.B; b += 64) all += seen_of(a, b);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) all += __shfl_xor(all, off, 64);
+  const int64_t each = (all * c.units + c.target - 1) / c.target;
+  return (int)(max((each + c.grain - 1) / c.grain, (int64_t)1) * c.grain);
+}
+
+// Number `id` of all chunks; false behind the last one.  The same for all lanes.
+__device__ __forceinline__ bool chunk_of(const Attention& a, const Chunks& c, int id,
+                                         Chunk* out) {
+  const int lane = threadIdx.x & 63;
+  const int length = chunk_length(a, c);
+  int before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int count = b0 + lane < a.B ? chunk_count(seen_of(a, b0 + lane), length) : 0;
+    int upto = count * c.units;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int other = __shfl_up(upto, off, 64);
+      if (lane >= off) upto += other;
+    }
+    const uint64_t behind = __ballot(before + upto > id);
+    if (behind) {
+      const int at = __builtin_ctzll(behind);
+      const int n = __builtin_amdgcn_readlane(count, at);
+      const int first = before + __builtin_amdgcn_readlane(upto, at) - n * c.units;
+      const int in = id - first;
+      out->b = b0 + at;
+      out->unit = in / n;
+      out->index = in - out->unit * n;
+      out->count = n;
+      out->length = length;
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+
+// PADDED: rows of fewer than DP values, or on any address.  SMALL: pages of fewer than 16
+// rows, whose rows are looked up one by one.
+template <typename T, bool EIGHT, int DP, bool PADDED, bool SMALL>
+__global__ __launch_bounds__(256) void cache_attention_tiles_kernel(
+    Attention a, Chunks chunks, float* __restrict__ part_o, float2* __restrict__ part_ml) {
+  typedef TileOf<T, EIGHT, DP> Tile;
+  constexpr int NS = Tile::NS, KC = Tile::KC, KV = Tile::KV, SIZE = Tile::SIZE;
+  constexpr int VD = Tile::VD, VP = Tile::VP, VE = Tile::VE, VB = Tile::VB;
+  constexpr int KW = 4;                              // words of a key's piece
+  constexpr int VW = VB / 4;                         // words of a value's piece
+  extern __shared__ __attribute__((aligned(16))) float joined[];
+  Chunk chunk;
+  if (!chunk_of(a, chunks, (int)blockIdx.x, &chunk)) return;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, j = lane >> 4;
+  const int b = __builtin_amdgcn_readfirstlane(chunk.b);
+  const int D = PADDED ? a.pages.D : DP, S = 1 << a.pages.shift;
+  const int tiles = (a.G + HEADS - 1) / HEADS;
+  const int kv_head = chunk.unit / tiles, head0 = (chunk.unit - kv_head * tiles) * HEADS;
+  const int heads = min(a.G - head0, HEADS);         // columns in use
+  const int columns = min(a.G, HEADS);
+  const int64_t first_head = (int64_t)kv_head * a.G + head0;
+  const int seen = seen_of(a, b);
+  const int first = chunk.index * chunk.length;
+  const int end = min((int64_t)first + chunk.length, (int64_t)seen);
+  const int last = a.position[b];
+  const int32_t* table = a.pages.table + (int64_t)b * a.pages.P;
+
+  // Where a lane's pieces of a row begin.  A piece that would end behind the row begins
+  // as much earlier; its first `extra` values are another piece's.
+  int k_at[KC], v_at[VP], k_extra[KC], v_extra[VP];
+#pragma unroll
+  for (int i = 0; i < KC; ++i) {
+    const int at = (j + 4 * i) * KV;
+    k_at[i] = PADDED ? min(at, D - KV) : at;
+    k_extra[i] = at - k_at[i];
+  }
+#pragma unroll
+  for (int p = 0; p < VP; ++p) {
+    const int at = p * 16 * VE + c * VE;
+    v_at[p] = PADDED ? min(at, D - VE) : at;
+    v_extra[p] = at - v_at[p];
+  }
+
+  // the queries, as the second operand of the first product; 0 where there is no head
+  constexpr int QN = Tile::WIDE ? KC * KV : KC * KV / 8;
+  typedef std::conditional_t<Tile::WIDE, float, bf16x8_t> query_t;
+  query_t q[QN];
+  {
+    const T* row = static_cast<const T*>(a.q) +
+                   ((int64_t)b * a.H + first_head + min(c, heads - 1)) * D;
+    constexpr int PER = 16 / sizeof(T);              // values of 16 bytes of q
+#pragma unroll
+    for (int i = 0; i < KC; ++i) {
+      const bool there = c < heads && (!PADDED || k_extra[i] < KV);
+#pragma unroll
+      for (int u = 0; u < KV / PER; ++u) {
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (there)
+          load_words<16>(reinterpret_cast<const uint8_t*>(row + k_at[i] + u * PER), w);
+        if constexpr (Tile::WIDE) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q[i * KV + u * 4 + e] = __uint_as_float(w[e]);
+        } else {
+          q[i * (KV / 8) + u] = __builtin_bit_cast(
+              bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
+        }
+      }
+    }
+  }
+
+  f32x4_t o[VD];
+#pragma unroll
+  for (int t = 0; t < VD; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+
+  const uint8_t* k_pages = static_cast<const uint8_t*>(a.k_pages);
+  const uint8_t* v_pages = static_cast<const uint8_t*>(a.v_pages);
+  for (int t0 = first + wave * (16 * NS); t0 < end; t0 += Tile::GRAIN) {
+    // ---- the rows' places, and which of them count
+    // (what does not count is read from a row that is there, and left out below)
+    int64_t k_row[NS], v_row[NS][SMALL ? 4 : 1];
+    bool v_there[NS][SMALL ? 4 : 1], whole = t0 + 16 * NS <= end;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      if constexpr (SMALL) {
+        const int t = t0 + 16 * s + c;
+        k_row[s] = t < end ? a.pages.row(b, t) : -1;
+        k_row[s] = a.pages.head(max(k_row[s], (int64_t)0), kv_head);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int u = t0 + 16 * s + 4 * j + r;
+          const int64_t row = u < end ? a.pages.row(b, u) : -1;
+          v_there[s][r] = row >= 0;
+          v_row[s][r] = a.pages.head(max(row, (int64_t)0), kv_head);
+        }
+        whole = false;
+      } else {
+        const int t = min(t0 + 16 * s, end - 1) & ~15;
+        const int page = table[t >> a.pages.shift];
+        const bool there = (unsigned)page < (unsigned)a.pages.N;
+        v_there[s][0] = there;
+        whole = whole && there;
+        k_row[s] = (((int64_t)(there ? page : 0) * a.pages.HK + kv_head)
+                    << a.pages.shift) + (t & (S - 1));
+        v_row[s][0] = k_row[s] + 4 * j;
+        k_row[s] += c;
+      }
+    }
+    // ---- keys and values
+    uint32_t kw[NS][KC][KW], vw[NS][4][VP][VW];
+    uint32_t k_unit[NS][2], v_unit[NS][4];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const uint8_t* row = k_pages + k_row[s] * D * SIZE;
+#pragma unroll
+      for (int i = 0; i < KC; ++i) {
+        if (!PADDED || k_extra[i] < KV) {
+          load_words<16>(row + k_at[i] * SIZE, kw[s][i]);
+        } else {
+#pragma unroll
+          for (int w = 0; w < KW; ++w) kw[s][i][w] = 0;
+        }
+      }
+      if constexpr (EIGHT) {
+        const uint8_t* unit = a.k_scales + k_row[s] * a.pages.DB;
+        k_unit[s][0] = unit[0];
+        if (DP == 256) k_unit[s][1] = unit[a.pages.DB - 1];
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int64_t at = SMALL ? v_row[s][SMALL ? r : 0] : v_row[s][0] + r;
+        const uint8_t* row = v_pages + at * D * SIZE;
+#pragma unroll
+        for (int p = 0; p < VP; ++p) {
+          if (!PADDED || v_extra[p] < VE) {
+            load_words<VB>(row + v_at[p] * SIZE, vw[s][r][p]);
+          } else {
+#pragma unroll
+            for (int w = 0; w < VW; ++w) vw[s][r][p][w] = 0;
+          }
+        }
+        if constexpr (EIGHT) {
+          const int block = DP == 256 ? min(c / 8, a.pages.DB - 1) : 0;
+          v_unit[s][r] = a.v_scales[at * a.pages.DB + block];
+        }
+      }
+    }
+    // ---- logits
+    float x[NS][4];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < KC; ++i) {
+        uint32_t* w = kw[s][i];
+        if constexpr (PADDED) {
+          // (another piece's values do not count twice)
+#pragma unroll
+          for (int e = 0; e < KW; ++e) {
+            const int bits = min(max(k_extra[i] * SIZE * 8 - 32 * e, 0), 32);
+            w[e] &= bits == 32 ? 0u : ~0u << bits;
+          }
+        }
+        if constexpr (EIGHT) {
+          const float unit = __uint_as_float(k_unit[s][DP == 256 ? i / 2 : 0] << 23);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if constexpr (Tile::WIDE) {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[2 * half + e], false);
+                const f32x2_t hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[2 * half + e], true);
+                const float f[4] = {lo[0] * unit, lo[1] * unit, hi[0] * unit, hi[1] * unit};
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                  sum = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                      f[u], q[i * KV + 8 * half + 4 * e + u], sum, 0, 0, 0);
+              }
+            } else {
+              uint4 wide;
+              wide.x = widened<false>(w[2 * half], unit);
+              wide.y = widened<true>(w[2 * half], unit);
+              wide.z = widened<false>(w[2 * half + 1], unit);
+              wide.w = widened<true>(w[2 * half + 1], unit);
+              sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                  __builtin_bit_cast(bf16x8_t, wide), q[i * 2 + half], sum, 0, 0, 0);
+            }
+          }
+        } else if constexpr (Tile::WIDE) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            sum = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                __uint_as_float(w[u]), q[i * KV + u], sum, 0, 0, 0);
+        } else {
+          sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3])), q[i], sum,
+              0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[s][r] = sum[r];
+    }
+    if (a.rel_values) {
+      const int h = (int)first_head + min(c, heads - 1);
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          x[s][r] += bias_of<T>(a, h, min(t0 + 16 * s + 4 * j + r, end - 1), last);
+    }
+    if (!whole) {
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const bool there = v_there[s][SMALL ? r : 0] && t0 + 16 * s + 4 * j + r < end;
+          if (there) continue;
+          x[s][r] = -INFINITY;
+#pragma unroll
+          for (int p = 0; p < VP; ++p)
+#pragma unroll
+            for (int w = 0; w < VW; ++w) vw[s][r][p][w] = 0;
+          if (EIGHT) v_unit[s][r] = FP8_UNIT;
+        }
+    }
+    // ---- weights
+    float top = m;
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) top = fmaxf(top, x[s][r]);
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    if (__any(top > m)) {
+      const float was = weight_of(m, top);
+      l *= was;
+#pragma unroll
+      for (int t = 0; t < VD; ++t) o[t] *= was;
+      m = top;
+    }
+    uint32_t wp[NS][2];                              // pairs of weights (bfloat16)
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[s][r] = weight_of(x[s][r], m);
+      if constexpr (!Tile::WIDE) {
+        wp[s][0] = f32x2_to_bf16x2(x[s][0], x[s][1]);
+        wp[s][1] = f32x2_to_bf16x2(x[s][2], x[s][3]);
+        l += __uint_as_float(wp[s][0] << 16) + __uint_as_float(wp[s][0] & 0xffff0000u);
+        l += __uint_as_float(wp[s][1] << 16) + __uint_as_float(wp[s][1] & 0xffff0000u);
+      } else {
+        l += (x[s][0] + x[s][1]) + (x[s][2] + x[s][3]);
+      }
+    }
+    // ---- sums of values
+    if constexpr (Tile::WIDE) {
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float unit = EIGHT ? __uint_as_float(v_unit[s][r] << 23) : 1.f;
+#pragma unroll
+          for (int p = 0; p < VP; ++p)
+#pragma unroll
+            for (int w = 0; w < VW; ++w) {
+              const uint32_t word = vw[s][r][p][w];
+              if constexpr (EIGHT) {
+                const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)word, false);
+                const f32x2_t hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)word, true);
+                const float f[4] = {lo[0] * unit, lo[1] * unit, hi[0] * unit, hi[1] * unit};
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                  o[p * VE + 4 * w + u] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                      f[u], x[s][r], o[p * VE + 4 * w + u], 0, 0, 0);
+              } else {
+                o[p * VE + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                    __uint_as_float(word), x[s][r], o[p * VE + w], 0, 0, 0);
+              }
+            }
+        }
+    } else {
+#pragma unroll
+      for (int s = 0; s < NS; s += 2) {
+        const bf16x8_t w = __builtin_bit_cast(
+            bf16x8_t, make_uint4(wp[s][0], wp[s][1], wp[s + 1][0], wp[s + 1][1]));
+#pragma unroll
+        for (int p = 0; p < VP; ++p)
+#pragma unroll
+          for (int pair = 0; pair < VE / 2; ++pair) {
+            uint32_t two[8];                         // values 2 pair, 2 pair + 1 of 8 positions
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int at = s + e / 4, r = e % 4;
+              if constexpr (EIGHT) {
+                const uint32_t word = vw[at][r][p][pair / 2];
+                const float unit = __uint_as_float(v_unit[at][r] << 23);
+                two[e] = pair & 1 ? widened<true>(word, unit) : widened<false>(word, unit);
+              } else {
+                two[e] = vw[at][r][p][pair];
+              }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              constexpr uint32_t PICK[2] = {0x05040100u, 0x07060302u};
+              uint4 v;
+              v.x = __builtin_amdgcn_perm(two[1], two[0], PICK[u]);
+              v.y = __builtin_amdgcn_perm(two[3], two[2], PICK[u]);
+              v.z = __builtin_amdgcn_perm(two[5], two[4], PICK[u]);
+              v.w = __builtin_amdgcn_perm(two[7], two[6], PICK[u]);
+              f32x4_t& sum = o[p * VE + 2 * pair + u];
+              sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                  __builtin_bit_cast(bf16x8_t, v), w, sum, 0, 0, 0);
+            }
+          }
+      }
+    }
+  }
+
+  // ---- the four wavefronts' triples
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  float* ms = joined;                                // [4][HEADS]
+  float* ls = ms + 4 * HEADS;                        // [4][HEADS]
+  float* os = ls + 4 * HEADS;                        // [4][heads][D]
+  if (lane < HEADS) {
+    ms[wave * HEADS + lane] = m;
+    ls[wave * HEADS + lane] = l;
+  }
+  if (c < heads) {
+    float* to = os + (wave * heads + c) * D;
+#pragma unroll
+    for (int p = 0; p < VP; ++p)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        // (row 4 j + r of the product is what lane c = 4 j + r read)
+        const int at = p * 16 * VE + (4 * j + r) * VE;
+        const int from = PADDED ? min(at, D - VE) : at;
+#pragma unroll
+        for (int u = 0; u < VE; ++u)
+          if (!PADDED || (from + u >= at && at < D)) to[from + u] = o[p * VE + u][r];
+      }
+  }
+  __syncthreads();
+  for (int h = 0; h < heads; ++h) {
+    float top = ms[h];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) top = fmaxf(top, ms[w * HEADS + h]);
+    float factor[4], all = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      factor[w] = weight_of(ms[w * HEADS + h], top);
+      all += ls[w * HEADS + h] * factor[w];
+    }
+    for (int d = threadIdx.x; d < D; d += 256) {
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) sum += os[(w * heads + h) * D + d] * factor[w];
+      if (chunk.count == 1) {
+        // (nothing seen: 0)
+        store_f32<T>(static_cast<T*>(a.out) +
+                         ((int64_t)b * a.H + first_head + h) * D + d,
+                     all == 0.f ? 0.f : sum / all);
+      } else {
+        part_o[((int64_t)blockIdx.x * columns + h) * D + d] = sum;
+      }
+    }
+    if (chunk.count > 1 && threadIdx.x == 0)
+      part_ml[(int64_t)blockIdx.x * columns + h] = make_float2(top, all);
+  }
+}
+
+// The chunks of a query head of a sequence put together: a block of 256 threads, whose
+// groups of as many as a row has values take every so many-th chunk.
+template <typename T>
+__global__ __launch_bounds__(256) void cache_attention_join_kernel(
+    Attention a, Chunks chunks, const float* __restrict__ part_o,
+    const float2* __restrict__ part_ml) {
+  extern __shared__ __attribute__((aligned(16))) float shared[];   // [chunks][256]
+  __shared__ float tops[4], sums[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int b = (int)(blockIdx.x / a.H), h = (int)(blockIdx.x - (int64_t)b * a.H);
+  const int D = a.pages.D;
+  const int length = chunk_length(a, chunks);
+  const int count = chunk_count(seen_of(a, b), length);
+  if (count == 1) return;
+  int before = 0;                                    // chunks of the sequences before
+  for (int i = lane; i < b; i += 64) before += chunk_count(seen_of(a, i), length);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) before += __shfl_xor(before, off, 64);
+  const int tiles = (a.G + HEADS - 1) / HEADS;
+  const int kv_head = h / a.G, in = h - kv_head * a.G;
+  const int unit = kv_head * tiles + in / HEADS;
+  const int64_t id = (int64_t)before * chunks.units + (int64_t)unit * count;
+  const int columns = min(a.G, HEADS);
+  const float2* ml = part_ml + id * columns + in % HEADS;
+  float top = -INFINITY;
+  for (int i = threadIdx.x; i < count; i += 256) {
+    const float m = ml[(int64_t)i * columns].x;
+    shared[i] = m;
+    top = fmaxf(top, m);
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  if (lane == 0) tops[wave] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; ++w) top = fmaxf(top, tops[w]);
+  float all = 0.f;
+  for (int i = threadIdx.x; i < count; i += 256) {
+    const float factor = weight_of(shared[i], top);
+    shared[i] = factor;
+    all += ml[(int64_t)i * columns].y * factor;
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) all += __shfl_xor(all, off, 64);
+  if (lane == 0) sums[wave] = all;
+  __syncthreads();
+  all = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  // (groups of 64, 128 or 256 threads)
+  const int wide = D <= 64 ? 64 : D <= 128 ? 128 : 256;
+  const int d = threadIdx.x & (wide - 1), group = threadIdx.x / wide;
+  float sum = 0.f;
+  if (d < D) {
+    const float* o = part_o + (id * columns + in % HEADS) * D + d;
+#pragma unroll 4
+    for (int i = group; i < count; i += 256 / wide)
+      sum += o[(int64_t)i * columns * D] * shared[i];
+  }
+  __shared__ float parts[256];
+  parts[threadIdx.x] = sum;
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  for (int g = 1; g < 256 / wide; ++g) sum += parts[g * wide + threadIdx.x];
+  store_f32<T>(static_cast<T*>(a.out) + ((int64_t)b * a.H + h) * D + d,
+               all == 0.f ? 0.f : sum / all);
+}
+
+// ---------------------------------------------------------------------------
 // the host's side
 // ---------------------------------------------------------------------------
 static bool on_16_bytes(std::initializer_list<const void*> all) {
@@ -344,6 +921,87 @@ static void run_read(const RowsOf& r, const void* k_pages, const void* v_pages,
                   : cache_read_kernel<T, EIGHT, false>;
   kern<<<grid, 256, 0, st>>>(r, k_pages, v_pages, k_scales, v_scales,
                              static_cast<T*>(k), static_cast<T*>(v));
+}
+
+constexpr int TARGET = 1024;      // chunks of all sequences: 4 for each of 256 CUs
+
+// How the tiles' kernel divides its work; no chunks where it does not apply.
+struct Division {
+  Chunks chunks;
+  int64_t blocks;                 // as many chunks as there can be
+  bool joins;                     // whether a sequence can have several
+  size_t part_o, part_ml, bytes;  // of the workspace
+};
+
+template <typename T, bool EIGHT>
+static int grain_of(int D) {
+  return D <= 64    ? TileOf<T, EIGHT, 64>::GRAIN
+         : D <= 128 ? TileOf<T, EIGHT, 128>::GRAIN
+                    : TileOf<T, EIGHT, 256>::GRAIN;
+}
+
+static Division divide(int B, int H, int HK, int D, int S, int P, int grain) {
+  Division v = {};
+  const int G = H / HK;
+  v.chunks.units = HK * ((G + HEADS - 1) / HEADS);
+  v.chunks.grain = grain;
+  v.chunks.target = TARGET;
+  const int64_t units = (int64_t)B * v.chunks.units, most = (int64_t)P * S;
+  v.blocks = std::min(units + v.chunks.target, units * ((most + grain - 1) / grain));
+  v.joins = most > grain;
+  if (v.joins) {
+    const size_t rows = (size_t)v.blocks * std::min(G, HEADS);
+    v.part_ml = (sizeof(float) * rows * D + 15) & ~(size_t)15;
+    v.bytes = v.part_ml + sizeof(float2) * rows + 16;
+  }
+  return v;
+}
+
+template <typename T, bool EIGHT, int DP, bool PADDED, bool SMALL>
+static int run_tiles(const Attention& a, const Division& v, char* workspace,
+                     hipStream_t st) {
+  auto kern = cache_attention_tiles_kernel<T, EIGHT, DP, PADDED, SMALL>;
+  const size_t lds =
+      sizeof(float) * 4 * (2 * HEADS + (size_t)std::min(a.G, HEADS) * a.pages.D);
+  MOE_ALLOW_LDS(kern, lds);
+  float* part_o = reinterpret_cast<float*>(workspace);
+  float2* part_ml = reinterpret_cast<float2*>(workspace + v.part_ml);
+  kern<<<(unsigned)v.blocks, 256, lds, st>>>(a, v.chunks, part_o, part_ml);
+  MOE_CHECK_LAUNCH("cache_attention");
+  if (v.joins) {
+    const size_t most = sizeof(float) * (v.chunks.target / v.chunks.units + 2);
+    cache_attention_join_kernel<T><<<(unsigned)((int64_t)a.B * a.H), 256, most, st>>>(
+        a, v.chunks, part_o, part_ml);
+    MOE_CHECK_LAUNCH("cache_attention");
+  }
+  return 0;
+}
+
+template <typename T, bool EIGHT>
+static int run_attention(const Attention& a, const Division& v, char* workspace,
+                         hipStream_t st) {
+  const int D = a.pages.D;
+  if (D < 16) {
+    cache_attention_kernel<T, EIGHT><<<(unsigned)((int64_t)a.B * a.H), 256, 0, st>>>(a);
+    MOE_CHECK_LAUNCH("cache_attention");
+    return 0;
+  }
+  const int DP = D <= 64 ? 64 : D <= 128 ? 128 : 256;
+  const bool small = a.pages.shift < 4;
+  const bool padded = small || D != DP || !on_16_bytes({a.q, a.k_pages, a.v_pages});
+#define TILES(dp)                                                                     \
+  (small    ? run_tiles<T, EIGHT, dp, true, true>                                     \
+   : padded ? run_tiles<T, EIGHT, dp, true, false>                                    \
+            : run_tiles<T, EIGHT, dp, false, false>)
+  auto run = DP == 64 ? TILES(64) : DP == 128 ? TILES(128) : TILES(256);
+#undef TILES
+  return run(a, v, workspace, st);
+}
+
+static int grain_of(int D, int dtype, bool eight) {
+  return dtype == MESH_MOE_BF16
+             ? (eight ? grain_of<bf16_t, true>(D) : grain_of<bf16_t, false>(D))
+             : (eight ? grain_of<float, true>(D) : grain_of<float, false>(D));
 }
 
 }  // namespace mesh_moe
@@ -410,9 +1068,12 @@ extern "C" int mesh_moe_cache_read(const void* k_pages, const void* v_pages,
 }
 
 extern "C" size_t mesh_moe_cache_attention_workspace_bytes(int B, int H, int HK, int D,
-                                                           int S, int P) {
-  (void)B, (void)H, (void)HK, (void)D, (void)S, (void)P;
-  return 0;
+                                                           int S, int P, int dtype,
+                                                           int eight_bit) {
+  if (B < 1 || H < 1 || HK < 1 || H % HK || D < 16 || D > MAX_WIDTH || S < 1 || P < 1 ||
+      !valid_dtype(dtype))
+    return 0;
+  return divide(B, H, HK, D, S, P, grain_of(D, dtype, eight_bit != 0)).bytes;
 }
 
 extern "C" int mesh_moe_cache_attention(
@@ -434,10 +1095,12 @@ extern "C" int mesh_moe_cache_attention(
               "reach go together");
   MOE_REQUIRE((int64_t)B * H <= MAX_BLOCKS, MESH_MOE_E_UNSUPPORTED,
               "cache_attention: %d sequences of %d heads are more than a launch has", B, H);
-  MOE_REQUIRE(workspace_bytes >=
-                  mesh_moe_cache_attention_workspace_bytes(B, H, HK, D, S, P),
-              MESH_MOE_E_ARG, "cache_attention: workspace too small");
-  (void)workspace;
+  Division v = {};
+  if (D >= 16) v = divide(B, H, HK, D, S, P, grain_of(D, dtype, k_scales != nullptr));
+  MOE_REQUIRE(v.blocks <= MAX_BLOCKS, MESH_MOE_E_UNSUPPORTED,
+              "cache_attention: %d sequences of %d heads are more than a launch has", B, H);
+  MOE_REQUIRE(v.bytes == 0 || (workspace && workspace_bytes >= v.bytes), MESH_MOE_E_ARG,
+              "cache_attention: workspace too small");
   if (k_new) {
     if (int rc = mesh_moe_cache_write(k_new, v_new, table, position, nullptr, k_pages,
                                       v_pages, k_scales, v_scales, B, 1, HK, D, N, S, P,
@@ -459,13 +1122,10 @@ extern "C" int mesh_moe_cache_attention(
   a.H = H;
   a.G = H / HK;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const unsigned grid = (unsigned)((int64_t)B * H);
-  auto kern = dtype == MESH_MOE_BF16
-                  ? (k_scales ? cache_attention_kernel<bf16_t, true>
-                              : cache_attention_kernel<bf16_t, false>)
-                  : (k_scales ? cache_attention_kernel<float, true>
-                              : cache_attention_kernel<float, false>);
-  kern<<<grid, 256, 0, st>>>(a);
-  MOE_CHECK_LAUNCH("cache_attention");
-  return 0;
+  char* at = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(workspace) + 15) &
+                                     ~(uintptr_t)15);
+  auto run = dtype == MESH_MOE_BF16
+                 ? (k_scales ? run_attention<bf16_t, true> : run_attention<bf16_t, false>)
+                 : (k_scales ? run_attention<float, true> : run_attention<float, false>);
+  return run(a, v, at, st);
 }

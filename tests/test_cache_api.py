@@ -156,7 +156,7 @@ def test_attention_refusals(lib):
   _refused(lib, with_(_21=5), -1, "dtype")
   _refused(lib, with_(_17=260), -2, "256")
   _refused(lib, with_(_14=1 << 30), -2, "more than a launch")
-  need = lib.mesh_moe_cache_attention_workspace_bytes(2, 8, 4, 64, 16, 1 << 20)
+  need = lib.mesh_moe_cache_attention_workspace_bytes(2, 8, 4, 64, 16, 1 << 20, 1, 1)
   if need:
     _refused(lib, with_(_20=1 << 20, _23=need - 1), -1, "workspace")
     _refused(lib, with_(_20=1 << 20, _22=None), -1, "workspace")
