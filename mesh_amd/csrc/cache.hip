@@ -1,6 +1,7 @@
 // The paged cache: rows of keys and values into pages and back, and attention of one new
 // token over them.
 #include "../../include/mesh_moe_cache.h"
+#include "arrival.h"
 #include "fp8.h"
 
 #include <algorithm>
@@ -185,6 +186,7 @@ struct Attention {
   Pages pages;
   const void *q, *k_pages, *v_pages;
   const uint8_t *k_scales, *v_scales;
+  const void *k_new, *v_new;      // the step's own row, which goes into the pages, or null
   const int32_t* position;        // [B]
   const void* rel_values;         // [H][NB] or null
   const int32_t* rel_bucket;      // [2 * reach - 1]
@@ -208,9 +210,11 @@ __device__ __forceinline__ float bias_of(const Attention& a, int h, int j, int l
                      min(max(bucket, 0), a.NB - 1));
 }
 
-// e^(x - m) with m >= x; 0 for x = -infinity
+// e^(x - m) with m >= x; 0 for x = -infinity.  (The difference first: it is exact where it
+// matters, and what is lost of a larger one is lost of a small weight.)
 __device__ __forceinline__ float weight_of(float x, float m) {
-  return x == -INFINITY ? 0.f : expf(x - m);
+  return x == -INFINITY ? 0.f
+                        : __builtin_amdgcn_exp2f((x - m) * 1.4426950408889634f);
 }
 
 template <typename T, bool EIGHT>
@@ -304,10 +308,10 @@ __global__ __launch_bounds__(256) void cache_attention_kernel(Attention a) {
 // wavefronts take turns with groups of NS x 16 positions, without barriers; what they have
 // in flight at once is what hides the memory's latency.
 //
-// Positions are dealt out in chunks of one length for all sequences, so many that the chip
-// is full, by what the sequences' lengths turn out to be on the device (chunk_of); a
-// chunk's triple goes to the workspace where its sequence has several, and
-// cache_attention_join_kernel puts them together.
+// The work is dealt out evenly to as many blocks as the chip holds at once, by what the
+// sequences' lengths turn out to be on the device (run_of).  Where a unit's positions fall
+// to several blocks, their triples go to the workspace, and the block that arrives there
+// last puts them together.
 // ---------------------------------------------------------------------------
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
@@ -356,95 +360,312 @@ struct TileOf {
   static constexpr int NS = WIDE ? (EIGHT ? (DP == 256 ? 1 : 2) : (DP == 64 ? 2 : 1))
                                  : (EIGHT ? (DP == 256 ? 2 : 4) : (DP == 64 ? 4 : 2));
   static constexpr int GRAIN = 4 * 16 * NS;                    // positions of four wavefronts
+  // blocks that a CU holds at once
+  template <bool PADDED>
+  static constexpr int at_once() {
+    return DP == 256 ? 1 : 2;
+  }
 };
 
-// The chunks of all sequences, numbered sequence by sequence, in each unit (key / value
-// head and tile of its query heads) by unit.
-struct Chunks {
+// How the work is divided.  A unit is a key / value head of a sequence with a tile of its
+// query heads; its positions come in grains of Tile::GRAIN (one at least).  The grains of
+// all units, sequence by sequence, are dealt out in runs of equal length, a block each.
+struct Shares {
   int units;                      // of a sequence
-  int grain;                      // a chunk's positions are a multiple
-  int target;                     // chunks that fill the chip
-};
-struct Chunk {
-  int b, unit, index, count;      // chunk `index` of `count` of a unit
-  int length;                     // of a chunk
+  int grain;
+  int blocks;                     // at most
 };
 
-__device__ __forceinline__ int chunk_count(int seen, int length) {
-  return max((int)(((int64_t)seen + length - 1) / length), 1);
+__device__ __forceinline__ int grains_of(int seen, int grain) {
+  return max((seen + grain - 1) / grain, 1);
 }
 
-// The positions of a chunk: all sequences' positions over `target` chunks.
-__device__ __forceinline__ int chunk_length(const Attention& a, const Chunks& c) {
-  const int lane = threadIdx.x & 63;
-  int64_t all = 0;
-  for (int b = lane; b < a.B; b += 64) all += seen_of(a, b);
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) all += __shfl_xor(all, off, 64);
-  const int64_t each = (all * c.units + c.target - 1) / c.target;
-  return (int)(max((each + c.grain - 1) / c.grain, (int64_t)1) * c.grain);
+// Sums over the lanes up to each, in six steps without LDS.
+__device__ __forceinline__ int sums_up_to(int v) {
+#define STEP(ctrl, rows)                                                              \
+  v += __builtin_amdgcn_update_dpp(0, v, ctrl, rows, 0xf, false)
+  STEP(0x111, 0xf);               // row_shr by 1, 2, 4, 8
+  STEP(0x112, 0xf);
+  STEP(0x114, 0xf);
+  STEP(0x118, 0xf);
+  STEP(0x142, 0xa);               // a row's last lane to the next row
+  STEP(0x143, 0xc);               // ... to the next two
+#undef STEP
+  return v;
 }
 
-// Number `id` of all chunks; false behind the last one.  The same for all lanes.
-__device__ __forceinline__ bool chunk_of(const Attention& a, const Chunks& c, int id,
-                                         Chunk* out) {
+// A block's run of grains, and where the first one is.
+struct Run {
+  int first, count;               // of all grains
+  int b, unit, grain;             // sequence, unit and grain of that
+  int of_unit;                    // grains of that unit
+};
+struct Runs {
+  int blocks, each, longer;       // `longer` of the blocks have one grain more than `each`
+  __device__ __forceinline__ int first(int block) const {
+    return block * each + min(block, longer);
+  }
+  __device__ __forceinline__ int block_of(int grain) const {
+    const int more = longer * (each + 1);
+    return grain < more ? grain / (each + 1) : longer + (grain - more) / each;
+  }
+};
+
+// false for a block without work.  The same for all lanes of a wavefront.
+__device__ __forceinline__ bool run_of(const Attention& a, const Shares& s, int block,
+                                       Runs* runs, Run* run) {
   const int lane = threadIdx.x & 63;
-  const int length = chunk_length(a, c);
-  int before = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int count = b0 + lane < a.B ? chunk_count(seen_of(a, b0 + lane), length) : 0;
-    int upto = count * c.units;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int other = __shfl_up(upto, off, 64);
-      if (lane >= off) upto += other;
-    }
-    const uint64_t behind = __ballot(before + upto > id);
+  auto grains = [&](int b) { return b < a.B ? grains_of(seen_of(a, b), s.grain) : 0; };
+  const int of_lane = grains(lane);
+  int up_to = sums_up_to(of_lane), all = __builtin_amdgcn_readlane(up_to, 63);
+  for (int b = 64; b < a.B; b += 64)
+    all += __builtin_amdgcn_readlane(sums_up_to(grains(b + lane)), 63);
+  all *= s.units;
+  runs->blocks = min(s.blocks, all);
+  if (block >= runs->blocks) return false;
+  runs->each = all / runs->blocks;
+  runs->longer = all - runs->each * runs->blocks;
+  run->first = runs->first(block);
+  run->count = runs->each + (block < runs->longer ? 1 : 0);
+  int before = 0, count = of_lane;                   // grains of units of one kind
+  for (int b = 0;; b += 64) {
+    const uint64_t behind =
+        __ballot((int64_t)(before + up_to) * s.units > (int64_t)run->first);
     if (behind) {
       const int at = __builtin_ctzll(behind);
-      const int n = __builtin_amdgcn_readlane(count, at);
-      const int first = before + __builtin_amdgcn_readlane(upto, at) - n * c.units;
-      const int in = id - first;
-      out->b = b0 + at;
-      out->unit = in / n;
-      out->index = in - out->unit * n;
-      out->count = n;
-      out->length = length;
+      run->b = b + at;
+      run->of_unit = __builtin_amdgcn_readlane(count, at);
+      const int in = run->first - (before + __builtin_amdgcn_readlane(up_to, at) -
+                                   run->of_unit) * s.units;
+      run->unit = in / run->of_unit;
+      run->grain = in - run->unit * run->of_unit;
       return true;
     }
-    before += __builtin_amdgcn_readlane(upto, 63);
+    before += __builtin_amdgcn_readlane(up_to, 63);
+    if (b + 64 >= a.B) return false;                 // (not reached)
+    count = grains(b + 64 + lane);
+    up_to = sums_up_to(count);
   }
-  return false;
+}
+
+// A wavefront keeps the step's key (of = 0) or value: in `row` and `units`, and in the page
+// where `writes` says so.
+template <typename T, bool EIGHT>
+__device__ __forceinline__ void keep_row(const Attention& a, int of, int b, int kv_head,
+                                         int64_t to, bool writes, uint8_t* row,
+                                         uint8_t* units) {
+  const int lane = threadIdx.x & 63, D = a.pages.D, at = lane * 8;
+  const bool own = of == 0 || a.v_new != nullptr;    // (else the key is the value)
+  const T* x = static_cast<const T*>(of && own ? a.v_new : a.k_new) +
+               ((int64_t)b * a.pages.HK + kv_head) * D;
+  void* pages = const_cast<void*>(of ? a.v_pages : a.k_pages);
+  uint8_t* scales = const_cast<uint8_t*>(of ? a.v_scales : a.k_scales);
+  float f[8];
+  load8<T, false>(x, at, D, f);
+  if constexpr (EIGHT) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, magnitude_bits(f[e]));
+    const Fp8Scale s = fp8_scale(max_of_lanes(top, 16));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] *= s.factor;
+    const uint32_t lo = fp8_pack4(f[0], f[1], f[2], f[3]);
+    const uint32_t hi = fp8_pack4(f[4], f[5], f[6], f[7]);
+    uint8_t* page = static_cast<uint8_t*>(pages) + to * D;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (at + e < D) {
+        const uint8_t byte = (uint8_t)((e < 4 ? lo : hi) >> 8 * (e & 3));
+        row[at + e] = byte;
+        if (writes && own) page[at + e] = byte;
+      }
+    if (at < D && lane % 16 == 0) {
+      units[lane / 16] = (uint8_t)s.byte;
+      if (writes && own) scales[to * a.pages.DB + lane / 16] = (uint8_t)s.byte;
+    }
+  } else {
+    T* page = static_cast<T*>(pages) + to * D;
+    T* kept = reinterpret_cast<T*>(row);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (at + e < D) {
+        store_f32<T>(kept + at + e, f[e]);
+        if (writes && own) store_f32<T>(page + at + e, f[e]);
+      }
+  }
+}
+
+// Units that fall to several blocks.  A block has a place in the workspace for the triple
+// of the unit it begins with (if that began before) and for the one it ends with.  A unit's
+// parts are put together by the block that arrives last; many of them (one sequence over
+// the whole chip has hundreds) in groups first, each by its last block, so that no block
+// reads more than PARTS.
+constexpr int PARTS = 32;
+
+__device__ __forceinline__ unsigned long long two_floats(float a, float b) {
+  return (unsigned long long)__float_as_uint(a) |
+         (unsigned long long)__float_as_uint(b) << 32;
+}
+__device__ __forceinline__ float low_float(unsigned long long v) {
+  return __uint_as_float((uint32_t)v);
+}
+__device__ __forceinline__ float high_float(unsigned long long v) {
+  return __uint_as_float((uint32_t)(v >> 32));
+}
+
+struct Joins {
+  unsigned long long* tops;       // [places][columns]: largest logit, sum of weights
+  unsigned long long* sums;       // [places][columns][(D + 1) / 2]: two values each
+  unsigned long long* group_counters;   // [places]: of a group's first part
+  unsigned long long* unit_counters;    // [places]: of a unit's first part
+  unsigned long long call;
+};
+
+// A block's part of a unit.
+struct Part {
+  int from, count;                // the unit's first block, and how many it has
+  int in_group, groups;           // parts of a group, groups
+  int group, index;               // this part's, and its number in the group
+  __device__ __forceinline__ int64_t place(int part) const {
+    return 2 * (int64_t)(from + part) + (part == 0 ? 1 : 0);
+  }
+  __device__ __forceinline__ Part(const Runs& runs, int first_grain, int grains) {
+    from = runs.block_of(first_grain);
+    count = runs.block_of(first_grain + grains - 1) - from + 1;
+    in_group = count <= PARTS ? count : (int)ceilf(sqrtf((float)count));
+    groups = (count + in_group - 1) / in_group;
+    index = (int)blockIdx.x - from;
+    group = index / in_group;
+    index -= group * in_group;
+  }
+};
+
+struct JoinSpace {
+  float factors[HEADS][PARTS], tops[HEADS], all[HEADS];
+  float sums[2][256];
+  int last;
+};
+
+// Joins `count` (up to PARTS) parts of a unit, the first being `first` and each `step`
+// behind the one before; the result goes to `out`, or (null) to the first part's place.  A
+// block of 256 threads.
+template <typename T>
+__device__ __forceinline__ void join_parts(const Joins& joins, const Part& part, int first,
+                                           int step, int count, int heads, int columns,
+                                           int D, JoinSpace& space, T* out) {
+  const int halves = (D + 1) / 2, items = heads * halves;
+  {
+    const int i = threadIdx.x & (PARTS - 1);
+    for (int h = threadIdx.x / PARTS; h < heads; h += 256 / PARTS) {
+      unsigned long long ml = two_floats(-INFINITY, 0.f);
+      if (i < count) ml = ld_dev(joins.tops + part.place(first + i * step) * columns + h);
+      float top = low_float(ml);
+#pragma unroll
+      for (int off = PARTS / 2; off > 0; off >>= 1)
+        top = fmaxf(top, __shfl_xor(top, off, 64));
+      const float factor = weight_of(low_float(ml), top);
+      float all = high_float(ml) * factor;
+#pragma unroll
+      for (int off = PARTS / 2; off > 0; off >>= 1) all += __shfl_xor(all, off, 64);
+      space.factors[h][i] = factor;
+      if (i == 0) {
+        space.tops[h] = top;
+        space.all[h] = all;
+      }
+    }
+  }
+  // (few items: the parts are dealt out to groups of threads, a power of two each)
+  int shift = 5;
+  while (shift < 8 && (1 << shift) < items) ++shift;
+  const int group = threadIdx.x >> shift, groups = 256 >> shift;
+  const int64_t place = part.place(first);
+  __syncthreads();
+  for (int item0 = threadIdx.x & ((1 << shift) - 1); item0 < ((items - 1) | 255) + 1;
+       item0 += 4 * 256) {
+    constexpr int IN_FLIGHT = 8;
+    float sum[4][2];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) sum[n][0] = sum[n][1] = 0.f;
+    for (int i0 = group; i0 < count; i0 += IN_FLIGHT * groups) {
+      unsigned long long v[4][IN_FLIGHT];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        if (n * 256 >= items) break;
+        const int item = min(item0 + n * 256, items - 1), h = item / halves;
+        const int64_t at = (int64_t)h * halves + (item - h * halves);
+#pragma unroll
+        for (int u = 0; u < IN_FLIGHT; ++u) {
+          const int i = min(i0 + u * groups, count - 1);
+          v[n][u] = ld_dev(joins.sums + part.place(first + i * step) * columns * halves + at);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        if (n * 256 >= items) break;
+        const int h = min(item0 + n * 256, items - 1) / halves;
+#pragma unroll
+        for (int u = 0; u < IN_FLIGHT; ++u) {
+          const int i = i0 + u * groups;
+          const float factor = i < count ? space.factors[h][i] : 0.f;
+          // (what is not a part is left out, whatever it is)
+          sum[n][0] += i < count ? low_float(v[n][u]) * factor : 0.f;
+          sum[n][1] += i < count ? high_float(v[n][u]) * factor : 0.f;
+        }
+      }
+    }
+    if (groups > 1) {
+      space.sums[0][threadIdx.x] = sum[0][0];
+      space.sums[1][threadIdx.x] = sum[0][1];
+      __syncthreads();
+      if (group == 0)
+        for (int g = 1; g < groups; ++g) {
+          sum[0][0] += space.sums[0][threadIdx.x + (g << shift)];
+          sum[0][1] += space.sums[1][threadIdx.x + (g << shift)];
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int item = item0 + n * 256;
+      if (item >= items || group != 0) break;
+      const int h = item / halves, d = 2 * (item - h * halves);
+      if (out) {
+        const float all = space.all[h];
+        // (no weights: 0)
+        store_f32<T>(out + (int64_t)h * D + d, all == 0.f ? 0.f : sum[n][0] / all);
+        if (d + 1 < D)
+          store_f32<T>(out + (int64_t)h * D + d + 1, all == 0.f ? 0.f : sum[n][1] / all);
+      } else {
+        st_dev(joins.sums + (place * columns + h) * halves + d / 2,
+               two_floats(sum[n][0], sum[n][1]));
+        if (d == 0)
+          st_dev(joins.tops + place * columns + h, two_floats(space.tops[h], space.all[h]));
+      }
+    }
+  }
 }
 
 // PADDED: rows of fewer than DP values, or on any address.  SMALL: pages of fewer than 16
 // rows, whose rows are looked up one by one.
 template <typename T, bool EIGHT, int DP, bool PADDED, bool SMALL>
-__global__ __launch_bounds__(256) void cache_attention_tiles_kernel(
-    Attention a, Chunks chunks, float* __restrict__ part_o, float2* __restrict__ part_ml) {
+__global__ __launch_bounds__(256, (TileOf<T, EIGHT, DP>::template at_once<PADDED>()))
+void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
   typedef TileOf<T, EIGHT, DP> Tile;
   constexpr int NS = Tile::NS, KC = Tile::KC, KV = Tile::KV, SIZE = Tile::SIZE;
   constexpr int VD = Tile::VD, VP = Tile::VP, VE = Tile::VE, VB = Tile::VB;
   constexpr int KW = 4;                              // words of a key's piece
   constexpr int VW = VB / 4;                         // words of a value's piece
   extern __shared__ __attribute__((aligned(16))) float joined[];
-  Chunk chunk;
-  if (!chunk_of(a, chunks, (int)blockIdx.x, &chunk)) return;
+  __shared__ JoinSpace space;
+  __shared__ __attribute__((aligned(16))) uint8_t fresh_rows[2][DP * SIZE];
+  __shared__ uint8_t fresh_units[2][2];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Runs runs;
+  Run run;
+  if (!run_of(a, shares, (int)blockIdx.x, &runs, &run)) return;
   const int c = lane & 15, j = lane >> 4;
-  const int b = __builtin_amdgcn_readfirstlane(chunk.b);
   const int D = PADDED ? a.pages.D : DP, S = 1 << a.pages.shift;
-  const int tiles = (a.G + HEADS - 1) / HEADS;
-  const int kv_head = chunk.unit / tiles, head0 = (chunk.unit - kv_head * tiles) * HEADS;
-  const int heads = min(a.G - head0, HEADS);         // columns in use
-  const int columns = min(a.G, HEADS);
-  const int64_t first_head = (int64_t)kv_head * a.G + head0;
-  const int seen = seen_of(a, b);
-  const int first = chunk.index * chunk.length;
-  const int end = min((int64_t)first + chunk.length, (int64_t)seen);
-  const int last = a.position[b];
-  const int32_t* table = a.pages.table + (int64_t)b * a.pages.P;
+  const int tiles = (a.G + HEADS - 1) / HEADS, columns = min(a.G, HEADS);
 
   // Where a lane's pieces of a row begin.  A piece that would end behind the row begins
   // as much earlier; its first `extra` values are another piece's.
@@ -460,6 +681,28 @@ __global__ __launch_bounds__(256) void cache_attention_tiles_kernel(
     const int at = p * 16 * VE + c * VE;
     v_at[p] = PADDED ? min(at, D - VE) : at;
     v_extra[p] = at - v_at[p];
+  }
+
+  for (int at_grain = run.first, left = run.count; left > 0;) {
+  // ---- the next unit, or what of it falls to this block
+  const int b = __builtin_amdgcn_readfirstlane(run.b);
+  const int unit = __builtin_amdgcn_readfirstlane(run.unit);
+  const int taken = min(left, run.of_unit - run.grain);
+  const bool begins = run.grain == 0, ends = run.grain + taken == run.of_unit;
+  const int kv_head = unit / tiles, head0 = (unit - kv_head * tiles) * HEADS;
+  const int heads = min(a.G - head0, HEADS);         // columns in use
+  const int64_t first_head = (int64_t)kv_head * a.G + head0;
+  const int seen = seen_of(a, b), last = a.position[b];
+  const int first = run.grain * Tile::GRAIN;
+  const int end = (int)min((int64_t)first + (int64_t)taken * Tile::GRAIN, (int64_t)seen);
+  const int32_t* table = a.pages.table + (int64_t)b * a.pages.P;
+  const Part part(runs, at_grain - run.grain, run.of_unit);
+  unsigned long long group_was = 0, unit_was = 0;
+  if (part.count > 1 && part.index == 0 && threadIdx.x == 0) {
+    group_was = counter_prepare(
+        joins.group_counters + part.place(part.group * part.in_group), joins.call);
+    if (part.group == 0 && part.groups > 1)
+      unit_was = counter_prepare(joins.unit_counters + part.place(0), joins.call);
   }
 
   // the queries, as the second operand of the first product; 0 where there is no head
@@ -493,6 +736,20 @@ __global__ __launch_bounds__(256) void cache_attention_tiles_kernel(
 #pragma unroll
   for (int t = 0; t < VD; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
+
+  // The step's own row: written by the block that ends its unit (of the head's first tile),
+  // which reads it from LDS.
+  bool fresh = false;
+  if (a.k_new && ends && last >= 0) {
+    const int64_t to = a.pages.row(b, last);
+    fresh = to >= 0;
+    if (fresh) {
+      __syncthreads();                               // (the unit before is done with them)
+      if (wave < 2) keep_row<T, EIGHT>(a, wave, b, kv_head, a.pages.head(to, kv_head),
+                                       head0 == 0, fresh_rows[wave], fresh_units[wave]);
+      __syncthreads();
+    }
+  }
 
   const uint8_t* k_pages = static_cast<const uint8_t*>(a.k_pages);
   const uint8_t* v_pages = static_cast<const uint8_t*>(a.v_pages);
@@ -566,6 +823,30 @@ __global__ __launch_bounds__(256) void cache_attention_tiles_kernel(
         if constexpr (EIGHT) {
           const int block = DP == 256 ? min(c / 8, a.pages.DB - 1) : 0;
           v_unit[s][r] = a.v_scales[at * a.pages.DB + block];
+        }
+      }
+    }
+    if (fresh && t0 <= last && last < t0 + 16 * NS) {
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        if (t0 + 16 * s + c == last) {
+#pragma unroll
+          for (int i = 0; i < KC; ++i)
+            if (!PADDED || k_extra[i] < KV)
+              load_words<16>(fresh_rows[0] + k_at[i] * SIZE, kw[s][i]);
+          if (EIGHT) {
+            k_unit[s][0] = fresh_units[0][0];
+            if (DP == 256) k_unit[s][1] = fresh_units[0][1];
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (t0 + 16 * s + 4 * j + r != last) continue;
+#pragma unroll
+          for (int p = 0; p < VP; ++p)
+            if (!PADDED || v_extra[p] < VE)
+              load_words<VB>(fresh_rows[1] + v_at[p] * SIZE, vw[s][r][p]);
+          if (EIGHT) v_unit[s][r] = fresh_units[1][DP == 256 ? c / 8 : 0];
         }
       }
     }
@@ -746,6 +1027,7 @@ __global__ __launch_bounds__(256) void cache_attention_tiles_kernel(
   float* ms = joined;                                // [4][HEADS]
   float* ls = ms + 4 * HEADS;                        // [4][HEADS]
   float* os = ls + 4 * HEADS;                        // [4][heads][D]
+  __syncthreads();                                   // (the unit before is done with them)
   if (lane < HEADS) {
     ms[wave * HEADS + lane] = m;
     ls[wave * HEADS + lane] = l;
@@ -765,98 +1047,76 @@ __global__ __launch_bounds__(256) void cache_attention_tiles_kernel(
       }
   }
   __syncthreads();
-  for (int h = 0; h < heads; ++h) {
+  const bool whole_unit = part.count == 1;
+  const int64_t place = part.place(part.group * part.in_group + part.index);
+  T* out = static_cast<T*>(a.out) + ((int64_t)b * a.H + first_head) * D;
+  // (two values a thread, as they go to the workspace)
+  const int halves = (D + 1) / 2;
+  for (int i = threadIdx.x; i < heads * halves; i += 256) {
+    const int h = i / halves, d = 2 * (i - h * halves);
     float top = ms[h];
 #pragma unroll
     for (int w = 1; w < 4; ++w) top = fmaxf(top, ms[w * HEADS + h]);
-    float factor[4], all = 0.f;
+    float sum[2] = {0.f, 0.f}, all = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      factor[w] = weight_of(ms[w * HEADS + h], top);
-      all += ls[w * HEADS + h] * factor[w];
+      const float factor = weight_of(ms[w * HEADS + h], top);
+      const float* from = os + (w * heads + h) * D + d;
+      sum[0] += from[0] * factor;
+      if (!PADDED || d + 1 < D) sum[1] += from[1] * factor;
+      all += ls[w * HEADS + h] * factor;
     }
-    for (int d = threadIdx.x; d < D; d += 256) {
-      float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) sum += os[(w * heads + h) * D + d] * factor[w];
-      if (chunk.count == 1) {
-        // (nothing seen: 0)
-        store_f32<T>(static_cast<T*>(a.out) +
-                         ((int64_t)b * a.H + first_head + h) * D + d,
-                     all == 0.f ? 0.f : sum / all);
-      } else {
-        part_o[((int64_t)blockIdx.x * columns + h) * D + d] = sum;
+    if (whole_unit) {
+      // (nothing seen: 0)
+      store_f32<T>(out + (int64_t)h * D + d, all == 0.f ? 0.f : sum[0] / all);
+      if (!PADDED || d + 1 < D)
+        store_f32<T>(out + (int64_t)h * D + d + 1, all == 0.f ? 0.f : sum[1] / all);
+    } else {
+      st_dev(joins.sums + (place * columns + h) * halves + d / 2, two_floats(sum[0], sum[1]));
+      if (d == 0) st_dev(joins.tops + place * columns + h, two_floats(top, all));
+    }
+  }
+  if (!whole_unit) {
+    // Once all stores of the block are out, it arrives at its group's counter, the last
+    // block of a group at the unit's (which part 0 stamped, and settles here).
+    const int group_first = part.group * part.in_group;
+    if (threadIdx.x == 0 && part.index == 0) {
+      counter_settle(joins.group_counters + place, joins.call, group_was);
+      if (group_first == 0 && part.groups > 1)
+        counter_settle(joins.unit_counters + place, joins.call, unit_was);
+    }
+    int join_first = group_first, step = 1;
+    int parts = min(part.in_group, part.count - group_first);
+    for (;;) {
+      unsigned long long* counter = (step == 1 ? joins.group_counters : joins.unit_counters) +
+                                    part.place(join_first);
+      wait_stores();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        space.last = arrive_is_last(counter, joins.call, (unsigned)parts);
+        if (space.last) st_dev(counter, 0ull);
       }
+      __syncthreads();
+      if (!space.last) break;
+      const bool done = step > 1 || part.groups == 1;
+      join_parts<T>(joins, part, join_first, step, parts, heads, columns, D, space,
+                    done ? out : nullptr);
+      if (done) break;
+      join_first = 0;
+      step = part.in_group;
+      parts = part.groups;
     }
-    if (chunk.count > 1 && threadIdx.x == 0)
-      part_ml[(int64_t)blockIdx.x * columns + h] = make_float2(top, all);
   }
-}
-
-// The chunks of a query head of a sequence put together: a block of 256 threads, whose
-// groups of as many as a row has values take every so many-th chunk.
-template <typename T>
-__global__ __launch_bounds__(256) void cache_attention_join_kernel(
-    Attention a, Chunks chunks, const float* __restrict__ part_o,
-    const float2* __restrict__ part_ml) {
-  extern __shared__ __attribute__((aligned(16))) float shared[];   // [chunks][256]
-  __shared__ float tops[4], sums[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int b = (int)(blockIdx.x / a.H), h = (int)(blockIdx.x - (int64_t)b * a.H);
-  const int D = a.pages.D;
-  const int length = chunk_length(a, chunks);
-  const int count = chunk_count(seen_of(a, b), length);
-  if (count == 1) return;
-  int before = 0;                                    // chunks of the sequences before
-  for (int i = lane; i < b; i += 64) before += chunk_count(seen_of(a, i), length);
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) before += __shfl_xor(before, off, 64);
-  const int tiles = (a.G + HEADS - 1) / HEADS;
-  const int kv_head = h / a.G, in = h - kv_head * a.G;
-  const int unit = kv_head * tiles + in / HEADS;
-  const int64_t id = (int64_t)before * chunks.units + (int64_t)unit * count;
-  const int columns = min(a.G, HEADS);
-  const float2* ml = part_ml + id * columns + in % HEADS;
-  float top = -INFINITY;
-  for (int i = threadIdx.x; i < count; i += 256) {
-    const float m = ml[(int64_t)i * columns].x;
-    shared[i] = m;
-    top = fmaxf(top, m);
+  at_grain += taken;
+  left -= taken;
+  run.grain = 0;
+  run.unit = unit + 1;
+  if (run.unit == shares.units) {
+    run.unit = 0;
+    run.b = b + 1;
+    if (left > 0) run.of_unit = grains_of(seen_of(a, b + 1), shares.grain);
   }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-  if (lane == 0) tops[wave] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 4; ++w) top = fmaxf(top, tops[w]);
-  float all = 0.f;
-  for (int i = threadIdx.x; i < count; i += 256) {
-    const float factor = weight_of(shared[i], top);
-    shared[i] = factor;
-    all += ml[(int64_t)i * columns].y * factor;
   }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) all += __shfl_xor(all, off, 64);
-  if (lane == 0) sums[wave] = all;
-  __syncthreads();
-  all = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-  // (groups of 64, 128 or 256 threads)
-  const int wide = D <= 64 ? 64 : D <= 128 ? 128 : 256;
-  const int d = threadIdx.x & (wide - 1), group = threadIdx.x / wide;
-  float sum = 0.f;
-  if (d < D) {
-    const float* o = part_o + (id * columns + in % HEADS) * D + d;
-#pragma unroll 4
-    for (int i = group; i < count; i += 256 / wide)
-      sum += o[(int64_t)i * columns * D] * shared[i];
-  }
-  __shared__ float parts[256];
-  parts[threadIdx.x] = sum;
-  __syncthreads();
-  if (threadIdx.x >= D) return;
-  for (int g = 1; g < 256 / wide; ++g) sum += parts[g * wide + threadIdx.x];
-  store_f32<T>(static_cast<T*>(a.out) + ((int64_t)b * a.H + h) * D + d,
-               all == 0.f ? 0.f : sum / all);
 }
 
 // ---------------------------------------------------------------------------
@@ -923,36 +1183,52 @@ static void run_read(const RowsOf& r, const void* k_pages, const void* v_pages,
                              static_cast<T*>(k), static_cast<T*>(v));
 }
 
-constexpr int TARGET = 1024;      // chunks of all sequences: 4 for each of 256 CUs
+constexpr int CUS = 256;
 
-// How the tiles' kernel divides its work; no chunks where it does not apply.
+// How the tiles' kernel divides its work and its workspace.
 struct Division {
-  Chunks chunks;
-  int64_t blocks;                 // as many chunks as there can be
-  bool joins;                     // whether a sequence can have several
-  size_t part_o, part_ml, bytes;  // of the workspace
+  Shares shares;
+  int64_t blocks;
+  bool joins;                     // whether a unit can fall to several blocks
+  size_t sums, counters, bytes;   // of the workspace: tops, sums, counters of both kinds
+  bool fits;                      // all grains can be counted
 };
 
+template <typename T, bool EIGHT, int DP>
+static Shares shares_of(bool padded) {
+  typedef TileOf<T, EIGHT, DP> Tile;
+  return Shares{0, Tile::GRAIN,
+                CUS * (padded ? Tile::template at_once<true>()
+                              : Tile::template at_once<false>())};
+}
 template <typename T, bool EIGHT>
-static int grain_of(int D) {
-  return D <= 64    ? TileOf<T, EIGHT, 64>::GRAIN
-         : D <= 128 ? TileOf<T, EIGHT, 128>::GRAIN
-                    : TileOf<T, EIGHT, 256>::GRAIN;
+static Shares shares_of(int D, bool padded) {
+  return D <= 64    ? shares_of<T, EIGHT, 64>(padded)
+         : D <= 128 ? shares_of<T, EIGHT, 128>(padded)
+                    : shares_of<T, EIGHT, 256>(padded);
 }
 
-static Division divide(int B, int H, int HK, int D, int S, int P, int grain) {
+static Division divide(int B, int H, int HK, int D, int S, int P, int dtype, bool eight,
+                       bool padded) {
   Division v = {};
+  v.shares = dtype == MESH_MOE_BF16
+                 ? (eight ? shares_of<bf16_t, true>(D, padded)
+                          : shares_of<bf16_t, false>(D, padded))
+                 : (eight ? shares_of<float, true>(D, padded)
+                          : shares_of<float, false>(D, padded));
   const int G = H / HK;
-  v.chunks.units = HK * ((G + HEADS - 1) / HEADS);
-  v.chunks.grain = grain;
-  v.chunks.target = TARGET;
-  const int64_t units = (int64_t)B * v.chunks.units, most = (int64_t)P * S;
-  v.blocks = std::min(units + v.chunks.target, units * ((most + grain - 1) / grain));
-  v.joins = most > grain;
+  const int64_t each = ((int64_t)P * S + v.shares.grain - 1) / v.shares.grain;
+  const int64_t units = (int64_t)HK * ((G + HEADS - 1) / HEADS);
+  v.fits = units <= 0x7fffffff / each / B;
+  if (!v.fits) return v;
+  v.shares.units = (int)units;
+  v.blocks = std::min<int64_t>(v.shares.blocks, units * each * B);
+  v.joins = each > 1;
   if (v.joins) {
-    const size_t rows = (size_t)v.blocks * std::min(G, HEADS);
-    v.part_ml = (sizeof(float) * rows * D + 15) & ~(size_t)15;
-    v.bytes = v.part_ml + sizeof(float2) * rows + 16;
+    const size_t rows = 2 * (size_t)v.blocks * std::min(G, HEADS);
+    v.sums = sizeof(unsigned long long) * rows;
+    v.counters = v.sums + sizeof(unsigned long long) * rows * ((D + 1) / 2);
+    v.bytes = v.counters + sizeof(unsigned long long) * 4 * v.blocks + 8;
   }
   return v;
 }
@@ -961,47 +1237,44 @@ template <typename T, bool EIGHT, int DP, bool PADDED, bool SMALL>
 static int run_tiles(const Attention& a, const Division& v, char* workspace,
                      hipStream_t st) {
   auto kern = cache_attention_tiles_kernel<T, EIGHT, DP, PADDED, SMALL>;
-  const size_t lds =
-      sizeof(float) * 4 * (2 * HEADS + (size_t)std::min(a.G, HEADS) * a.pages.D);
+  const int heads = std::min(a.G, HEADS);
+  const size_t lds = sizeof(float) * 4 * (2 * HEADS + (size_t)heads * a.pages.D);
   MOE_ALLOW_LDS(kern, lds);
-  float* part_o = reinterpret_cast<float*>(workspace);
-  float2* part_ml = reinterpret_cast<float2*>(workspace + v.part_ml);
-  kern<<<(unsigned)v.blocks, 256, lds, st>>>(a, v.chunks, part_o, part_ml);
+  Joins joins = {};
+  joins.tops = reinterpret_cast<unsigned long long*>(workspace);
+  joins.sums = reinterpret_cast<unsigned long long*>(workspace + v.sums);
+  joins.group_counters = reinterpret_cast<unsigned long long*>(workspace + v.counters);
+  joins.unit_counters = joins.group_counters + 2 * v.blocks;
+  joins.call = next_call_number();
+  kern<<<(unsigned)v.blocks, 256, lds, st>>>(a, v.shares, joins);
   MOE_CHECK_LAUNCH("cache_attention");
-  if (v.joins) {
-    const size_t most = sizeof(float) * (v.chunks.target / v.chunks.units + 2);
-    cache_attention_join_kernel<T><<<(unsigned)((int64_t)a.B * a.H), 256, most, st>>>(
-        a, v.chunks, part_o, part_ml);
-    MOE_CHECK_LAUNCH("cache_attention");
-  }
   return 0;
 }
 
+// whether the tiles' kernel takes its PADDED form
+static bool rows_padded(const Attention& a) {
+  const int D = a.pages.D;
+  return a.pages.shift < 4 || (D != 64 && D != 128 && D != 256) ||
+         !on_16_bytes({a.q, a.k_pages, a.v_pages});
+}
+
 template <typename T, bool EIGHT>
-static int run_attention(const Attention& a, const Division& v, char* workspace,
-                         hipStream_t st) {
+static int run_attention(const Attention& a, const Division& v, bool padded,
+                         char* workspace, hipStream_t st) {
   const int D = a.pages.D;
   if (D < 16) {
     cache_attention_kernel<T, EIGHT><<<(unsigned)((int64_t)a.B * a.H), 256, 0, st>>>(a);
     MOE_CHECK_LAUNCH("cache_attention");
     return 0;
   }
-  const int DP = D <= 64 ? 64 : D <= 128 ? 128 : 256;
   const bool small = a.pages.shift < 4;
-  const bool padded = small || D != DP || !on_16_bytes({a.q, a.k_pages, a.v_pages});
 #define TILES(dp)                                                                     \
   (small    ? run_tiles<T, EIGHT, dp, true, true>                                     \
    : padded ? run_tiles<T, EIGHT, dp, true, false>                                    \
             : run_tiles<T, EIGHT, dp, false, false>)
-  auto run = DP == 64 ? TILES(64) : DP == 128 ? TILES(128) : TILES(256);
+  auto run = D <= 64 ? TILES(64) : D <= 128 ? TILES(128) : TILES(256);
 #undef TILES
   return run(a, v, workspace, st);
-}
-
-static int grain_of(int D, int dtype, bool eight) {
-  return dtype == MESH_MOE_BF16
-             ? (eight ? grain_of<bf16_t, true>(D) : grain_of<bf16_t, false>(D))
-             : (eight ? grain_of<float, true>(D) : grain_of<float, false>(D));
 }
 
 }  // namespace mesh_moe
@@ -1073,7 +1346,8 @@ extern "C" size_t mesh_moe_cache_attention_workspace_bytes(int B, int H, int HK,
   if (B < 1 || H < 1 || HK < 1 || H % HK || D < 16 || D > MAX_WIDTH || S < 1 || P < 1 ||
       !valid_dtype(dtype))
     return 0;
-  return divide(B, H, HK, D, S, P, grain_of(D, dtype, eight_bit != 0)).bytes;
+  // (the form with more blocks, wherever the operands lie)
+  return divide(B, H, HK, D, S, P, dtype, eight_bit != 0, false).bytes;
 }
 
 extern "C" int mesh_moe_cache_attention(
@@ -1093,25 +1367,13 @@ extern "C" int mesh_moe_cache_attention(
                   (!rel_values || (num_buckets >= 1 && reach >= 1)),
               MESH_MOE_E_ARG, "cache_attention: rel_values, rel_bucket, num_buckets and "
               "reach go together");
-  MOE_REQUIRE((int64_t)B * H <= MAX_BLOCKS, MESH_MOE_E_UNSUPPORTED,
-              "cache_attention: %d sequences of %d heads are more than a launch has", B, H);
-  Division v = {};
-  if (D >= 16) v = divide(B, H, HK, D, S, P, grain_of(D, dtype, k_scales != nullptr));
-  MOE_REQUIRE(v.blocks <= MAX_BLOCKS, MESH_MOE_E_UNSUPPORTED,
-              "cache_attention: %d sequences of %d heads are more than a launch has", B, H);
-  MOE_REQUIRE(v.bytes == 0 || (workspace && workspace_bytes >= v.bytes), MESH_MOE_E_ARG,
-              "cache_attention: workspace too small");
-  if (k_new) {
-    if (int rc = mesh_moe_cache_write(k_new, v_new, table, position, nullptr, k_pages,
-                                      v_pages, k_scales, v_scales, B, 1, HK, D, N, S, P,
-                                      dtype, stream))
-      return rc;
-  }
   a.q = q;
   a.k_pages = k_pages;
   a.v_pages = v_pages ? v_pages : k_pages;
   a.k_scales = k_scales;
   a.v_scales = v_pages ? v_scales : k_scales;
+  a.k_new = D < 16 ? nullptr : k_new;
+  a.v_new = D < 16 ? nullptr : v_new;
   a.position = position;
   a.rel_values = rel_values;
   a.rel_bucket = rel_bucket;
@@ -1121,11 +1383,25 @@ extern "C" int mesh_moe_cache_attention(
   a.B = B;
   a.H = H;
   a.G = H / HK;
+  const bool padded = rows_padded(a);
+  const Division v = divide(B, H, HK, std::max(D, 16), S, P, dtype, k_scales != nullptr,
+                            padded);
+  MOE_REQUIRE(v.fits && (D >= 16 || (int64_t)B * H <= MAX_BLOCKS), MESH_MOE_E_UNSUPPORTED,
+              "cache_attention: %d sequences of %d heads and %d pages are more than a "
+              "launch has", B, H, P);
+  MOE_REQUIRE(D < 16 || v.bytes == 0 || (workspace && workspace_bytes >= v.bytes),
+              MESH_MOE_E_ARG, "cache_attention: workspace too small");
+  if (k_new && D < 16) {
+    if (int rc = mesh_moe_cache_write(k_new, v_new, table, position, nullptr, k_pages,
+                                      v_pages, k_scales, v_scales, B, 1, HK, D, N, S, P,
+                                      dtype, stream))
+      return rc;
+  }
   hipStream_t st = static_cast<hipStream_t>(stream);
-  char* at = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(workspace) + 15) &
-                                     ~(uintptr_t)15);
+  char* at = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(workspace) + 7) &
+                                     ~(uintptr_t)7);
   auto run = dtype == MESH_MOE_BF16
                  ? (k_scales ? run_attention<bf16_t, true> : run_attention<bf16_t, false>)
                  : (k_scales ? run_attention<float, true> : run_attention<float, false>);
-  return run(a, v, at, st);
+  return run(a, v, padded, at, st);
 }
