@@ -1,7 +1,6 @@
 // The paged cache: rows of keys and values into pages and back, and attention of one new
 // token over them.
 #include "../../include/mesh_moe_cache.h"
-#include "arrival.h"
 #include "fp8.h"
 
 #include <algorithm>
@@ -310,8 +309,10 @@ __global__ __launch_bounds__(256) void cache_attention_kernel(Attention a) {
 //
 // The work is dealt out evenly to as many blocks as the chip holds at once, by what the
 // sequences' lengths turn out to be on the device (run_of).  Where a unit's positions fall
-// to several blocks, their triples go to the workspace, and the block that arrives there
-// last puts them together.
+// to several blocks, their triples go to the workspace, and cache_attention_join_kernel
+// puts them together.  (In the same launch, by the block of a unit that is done last, a
+// join costs its block three or four round trips to a memory that is busy with the others'
+// streams: 64 sequences of up to 8192, 129 us instead of 98.)
 // ---------------------------------------------------------------------------
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
@@ -402,6 +403,11 @@ struct Run {
 };
 struct Runs {
   int blocks, each, longer;       // `longer` of the blocks have one grain more than `each`
+  __device__ __forceinline__ Runs(const Shares& s, int grains) {
+    blocks = min(s.blocks, grains);
+    each = grains / blocks;
+    longer = grains - each * blocks;
+  }
   __device__ __forceinline__ int first(int block) const {
     return block * each + min(block, longer);
   }
@@ -413,20 +419,17 @@ struct Runs {
 
 // false for a block without work.  The same for all lanes of a wavefront.
 __device__ __forceinline__ bool run_of(const Attention& a, const Shares& s, int block,
-                                       Runs* runs, Run* run) {
+                                       Run* run) {
   const int lane = threadIdx.x & 63;
   auto grains = [&](int b) { return b < a.B ? grains_of(seen_of(a, b), s.grain) : 0; };
   const int of_lane = grains(lane);
   int up_to = sums_up_to(of_lane), all = __builtin_amdgcn_readlane(up_to, 63);
   for (int b = 64; b < a.B; b += 64)
     all += __builtin_amdgcn_readlane(sums_up_to(grains(b + lane)), 63);
-  all *= s.units;
-  runs->blocks = min(s.blocks, all);
-  if (block >= runs->blocks) return false;
-  runs->each = all / runs->blocks;
-  runs->longer = all - runs->each * runs->blocks;
-  run->first = runs->first(block);
-  run->count = runs->each + (block < runs->longer ? 1 : 0);
+  const Runs runs(s, all * s.units);
+  if (block >= runs.blocks) return false;
+  run->first = runs.first(block);
+  run->count = runs.each + (block < runs.longer ? 1 : 0);
   int before = 0, count = of_lane;                   // grains of units of one kind
   for (int b = 0;; b += 64) {
     const uint64_t behind =
@@ -496,152 +499,38 @@ __device__ __forceinline__ void keep_row(const Attention& a, int of, int b, int 
 }
 
 // Units that fall to several blocks.  A block has a place in the workspace for the triple
-// of the unit it begins with (if that began before) and for the one it ends with.  A unit's
-// parts are put together by the block that arrives last; many of them (one sequence over
-// the whole chip has hundreds) in groups first, each by its last block, so that no block
-// reads more than PARTS.
-constexpr int PARTS = 32;
-
-__device__ __forceinline__ unsigned long long two_floats(float a, float b) {
-  return (unsigned long long)__float_as_uint(a) |
-         (unsigned long long)__float_as_uint(b) << 32;
-}
-__device__ __forceinline__ float low_float(unsigned long long v) {
-  return __uint_as_float((uint32_t)v);
-}
-__device__ __forceinline__ float high_float(unsigned long long v) {
-  return __uint_as_float((uint32_t)(v >> 32));
-}
-
+// of the unit it begins with (if that began before) and one for the unit it ends with.
 struct Joins {
-  unsigned long long* tops;       // [places][columns]: largest logit, sum of weights
-  unsigned long long* sums;       // [places][columns][(D + 1) / 2]: two values each
-  unsigned long long* group_counters;   // [places]: of a group's first part
-  unsigned long long* unit_counters;    // [places]: of a unit's first part
-  unsigned long long call;
+  float2* tops;                   // [places][columns]: largest logit, sum of weights
+  float2* sums;                   // [places][columns][(D + 1) / 2]: two values each
 };
+// the place of part `part` of a unit whose first block is `from`
+__device__ __forceinline__ int64_t place_of(int from, int part) {
+  return 2 * (int64_t)(from + part) + (part == 0 ? 1 : 0);
+}
 
-// A block's part of a unit.
-struct Part {
-  int from, count;                // the unit's first block, and how many it has
-  int in_group, groups;           // parts of a group, groups
-  int group, index;               // this part's, and its number in the group
-  __device__ __forceinline__ int64_t place(int part) const {
-    return 2 * (int64_t)(from + part) + (part == 0 ? 1 : 0);
-  }
-  __device__ __forceinline__ Part(const Runs& runs, int first_grain, int grains) {
-    from = runs.block_of(first_grain);
-    count = runs.block_of(first_grain + grains - 1) - from + 1;
-    in_group = count <= PARTS ? count : (int)ceilf(sqrtf((float)count));
-    groups = (count + in_group - 1) / in_group;
-    index = (int)blockIdx.x - from;
-    group = index / in_group;
-    index -= group * in_group;
-  }
-};
-
-struct JoinSpace {
-  float factors[HEADS][PARTS], tops[HEADS], all[HEADS];
-  float sums[2][256];
-  int last;
-};
-
-// Joins `count` (up to PARTS) parts of a unit, the first being `first` and each `step`
-// behind the one before; the result goes to `out`, or (null) to the first part's place.  A
-// block of 256 threads.
-template <typename T>
-__device__ __forceinline__ void join_parts(const Joins& joins, const Part& part, int first,
-                                           int step, int count, int heads, int columns,
-                                           int D, JoinSpace& space, T* out) {
-  const int halves = (D + 1) / 2, items = heads * halves;
-  {
-    const int i = threadIdx.x & (PARTS - 1);
-    for (int h = threadIdx.x / PARTS; h < heads; h += 256 / PARTS) {
-      unsigned long long ml = two_floats(-INFINITY, 0.f);
-      if (i < count) ml = ld_dev(joins.tops + part.place(first + i * step) * columns + h);
-      float top = low_float(ml);
-#pragma unroll
-      for (int off = PARTS / 2; off > 0; off >>= 1)
-        top = fmaxf(top, __shfl_xor(top, off, 64));
-      const float factor = weight_of(low_float(ml), top);
-      float all = high_float(ml) * factor;
-#pragma unroll
-      for (int off = PARTS / 2; off > 0; off >>= 1) all += __shfl_xor(all, off, 64);
-      space.factors[h][i] = factor;
-      if (i == 0) {
-        space.tops[h] = top;
-        space.all[h] = all;
-      }
+// The parts of unit `id` (of all units): false where it is whole.  The same for all lanes.
+__device__ __forceinline__ bool parts_of(const Attention& a, const Shares& s, int id,
+                                         int* b, int* unit, int* from, int* parts) {
+  const int lane = threadIdx.x & 63;
+  *b = id / s.units;
+  *unit = id - *b * s.units;
+  int before = 0, all = 0, own = 0;                  // grains of units of one kind
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int grains =
+        b0 + lane < a.B ? grains_of(seen_of(a, b0 + lane), s.grain) : 0;
+    const int up_to = sums_up_to(grains);
+    if (*b >= b0 && *b < b0 + 64) {
+      own = __builtin_amdgcn_readlane(grains, *b - b0);
+      before = all + __builtin_amdgcn_readlane(up_to, *b - b0) - own;
     }
+    all += __builtin_amdgcn_readlane(up_to, 63);
   }
-  // (few items: the parts are dealt out to groups of threads, a power of two each)
-  int shift = 5;
-  while (shift < 8 && (1 << shift) < items) ++shift;
-  const int group = threadIdx.x >> shift, groups = 256 >> shift;
-  const int64_t place = part.place(first);
-  __syncthreads();
-  for (int item0 = threadIdx.x & ((1 << shift) - 1); item0 < ((items - 1) | 255) + 1;
-       item0 += 4 * 256) {
-    constexpr int IN_FLIGHT = 8;
-    float sum[4][2];
-#pragma unroll
-    for (int n = 0; n < 4; ++n) sum[n][0] = sum[n][1] = 0.f;
-    for (int i0 = group; i0 < count; i0 += IN_FLIGHT * groups) {
-      unsigned long long v[4][IN_FLIGHT];
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        if (n * 256 >= items) break;
-        const int item = min(item0 + n * 256, items - 1), h = item / halves;
-        const int64_t at = (int64_t)h * halves + (item - h * halves);
-#pragma unroll
-        for (int u = 0; u < IN_FLIGHT; ++u) {
-          const int i = min(i0 + u * groups, count - 1);
-          v[n][u] = ld_dev(joins.sums + part.place(first + i * step) * columns * halves + at);
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        if (n * 256 >= items) break;
-        const int h = min(item0 + n * 256, items - 1) / halves;
-#pragma unroll
-        for (int u = 0; u < IN_FLIGHT; ++u) {
-          const int i = i0 + u * groups;
-          const float factor = i < count ? space.factors[h][i] : 0.f;
-          // (what is not a part is left out, whatever it is)
-          sum[n][0] += i < count ? low_float(v[n][u]) * factor : 0.f;
-          sum[n][1] += i < count ? high_float(v[n][u]) * factor : 0.f;
-        }
-      }
-    }
-    if (groups > 1) {
-      space.sums[0][threadIdx.x] = sum[0][0];
-      space.sums[1][threadIdx.x] = sum[0][1];
-      __syncthreads();
-      if (group == 0)
-        for (int g = 1; g < groups; ++g) {
-          sum[0][0] += space.sums[0][threadIdx.x + (g << shift)];
-          sum[0][1] += space.sums[1][threadIdx.x + (g << shift)];
-        }
-    }
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const int item = item0 + n * 256;
-      if (item >= items || group != 0) break;
-      const int h = item / halves, d = 2 * (item - h * halves);
-      if (out) {
-        const float all = space.all[h];
-        // (no weights: 0)
-        store_f32<T>(out + (int64_t)h * D + d, all == 0.f ? 0.f : sum[n][0] / all);
-        if (d + 1 < D)
-          store_f32<T>(out + (int64_t)h * D + d + 1, all == 0.f ? 0.f : sum[n][1] / all);
-      } else {
-        st_dev(joins.sums + (place * columns + h) * halves + d / 2,
-               two_floats(sum[n][0], sum[n][1]));
-        if (d == 0)
-          st_dev(joins.tops + place * columns + h, two_floats(space.tops[h], space.all[h]));
-      }
-    }
-  }
+  const Runs runs(s, all * s.units);
+  const int first = before * s.units + *unit * own;
+  *from = runs.block_of(first);
+  *parts = runs.block_of(first + own - 1) - *from + 1;
+  return *parts > 1;
 }
 
 // PADDED: rows of fewer than DP values, or on any address.  SMALL: pages of fewer than 16
@@ -655,14 +544,12 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
   constexpr int KW = 4;                              // words of a key's piece
   constexpr int VW = VB / 4;                         // words of a value's piece
   extern __shared__ __attribute__((aligned(16))) float joined[];
-  __shared__ JoinSpace space;
   __shared__ __attribute__((aligned(16))) uint8_t fresh_rows[2][DP * SIZE];
   __shared__ uint8_t fresh_units[2][2];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  Runs runs;
   Run run;
-  if (!run_of(a, shares, (int)blockIdx.x, &runs, &run)) return;
+  if (!run_of(a, shares, (int)blockIdx.x, &run)) return;
   const int c = lane & 15, j = lane >> 4;
   const int D = PADDED ? a.pages.D : DP, S = 1 << a.pages.shift;
   const int tiles = (a.G + HEADS - 1) / HEADS, columns = min(a.G, HEADS);
@@ -683,7 +570,7 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
     v_extra[p] = at - v_at[p];
   }
 
-  for (int at_grain = run.first, left = run.count; left > 0;) {
+  for (int left = run.count; left > 0;) {
   // ---- the next unit, or what of it falls to this block
   const int b = __builtin_amdgcn_readfirstlane(run.b);
   const int unit = __builtin_amdgcn_readfirstlane(run.unit);
@@ -696,15 +583,6 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
   const int first = run.grain * Tile::GRAIN;
   const int end = (int)min((int64_t)first + (int64_t)taken * Tile::GRAIN, (int64_t)seen);
   const int32_t* table = a.pages.table + (int64_t)b * a.pages.P;
-  const Part part(runs, at_grain - run.grain, run.of_unit);
-  unsigned long long group_was = 0, unit_was = 0;
-  if (part.count > 1 && part.index == 0 && threadIdx.x == 0) {
-    group_was = counter_prepare(
-        joins.group_counters + part.place(part.group * part.in_group), joins.call);
-    if (part.group == 0 && part.groups > 1)
-      unit_was = counter_prepare(joins.unit_counters + part.place(0), joins.call);
-  }
-
   // the queries, as the second operand of the first product; 0 where there is no head
   constexpr int QN = Tile::WIDE ? KC * KV : KC * KV / 8;
   typedef std::conditional_t<Tile::WIDE, float, bf16x8_t> query_t;
@@ -1047,8 +925,8 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
       }
   }
   __syncthreads();
-  const bool whole_unit = part.count == 1;
-  const int64_t place = part.place(part.group * part.in_group + part.index);
+  const bool whole_unit = begins && ends;
+  const int64_t place = 2 * (int64_t)blockIdx.x + (begins ? 1 : 0);
   T* out = static_cast<T*>(a.out) + ((int64_t)b * a.H + first_head) * D;
   // (two values a thread, as they go to the workspace)
   const int halves = (D + 1) / 2;
@@ -1072,42 +950,10 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
       if (!PADDED || d + 1 < D)
         store_f32<T>(out + (int64_t)h * D + d + 1, all == 0.f ? 0.f : sum[1] / all);
     } else {
-      st_dev(joins.sums + (place * columns + h) * halves + d / 2, two_floats(sum[0], sum[1]));
-      if (d == 0) st_dev(joins.tops + place * columns + h, two_floats(top, all));
+      joins.sums[(place * columns + h) * halves + d / 2] = make_float2(sum[0], sum[1]);
+      if (d == 0) joins.tops[place * columns + h] = make_float2(top, all);
     }
   }
-  if (!whole_unit) {
-    // Once all stores of the block are out, it arrives at its group's counter, the last
-    // block of a group at the unit's (which part 0 stamped, and settles here).
-    const int group_first = part.group * part.in_group;
-    if (threadIdx.x == 0 && part.index == 0) {
-      counter_settle(joins.group_counters + place, joins.call, group_was);
-      if (group_first == 0 && part.groups > 1)
-        counter_settle(joins.unit_counters + place, joins.call, unit_was);
-    }
-    int join_first = group_first, step = 1;
-    int parts = min(part.in_group, part.count - group_first);
-    for (;;) {
-      unsigned long long* counter = (step == 1 ? joins.group_counters : joins.unit_counters) +
-                                    part.place(join_first);
-      wait_stores();
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        space.last = arrive_is_last(counter, joins.call, (unsigned)parts);
-        if (space.last) st_dev(counter, 0ull);
-      }
-      __syncthreads();
-      if (!space.last) break;
-      const bool done = step > 1 || part.groups == 1;
-      join_parts<T>(joins, part, join_first, step, parts, heads, columns, D, space,
-                    done ? out : nullptr);
-      if (done) break;
-      join_first = 0;
-      step = part.in_group;
-      parts = part.groups;
-    }
-  }
-  at_grain += taken;
   left -= taken;
   run.grain = 0;
   run.unit = unit + 1;
@@ -1117,6 +963,74 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
     if (left > 0) run.of_unit = grains_of(seen_of(a, b + 1), shares.grain);
   }
   }
+}
+
+// Puts the parts of a unit together.  Block (x, y): unit x, `per` (a power of two) of its
+// heads' pairs of values; 256 / per groups of threads take every so many-th part.
+template <typename T>
+__global__ __launch_bounds__(256) void cache_attention_join_kernel(
+    Attention a, Shares shares, Joins joins, int per) {
+  constexpr int IN_FLIGHT = 16;
+  __shared__ float tops[256], alls[256], sums[2][256];
+  int b, unit, from, parts;
+  if (!parts_of(a, shares, (int)blockIdx.x, &b, &unit, &from, &parts)) return;
+  const int D = a.pages.D, halves = (D + 1) / 2;
+  const int tiles = (a.G + HEADS - 1) / HEADS, columns = min(a.G, HEADS);
+  const int kv_head = unit / tiles, head0 = (unit - kv_head * tiles) * HEADS;
+  const int items = min(a.G - head0, HEADS) * halves;
+  const int lane_item = threadIdx.x & (per - 1), group = threadIdx.x / per;
+  const int groups = 256 / per;
+  const int item = min((int)blockIdx.y * per + lane_item, items - 1);
+  const int h = item / halves, d = item - h * halves;
+  float top = -INFINITY, all = 0.f, sum[2] = {0.f, 0.f};
+  for (int i0 = group; i0 < parts; i0 += IN_FLIGHT * groups) {
+    float2 ml[IN_FLIGHT], o[IN_FLIGHT];
+#pragma unroll
+    for (int u = 0; u < IN_FLIGHT; ++u) {
+      const int i = i0 + u * groups;
+      ml[u] = make_float2(-INFINITY, 0.f);
+      o[u] = make_float2(0.f, 0.f);
+      if (i >= parts) continue;
+      const int64_t at = place_of(from, i) * columns + h;
+      ml[u] = joins.tops[at];
+      o[u] = joins.sums[at * halves + d];
+    }
+    float most = top;
+#pragma unroll
+    for (int u = 0; u < IN_FLIGHT; ++u) most = fmaxf(most, ml[u].x);
+    const float was = weight_of(top, most);
+    top = most;
+    all *= was;
+    sum[0] *= was;
+    sum[1] *= was;
+#pragma unroll
+    for (int u = 0; u < IN_FLIGHT; ++u) {
+      const float factor = weight_of(ml[u].x, top);
+      all += ml[u].y * factor;
+      sum[0] += o[u].x * factor;
+      sum[1] += o[u].y * factor;
+    }
+  }
+  tops[threadIdx.x] = top;
+  alls[threadIdx.x] = all;
+  sums[0][threadIdx.x] = sum[0];
+  sums[1][threadIdx.x] = sum[1];
+  __syncthreads();
+  if (group != 0 || (int)blockIdx.y * per + lane_item >= items) return;
+  for (int g = 1; g < groups; ++g) top = fmaxf(top, tops[lane_item + g * per]);
+  all = sum[0] = sum[1] = 0.f;
+  for (int g = 0; g < groups; ++g) {
+    const int at = lane_item + g * per;
+    const float factor = weight_of(tops[at], top);
+    all += alls[at] * factor;
+    sum[0] += sums[0][at] * factor;
+    sum[1] += sums[1][at] * factor;
+  }
+  T* out = static_cast<T*>(a.out) +
+           ((int64_t)b * a.H + (int64_t)kv_head * a.G + head0 + h) * D + 2 * d;
+  // (no weights: 0)
+  store_f32<T>(out, all == 0.f ? 0.f : sum[0] / all);
+  if (2 * d + 1 < D) store_f32<T>(out + 1, all == 0.f ? 0.f : sum[1] / all);
 }
 
 // ---------------------------------------------------------------------------
@@ -1190,7 +1104,7 @@ struct Division {
   Shares shares;
   int64_t blocks;
   bool joins;                     // whether a unit can fall to several blocks
-  size_t sums, counters, bytes;   // of the workspace: tops, sums, counters of both kinds
+  size_t sums, bytes;             // of the workspace: tops, sums
   bool fits;                      // all grains can be counted
 };
 
@@ -1219,16 +1133,15 @@ static Division divide(int B, int H, int HK, int D, int S, int P, int dtype, boo
   const int G = H / HK;
   const int64_t each = ((int64_t)P * S + v.shares.grain - 1) / v.shares.grain;
   const int64_t units = (int64_t)HK * ((G + HEADS - 1) / HEADS);
-  v.fits = units <= 0x7fffffff / each / B;
+  v.fits = units <= 0x7fffffff / each / B && units * B <= MAX_BLOCKS;
   if (!v.fits) return v;
   v.shares.units = (int)units;
   v.blocks = std::min<int64_t>(v.shares.blocks, units * each * B);
   v.joins = each > 1;
   if (v.joins) {
     const size_t rows = 2 * (size_t)v.blocks * std::min(G, HEADS);
-    v.sums = sizeof(unsigned long long) * rows;
-    v.counters = v.sums + sizeof(unsigned long long) * rows * ((D + 1) / 2);
-    v.bytes = v.counters + sizeof(unsigned long long) * 4 * v.blocks + 8;
+    v.sums = sizeof(float2) * rows;
+    v.bytes = v.sums + sizeof(float2) * rows * ((D + 1) / 2) + 8;
   }
   return v;
 }
@@ -1241,13 +1154,22 @@ static int run_tiles(const Attention& a, const Division& v, char* workspace,
   const size_t lds = sizeof(float) * 4 * (2 * HEADS + (size_t)heads * a.pages.D);
   MOE_ALLOW_LDS(kern, lds);
   Joins joins = {};
-  joins.tops = reinterpret_cast<unsigned long long*>(workspace);
-  joins.sums = reinterpret_cast<unsigned long long*>(workspace + v.sums);
-  joins.group_counters = reinterpret_cast<unsigned long long*>(workspace + v.counters);
-  joins.unit_counters = joins.group_counters + 2 * v.blocks;
-  joins.call = next_call_number();
+  joins.tops = reinterpret_cast<float2*>(workspace);
+  joins.sums = reinterpret_cast<float2*>(workspace + v.sums);
   kern<<<(unsigned)v.blocks, 256, lds, st>>>(a, v.shares, joins);
   MOE_CHECK_LAUNCH("cache_attention");
+  if (v.joins) {
+    // (blocks for every CU twice, as far as there are pairs of values)
+    const int64_t units = (int64_t)a.B * v.shares.units;
+    const int items = heads * ((a.pages.D + 1) / 2);
+    int per = 256;
+    while (per > 32 && (per >= 2 * items || units * ((items + per - 1) / per) < 2 * CUS))
+      per /= 2;
+    cache_attention_join_kernel<T>
+        <<<dim3((unsigned)units, (items + per - 1) / per), 256, 0, st>>>(a, v.shares, joins,
+                                                                       per);
+    MOE_CHECK_LAUNCH("cache_attention");
+  }
   return 0;
 }
 

@@ -6,9 +6,9 @@
 // (ops.py:4937-4940).  The dense [G,S,E] masks and the S x S cumsum matmul
 // (ops.py:2761-2781) are replaced by a per-token record and integer counting.
 #include <algorithm>
+#include <atomic>
 #include <mutex>
 
-#include "arrival.h"
 #include "common.h"
 
 namespace mesh_moe {
@@ -401,12 +401,37 @@ __global__ __launch_bounds__(64) void router_few_kernel(
 // policy; per block column sums of the balancing-loss proxies.
 // Grid (blocks per group, G).
 // ---------------------------------------------------------------------------
+// Accesses that are coherent across the GPU's compute dies without a cache
+// flush.  Each die (XCD) has its own L2; an ordinary store may sit there, and
+// an ordinary load may hit a stale line there, until a device-scope fence
+// writes back / invalidates that whole L2 -- too expensive to issue from
+// every block of a kernel whose other blocks are still streaming through the
+// same L2.  A relaxed atomic store / load at device scope is a write-through
+// store / a load that bypasses lines the L2 cannot vouch for.  The blocks of
+// the single-launch gating kernel exchange their data only through these:
+// the writer waits until its stores have completed (vmcnt 0) before it bumps
+// the arrival counter, the reader loads after it has seen the counter.
+template <typename T>
+__device__ __forceinline__ void st_dev(T* p, T v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename T>
+__device__ __forceinline__ T ld_dev(const T* p) {
+  return __hip_atomic_load(const_cast<T*>(p), __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+}
 __device__ __forceinline__ unsigned long long pack_i2(int a, int b) {
   return (unsigned long long)(unsigned)a | ((unsigned long long)(unsigned)b << 32);
 }
 __device__ __forceinline__ unsigned long long pack_f2(float a, float b) {
   return pack_i2((int)__float_as_uint(a), (int)__float_as_uint(b));
 }
+// this wavefront's global stores (and loads) have completed
+__device__ __forceinline__ void wait_stores() {
+  __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0), nothing else
+  asm volatile("" ::: "memory");
+}
+
 struct GateParams {
   int G, S, E, C;
   int policy;
@@ -1063,7 +1088,9 @@ __global__ __launch_bounds__(SELECT_THREADS) void gate_select_kernel(
 // terms up.  Nobody waits for anybody, so the scheme does not depend on which
 // blocks are resident together.
 //
-// The counters are those of arrival.h; the last arrival leaves zero behind.
+// A counter is a 64-bit word: call number << 16 | arrivals.  A word that does
+// not carry the current call's number counts as zero, so the workspace may
+// hold anything when the call starts; the last arrival leaves zero behind.
 // ---------------------------------------------------------------------------
 struct GateParams;
 template <bool COHERENT>
@@ -1079,6 +1106,54 @@ struct FusedTail {
   float* loss;                // [1]
   unsigned long long call;    // number of this call, < 2^48, never 0
 };
+
+// Puts a counter word into this call's state "no arrivals yet", whatever it holds: zero
+// where the last arrival of a call left it, anything where the workspace's memory has
+// served something else since (between two passes of a training step it has).  One
+// thread of a block that arrives at the word itself; it hands the returned word to
+// counter_settle once its work is done (nobody waits for it before) and arrives behind
+// that.
+__device__ __forceinline__ unsigned long long counter_prepare(
+    unsigned long long* word, unsigned long long call) {
+  return __hip_atomic_exchange(word, call << 16, __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Puts back the arrivals that came before counter_prepare.  Until then the word counts
+// too few, so no arrival takes itself for the last one, and this block's own arrival is
+// still to come.
+__device__ __forceinline__ void counter_settle(unsigned long long* word,
+                                               unsigned long long call,
+                                               unsigned long long prepared) {
+  if ((prepared >> 16) == call)
+    (void)__hip_atomic_fetch_add(word, prepared & 0xffffu, __ATOMIC_RELAXED,
+                                 __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// true for the last of `expected` arrivals; one thread per arrival.  The
+// common case is one fetch-add on a word that counter_prepare stamped long
+// ago.  An arrival that finds another stamp (its add then changed a word
+// nobody relies on) installs the stamp itself or, if somebody else just did,
+// adds again: every arrival ends with exactly one successful operation on a
+// word that carries this call's stamp.
+__device__ __forceinline__ bool arrive_is_last(unsigned long long* word,
+                                               unsigned long long call,
+                                               unsigned expected) {
+  unsigned long long old = __hip_atomic_fetch_add(
+      word, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if ((old >> 16) == call) return (unsigned)((old + 1) & 0xffffu) == expected;
+  old = __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (;;) {
+    if ((old >> 16) == call) {
+      old = __hip_atomic_fetch_add(word, 1ull, __ATOMIC_RELAXED,
+                                   __HIP_MEMORY_SCOPE_AGENT);
+      return (unsigned)((old + 1) & 0xffffu) == expected;
+    }
+    const unsigned long long seen = atomicCAS(word, old, (call << 16) | 1ull);
+    if (seen == old) return expected == 1u;
+    old = seen;
+  }
+}
 
 // Ranks of the block's choices.  ch [3][128] int16 in LDS as written by
 // gate_select_kernel; wcnt [3][2][E] int32 in LDS.  Wavefront w ranks choice
@@ -2291,6 +2366,14 @@ extern "C" size_t mesh_moe_gating_workspace_bytes(int G, int S, int E) {
   return sizeof(float) * (2 * (size_t)G * nblk * E + GSUM * (size_t)G) +
          sizeof(int32_t) * 3 * (size_t)G * nblk * E +
          sizeof(unsigned long long) * ((size_t)G + 1) + 3 * 256;
+}
+
+// Number of a single-launch gating call: the arrival counters in the
+// workspace are read relative to it (see arrive_is_last).
+static unsigned long long next_call_number() {
+  static std::atomic<unsigned long long> counter{1};
+  unsigned long long n = counter.fetch_add(1, std::memory_order_relaxed);
+  return (n & ((1ull << 48) - 1)) | (1ull << 47);
 }
 
 // Whether the gating of one group can make the slot map of the first expert product.
