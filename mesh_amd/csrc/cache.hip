@@ -374,11 +374,15 @@ struct TileOf {
 struct Shares {
   int units;                      // of a sequence
   int grain;
-  int blocks;                     // at most
+  int blocks;                     // at most; 0: a block for every unit
 };
+// A unit's first positions take their block about as long to begin with and to put away as
+// a grain of them to go through: units count as that much longer.
+constexpr int AHEAD = 1;
 
+// grains of a unit, those ahead of the first included
 __device__ __forceinline__ int grains_of(int seen, int grain) {
-  return max((seen + grain - 1) / grain, 1);
+  return max((seen + grain - 1) / grain, 1) + AHEAD;
 }
 
 // Sums over the lanes up to each, in six steps without LDS.
@@ -421,6 +425,13 @@ struct Runs {
 __device__ __forceinline__ bool run_of(const Attention& a, const Shares& s, int block,
                                        Run* run) {
   const int lane = threadIdx.x & 63;
+  if (s.blocks == 0) {
+    run->b = block / s.units;
+    run->unit = block - run->b * s.units;
+    run->first = run->grain = 0;
+    run->count = run->of_unit = grains_of(seen_of(a, run->b), s.grain);
+    return true;
+  }
   auto grains = [&](int b) { return b < a.B ? grains_of(seen_of(a, b), s.grain) : 0; };
   const int of_lane = grains(lane);
   int up_to = sums_up_to(of_lane), all = __builtin_amdgcn_readlane(up_to, 63);
@@ -528,7 +539,7 @@ __device__ __forceinline__ bool parts_of(const Attention& a, const Shares& s, in
   }
   const Runs runs(s, all * s.units);
   const int first = before * s.units + *unit * own;
-  *from = runs.block_of(first);
+  *from = runs.block_of(first + AHEAD);
   *parts = runs.block_of(first + own - 1) - *from + 1;
   return *parts > 1;
 }
@@ -575,13 +586,16 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
   const int b = __builtin_amdgcn_readfirstlane(run.b);
   const int unit = __builtin_amdgcn_readfirstlane(run.unit);
   const int taken = min(left, run.of_unit - run.grain);
-  const bool begins = run.grain == 0, ends = run.grain + taken == run.of_unit;
+  const int from_grain = max(run.grain - AHEAD, 0), to_grain = run.grain + taken - AHEAD;
+  const bool begins = from_grain == 0, ends = run.grain + taken == run.of_unit;
+  left -= taken;
+  if (to_grain <= 0) break;                          // (only what is ahead: the end of the run)
   const int kv_head = unit / tiles, head0 = (unit - kv_head * tiles) * HEADS;
   const int heads = min(a.G - head0, HEADS);         // columns in use
   const int64_t first_head = (int64_t)kv_head * a.G + head0;
   const int seen = seen_of(a, b), last = a.position[b];
-  const int first = run.grain * Tile::GRAIN;
-  const int end = (int)min((int64_t)first + (int64_t)taken * Tile::GRAIN, (int64_t)seen);
+  const int first = from_grain * Tile::GRAIN;
+  const int end = (int)min((int64_t)to_grain * Tile::GRAIN, (int64_t)seen);
   const int32_t* table = a.pages.table + (int64_t)b * a.pages.P;
   // the queries, as the second operand of the first product; 0 where there is no head
   constexpr int QN = Tile::WIDE ? KC * KV : KC * KV / 8;
@@ -954,7 +968,6 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
       if (d == 0) joins.tops[place * columns + h] = make_float2(top, all);
     }
   }
-  left -= taken;
   run.grain = 0;
   run.unit = unit + 1;
   if (run.unit == shares.units) {
@@ -1098,6 +1111,7 @@ static void run_read(const RowsOf& r, const void* k_pages, const void* v_pages,
 }
 
 constexpr int CUS = 256;
+constexpr int WHOLE = 4;          // units of up to so many grains are not divided
 
 // How the tiles' kernel divides its work and its workspace.
 struct Division {
@@ -1131,13 +1145,15 @@ static Division divide(int B, int H, int HK, int D, int S, int P, int dtype, boo
                  : (eight ? shares_of<float, true>(D, padded)
                           : shares_of<float, false>(D, padded));
   const int G = H / HK;
-  const int64_t each = ((int64_t)P * S + v.shares.grain - 1) / v.shares.grain;
+  const int64_t most = ((int64_t)P * S + v.shares.grain - 1) / v.shares.grain;
+  const int64_t each = most + AHEAD;
   const int64_t units = (int64_t)HK * ((G + HEADS - 1) / HEADS);
   v.fits = units <= 0x7fffffff / each / B && units * B <= MAX_BLOCKS;
   if (!v.fits) return v;
   v.shares.units = (int)units;
-  v.blocks = std::min<int64_t>(v.shares.blocks, units * each * B);
-  v.joins = each > 1;
+  v.joins = most > WHOLE;
+  if (!v.joins) v.shares.blocks = 0;
+  v.blocks = v.joins ? std::min<int64_t>(v.shares.blocks, units * each * B) : units * B;
   if (v.joins) {
     const size_t rows = 2 * (size_t)v.blocks * std::min(G, HEADS);
     v.sums = sizeof(float2) * rows;
