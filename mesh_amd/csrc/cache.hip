@@ -194,19 +194,26 @@ struct Attention {
   int B, H, G;                    // G query heads share a key / value head
 };
 
-// visible positions of sequence b
-__device__ __forceinline__ int seen_of(const Attention& a, int b) {
-  const int64_t all = (int64_t)a.pages.P << a.pages.shift;
-  return (int)min(max((int64_t)a.position[b] + 1, (int64_t)0), all);
+// What nothing in a launch writes, from an address that is the same for all lanes: a load
+// through the scalar cache, which does not wait for the vector loads before it.
+__device__ __forceinline__ int32_t scalar_load(const int32_t* p) {
+  typedef const __attribute__((address_space(4))) int32_t* constant_t;
+  return *reinterpret_cast<constant_t>(reinterpret_cast<uintptr_t>(p));
 }
 
-// the relative bias of head h for position j, `last` being the query's
-template <typename T>
-__device__ __forceinline__ float bias_of(const Attention& a, int h, int j, int last) {
-  const int back = max(j - last, 1 - a.reach);
-  const int bucket = a.rel_bucket[back + a.reach - 1];
-  return load_f32<T>(static_cast<const T*>(a.rel_values) + (int64_t)h * a.NB +
-                     min(max(bucket, 0), a.NB - 1));
+// visible positions of a sequence whose query is at `position`
+__device__ __forceinline__ int seen_from(const Attention& a, int position) {
+  const int64_t all = (int64_t)a.pages.P << a.pages.shift;
+  return (int)min(max((int64_t)position + 1, (int64_t)0), all);
+}
+__device__ __forceinline__ int seen_of(const Attention& a, int b) {
+  return seen_from(a, a.position[b]);
+}
+
+// the bucket of a position `distance` (0 or less) from the query's
+__device__ __forceinline__ int bucket_of(const Attention& a, int distance) {
+  const int bucket = a.rel_bucket[max(distance, 1 - a.reach) + a.reach - 1];
+  return min(max(bucket, 0), a.NB - 1);
 }
 
 // e^(x - m) with m >= x; 0 for x = -infinity.  (The difference first: it is exact where it
@@ -255,7 +262,9 @@ __global__ __launch_bounds__(256) void cache_attention_kernel(Attention a) {
                                             a.pages.DB), x);
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
-    if (a.rel_values) x += bias_of<T>(a, h, j, last);
+    if (a.rel_values)
+      x += load_f32<T>(static_cast<const T*>(a.rel_values) + (int64_t)h * a.NB +
+                       bucket_of(a, j - last));
     const float top = fmaxf(m, x), was = weight_of(m, top);
     const float w = round_to<T>(weight_of(x, top));
     m = top;
@@ -333,6 +342,16 @@ __device__ __forceinline__ uint32_t widened(uint32_t word, float unit) {
       uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, unit, HIGH));
 }
 
+// ... the four of a word in float32
+__device__ __forceinline__ void four_floats(uint32_t word, float unit, float (&f)[4]) {
+  const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)word, false);
+  const f32x2_t hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)word, true);
+  f[0] = lo[0] * unit;
+  f[1] = lo[1] * unit;
+  f[2] = hi[0] * unit;
+  f[3] = hi[1] * unit;
+}
+
 template <int BYTES>
 __device__ __forceinline__ void load_words(const uint8_t* at, uint32_t* to) {
   typedef typename Words<BYTES>::type words_t;
@@ -361,11 +380,7 @@ struct TileOf {
   static constexpr int NS = WIDE ? (EIGHT ? (DP == 256 ? 1 : 2) : (DP == 64 ? 2 : 1))
                                  : (EIGHT ? (DP == 256 ? 2 : 4) : (DP == 64 ? 4 : 2));
   static constexpr int GRAIN = 4 * 16 * NS;                    // positions of four wavefronts
-  // blocks that a CU holds at once
-  template <bool PADDED>
-  static constexpr int at_once() {
-    return DP == 256 ? 1 : 2;
-  }
+  static constexpr int AT_ONCE = DP == 256 ? 1 : 2;            // blocks that a CU holds
 };
 
 // How the work is divided.  A unit is a key / value head of a sequence with a tile of its
@@ -544,15 +559,32 @@ __device__ __forceinline__ bool parts_of(const Attention& a, const Shares& s, in
   return *parts > 1;
 }
 
-// PADDED: rows of fewer than DP values, or on any address.  SMALL: pages of fewer than 16
+// What a wavefront has of NS x 16 positions: words of keys and values as the products take
+// them, their scale bytes, and which of the pages are there.  SMALL: pages of fewer than 16
 // rows, whose rows are looked up one by one.
+template <typename T, bool EIGHT, int DP, bool SMALL>
+struct Group {
+  typedef TileOf<T, EIGHT, DP> Tile;
+  static constexpr int NS = Tile::NS, BLOCKS = DP == 256 ? 2 : 1;
+  uint32_t k[NS][Tile::KC][4], v[NS][4][Tile::VP][Tile::VB / 4];
+  uint32_t k_units[NS];                      // a byte for each block of the lane's key
+  uint32_t v_units[NS][SMALL ? 4 : BLOCKS];  // [4 rows][blocks] bytes, SMALL: as the keys'
+  bool there[NS][SMALL ? 4 : 1];
+};
+
+// What a scale byte (bits 8 n .. of the word) stands for.
+__device__ __forceinline__ float unit_in(uint32_t word, int n) {
+  return __uint_as_float((n < 3 ? word << (23 - 8 * n) : word >> 1) & 0x7f800000u);
+}
+
+// PADDED: rows of fewer than DP values, or on any address.
 template <typename T, bool EIGHT, int DP, bool PADDED, bool SMALL>
-__global__ __launch_bounds__(256, (TileOf<T, EIGHT, DP>::template at_once<PADDED>()))
+__global__ __launch_bounds__(256, (TileOf<T, EIGHT, DP>::AT_ONCE))
 void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
   typedef TileOf<T, EIGHT, DP> Tile;
+  typedef Group<T, EIGHT, DP, SMALL> Group;
   constexpr int NS = Tile::NS, KC = Tile::KC, KV = Tile::KV, SIZE = Tile::SIZE;
   constexpr int VD = Tile::VD, VP = Tile::VP, VE = Tile::VE, VB = Tile::VB;
-  constexpr int KW = 4;                              // words of a key's piece
   constexpr int VW = VB / 4;                         // words of a value's piece
   extern __shared__ __attribute__((aligned(16))) float joined[];
   __shared__ __attribute__((aligned(16))) uint8_t fresh_rows[2][DP * SIZE];
@@ -563,7 +595,10 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
   if (!run_of(a, shares, (int)blockIdx.x, &run)) return;
   const int c = lane & 15, j = lane >> 4;
   const int D = PADDED ? a.pages.D : DP, S = 1 << a.pages.shift;
+  const int DB = DP == 256 ? 2 : 1;
   const int tiles = (a.G + HEADS - 1) / HEADS, columns = min(a.G, HEADS);
+  const uint8_t* k_pages = static_cast<const uint8_t*>(a.k_pages);
+  const uint8_t* v_pages = static_cast<const uint8_t*>(a.v_pages);
 
   // Where a lane's pieces of a row begin.  A piece that would end behind the row begins
   // as much earlier; its first `extra` values are another piece's.
@@ -582,399 +617,472 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
   }
 
   for (int left = run.count; left > 0;) {
-  // ---- the next unit, or what of it falls to this block
-  const int b = __builtin_amdgcn_readfirstlane(run.b);
-  const int unit = __builtin_amdgcn_readfirstlane(run.unit);
-  const int taken = min(left, run.of_unit - run.grain);
-  const int from_grain = max(run.grain - AHEAD, 0), to_grain = run.grain + taken - AHEAD;
-  const bool begins = from_grain == 0, ends = run.grain + taken == run.of_unit;
-  left -= taken;
-  if (to_grain <= 0) break;                          // (only what is ahead: the end of the run)
-  const int kv_head = unit / tiles, head0 = (unit - kv_head * tiles) * HEADS;
-  const int heads = min(a.G - head0, HEADS);         // columns in use
-  const int64_t first_head = (int64_t)kv_head * a.G + head0;
-  const int seen = seen_of(a, b), last = a.position[b];
-  const int first = from_grain * Tile::GRAIN;
-  const int end = (int)min((int64_t)to_grain * Tile::GRAIN, (int64_t)seen);
-  const int32_t* table = a.pages.table + (int64_t)b * a.pages.P;
-  // the queries, as the second operand of the first product; 0 where there is no head
-  constexpr int QN = Tile::WIDE ? KC * KV : KC * KV / 8;
-  typedef std::conditional_t<Tile::WIDE, float, bf16x8_t> query_t;
-  query_t q[QN];
-  {
-    const T* row = static_cast<const T*>(a.q) +
-                   ((int64_t)b * a.H + first_head + min(c, heads - 1)) * D;
-    constexpr int PER = 16 / sizeof(T);              // values of 16 bytes of q
-#pragma unroll
-    for (int i = 0; i < KC; ++i) {
-      const bool there = c < heads && (!PADDED || k_extra[i] < KV);
-#pragma unroll
-      for (int u = 0; u < KV / PER; ++u) {
-        uint32_t w[4] = {0, 0, 0, 0};
-        if (there)
-          load_words<16>(reinterpret_cast<const uint8_t*>(row + k_at[i] + u * PER), w);
-        if constexpr (Tile::WIDE) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) q[i * KV + u * 4 + e] = __uint_as_float(w[e]);
-        } else {
-          q[i * (KV / 8) + u] = __builtin_bit_cast(
-              bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
-        }
-      }
-    }
-  }
+    // ---- the next unit, or what of it falls to this block
+    const int b = __builtin_amdgcn_readfirstlane(run.b);
+    const int unit = __builtin_amdgcn_readfirstlane(run.unit);
+    const int taken = min(left, run.of_unit - run.grain);
+    const int from_grain = max(run.grain - AHEAD, 0), to_grain = run.grain + taken - AHEAD;
+    const bool begins = from_grain == 0, ends = run.grain + taken == run.of_unit;
+    left -= taken;
+    if (to_grain <= 0) break;                        // (only what is ahead: the run's end)
+    const int kv_head = unit / tiles, head0 = (unit - kv_head * tiles) * HEADS;
+    const int heads = min(a.G - head0, HEADS);       // columns in use
+    const int64_t first_head = (int64_t)kv_head * a.G + head0;
+    const int last = scalar_load(a.position + b), seen = seen_from(a, last);
+    const int first = from_grain * Tile::GRAIN;
+    const int end = (int)min((int64_t)to_grain * Tile::GRAIN, (int64_t)seen);
+    const int32_t* table = a.pages.table + (int64_t)b * a.pages.P;
+    const int step = Tile::GRAIN, start = first + wave * (16 * NS);
 
-  f32x4_t o[VD];
+    // The pages of the 16 positions from t0 + 16 s on (not SMALL); behind the end, that of
+    // the last one.
+    auto look_up = [&](int t0, int (&page)[NS]) {
 #pragma unroll
-  for (int t = 0; t < VD; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
-
-  // The step's own row: written by the block that ends its unit (of the head's first tile),
-  // which reads it from LDS.
-  bool fresh = false;
-  if (a.k_new && ends && last >= 0) {
-    const int64_t to = a.pages.row(b, last);
-    fresh = to >= 0;
-    if (fresh) {
-      __syncthreads();                               // (the unit before is done with them)
-      if (wave < 2) keep_row<T, EIGHT>(a, wave, b, kv_head, a.pages.head(to, kv_head),
-                                       head0 == 0, fresh_rows[wave], fresh_units[wave]);
-      __syncthreads();
-    }
-  }
-
-  const uint8_t* k_pages = static_cast<const uint8_t*>(a.k_pages);
-  const uint8_t* v_pages = static_cast<const uint8_t*>(a.v_pages);
-  for (int t0 = first + wave * (16 * NS); t0 < end; t0 += Tile::GRAIN) {
-    // ---- the rows' places, and which of them count
-    // (what does not count is read from a row that is there, and left out below)
-    int64_t k_row[NS], v_row[NS][SMALL ? 4 : 1];
-    bool v_there[NS][SMALL ? 4 : 1], whole = t0 + 16 * NS <= end;
+      for (int s = 0; s < NS; ++s)
+        page[s] = scalar_load(table + (max(min(t0 + 16 * s, end - 1), 0) >> a.pages.shift));
+    };
+    // Loads positions t0 .. t0 + 16 NS - 1; what of them is not there, or not before the end,
+    // is read from rows that are, and left out when it is used.
+    auto load = [&](int t0, const int (&page)[NS], Group& g) {
+      int64_t k_row[NS], v_row[NS][SMALL ? 4 : 1];   // of lane 0's keys and values, SMALL:
+#pragma unroll                                       // of every lane's
+      for (int s = 0; s < NS; ++s) {
+        if constexpr (SMALL) {
+          const int t = t0 + 16 * s + c;
+          k_row[s] = t < end ? a.pages.row(b, t) : -1;
+          k_row[s] = a.pages.head(max(k_row[s], (int64_t)0), kv_head);
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      if constexpr (SMALL) {
-        const int t = t0 + 16 * s + c;
-        k_row[s] = t < end ? a.pages.row(b, t) : -1;
-        k_row[s] = a.pages.head(max(k_row[s], (int64_t)0), kv_head);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int u = t0 + 16 * s + 4 * j + r;
-          const int64_t row = u < end ? a.pages.row(b, u) : -1;
-          v_there[s][r] = row >= 0;
-          v_row[s][r] = a.pages.head(max(row, (int64_t)0), kv_head);
-        }
-        whole = false;
-      } else {
-        const int t = min(t0 + 16 * s, end - 1) & ~15;
-        const int page = table[t >> a.pages.shift];
-        const bool there = (unsigned)page < (unsigned)a.pages.N;
-        v_there[s][0] = there;
-        whole = whole && there;
-        k_row[s] = (((int64_t)(there ? page : 0) * a.pages.HK + kv_head)
-                    << a.pages.shift) + (t & (S - 1));
-        v_row[s][0] = k_row[s] + 4 * j;
-        k_row[s] += c;
-      }
-    }
-    // ---- keys and values
-    uint32_t kw[NS][KC][KW], vw[NS][4][VP][VW];
-    uint32_t k_unit[NS][2], v_unit[NS][4];
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      const uint8_t* row = k_pages + k_row[s] * D * SIZE;
-#pragma unroll
-      for (int i = 0; i < KC; ++i) {
-        if (!PADDED || k_extra[i] < KV) {
-          load_words<16>(row + k_at[i] * SIZE, kw[s][i]);
-        } else {
-#pragma unroll
-          for (int w = 0; w < KW; ++w) kw[s][i][w] = 0;
-        }
-      }
-      if constexpr (EIGHT) {
-        const uint8_t* unit = a.k_scales + k_row[s] * a.pages.DB;
-        k_unit[s][0] = unit[0];
-        if (DP == 256) k_unit[s][1] = unit[a.pages.DB - 1];
-      }
-    }
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int64_t at = SMALL ? v_row[s][SMALL ? r : 0] : v_row[s][0] + r;
-        const uint8_t* row = v_pages + at * D * SIZE;
-#pragma unroll
-        for (int p = 0; p < VP; ++p) {
-          if (!PADDED || v_extra[p] < VE) {
-            load_words<VB>(row + v_at[p] * SIZE, vw[s][r][p]);
-          } else {
-#pragma unroll
-            for (int w = 0; w < VW; ++w) vw[s][r][p][w] = 0;
+          for (int r = 0; r < 4; ++r) {
+            const int u = t0 + 16 * s + 4 * j + r;
+            const int64_t row = u < end ? a.pages.row(b, u) : -1;
+            g.there[s][r] = row >= 0;
+            v_row[s][r] = a.pages.head(max(row, (int64_t)0), kv_head);
           }
-        }
-        if constexpr (EIGHT) {
-          const int block = DP == 256 ? min(c / 8, a.pages.DB - 1) : 0;
-          v_unit[s][r] = a.v_scales[at * a.pages.DB + block];
+        } else {
+          const int t = min(t0 + 16 * s, end - 1) & ~15;
+          g.there[s][0] = (unsigned)page[s] < (unsigned)a.pages.N;
+          k_row[s] = v_row[s][0] =
+              (((int64_t)(g.there[s][0] ? page[s] : 0) * a.pages.HK + kv_head)
+               << a.pages.shift) + (t & (S - 1));
         }
       }
-    }
-    if (fresh && t0 <= last && last < t0 + 16 * NS) {
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        if (t0 + 16 * s + c == last) {
+        const uint8_t* from = k_pages + k_row[s] * D * SIZE;
 #pragma unroll
-          for (int i = 0; i < KC; ++i)
-            if (!PADDED || k_extra[i] < KV)
-              load_words<16>(fresh_rows[0] + k_at[i] * SIZE, kw[s][i]);
-          if (EIGHT) {
-            k_unit[s][0] = fresh_units[0][0];
-            if (DP == 256) k_unit[s][1] = fresh_units[0][1];
-          }
+        for (int i = 0; i < KC; ++i)
+          if (!PADDED || k_extra[i] < KV)
+            load_words<16>(from + (uint32_t)(((SMALL ? 0 : c * D) + k_at[i]) * SIZE),
+                           g.k[s][i]);
+        if constexpr (EIGHT) {
+          const uint8_t* units = a.k_scales + k_row[s] * DB + (SMALL ? 0 : c * DB);
+          g.k_units[s] = DB == 2 ? units[0] | (uint32_t)units[1] << 8 : units[0];
         }
+      }
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          if (t0 + 16 * s + 4 * j + r != last) continue;
+          const uint8_t* from = v_pages + v_row[s][SMALL ? r : 0] * D * SIZE;
 #pragma unroll
           for (int p = 0; p < VP; ++p)
             if (!PADDED || v_extra[p] < VE)
-              load_words<VB>(fresh_rows[1] + v_at[p] * SIZE, vw[s][r][p]);
-          if (EIGHT) v_unit[s][r] = fresh_units[1][DP == 256 ? c / 8 : 0];
+              load_words<VB>(from + (SMALL ? 0 : r * D * SIZE) +
+                                 (uint32_t)(((SMALL ? 0 : 4 * j * D) + v_at[p]) * SIZE),
+                             g.v[s][r][p]);
+          if constexpr (EIGHT && SMALL) {
+            const uint8_t* units = a.v_scales + v_row[s][r] * DB;
+            g.v_units[s][r] = DB == 2 ? units[0] | (uint32_t)units[1] << 8 : units[0];
+          }
         }
+        if constexpr (EIGHT && !SMALL)
+          load_words<4 * Group::BLOCKS>(a.v_scales + v_row[s][0] * DB + 4 * j * DB,
+                                        g.v_units[s]);
       }
-    }
-    // ---- logits
-    float x[NS][4];
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+    };
+
+    // ---- the queries, as the second operand of the first product; 0 where there is no head
+    int page[NS];
+    if (!SMALL) look_up(start, page);
+    constexpr int QN = Tile::WIDE ? KC * KV : KC * KV / 8;
+    typedef std::conditional_t<Tile::WIDE, float, bf16x8_t> query_t;
+    query_t q[QN];
+    {
+      const T* row = static_cast<const T*>(a.q) +
+                     ((int64_t)b * a.H + first_head + min(c, heads - 1)) * D;
+      constexpr int PER = 16 / sizeof(T);            // values of 16 bytes of q
 #pragma unroll
       for (int i = 0; i < KC; ++i) {
-        uint32_t* w = kw[s][i];
-        if constexpr (PADDED) {
-          // (another piece's values do not count twice)
+        const bool there = c < heads && (!PADDED || k_extra[i] < KV);
 #pragma unroll
-          for (int e = 0; e < KW; ++e) {
-            const int bits = min(max(k_extra[i] * SIZE * 8 - 32 * e, 0), 32);
-            w[e] &= bits == 32 ? 0u : ~0u << bits;
+        for (int u = 0; u < KV / PER; ++u) {
+          uint32_t w[4] = {0, 0, 0, 0};
+          if (there)
+            load_words<16>(reinterpret_cast<const uint8_t*>(row + k_at[i] + u * PER), w);
+          if constexpr (Tile::WIDE) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[i * KV + u * 4 + e] = __uint_as_float(w[e]);
+          } else {
+            q[i * (KV / 8) + u] =
+                __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
           }
         }
-        if constexpr (EIGHT) {
-          const float unit = __uint_as_float(k_unit[s][DP == 256 ? i / 2 : 0] << 23);
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            if constexpr (Tile::WIDE) {
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[2 * half + e], false);
-                const f32x2_t hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[2 * half + e], true);
-                const float f[4] = {lo[0] * unit, lo[1] * unit, hi[0] * unit, hi[1] * unit};
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-                  sum = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                      f[u], q[i * KV + 8 * half + 4 * e + u], sum, 0, 0, 0);
-              }
-            } else {
-              uint4 wide;
-              wide.x = widened<false>(w[2 * half], unit);
-              wide.y = widened<true>(w[2 * half], unit);
-              wide.z = widened<false>(w[2 * half + 1], unit);
-              wide.w = widened<true>(w[2 * half + 1], unit);
-              sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                  __builtin_bit_cast(bf16x8_t, wide), q[i * 2 + half], sum, 0, 0, 0);
-            }
-          }
-        } else if constexpr (Tile::WIDE) {
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            sum = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                __uint_as_float(w[u]), q[i * KV + u], sum, 0, 0, 0);
-        } else {
-          sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3])), q[i], sum,
-              0, 0, 0);
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) x[s][r] = sum[r];
-    }
-    if (a.rel_values) {
-      const int h = (int)first_head + min(c, heads - 1);
-#pragma unroll
-      for (int s = 0; s < NS; ++s)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          x[s][r] += bias_of<T>(a, h, min(t0 + 16 * s + 4 * j + r, end - 1), last);
-    }
-    if (!whole) {
-#pragma unroll
-      for (int s = 0; s < NS; ++s)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const bool there = v_there[s][SMALL ? r : 0] && t0 + 16 * s + 4 * j + r < end;
-          if (there) continue;
-          x[s][r] = -INFINITY;
-#pragma unroll
-          for (int p = 0; p < VP; ++p)
-#pragma unroll
-            for (int w = 0; w < VW; ++w) vw[s][r][p][w] = 0;
-          if (EIGHT) v_unit[s][r] = FP8_UNIT;
-        }
-    }
-    // ---- weights
-    float top = m;
-#pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) top = fmaxf(top, x[s][r]);
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    if (__any(top > m)) {
-      const float was = weight_of(m, top);
-      l *= was;
-#pragma unroll
-      for (int t = 0; t < VD; ++t) o[t] *= was;
-      m = top;
-    }
-    uint32_t wp[NS][2];                              // pairs of weights (bfloat16)
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) x[s][r] = weight_of(x[s][r], m);
-      if constexpr (!Tile::WIDE) {
-        wp[s][0] = f32x2_to_bf16x2(x[s][0], x[s][1]);
-        wp[s][1] = f32x2_to_bf16x2(x[s][2], x[s][3]);
-        l += __uint_as_float(wp[s][0] << 16) + __uint_as_float(wp[s][0] & 0xffff0000u);
-        l += __uint_as_float(wp[s][1] << 16) + __uint_as_float(wp[s][1] & 0xffff0000u);
-      } else {
-        l += (x[s][0] + x[s][1]) + (x[s][2] + x[s][3]);
       }
     }
-    // ---- sums of values
-    if constexpr (Tile::WIDE) {
-#pragma unroll
-      for (int s = 0; s < NS; ++s)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float unit = EIGHT ? __uint_as_float(v_unit[s][r] << 23) : 1.f;
-#pragma unroll
-          for (int p = 0; p < VP; ++p)
-#pragma unroll
-            for (int w = 0; w < VW; ++w) {
-              const uint32_t word = vw[s][r][p][w];
-              if constexpr (EIGHT) {
-                const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)word, false);
-                const f32x2_t hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)word, true);
-                const float f[4] = {lo[0] * unit, lo[1] * unit, hi[0] * unit, hi[1] * unit};
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-                  o[p * VE + 4 * w + u] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                      f[u], x[s][r], o[p * VE + 4 * w + u], 0, 0, 0);
-              } else {
-                o[p * VE + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                    __uint_as_float(word), x[s][r], o[p * VE + w], 0, 0, 0);
-              }
-            }
-        }
-    } else {
-#pragma unroll
-      for (int s = 0; s < NS; s += 2) {
-        const bf16x8_t w = __builtin_bit_cast(
-            bf16x8_t, make_uint4(wp[s][0], wp[s][1], wp[s + 1][0], wp[s + 1][1]));
-#pragma unroll
-        for (int p = 0; p < VP; ++p)
-#pragma unroll
-          for (int pair = 0; pair < VE / 2; ++pair) {
-            uint32_t two[8];                         // values 2 pair, 2 pair + 1 of 8 positions
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int at = s + e / 4, r = e % 4;
-              if constexpr (EIGHT) {
-                const uint32_t word = vw[at][r][p][pair / 2];
-                const float unit = __uint_as_float(v_unit[at][r] << 23);
-                two[e] = pair & 1 ? widened<true>(word, unit) : widened<false>(word, unit);
-              } else {
-                two[e] = vw[at][r][p][pair];
-              }
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              constexpr uint32_t PICK[2] = {0x05040100u, 0x07060302u};
-              uint4 v;
-              v.x = __builtin_amdgcn_perm(two[1], two[0], PICK[u]);
-              v.y = __builtin_amdgcn_perm(two[3], two[2], PICK[u]);
-              v.z = __builtin_amdgcn_perm(two[5], two[4], PICK[u]);
-              v.w = __builtin_amdgcn_perm(two[7], two[6], PICK[u]);
-              f32x4_t& sum = o[p * VE + 2 * pair + u];
-              sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                  __builtin_bit_cast(bf16x8_t, v), w, sum, 0, 0, 0);
-            }
-          }
-      }
-    }
-  }
 
-  // ---- the four wavefronts' triples
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
-  float* ms = joined;                                // [4][HEADS]
-  float* ls = ms + 4 * HEADS;                        // [4][HEADS]
-  float* os = ls + 4 * HEADS;                        // [4][heads][D]
-  __syncthreads();                                   // (the unit before is done with them)
-  if (lane < HEADS) {
-    ms[wave * HEADS + lane] = m;
-    ls[wave * HEADS + lane] = l;
-  }
-  if (c < heads) {
-    float* to = os + (wave * heads + c) * D;
-#pragma unroll
-    for (int p = 0; p < VP; ++p)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        // (row 4 j + r of the product is what lane c = 4 j + r read)
-        const int at = p * 16 * VE + (4 * j + r) * VE;
-        const int from = PADDED ? min(at, D - VE) : at;
-#pragma unroll
-        for (int u = 0; u < VE; ++u)
-          if (!PADDED || (from + u >= at && at < D)) to[from + u] = o[p * VE + u][r];
+    // The step's own row: written by the block that ends its unit (of the head's first
+    // tile), which reads it from LDS.
+    bool fresh = false;
+    if (a.k_new && ends && last >= 0) {
+      const int64_t to = a.pages.row(b, last);
+      fresh = to >= 0;
+      if (fresh) {
+        __syncthreads();                             // (the unit before is done with them)
+        if (wave < 2)
+          keep_row<T, EIGHT>(a, wave, b, kv_head, a.pages.head(to, kv_head), head0 == 0,
+                             fresh_rows[wave], fresh_units[wave]);
+        __syncthreads();
       }
-  }
-  __syncthreads();
-  const bool whole_unit = begins && ends;
-  const int64_t place = 2 * (int64_t)blockIdx.x + (begins ? 1 : 0);
-  T* out = static_cast<T*>(a.out) + ((int64_t)b * a.H + first_head) * D;
-  // (two values a thread, as they go to the workspace)
-  const int halves = (D + 1) / 2;
-  for (int i = threadIdx.x; i < heads * halves; i += 256) {
-    const int h = i / halves, d = 2 * (i - h * halves);
-    float top = ms[h];
-#pragma unroll
-    for (int w = 1; w < 4; ++w) top = fmaxf(top, ms[w * HEADS + h]);
-    float sum[2] = {0.f, 0.f}, all = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float factor = weight_of(ms[w * HEADS + h], top);
-      const float* from = os + (w * heads + h) * D + d;
-      sum[0] += from[0] * factor;
-      if (!PADDED || d + 1 < D) sum[1] += from[1] * factor;
-      all += ls[w * HEADS + h] * factor;
     }
-    if (whole_unit) {
-      // (nothing seen: 0)
-      store_f32<T>(out + (int64_t)h * D + d, all == 0.f ? 0.f : sum[0] / all);
-      if (!PADDED || d + 1 < D)
-        store_f32<T>(out + (int64_t)h * D + d + 1, all == 0.f ? 0.f : sum[1] / all);
-    } else {
-      joins.sums[(place * columns + h) * halves + d / 2] = make_float2(sum[0], sum[1]);
-      if (d == 0) joins.tops[place * columns + h] = make_float2(top, all);
+
+    // the relative biases of the lane's head, and that of all positions far away
+    const T* rel_row = nullptr;
+    float far_bias = 0.f;
+    if (a.rel_values) {
+      rel_row = static_cast<const T*>(a.rel_values) +
+                (first_head + min(c, heads - 1)) * a.NB;
+      far_bias = load_f32<T>(rel_row + bucket_of(a, 1 - a.reach));
     }
-  }
-  run.grain = 0;
-  run.unit = unit + 1;
-  if (run.unit == shares.units) {
-    run.unit = 0;
-    run.b = b + 1;
-    if (left > 0) run.of_unit = grains_of(seen_of(a, b + 1), shares.grain);
-  }
+
+    f32x4_t o[VD];
+#pragma unroll
+    for (int t = 0; t < VD; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+
+    // ---- a group's positions into m, l and o
+    auto use = [&](int t0, Group& g) {
+      if (PADDED) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+#pragma unroll
+          for (int i = 0; i < KC; ++i)
+            if (k_extra[i] >= KV)
+#pragma unroll
+              for (int w = 0; w < 4; ++w) g.k[s][i][w] = 0;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int p = 0; p < VP; ++p)
+              if (v_extra[p] >= VE)
+#pragma unroll
+                for (int w = 0; w < VW; ++w) g.v[s][r][p][w] = 0;
+        }
+      }
+      if (fresh && t0 <= last && last < t0 + 16 * NS) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          if (t0 + 16 * s + c == last) {
+#pragma unroll
+            for (int i = 0; i < KC; ++i)
+              if (!PADDED || k_extra[i] < KV)
+                load_words<16>(fresh_rows[0] + k_at[i] * SIZE, g.k[s][i]);
+            if (EIGHT) g.k_units[s] = fresh_units[0][0] | (uint32_t)fresh_units[0][1] << 8;
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (t0 + 16 * s + 4 * j + r != last) continue;
+#pragma unroll
+            for (int p = 0; p < VP; ++p)
+              if (!PADDED || v_extra[p] < VE)
+                load_words<VB>(fresh_rows[1] + v_at[p] * SIZE, g.v[s][r][p]);
+            if (EIGHT) {
+              const uint32_t units = fresh_units[1][0] | (uint32_t)fresh_units[1][1] << 8;
+              if constexpr (SMALL) {
+                g.v_units[s][r] = units;
+              } else {
+                const int bits = 8 * DB * (r % (4 / DB));
+                uint32_t& word = g.v_units[s][r * DB / 4];
+                word = (word & ~((DB == 2 ? 0xffffu : 0xffu) << bits)) |
+                       (DB == 2 ? units : units & 0xffu) << bits;
+              }
+            }
+          }
+        }
+      }
+      // -- logits
+      float x[NS][4];
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < KC; ++i) {
+          uint32_t* w = g.k[s][i];
+          if constexpr (PADDED) {
+            // (another piece's values do not count twice)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int bits = min(max(k_extra[i] * SIZE * 8 - 32 * e, 0), 32);
+              w[e] &= bits == 32 ? 0u : ~0u << bits;
+            }
+          }
+          if constexpr (EIGHT) {
+            const float unit = unit_in(g.k_units[s], DP == 256 ? i / 2 : 0);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              if constexpr (Tile::WIDE) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  float f[4];
+                  four_floats(w[2 * half + e], unit, f);
+#pragma unroll
+                  for (int u = 0; u < 4; ++u)
+                    sum = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                        f[u], q[i * KV + 8 * half + 4 * e + u], sum, 0, 0, 0);
+                }
+              } else {
+                uint4 wide;
+                wide.x = widened<false>(w[2 * half], unit);
+                wide.y = widened<true>(w[2 * half], unit);
+                wide.z = widened<false>(w[2 * half + 1], unit);
+                wide.w = widened<true>(w[2 * half + 1], unit);
+                sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    __builtin_bit_cast(bf16x8_t, wide), q[i * 2 + half], sum, 0, 0, 0);
+              }
+            }
+          } else if constexpr (Tile::WIDE) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              sum = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                  __uint_as_float(w[u]), q[i * KV + u], sum, 0, 0, 0);
+          } else {
+            sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3])), q[i], sum,
+                0, 0, 0);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[s][r] = sum[r];
+      }
+      if (a.rel_values) {
+        if (last - (t0 + 16 * NS - 1) >= a.reach - 1) {
+#pragma unroll
+          for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[s][r] += far_bias;
+        } else {
+          // (all loads of a kind at once)
+          int bucket[NS][4];
+#pragma unroll
+          for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              bucket[s][r] = bucket_of(a, min(t0 + 16 * s + 4 * j + r, end - 1) - last);
+          float bias[NS][4];
+#pragma unroll
+          for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) bias[s][r] = load_f32<T>(rel_row + bucket[s][r]);
+#pragma unroll
+          for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[s][r] += bias[s][r];
+        }
+      }
+      bool whole = !SMALL && t0 + 16 * NS <= end;
+      if constexpr (!SMALL)
+#pragma unroll
+        for (int s = 0; s < NS; ++s) whole = whole && g.there[s][0];
+      if (!whole) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (g.there[s][SMALL ? r : 0] && t0 + 16 * s + 4 * j + r < end) continue;
+            x[s][r] = -INFINITY;
+#pragma unroll
+            for (int p = 0; p < VP; ++p)
+#pragma unroll
+              for (int w = 0; w < VW; ++w) g.v[s][r][p][w] = 0;
+          }
+      }
+      // -- weights
+      float top = m;
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) top = fmaxf(top, x[s][r]);
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      if (__any(top > m)) {
+        const float was = weight_of(m, top);
+        l *= was;
+#pragma unroll
+        for (int t = 0; t < VD; ++t) o[t] *= was;
+        m = top;
+      }
+      uint32_t pairs[NS][2];                         // of weights (bfloat16)
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[s][r] = weight_of(x[s][r], m);
+        if constexpr (!Tile::WIDE) {
+          pairs[s][0] = f32x2_to_bf16x2(x[s][0], x[s][1]);
+          pairs[s][1] = f32x2_to_bf16x2(x[s][2], x[s][3]);
+          // (the sum of what is multiplied, so that weights add up to 1)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            l += __uint_as_float(pairs[s][e] << 16) +
+                 __uint_as_float(pairs[s][e] & 0xffff0000u);
+        } else {
+          l += (x[s][0] + x[s][1]) + (x[s][2] + x[s][3]);
+        }
+      }
+      // -- sums of values
+      auto v_unit = [&](int s, int r) {
+        if constexpr (!EIGHT) return 1.f;
+        else if constexpr (SMALL)
+          return DB == 2 && c >= 8 ? unit_in(g.v_units[s][r], 1) : unit_in(g.v_units[s][r], 0);
+        else if constexpr (DB == 2)
+          return c >= 8 ? unit_in(g.v_units[s][r / 2], r % 2 * 2 + 1)
+                        : unit_in(g.v_units[s][r / 2], r % 2 * 2);
+        else
+          return unit_in(g.v_units[s][0], r);
+      };
+      if constexpr (Tile::WIDE) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float unit = v_unit(s, r);
+#pragma unroll
+            for (int p = 0; p < VP; ++p)
+#pragma unroll
+              for (int w = 0; w < VW; ++w) {
+                const uint32_t word = g.v[s][r][p][w];
+                if constexpr (EIGHT) {
+                  float f[4];
+                  four_floats(word, unit, f);
+#pragma unroll
+                  for (int u = 0; u < 4; ++u)
+                    o[p * VE + 4 * w + u] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                        f[u], x[s][r], o[p * VE + 4 * w + u], 0, 0, 0);
+                } else {
+                  o[p * VE + w] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                      __uint_as_float(word), x[s][r], o[p * VE + w], 0, 0, 0);
+                }
+              }
+          }
+      } else {
+#pragma unroll
+        for (int s = 0; s < NS; s += 2) {
+          const bf16x8_t w = __builtin_bit_cast(
+              bf16x8_t,
+              make_uint4(pairs[s][0], pairs[s][1], pairs[s + 1][0], pairs[s + 1][1]));
+          float unit[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) unit[e] = v_unit(s + e / 4, e % 4);
+#pragma unroll
+          for (int p = 0; p < VP; ++p)
+#pragma unroll
+            for (int pair = 0; pair < VE / 2; ++pair) {
+              uint32_t two[8];                       // values 2 pair, 2 pair + 1 of 8 positions
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const uint32_t* words = g.v[s + e / 4][e % 4][p];
+                if constexpr (EIGHT)
+                  two[e] = pair & 1 ? widened<true>(words[pair / 2], unit[e])
+                                    : widened<false>(words[pair / 2], unit[e]);
+                else
+                  two[e] = words[pair];
+              }
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                constexpr uint32_t PICK[2] = {0x05040100u, 0x07060302u};
+                uint4 v;
+                v.x = __builtin_amdgcn_perm(two[1], two[0], PICK[u]);
+                v.y = __builtin_amdgcn_perm(two[3], two[2], PICK[u]);
+                v.z = __builtin_amdgcn_perm(two[5], two[4], PICK[u]);
+                v.w = __builtin_amdgcn_perm(two[7], two[6], PICK[u]);
+                f32x4_t& sum = o[p * VE + 2 * pair + u];
+                sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    __builtin_bit_cast(bf16x8_t, v), w, sum, 0, 0, 0);
+              }
+            }
+        }
+      }
+    };
+
+    // (the pages of the next group are looked up while this one is used)
+    for (int t0 = start; t0 < end; t0 += step) {
+      Group g;
+      load(t0, page, g);
+      if (!SMALL) look_up(t0 + step, page);
+      use(t0, g);
+    }
+
+    // ---- the four wavefronts' triples
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    float* ms = joined;                              // [4][HEADS]
+    float* ls = ms + 4 * HEADS;                      // [4][HEADS]
+    float* os = ls + 4 * HEADS;                      // [4][heads][D]
+    __syncthreads();                                 // (the unit before is done with them)
+    if (lane < HEADS) {
+      ms[wave * HEADS + lane] = m;
+      ls[wave * HEADS + lane] = l;
+    }
+    if (c < heads) {
+      float* to = os + (wave * heads + c) * D;
+#pragma unroll
+      for (int p = 0; p < VP; ++p)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          // (row 4 j + r of the product is what lane c = 4 j + r read)
+          const int at = p * 16 * VE + (4 * j + r) * VE;
+          const int from = PADDED ? min(at, D - VE) : at;
+#pragma unroll
+          for (int u = 0; u < VE; ++u)
+            if (!PADDED || (from + u >= at && at < D)) to[from + u] = o[p * VE + u][r];
+        }
+    }
+    __syncthreads();
+    const bool whole_unit = begins && ends;
+    const int64_t place = 2 * (int64_t)blockIdx.x + (begins ? 1 : 0);
+    T* out = static_cast<T*>(a.out) + ((int64_t)b * a.H + first_head) * D;
+    // (two values a thread, as they go to the workspace)
+    const int halves = (D + 1) / 2;
+    for (int i = threadIdx.x; i < heads * halves; i += 256) {
+      const int h = i / halves, d = 2 * (i - h * halves);
+      float top = ms[h];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) top = fmaxf(top, ms[w * HEADS + h]);
+      float sum[2] = {0.f, 0.f}, all = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float factor = weight_of(ms[w * HEADS + h], top);
+        const float* from = os + (w * heads + h) * D + d;
+        sum[0] += from[0] * factor;
+        if (!PADDED || d + 1 < D) sum[1] += from[1] * factor;
+        all += ls[w * HEADS + h] * factor;
+      }
+      if (whole_unit) {
+        // (nothing seen: 0)
+        store_f32<T>(out + (int64_t)h * D + d, all == 0.f ? 0.f : sum[0] / all);
+        if (!PADDED || d + 1 < D)
+          store_f32<T>(out + (int64_t)h * D + d + 1, all == 0.f ? 0.f : sum[1] / all);
+      } else {
+        joins.sums[(place * columns + h) * halves + d / 2] = make_float2(sum[0], sum[1]);
+        if (d == 0) joins.tops[place * columns + h] = make_float2(top, all);
+      }
+    }
+    run.grain = 0;
+    run.unit = unit + 1;
+    if (run.unit == shares.units) {
+      run.unit = 0;
+      run.b = b + 1;
+      if (left > 0)
+        run.of_unit = grains_of(seen_from(a, scalar_load(a.position + b + 1)), shares.grain);
+    }
   }
 }
 
@@ -1111,7 +1219,11 @@ static void run_read(const RowsOf& r, const void* k_pages, const void* v_pages,
 }
 
 constexpr int CUS = 256;
-constexpr int WHOLE = 4;          // units of up to so many grains are not divided
+// Units of up to so many grains are not divided, where there are as many as CUs twice as
+// long ones: 64 sequences of 1024, 8 heads of 128 (8 grains) take 49 us whole, 52 divided;
+// one of 2001, 1 head of 128 in 8 bits (8 grains) 19 whole, 12 divided, and one of 700, 16
+// heads of 64 (3 grains) 8.4 whole, 10.3 divided.
+constexpr int WHOLE = 4;
 
 // How the tiles' kernel divides its work and its workspace.
 struct Division {
@@ -1123,27 +1235,22 @@ struct Division {
 };
 
 template <typename T, bool EIGHT, int DP>
-static Shares shares_of(bool padded) {
+static Shares shares_of() {
   typedef TileOf<T, EIGHT, DP> Tile;
-  return Shares{0, Tile::GRAIN,
-                CUS * (padded ? Tile::template at_once<true>()
-                              : Tile::template at_once<false>())};
+  return Shares{0, Tile::GRAIN, CUS * Tile::AT_ONCE};
 }
 template <typename T, bool EIGHT>
-static Shares shares_of(int D, bool padded) {
-  return D <= 64    ? shares_of<T, EIGHT, 64>(padded)
-         : D <= 128 ? shares_of<T, EIGHT, 128>(padded)
-                    : shares_of<T, EIGHT, 256>(padded);
+static Shares shares_of(int D) {
+  return D <= 64    ? shares_of<T, EIGHT, 64>()
+         : D <= 128 ? shares_of<T, EIGHT, 128>()
+                    : shares_of<T, EIGHT, 256>();
 }
 
-static Division divide(int B, int H, int HK, int D, int S, int P, int dtype, bool eight,
-                       bool padded) {
+static Division divide(int B, int H, int HK, int D, int S, int P, int dtype, bool eight) {
   Division v = {};
   v.shares = dtype == MESH_MOE_BF16
-                 ? (eight ? shares_of<bf16_t, true>(D, padded)
-                          : shares_of<bf16_t, false>(D, padded))
-                 : (eight ? shares_of<float, true>(D, padded)
-                          : shares_of<float, false>(D, padded));
+                 ? (eight ? shares_of<bf16_t, true>(D) : shares_of<bf16_t, false>(D))
+                 : (eight ? shares_of<float, true>(D) : shares_of<float, false>(D));
   const int G = H / HK;
   const int64_t most = ((int64_t)P * S + v.shares.grain - 1) / v.shares.grain;
   const int64_t each = most + AHEAD;
@@ -1151,7 +1258,7 @@ static Division divide(int B, int H, int HK, int D, int S, int P, int dtype, boo
   v.fits = units <= 0x7fffffff / each / B && units * B <= MAX_BLOCKS;
   if (!v.fits) return v;
   v.shares.units = (int)units;
-  v.joins = most > WHOLE;
+  v.joins = most > (units * B >= CUS ? 2 * WHOLE : WHOLE);
   if (!v.joins) v.shares.blocks = 0;
   v.blocks = v.joins ? std::min<int64_t>(v.shares.blocks, units * each * B) : units * B;
   if (v.joins) {
@@ -1284,8 +1391,7 @@ extern "C" size_t mesh_moe_cache_attention_workspace_bytes(int B, int H, int HK,
   if (B < 1 || H < 1 || HK < 1 || H % HK || D < 16 || D > MAX_WIDTH || S < 1 || P < 1 ||
       !valid_dtype(dtype))
     return 0;
-  // (the form with more blocks, wherever the operands lie)
-  return divide(B, H, HK, D, S, P, dtype, eight_bit != 0, false).bytes;
+  return divide(B, H, HK, D, S, P, dtype, eight_bit != 0).bytes;
 }
 
 extern "C" int mesh_moe_cache_attention(
@@ -1322,8 +1428,7 @@ extern "C" int mesh_moe_cache_attention(
   a.H = H;
   a.G = H / HK;
   const bool padded = rows_padded(a);
-  const Division v = divide(B, H, HK, std::max(D, 16), S, P, dtype, k_scales != nullptr,
-                            padded);
+  const Division v = divide(B, H, HK, std::max(D, 16), S, P, dtype, k_scales != nullptr);
   MOE_REQUIRE(v.fits && (D >= 16 || (int64_t)B * H <= MAX_BLOCKS), MESH_MOE_E_UNSUPPORTED,
               "cache_attention: %d sequences of %d heads and %d pages are more than a "
               "launch has", B, H, P);
