@@ -377,10 +377,17 @@ struct TileOf {
   static constexpr int VE = VB / SIZE;                         // values of a piece
   static constexpr bool WIDE = sizeof(T) == 4;                 // float32 products
   // groups of 16 positions that a wavefront has in registers at once
-  static constexpr int NS = WIDE ? (EIGHT ? (DP == 256 ? 1 : 2) : (DP == 64 ? 2 : 1))
-                                 : (EIGHT ? (DP == 256 ? 2 : 4) : (DP == 64 ? 4 : 2));
+  static constexpr int NS =
+      WIDE ? (EIGHT ? (DP == 256 ? 1 : 2) : (DP == 64 ? 2 : 1))
+           : (EIGHT && DP < 256 ? 4 : 2);
   static constexpr int GRAIN = 4 * 16 * NS;                    // positions of four wavefronts
-  static constexpr int AT_ONCE = DP == 256 ? 1 : 2;            // blocks that a CU holds
+  // blocks that a CU holds
+  template <bool PADDED>
+  static constexpr int at_once() {
+    return DP == 256 && !(EIGHT && !PADDED) ? 1 : DP == 64 && !EIGHT && !WIDE ? 3 : 2;
+  }
+  // grains that are not divided among blocks (see divide)
+  static constexpr int WHOLE = DP == 64 && !EIGHT && !WIDE ? 8 : 4;
 };
 
 // How the work is divided.  A unit is a key / value head of a sequence with a tile of its
@@ -568,8 +575,8 @@ struct Group {
   static constexpr int NS = Tile::NS, BLOCKS = DP == 256 ? 2 : 1;
   uint32_t k[NS][Tile::KC][4], v[NS][4][Tile::VP][Tile::VB / 4];
   uint32_t k_units[NS];                      // a byte for each block of the lane's key
-  uint32_t v_units[NS][SMALL ? 4 : BLOCKS];  // [4 rows][blocks] bytes, SMALL: as the keys'
-  bool there[NS][SMALL ? 4 : 1];
+  uint32_t v_units[NS][BLOCKS];              // [4 rows][blocks] bytes
+  bool there[NS];                            // the values' page
 };
 
 // What a scale byte (bits 8 n .. of the word) stands for.
@@ -579,7 +586,7 @@ __device__ __forceinline__ float unit_in(uint32_t word, int n) {
 
 // PADDED: rows of fewer than DP values, or on any address.
 template <typename T, bool EIGHT, int DP, bool PADDED, bool SMALL>
-__global__ __launch_bounds__(256, (TileOf<T, EIGHT, DP>::AT_ONCE))
+__global__ __launch_bounds__(256, (TileOf<T, EIGHT, DP>::template at_once<PADDED>()))
 void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
   typedef TileOf<T, EIGHT, DP> Tile;
   typedef Group<T, EIGHT, DP, SMALL> Group;
@@ -634,76 +641,68 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
     const int32_t* table = a.pages.table + (int64_t)b * a.pages.P;
     const int step = Tile::GRAIN, start = first + wave * (16 * NS);
 
-    // The pages of the 16 positions from t0 + 16 s on (not SMALL); behind the end, that of
-    // the last one.
-    auto look_up = [&](int t0, int (&page)[NS]) {
+    // The pages of the 16 positions from t0 + 16 s on, SMALL: of the lane's key and values;
+    // behind the end, that of the last one.
+    struct Looked { int k, v; };
+    auto look_up = [&](int t0, Looked (&page)[NS]) {
 #pragma unroll
-      for (int s = 0; s < NS; ++s)
-        page[s] = scalar_load(table + (max(min(t0 + 16 * s, end - 1), 0) >> a.pages.shift));
+      for (int s = 0; s < NS; ++s) {
+        const int t = t0 + 16 * s, most = max(end - 1, 0);
+        if constexpr (SMALL) {
+          page[s].k = table[min(t + c, most) >> a.pages.shift];
+          page[s].v = table[min(t + 4 * j, most) >> a.pages.shift];
+        } else {
+          page[s].k = page[s].v = scalar_load(table + (min(t, most) >> a.pages.shift));
+        }
+      }
     };
     // Loads positions t0 .. t0 + 16 NS - 1; what of them is not there, or not before the end,
     // is read from rows that are, and left out when it is used.
-    auto load = [&](int t0, const int (&page)[NS], Group& g) {
-      int64_t k_row[NS], v_row[NS][SMALL ? 4 : 1];   // of lane 0's keys and values, SMALL:
-#pragma unroll                                       // of every lane's
-      for (int s = 0; s < NS; ++s) {
-        if constexpr (SMALL) {
-          const int t = t0 + 16 * s + c;
-          k_row[s] = t < end ? a.pages.row(b, t) : -1;
-          k_row[s] = a.pages.head(max(k_row[s], (int64_t)0), kv_head);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int u = t0 + 16 * s + 4 * j + r;
-            const int64_t row = u < end ? a.pages.row(b, u) : -1;
-            g.there[s][r] = row >= 0;
-            v_row[s][r] = a.pages.head(max(row, (int64_t)0), kv_head);
-          }
-        } else {
-          const int t = min(t0 + 16 * s, end - 1) & ~15;
-          g.there[s][0] = (unsigned)page[s] < (unsigned)a.pages.N;
-          k_row[s] = v_row[s][0] =
-              (((int64_t)(g.there[s][0] ? page[s] : 0) * a.pages.HK + kv_head)
-               << a.pages.shift) + (t & (S - 1));
-        }
-      }
+    auto load = [&](int t0, const Looked (&page)[NS], Group& g) {
+      // row number of position t in a page, 0 for a page that is not there
+      auto row_in = [&](int page, int t) {
+        const int there = (unsigned)page < (unsigned)a.pages.N ? page : 0;
+        return (((int64_t)there * a.pages.HK + kv_head) << a.pages.shift) + (t & (S - 1));
+      };
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        const uint8_t* from = k_pages + k_row[s] * D * SIZE;
+        // (not SMALL: of the 16 positions' first)
+        const int64_t row =
+            row_in(page[s].k, SMALL ? t0 + 16 * s + c : min(t0 + 16 * s, end - 1) & ~15);
+        const uint8_t* from = k_pages + row * D * SIZE;
 #pragma unroll
         for (int i = 0; i < KC; ++i)
           if (!PADDED || k_extra[i] < KV)
             load_words<16>(from + (uint32_t)(((SMALL ? 0 : c * D) + k_at[i]) * SIZE),
                            g.k[s][i]);
         if constexpr (EIGHT) {
-          const uint8_t* units = a.k_scales + k_row[s] * DB + (SMALL ? 0 : c * DB);
+          const uint8_t* units = a.k_scales + row * DB + (SMALL ? 0 : c * DB);
           g.k_units[s] = DB == 2 ? units[0] | (uint32_t)units[1] << 8 : units[0];
         }
       }
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
+        const int64_t row =
+            row_in(page[s].v, SMALL ? t0 + 16 * s + 4 * j : min(t0 + 16 * s, end - 1) & ~15);
+        const uint8_t* from = v_pages + row * D * SIZE;
+        g.there[s] = (unsigned)page[s].v < (unsigned)a.pages.N;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const uint8_t* from = v_pages + v_row[s][SMALL ? r : 0] * D * SIZE;
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
           for (int p = 0; p < VP; ++p)
             if (!PADDED || v_extra[p] < VE)
-              load_words<VB>(from + (SMALL ? 0 : r * D * SIZE) +
+              load_words<VB>(from + r * D * SIZE +
                                  (uint32_t)(((SMALL ? 0 : 4 * j * D) + v_at[p]) * SIZE),
                              g.v[s][r][p]);
-          if constexpr (EIGHT && SMALL) {
-            const uint8_t* units = a.v_scales + v_row[s][r] * DB;
-            g.v_units[s][r] = DB == 2 ? units[0] | (uint32_t)units[1] << 8 : units[0];
-          }
-        }
-        if constexpr (EIGHT && !SMALL)
-          load_words<4 * Group::BLOCKS>(a.v_scales + v_row[s][0] * DB + 4 * j * DB,
-                                        g.v_units[s]);
+        if constexpr (EIGHT)
+          load_words<4 * Group::BLOCKS>(
+              a.v_scales + row * DB + (SMALL ? 0 : 4 * j * DB), g.v_units[s]);
       }
     };
 
     // ---- the queries, as the second operand of the first product; 0 where there is no head
-    int page[NS];
-    if (!SMALL) look_up(start, page);
+    Looked page[NS];
+    look_up(start, page);
     constexpr int QN = Tile::WIDE ? KC * KV : KC * KV / 8;
     typedef std::conditional_t<Tile::WIDE, float, bf16x8_t> query_t;
     query_t q[QN];
@@ -797,14 +796,10 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
                 load_words<VB>(fresh_rows[1] + v_at[p] * SIZE, g.v[s][r][p]);
             if (EIGHT) {
               const uint32_t units = fresh_units[1][0] | (uint32_t)fresh_units[1][1] << 8;
-              if constexpr (SMALL) {
-                g.v_units[s][r] = units;
-              } else {
-                const int bits = 8 * DB * (r % (4 / DB));
-                uint32_t& word = g.v_units[s][r * DB / 4];
-                word = (word & ~((DB == 2 ? 0xffffu : 0xffu) << bits)) |
-                       (DB == 2 ? units : units & 0xffu) << bits;
-              }
+              const int bits = 8 * DB * (r % (4 / DB));
+              uint32_t& word = g.v_units[s][r * DB / 4];
+              word = (word & ~((DB == 2 ? 0xffffu : 0xffu) << bits)) |
+                     (DB == 2 ? units : units & 0xffu) << bits;
             }
           }
         }
@@ -888,16 +883,15 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
             for (int r = 0; r < 4; ++r) x[s][r] += bias[s][r];
         }
       }
-      bool whole = !SMALL && t0 + 16 * NS <= end;
-      if constexpr (!SMALL)
+      bool whole = t0 + 16 * NS <= end;
 #pragma unroll
-        for (int s = 0; s < NS; ++s) whole = whole && g.there[s][0];
-      if (!whole) {
+      for (int s = 0; s < NS; ++s) whole = whole && g.there[s];
+      if (SMALL ? !__all(whole) : !whole) {
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            if (g.there[s][SMALL ? r : 0] && t0 + 16 * s + 4 * j + r < end) continue;
+            if (g.there[s] && t0 + 16 * s + 4 * j + r < end) continue;
             x[s][r] = -INFINITY;
 #pragma unroll
             for (int p = 0; p < VP; ++p)
@@ -940,8 +934,6 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
       // -- sums of values
       auto v_unit = [&](int s, int r) {
         if constexpr (!EIGHT) return 1.f;
-        else if constexpr (SMALL)
-          return DB == 2 && c >= 8 ? unit_in(g.v_units[s][r], 1) : unit_in(g.v_units[s][r], 0);
         else if constexpr (DB == 2)
           return c >= 8 ? unit_in(g.v_units[s][r / 2], r % 2 * 2 + 1)
                         : unit_in(g.v_units[s][r / 2], r % 2 * 2);
@@ -1016,7 +1008,7 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
     for (int t0 = start; t0 < end; t0 += step) {
       Group g;
       load(t0, page, g);
-      if (!SMALL) look_up(t0 + step, page);
+      look_up(t0 + step, page);
       use(t0, g);
     }
 
@@ -1219,12 +1211,6 @@ static void run_read(const RowsOf& r, const void* k_pages, const void* v_pages,
 }
 
 constexpr int CUS = 256;
-// Units of up to so many grains are not divided, where there are as many as CUs twice as
-// long ones: 64 sequences of 1024, 8 heads of 128 (8 grains) take 49 us whole, 52 divided;
-// one of 2001, 1 head of 128 in 8 bits (8 grains) 19 whole, 12 divided, and one of 700, 16
-// heads of 64 (3 grains) 8.4 whole, 10.3 divided.
-constexpr int WHOLE = 4;
-
 // How the tiles' kernel divides its work and its workspace.
 struct Division {
   Shares shares;
@@ -1235,22 +1221,29 @@ struct Division {
 };
 
 template <typename T, bool EIGHT, int DP>
-static Shares shares_of() {
+static Shares shares_of(bool padded, int* whole) {
   typedef TileOf<T, EIGHT, DP> Tile;
-  return Shares{0, Tile::GRAIN, CUS * Tile::AT_ONCE};
+  *whole = Tile::WHOLE;
+  return Shares{0, Tile::GRAIN,
+                CUS * (padded ? Tile::template at_once<true>()
+                              : Tile::template at_once<false>())};
 }
 template <typename T, bool EIGHT>
-static Shares shares_of(int D) {
-  return D <= 64    ? shares_of<T, EIGHT, 64>()
-         : D <= 128 ? shares_of<T, EIGHT, 128>()
-                    : shares_of<T, EIGHT, 256>();
+static Shares shares_of(int D, bool padded, int* whole) {
+  return D <= 64    ? shares_of<T, EIGHT, 64>(padded, whole)
+         : D <= 128 ? shares_of<T, EIGHT, 128>(padded, whole)
+                    : shares_of<T, EIGHT, 256>(padded, whole);
 }
 
-static Division divide(int B, int H, int HK, int D, int S, int P, int dtype, bool eight) {
+static Division divide(int B, int H, int HK, int D, int S, int P, int dtype, bool eight,
+                       bool padded) {
   Division v = {};
+  int whole = 0;
   v.shares = dtype == MESH_MOE_BF16
-                 ? (eight ? shares_of<bf16_t, true>(D) : shares_of<bf16_t, false>(D))
-                 : (eight ? shares_of<float, true>(D) : shares_of<float, false>(D));
+                 ? (eight ? shares_of<bf16_t, true>(D, padded, &whole)
+                          : shares_of<bf16_t, false>(D, padded, &whole))
+                 : (eight ? shares_of<float, true>(D, padded, &whole)
+                          : shares_of<float, false>(D, padded, &whole));
   const int G = H / HK;
   const int64_t most = ((int64_t)P * S + v.shares.grain - 1) / v.shares.grain;
   const int64_t each = most + AHEAD;
@@ -1258,7 +1251,11 @@ static Division divide(int B, int H, int HK, int D, int S, int P, int dtype, boo
   v.fits = units <= 0x7fffffff / each / B && units * B <= MAX_BLOCKS;
   if (!v.fits) return v;
   v.shares.units = (int)units;
-  v.joins = most > (units * B >= CUS ? 2 * WHOLE : WHOLE);
+  // Units that are this short are not divided, with as many of them as CUs twice as long
+  // ones: 64 sequences of 1024, 8 heads of 128 (8 grains) take 49 us whole, 52 divided; one
+  // of 2001, 1 head of 128 in 8 bits (8 grains) 19 whole, 12 divided; one of 700, 16 heads
+  // of 64 (6 grains) 8.4 whole, 10.3 divided.
+  v.joins = most > (units * B >= CUS ? 2 * whole : whole);
   if (!v.joins) v.shares.blocks = 0;
   v.blocks = v.joins ? std::min<int64_t>(v.shares.blocks, units * each * B) : units * B;
   if (v.joins) {
@@ -1296,7 +1293,9 @@ static int run_tiles(const Attention& a, const Division& v, char* workspace,
   return 0;
 }
 
-// whether the tiles' kernel takes its PADDED form
+// what the tiles' kernel takes
+static bool takes_tiles(int D, int S) { return D >= 16 && S >= 4; }
+// whether it is its PADDED form
 static bool rows_padded(const Attention& a) {
   const int D = a.pages.D;
   return a.pages.shift < 4 || (D != 64 && D != 128 && D != 256) ||
@@ -1307,7 +1306,7 @@ template <typename T, bool EIGHT>
 static int run_attention(const Attention& a, const Division& v, bool padded,
                          char* workspace, hipStream_t st) {
   const int D = a.pages.D;
-  if (D < 16) {
+  if (!takes_tiles(D, 1 << a.pages.shift)) {
     cache_attention_kernel<T, EIGHT><<<(unsigned)((int64_t)a.B * a.H), 256, 0, st>>>(a);
     MOE_CHECK_LAUNCH("cache_attention");
     return 0;
@@ -1388,10 +1387,11 @@ extern "C" int mesh_moe_cache_read(const void* k_pages, const void* v_pages,
 extern "C" size_t mesh_moe_cache_attention_workspace_bytes(int B, int H, int HK, int D,
                                                            int S, int P, int dtype,
                                                            int eight_bit) {
-  if (B < 1 || H < 1 || HK < 1 || H % HK || D < 16 || D > MAX_WIDTH || S < 1 || P < 1 ||
+  if (B < 1 || H < 1 || HK < 1 || H % HK || !takes_tiles(D, S) || D > MAX_WIDTH || P < 1 ||
       !valid_dtype(dtype))
     return 0;
-  return divide(B, H, HK, D, S, P, dtype, eight_bit != 0).bytes;
+  // (the form with more blocks, wherever the operands lie)
+  return divide(B, H, HK, D, S, P, dtype, eight_bit != 0, false).bytes;
 }
 
 extern "C" int mesh_moe_cache_attention(
@@ -1416,8 +1416,9 @@ extern "C" int mesh_moe_cache_attention(
   a.v_pages = v_pages ? v_pages : k_pages;
   a.k_scales = k_scales;
   a.v_scales = v_pages ? v_scales : k_scales;
-  a.k_new = D < 16 ? nullptr : k_new;
-  a.v_new = D < 16 ? nullptr : v_new;
+  const bool tiles = takes_tiles(D, S);
+  a.k_new = tiles ? k_new : nullptr;
+  a.v_new = tiles ? v_new : nullptr;
   a.position = position;
   a.rel_values = rel_values;
   a.rel_bucket = rel_bucket;
@@ -1428,13 +1429,14 @@ extern "C" int mesh_moe_cache_attention(
   a.H = H;
   a.G = H / HK;
   const bool padded = rows_padded(a);
-  const Division v = divide(B, H, HK, std::max(D, 16), S, P, dtype, k_scales != nullptr);
-  MOE_REQUIRE(v.fits && (D >= 16 || (int64_t)B * H <= MAX_BLOCKS), MESH_MOE_E_UNSUPPORTED,
+  const Division v = divide(B, H, HK, std::max(D, 16), S, P, dtype, k_scales != nullptr,
+                            padded);
+  MOE_REQUIRE(v.fits && (tiles || (int64_t)B * H <= MAX_BLOCKS), MESH_MOE_E_UNSUPPORTED,
               "cache_attention: %d sequences of %d heads and %d pages are more than a "
               "launch has", B, H, P);
-  MOE_REQUIRE(D < 16 || v.bytes == 0 || (workspace && workspace_bytes >= v.bytes),
+  MOE_REQUIRE(!tiles || v.bytes == 0 || (workspace && workspace_bytes >= v.bytes),
               MESH_MOE_E_ARG, "cache_attention: workspace too small");
-  if (k_new && D < 16) {
+  if (k_new && !tiles) {
     if (int rc = mesh_moe_cache_write(k_new, v_new, table, position, nullptr, k_pages,
                                       v_pages, k_scales, v_scales, B, 1, HK, D, N, S, P,
                                       dtype, stream))
