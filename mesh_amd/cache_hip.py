@@ -18,6 +18,7 @@ the page of every page_size positions, -1 one that it does not have (yet).
 """
 
 import ctypes
+import functools
 
 import torch
 
@@ -62,6 +63,8 @@ def load_library():
 
 
 _empty = torch.empty
+_empty_like = torch.empty_like
+_current_device = moe_hip.current_device
 _dev = fp8_hip._dev        # pylint: disable=protected-access
 _stage = moe_hip._stage    # pylint: disable=protected-access
 _check = moe_hip._check    # pylint: disable=protected-access
@@ -80,7 +83,7 @@ class PagedCache(object):
   page_size, scale_blocks(d_kv)] uint8; value i of a row stands for value *
   2^(scales[i // 128] - 127).  v_pages None: the keys are the values (shared_kv)."""
 
-  __slots__ = ("_k", "_v", "_k_scales", "_v_scales", "_shape")
+  __slots__ = ("_k", "_v", "_k_scales", "_v_scales", "_shape", "_device")
 
   def __init__(self, k_pages, v_pages=None, k_scales=None, v_scales=None):
     shape = k_pages.shape
@@ -106,6 +109,13 @@ class PagedCache(object):
     self._k, self._v = k_pages, v_pages
     self._k_scales, self._v_scales = k_scales, v_scales
     self._shape = tuple(shape)
+    # the device of all buffers, where they are what the library takes
+    self._device = None
+    if k_pages.is_cuda:
+      device = k_pages.get_device()
+      if all(x is None or (x.is_cuda and x.get_device() == device and x.is_contiguous())
+             for x in (k_pages, v_pages, k_scales, v_scales)):
+        self._device = device
 
   @classmethod
   def empty(cls, pages, page_size, heads, d_kv, dtype=torch.bfloat16, device="cuda",
@@ -144,9 +154,12 @@ def _pointers(cache):
     raise MoeHipError("cache must be a PagedCache")
   # pylint: disable=protected-access
   k, v, ks, vs = cache._k, cache._v, cache._k_scales, cache._v_scales
-  return (_dev(k, "k_pages"), None if v is None else _dev(v, "v_pages"),
-          None if ks is None else _dev(ks, "k_scales"),
-          None if vs is None else _dev(vs, "v_scales"))
+  if cache._device is None or cache._device != _current_device():
+    for t, name in ((k, "k_pages"), (v, "v_pages"), (ks, "k_scales"), (vs, "v_scales")):
+      if t is not None:
+        _dev(t, name)            # (says what is wrong with it)
+  return (k.data_ptr(), None if v is None else v.data_ptr(),
+          None if ks is None else ks.data_ptr(), None if vs is None else vs.data_ptr())
 
 
 def _type(cache, dtype):
@@ -160,7 +173,13 @@ def _type(cache, dtype):
 def _table(table, batch):
   if table.dim() != 2:
     raise MoeHipError("table %s, expected [batch, columns]" % (tuple(table.shape),))
-  return _dev(table, "table", torch.int32, (batch, table.shape[1])), table.shape[1]
+  columns = table.shape[1]
+  return _dev(table, "table", torch.int32, (batch, columns)), columns
+
+
+@functools.lru_cache(maxsize=None)
+def _workspace_bytes(*sizes):
+  return load_library().mesh_moe_cache_attention_workspace_bytes(*sizes)
 
 
 def write(cache, k, v, table, position, count=None):
@@ -211,7 +230,7 @@ def read(cache, table, position, length, count=None, dtype=None):
   cp = None if count is None else _dev(count, "count", torch.int32, (b,))
   make = _empty if columns else torch.zeros
   k = make((b, length, heads * d), dtype=dtype, device=position.device)
-  v = None if cache.shared_kv else make(k.shape, dtype=dtype, device=position.device)
+  v = None if cache.shared_kv else _empty_like(k) if columns else k.clone()
   if k.numel() and columns:
     with _stage("cache_read"):
       _check(lib.mesh_moe_cache_read(
@@ -266,9 +285,8 @@ def attention(q, cache, table, position, k_new=None, v_new=None, relative_bias=N
   relative = _relative_bias(relative_bias, dtype, h)
   if not (b and columns):
     return torch.zeros_like(q)
-  out = _empty(shape, dtype=dtype, device=q.device)
-  ws_bytes = lib.mesh_moe_cache_attention_workspace_bytes(
-      b, h, heads, d, s, columns, code, int(cache._k_scales is not None))  # pylint: disable=protected-access
+  out = _empty_like(q)
+  ws_bytes = _workspace_bytes(b, h, heads, d, s, columns, code, cache.eight_bit)
   ws = _empty((ws_bytes,), dtype=torch.uint8, device=q.device) if ws_bytes else None
   with _stage("cache_attention"):
     _check(lib.mesh_moe_cache_attention(

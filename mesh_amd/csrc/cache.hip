@@ -33,6 +33,13 @@ struct Pages {
   }
 };
 
+// What nothing in a launch writes, from an address that is the same for all lanes: a load
+// through the scalar cache, which does not wait for the vector loads before it.
+__device__ __forceinline__ int32_t scalar_load(const int32_t* p) {
+  typedef const __attribute__((address_space(4))) int32_t* constant_t;
+  return *reinterpret_cast<constant_t>(reinterpret_cast<uintptr_t>(p));
+}
+
 // What a scale byte stands for (2^-127 is not a normal number).
 __device__ __forceinline__ float unit_of(uint32_t byte) {
   return __uint_as_float(byte == 255 ? 0x7fc00000u
@@ -49,11 +56,56 @@ __device__ __forceinline__ uint32_t max_of_lanes(uint32_t v, int lanes) {
   return v;
 }
 
+template <int BYTES> struct Words;                 // of any address
+template <> struct Words<4> { typedef uint32_t type __attribute__((aligned(1))); };
+template <> struct Words<8> {
+  typedef uint32_t type __attribute__((ext_vector_type(2), aligned(1)));
+};
+template <> struct Words<16> {
+  typedef uint32_t type __attribute__((ext_vector_type(4), aligned(1)));
+};
+template <int BYTES>
+__device__ __forceinline__ void load_words(const uint8_t* at, uint32_t* to) {
+  typedef typename Words<BYTES>::type words_t;
+  const words_t v = *reinterpret_cast<const words_t*>(at);
+  if constexpr (BYTES == 4) {
+    to[0] = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < BYTES / 4; ++i) to[i] = v[i];
+  }
+}
+
+// 8 values of 8 bits of a row of D from value `at` on, zeros behind the row, and back.
+template <bool ALIGNED>
+__device__ __forceinline__ void load_eight(const uint8_t* row, int at, int D,
+                                           uint32_t (&w)[2]) {
+  if (ALIGNED || at + 8 <= D) {
+    load_words<8>(row + at, w);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 7; ++j)
+    if (at + j < D) w[j / 4] |= (uint32_t)row[at + j] << 8 * (j & 3);
+}
+template <bool ALIGNED>
+__device__ __forceinline__ void store_eight(uint8_t* row, int at, int D, uint32_t lo,
+                                            uint32_t hi) {
+  if (ALIGNED || at + 8 <= D) {
+    *reinterpret_cast<Words<8>::type*>(row + at) = Words<8>::type{lo, hi};
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 7; ++j)
+    if (at + j < D) row[at + j] = (uint8_t)((j < 4 ? lo : hi) >> 8 * (j & 3));
+}
+
 // ---------------------------------------------------------------------------
-// Rows into pages and back.  A wavefront has a row of keys or of values (blockIdx.y),
-// whose page is the same for all its lanes; a lane has 8 values, and a head's lanes are a
-// power of two (16 for each block of 128 where it has more than one), so that a block's
-// largest magnitude is found by DPP steps among neighbours.
+// Rows into pages and back.  A wavefront has R rows of keys or of values (blockIdx.z) that
+// follow each other in a sequence (blockIdx.y), so that loads of R rows are on their way at
+// once; with one row a sequence the wavefronts of a block share it.  A lane has 8 values of
+// each, and a head's lanes are a power of two (16 for each block of 128 where it has more
+// than one), so that a block's largest magnitude is found by DPP steps among neighbours.
 // ---------------------------------------------------------------------------
 struct RowsOf {
   Pages pages;
@@ -62,114 +114,140 @@ struct RowsOf {
   int B, T;
   int lanes;                      // of a head, log2
 };
+// Rows of a wavefront, where a sequence has several: 4 x 16384 rows of 1024 values out of
+// an 8-bit cache take 84 us by one, 82 by two, 69 by four; 23 x 1000 of 480 out of a
+// bfloat16 one 24 by one, 17 by two, 21 by four.
+template <bool EIGHT> constexpr int ROWS = EIGHT ? 4 : 2;
 
-template <typename T, bool EIGHT, bool ALIGNED>
-__global__ __launch_bounds__(256) void cache_write_kernel(
-    RowsOf r, const T* __restrict__ k, const T* __restrict__ v, void* k_pages,
-    void* v_pages, uint8_t* k_scales, uint8_t* v_scales) {
-  const bool is_v = blockIdx.y != 0;
-  const T* x = is_v ? v : k;
-  uint8_t* values = static_cast<uint8_t*>(is_v ? v_pages : k_pages);
-  uint8_t* scales = is_v ? v_scales : k_scales;
-  const int lane = threadIdx.x & 63, D = r.pages.D, HK = r.pages.HK;
-  const int pieces = HK << r.lanes, group = min(1 << r.lanes, 16);
-  const int64_t rows = (int64_t)r.B * r.T;
-  for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < rows;
-       i += (int64_t)gridDim.x * 4) {
-    const int b = (int)(i / r.T), t = (int)(i - (int64_t)b * r.T);
-    if (r.count && t >= r.count[b]) continue;
-    const int64_t to = r.pages.row(b, (int64_t)r.position[b] + t);
-    if (to < 0) continue;
-    const T* from = x + i * HK * D;
-    for (int piece = lane; piece < (pieces + 63) / 64 * 64; piece += 64) {
-      const int h = piece >> r.lanes;
-      const int at = h < HK ? (piece & ((1 << r.lanes) - 1)) * 8 : D;
-      float f[8];
-      load8<T, ALIGNED>(from + (int64_t)min(h, HK - 1) * D, at, D, f);
-      const int64_t row = r.pages.head(to, h);
-      if constexpr (EIGHT) {
-        uint32_t top = 0;
+// Calls f(b, t0, rows, from, piece, step): rows t0 .. of sequence b, which lie (from) in
+// rows of the pages or nowhere (-1), of which this lane has the pieces piece, piece + step,
+// ...  `rows` of them are before the count.
+template <int R, typename F>
+__device__ __forceinline__ void for_rows(const RowsOf& r, F f) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int groups = (r.T + R - 1) / R;
+  for (int b = blockIdx.y; b < r.B; b += gridDim.y) {
+    const int count = r.count ? min(max(scalar_load(r.count + b), 0), r.T) : r.T;
+    const int position = scalar_load(r.position + b);
+    const int32_t* table = r.pages.table + (int64_t)b * r.pages.P;
+    for (int64_t g = R == 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+         g < groups; g += R == 1 ? (int64_t)gridDim.x : (int64_t)gridDim.x * 4) {
+      const int t0 = (int)g * R;
+      int64_t rows[R];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, magnitude_bits(f[j]));
-        const Fp8Scale s = fp8_scale(max_of_lanes(top, group));
-        if (at >= D) continue;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] *= s.factor;
-        const uint32_t lo = fp8_pack4(f[0], f[1], f[2], f[3]);
-        const uint32_t hi = fp8_pack4(f[4], f[5], f[6], f[7]);
-        uint8_t* q = values + row * D + at;
-        if (ALIGNED) {
-          *reinterpret_cast<uint2*>(q) = make_uint2(lo, hi);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (at + j < D) q[j] = (uint8_t)((j < 4 ? lo : hi) >> 8 * (j & 3));
-        }
-        if ((piece & (group - 1)) == 0)
-          scales[row * r.pages.DB + at / FP8_BLOCK] = (uint8_t)s.byte;
-      } else {
-        if (at < D)
-          store8<T, ALIGNED>(reinterpret_cast<T*>(values) + row * D, at, D, f);
+      for (int i = 0; i < R; ++i) {
+        const int64_t p = (int64_t)position + t0 + i;
+        rows[i] = -1;
+        if (t0 + i >= count || p < 0 || (p >> r.pages.shift) >= r.pages.P) continue;
+        const int page = scalar_load(table + (p >> r.pages.shift));
+        if ((unsigned)page < (unsigned)r.pages.N)
+          rows[i] = (((int64_t)page * r.pages.HK) << r.pages.shift) +
+                    (p & ((1 << r.pages.shift) - 1));
       }
+      f(b, t0, min(r.T - t0, R), rows, R == 1 ? (int)threadIdx.x : lane,
+        R == 1 ? 256 : 64);
     }
   }
 }
 
-template <typename T, bool EIGHT, bool ALIGNED>
+template <typename T, bool EIGHT, bool ALIGNED, int R>
+__global__ __launch_bounds__(256) void cache_write_kernel(
+    RowsOf r, const T* __restrict__ k, const T* __restrict__ v, void* k_pages,
+    void* v_pages, uint8_t* k_scales, uint8_t* v_scales) {
+  const bool is_v = blockIdx.z != 0;
+  const T* x = is_v ? v : k;
+  uint8_t* values = static_cast<uint8_t*>(is_v ? v_pages : k_pages);
+  uint8_t* scales = is_v ? v_scales : k_scales;
+  const int D = r.pages.D, HK = r.pages.HK;
+  const int pieces = HK << r.lanes, group = min(1 << r.lanes, 16);
+  for_rows<R>(r, [&](int b, int t0, int, const int64_t (&to)[R], int first, int step) {
+    const T* from = x + ((int64_t)b * r.T + t0) * HK * D;
+    // (whole wavefronts, as the maxima take them)
+    for (int piece = first; piece < (pieces + 63) / 64 * 64; piece += step) {
+      const int h = piece >> r.lanes;
+      const int at = h < HK ? (piece & ((1 << r.lanes) - 1)) * 8 : D;
+      float f[R][8];
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        load8<T, ALIGNED>(from + ((int64_t)i * HK + min(h, HK - 1)) * D,
+                          to[i] < 0 ? D : at, D, f[i]);
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        if (to[i] < 0) continue;
+        const int64_t row = r.pages.head(to[i], h);
+        if constexpr (EIGHT) {
+          uint32_t top = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) top = max(top, magnitude_bits(f[i][j]));
+          const Fp8Scale s = fp8_scale(max_of_lanes(top, group));
+          if (at >= D) continue;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[i][j] *= s.factor;
+          const uint32_t lo = fp8_pack4(f[i][0], f[i][1], f[i][2], f[i][3]);
+          const uint32_t hi = fp8_pack4(f[i][4], f[i][5], f[i][6], f[i][7]);
+          store_eight<ALIGNED>(values + row * D, at, D, lo, hi);
+          if ((piece & (group - 1)) == 0)
+            scales[row * r.pages.DB + at / FP8_BLOCK] = (uint8_t)s.byte;
+        } else {
+          if (at < D)
+            store8<T, ALIGNED>(reinterpret_cast<T*>(values) + row * D, at, D, f[i]);
+        }
+      }
+    }
+  });
+}
+
+template <typename T, bool EIGHT, bool ALIGNED, int R>
 __global__ __launch_bounds__(256) void cache_read_kernel(
     RowsOf r, const void* __restrict__ k_pages, const void* __restrict__ v_pages,
     const uint8_t* __restrict__ k_scales, const uint8_t* __restrict__ v_scales,
     T* __restrict__ k, T* __restrict__ v) {
-  const bool is_v = blockIdx.y != 0;
+  const bool is_v = blockIdx.z != 0;
   T* y = is_v ? v : k;
   const uint8_t* values = static_cast<const uint8_t*>(is_v ? v_pages : k_pages);
   const uint8_t* scales = is_v ? v_scales : k_scales;
-  const int lane = threadIdx.x & 63, D = r.pages.D, HK = r.pages.HK;
+  const int D = r.pages.D, HK = r.pages.HK;
   const int pieces = HK << r.lanes;
-  const int64_t rows = (int64_t)r.B * r.T;
-  for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < rows;
-       i += (int64_t)gridDim.x * 4) {
-    const int b = (int)(i / r.T), t = (int)(i - (int64_t)b * r.T);
-    const int64_t from = r.count && t >= r.count[b]
-                             ? -1 : r.pages.row(b, (int64_t)r.position[b] + t);
-    T* to = y + i * HK * D;
-    for (int piece = lane; piece < pieces; piece += 64) {
+  for_rows<R>(r, [&](int b, int t0, int n, const int64_t (&from)[R], int first, int step) {
+    T* to = y + ((int64_t)b * r.T + t0) * HK * D;
+    for (int piece = first; piece < pieces; piece += step) {
       const int h = piece >> r.lanes, at = (piece & ((1 << r.lanes) - 1)) * 8;
       if (at >= D) continue;
-      const int64_t row = r.pages.head(from, h);
-      float f[8];
+      float f[R][8];
+      uint32_t w[R][2], byte[R];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = 0.f;
-      if (from >= 0) {
-        if constexpr (EIGHT) {
-          const uint8_t* q = values + row * D + at;
-          uint32_t w[2] = {0, 0};
-          if (ALIGNED) {
-            const uint2 both = *reinterpret_cast<const uint2*>(q);
-            w[0] = both.x;
-            w[1] = both.y;
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (at + j < D) w[j / 4] |= (uint32_t)q[j] << 8 * (j & 3);
-          }
-          const float unit = unit_of(scales[row * r.pages.DB + at / FP8_BLOCK]);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[j], false);
-            const f32x2_t hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[j], true);
-            f[4 * j] = lo[0] * unit;
-            f[4 * j + 1] = lo[1] * unit;
-            f[4 * j + 2] = hi[0] * unit;
-            f[4 * j + 3] = hi[1] * unit;
-          }
-        } else {
-          load8<T, ALIGNED>(reinterpret_cast<const T*>(values) + row * D, at, D, f);
+      for (int i = 0; i < R; ++i) {
+        const int64_t row = r.pages.head(from[i], h);
+        w[i][0] = w[i][1] = 0;
+        byte[i] = FP8_UNIT;
+        if constexpr (!EIGHT) {
+          load8<T, ALIGNED>(reinterpret_cast<const T*>(values) + row * D,
+                            from[i] < 0 ? D : at, D, f[i]);
+        } else if (from[i] >= 0) {
+          load_eight<ALIGNED>(values + row * D, at, D, w[i]);
+          byte[i] = scales[row * r.pages.DB + at / FP8_BLOCK];
         }
       }
-      store8<T, ALIGNED>(to + (int64_t)h * D, at, D, f);
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        if (i >= n) continue;
+        if constexpr (EIGHT) {
+          const float unit = unit_of(byte[i]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i][j], false);
+            const f32x2_t hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i][j], true);
+            f[i][4 * j] = lo[0] * unit;
+            f[i][4 * j + 1] = lo[1] * unit;
+            f[i][4 * j + 2] = hi[0] * unit;
+            f[i][4 * j + 3] = hi[1] * unit;
+          }
+        }
+        store8<T, ALIGNED>(to + ((int64_t)i * HK + h) * D, at, D, f[i]);
+      }
     }
-  }
+  });
 }
 
 // ---------------------------------------------------------------------------
@@ -193,13 +271,6 @@ struct Attention {
   void* out;
   int B, H, G;                    // G query heads share a key / value head
 };
-
-// What nothing in a launch writes, from an address that is the same for all lanes: a load
-// through the scalar cache, which does not wait for the vector loads before it.
-__device__ __forceinline__ int32_t scalar_load(const int32_t* p) {
-  typedef const __attribute__((address_space(4))) int32_t* constant_t;
-  return *reinterpret_cast<constant_t>(reinterpret_cast<uintptr_t>(p));
-}
 
 // visible positions of a sequence whose query is at `position`
 __device__ __forceinline__ int seen_from(const Attention& a, int position) {
@@ -327,14 +398,6 @@ typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-template <int BYTES> struct Words;                 // of any address
-template <> struct Words<4> { typedef uint32_t type __attribute__((aligned(1))); };
-template <> struct Words<8> {
-  typedef uint32_t type __attribute__((ext_vector_type(2), aligned(1)));
-};
-template <> struct Words<16> {
-  typedef uint32_t type __attribute__((ext_vector_type(4), aligned(1)));
-};
 // two 8-bit values of a word, times their unit, in bfloat16 (exact)
 template <bool HIGH>
 __device__ __forceinline__ uint32_t widened(uint32_t word, float unit) {
@@ -350,18 +413,6 @@ __device__ __forceinline__ void four_floats(uint32_t word, float unit, float (&f
   f[1] = lo[1] * unit;
   f[2] = hi[0] * unit;
   f[3] = hi[1] * unit;
-}
-
-template <int BYTES>
-__device__ __forceinline__ void load_words(const uint8_t* at, uint32_t* to) {
-  typedef typename Words<BYTES>::type words_t;
-  const words_t v = *reinterpret_cast<const words_t*>(at);
-  if constexpr (BYTES == 4) {
-    to[0] = v;
-  } else {
-#pragma unroll
-    for (int i = 0; i < BYTES / 4; ++i) to[i] = v[i];
-  }
 }
 
 constexpr int HEADS = 16;                          // columns of a tile
@@ -507,27 +558,23 @@ __device__ __forceinline__ void keep_row(const Attention& a, int of, int b, int 
     for (int e = 0; e < 8; ++e) f[e] *= s.factor;
     const uint32_t lo = fp8_pack4(f[0], f[1], f[2], f[3]);
     const uint32_t hi = fp8_pack4(f[4], f[5], f[6], f[7]);
-    uint8_t* page = static_cast<uint8_t*>(pages) + to * D;
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (at + e < D) {
-        const uint8_t byte = (uint8_t)((e < 4 ? lo : hi) >> 8 * (e & 3));
-        row[at + e] = byte;
-        if (writes && own) page[at + e] = byte;
-      }
+    if (at < D) {
+      store_eight<false>(row, at, D, lo, hi);
+      if (writes && own)
+        store_eight<false>(static_cast<uint8_t*>(pages) + to * D, at, D, lo, hi);
+    }
     if (at < D && lane % 16 == 0) {
       units[lane / 16] = (uint8_t)s.byte;
       if (writes && own) scales[to * a.pages.DB + lane / 16] = (uint8_t)s.byte;
     }
   } else {
-    T* page = static_cast<T*>(pages) + to * D;
-    T* kept = reinterpret_cast<T*>(row);
+    if (at < D) {
+      T* kept = reinterpret_cast<T*>(row);
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (at + e < D) {
-        store_f32<T>(kept + at + e, f[e]);
-        if (writes && own) store_f32<T>(page + at + e, f[e]);
-      }
+      for (int e = 0; e < 8; ++e)
+        if (at + e < D) store_f32<T>(kept + at + e, f[e]);
+      if (writes && own) store8<T, false>(static_cast<T*>(pages) + to * D, at, D, f);
+    }
   }
 }
 
@@ -1181,33 +1228,40 @@ static int lanes_of(int D) {
   return n;
 }
 
-// blocks of the kernels that have a wavefront per row
-static unsigned row_blocks(int64_t rows) {
-  return (unsigned)std::min<int64_t>((rows + 3) / 4, 1 << 20);
+// the grid of the kernels that have rows
+static dim3 row_grid(const RowsOf& r, int rows, bool v) {
+  const int64_t groups = rows == 1 ? r.T : ((int64_t)r.T + 4 * rows - 1) / (4 * rows);
+  return dim3((unsigned)std::min<int64_t>(groups, 1 << 14),
+              (unsigned)std::min(r.B, 1 << 14), v ? 2 : 1);
 }
 
 template <typename T, bool EIGHT>
 static void run_write(const RowsOf& r, const void* k, const void* v, void* k_pages,
                       void* v_pages, uint8_t* k_scales, uint8_t* v_scales,
                       hipStream_t st) {
-  const dim3 grid(row_blocks((int64_t)r.B * r.T), v ? 2 : 1);
-  auto kern = r.pages.D % 8 == 0 && on_16_bytes({k, v, k_pages, v_pages})
-                  ? cache_write_kernel<T, EIGHT, true>
-                  : cache_write_kernel<T, EIGHT, false>;
-  kern<<<grid, 256, 0, st>>>(r, static_cast<const T*>(k), static_cast<const T*>(v),
-                             k_pages, v_pages, k_scales, v_scales);
+  const bool aligned = r.pages.D % 8 == 0 && on_16_bytes({k, v, k_pages, v_pages});
+  const bool one = r.T == 1;
+  auto kern = aligned ? (one ? cache_write_kernel<T, EIGHT, true, 1>
+                             : cache_write_kernel<T, EIGHT, true, ROWS<EIGHT>>)
+                      : (one ? cache_write_kernel<T, EIGHT, false, 1>
+                             : cache_write_kernel<T, EIGHT, false, ROWS<EIGHT>>);
+  kern<<<row_grid(r, one ? 1 : ROWS<EIGHT>, v != nullptr), 256, 0, st>>>(
+      r, static_cast<const T*>(k), static_cast<const T*>(v), k_pages, v_pages, k_scales,
+      v_scales);
 }
 
 template <typename T, bool EIGHT>
 static void run_read(const RowsOf& r, const void* k_pages, const void* v_pages,
                      const uint8_t* k_scales, const uint8_t* v_scales, void* k, void* v,
                      hipStream_t st) {
-  const dim3 grid(row_blocks((int64_t)r.B * r.T), v ? 2 : 1);
-  auto kern = r.pages.D % 8 == 0 && on_16_bytes({k, v, k_pages, v_pages})
-                  ? cache_read_kernel<T, EIGHT, true>
-                  : cache_read_kernel<T, EIGHT, false>;
-  kern<<<grid, 256, 0, st>>>(r, k_pages, v_pages, k_scales, v_scales,
-                             static_cast<T*>(k), static_cast<T*>(v));
+  const bool aligned = r.pages.D % 8 == 0 && on_16_bytes({k, v, k_pages, v_pages});
+  const bool one = r.T == 1;
+  auto kern = aligned ? (one ? cache_read_kernel<T, EIGHT, true, 1>
+                             : cache_read_kernel<T, EIGHT, true, ROWS<EIGHT>>)
+                      : (one ? cache_read_kernel<T, EIGHT, false, 1>
+                             : cache_read_kernel<T, EIGHT, false, ROWS<EIGHT>>);
+  kern<<<row_grid(r, one ? 1 : ROWS<EIGHT>, v != nullptr), 256, 0, st>>>(
+      r, k_pages, v_pages, k_scales, v_scales, static_cast<T*>(k), static_cast<T*>(v));
 }
 
 constexpr int CUS = 256;
