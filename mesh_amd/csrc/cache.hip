@@ -119,6 +119,16 @@ struct RowsOf {
 // bfloat16 one 24 by one, 17 by two, 21 by four.
 template <bool EIGHT> constexpr int ROWS = EIGHT ? 4 : 2;
 
+// Where piece `piece` of a head's row begins: a piece that would end behind the row begins as
+// much earlier, if that is in its block of 128 (EIGHT) or row, and the values that two lanes
+// have then are the same.  D for a piece that the row does not have.
+template <bool EIGHT, bool ALIGNED>
+__device__ __forceinline__ int piece_at(int piece, int D) {
+  const int at = min(piece * 8, D);
+  if (ALIGNED || at == D || at + 8 <= D) return at;
+  return D - (EIGHT ? at / FP8_BLOCK * FP8_BLOCK : 0) >= 8 ? D - 8 : at;
+}
+
 // Calls f(b, t0, rows, from, piece, step): rows t0 .. of sequence b, which lie (from) in
 // rows of the pages or nowhere (-1), of which this lane has the pieces piece, piece + step,
 // ...  `rows` of them are before the count.
@@ -166,7 +176,8 @@ __global__ __launch_bounds__(256) void cache_write_kernel(
     // (whole wavefronts, as the maxima take them)
     for (int piece = first; piece < (pieces + 63) / 64 * 64; piece += step) {
       const int h = piece >> r.lanes;
-      const int at = h < HK ? (piece & ((1 << r.lanes) - 1)) * 8 : D;
+      const int at =
+          h < HK ? piece_at<EIGHT, ALIGNED>(piece & ((1 << r.lanes) - 1), D) : D;
       float f[R][8];
 #pragma unroll
       for (int i = 0; i < R; ++i)
@@ -212,7 +223,8 @@ __global__ __launch_bounds__(256) void cache_read_kernel(
   for_rows<R>(r, [&](int b, int t0, int n, const int64_t (&from)[R], int first, int step) {
     T* to = y + ((int64_t)b * r.T + t0) * HK * D;
     for (int piece = first; piece < pieces; piece += step) {
-      const int h = piece >> r.lanes, at = (piece & ((1 << r.lanes) - 1)) * 8;
+      const int h = piece >> r.lanes;
+      const int at = piece_at<EIGHT, ALIGNED>(piece & ((1 << r.lanes) - 1), D);
       if (at >= D) continue;
       float f[R][8];
       uint32_t w[R][2], byte[R];
