@@ -205,8 +205,11 @@ class ExpertsAttentionParams(AttentionParams):
     raise NotImplementedError("ExpertsAttention uses shared_kv = True.")
 
 
+MAX_DISTANCE = 128     # of relative_position_bucket
+
+
 def relative_position_bucket(relative_position, bidirectional=True,
-                             num_buckets=32, max_distance=128):
+                             num_buckets=32, max_distance=MAX_DISTANCE):
   """_relative_position_bucket (transformer_layers.py:1000-1042) on host
   integers: relative_position = memory position - query position -> bucket in
   [0, num_buckets).  Half of the buckets hold exact small distances, the rest
@@ -410,6 +413,113 @@ class AttentionDecodeOperation(mtf.Operation):
     outs = mesh_impl.slicewise(fn, *[lowering.tensors[t] for t in self.inputs])
     for tensor, value in zip(self.outputs, outs):
       lowering.set_tensor_lowering(tensor, value)
+
+
+class PagedState(object):
+  """A layer's recurrent states kept in pages: `cache` (a cache_hip.PagedCache of the
+  activations' type or of 8 bits) and `table` [batch dims..., columns] int32 on the GPU,
+  which page has every page_size positions of a batch entry (-1: none yet).  Passed as the
+  layer's one state in "first_part" and "incremental" mode, and recorded as its new one;
+  the cache itself is updated in place, and the program gives sequences pages by writing
+  into `table`, also between the replays of a recorded step."""
+
+  def __init__(self, cache, table):
+    self.cache, self.table = cache, table
+
+  def check(self, channels, num_heads, batch_shape, shared_kv):
+    """Raises where the state is not one of an attention layer of these sizes."""
+    cache = self.cache
+    if (cache.heads * cache.d_kv != channels or cache.heads != num_heads or
+        cache.shared_kv != shared_kv):
+      raise ValueError("%r is no state of %d heads with %d channels%s"
+                       % (cache, num_heads, channels,
+                          " shared by keys and values" if shared_kv else ""))
+    if tuple(self.table.shape[:-1]) != tuple(batch_shape):
+      raise ValueError("table %s does not match the batch %s"
+                       % (tuple(self.table.shape), tuple(batch_shape)))
+
+  @property
+  def flat_table(self):
+    return self.table.reshape(-1, self.table.shape[-1])
+
+
+class PagedWriteOperation(mtf.Operation):
+  """The keys and values of a first part, [batch..., length, heads * d_kv], become the
+  positions 0 .. length - 1 of a PagedState (v None: shared_kv); positions without a page
+  are left out.  The output is k, for whoever wants to depend on it."""
+
+  def __init__(self, k, v, state, num_heads, name=None):
+    super(PagedWriteOperation, self).__init__([k] if v is None else [k, v],
+                                              name=name or "paged_write")
+    sizes = k.shape.to_integer_list
+    state.check(sizes[-1], num_heads, sizes[:-2], v is None)
+    self._state = state
+    self._outputs = [mtf.Tensor(self, k.shape, k.dtype)]
+
+  has_gradient = False
+
+  def lower(self, lowering):
+    from mesh_amd import cache_hip
+    state, sizes = self._state, self.outputs[0].shape.to_integer_list
+
+    def fn(k, *v):
+      rows = [t.reshape(-1, *sizes[-2:]).contiguous() for t in (k,) + v]
+      start = torch.zeros(rows[0].shape[0], dtype=torch.int32, device=k.device)
+      cache_hip.write(state.cache, rows[0], rows[1] if v else None, state.flat_table,
+                      start)
+      return k
+    lowering.set_tensor_lowering(
+        self.outputs[0], lowering.mesh_impl(self).slicewise(
+            fn, *[lowering.tensors[t] for t in self.inputs]))
+
+
+class PagedDecodeOperation(mtf.Operation):
+  """AttentionDecodeOperation over a PagedState: q, k, v [batch..., heads * d_kv] of the
+  step (v None: shared_kv) and position [batch...] (int32) -> the attention outputs.  The
+  step's row is written into the state in the same pass; nothing else of it is touched.
+  A position of -1 is a batch entry without a sequence, whose outputs are zeros."""
+
+  def __init__(self, q, k, v, position, state, num_heads, relative_values=None,
+               relative_bidirectional=False, name=None):
+    super(PagedDecodeOperation, self).__init__(
+        [q, k, position] + ([] if v is None else [v]) + (
+            [] if relative_values is None else [relative_values]),
+        name=name or "paged_decode")
+    if q.shape != k.shape or (v is not None and q.shape != v.shape):
+      raise ValueError("q, k, v %s %s %s" % (q.shape, k.shape, v and v.shape))
+    if position.shape.dims != q.shape.dims[:-1]:
+      raise ValueError("position %s does not match q %s" % (position.shape, q.shape))
+    sizes = q.shape.to_integer_list
+    state.check(sizes[-1], num_heads, sizes[:-1], v is None)
+    self._state = state
+    self._has_v, self._has_rel = v is not None, relative_values is not None
+    self._rel_bidirectional = bool(relative_bidirectional)
+    self._outputs = [mtf.Tensor(self, q.shape, q.dtype)]
+
+  has_gradient = False
+
+  def lower(self, lowering):
+    from mesh_amd import cache_hip
+    state, bidirectional = self._state, self._rel_bidirectional
+    has_v, has_rel = self._has_v, self._has_rel
+    sizes = self.outputs[0].shape.to_integer_list
+
+    def fn(q, k, position, *extra):
+      q2, k2 = (t.reshape(-1, sizes[-1]).contiguous() for t in (q, k))
+      v2 = extra[0].reshape(-1, sizes[-1]).contiguous() if has_v else None
+      rel = None
+      if has_rel:
+        values = extra[-1].to(q.dtype).contiguous()
+        # (from MAX_DISTANCE on all positions are in one bucket)
+        reach = min(state.table.shape[-1] * state.cache.page_size, MAX_DISTANCE + 1)
+        rel = (values, relative_bucket_table(reach, bidirectional, values.shape[-1],
+                                             values.device))
+      return cache_hip.attention(
+          q2, state.cache, state.flat_table, position.reshape(-1).to(torch.int32), k_new=k2,
+          v_new=v2, relative_bias=rel).reshape(sizes)
+    lowering.set_tensor_lowering(
+        self.outputs[0], lowering.mesh_impl(self).slicewise(
+            fn, *[lowering.tensors[t] for t in self.inputs]))
 
 
 class SelfAttentionGradOperation(mtf.Operation):

@@ -116,6 +116,15 @@ class Context(object):
                                               len(self.new_states) + n - 1))
     return got
 
+  def paged_state(self):
+    """The next recurrent state, where it is kept in pages (attention.PagedState), else
+    None."""
+    from mesh_amd.transformer import attention
+    states = self.states[len(self.new_states):len(self.new_states) + 1]
+    if states and isinstance(states[0], attention.PagedState):
+      return states[0]
+    return None
+
   def record_new_states(self, new_states):
     """transformer.py:263-271."""
     self.new_states.extend(new_states)
@@ -598,6 +607,9 @@ class Unitransformer(object):
     x [batch dims..., d_model] (one position per batch entry), `position`
     [batch dims...] int32, the states of the previous call as `states`, the
     sequences' `length_dim`, and appends the updated states to `new_states`.
+    Where the states passed in either mode are attention.PagedState objects, one per
+    attention layer, keys and values are written into their pages instead, and the same
+    objects are the new states (`new_states` may be left out).
     The loop around it (sampling, stopping) stays with the caller.  `reuse`:
     take the variables an earlier call on this graph created (the default in
     "incremental" mode, as the reference's loop body does)."""

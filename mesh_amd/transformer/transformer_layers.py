@@ -150,6 +150,14 @@ class SelfAttention(transformer.TransformerLayer):
       if context.read_priority is not transformer.POSITION:
         raise NotImplementedError("incremental mode of a model that is not "
                                   "autoregressive")
+      paged = context.paged_state()
+      if paged is not None:
+        o = attention.PagedDecodeOperation(
+            q, k, None if self.shared_kv else v, context.position, paged,
+            params.num_heads, relative_values=relative_values,
+            relative_bidirectional=not context.model.fully_autoregressive).outputs[0]
+        context.record_new_states([paged])
+        return params.compute_output(o, output_shape=x.shape)
       if self.shared_kv:                     # one state: the shared tensor
         old_k = old_v = context.get_states(1)[0]
       else:
@@ -161,7 +169,12 @@ class SelfAttention(transformer.TransformerLayer):
       o, k_all, v_all = op.outputs
       context.record_new_states([k_all] if self.shared_kv else [k_all, v_all])
       return params.compute_output(o, output_shape=x.shape)
-    if context.mode == transformer.FIRST_PART:
+    paged = context.paged_state() if context.mode == transformer.FIRST_PART else None
+    if paged is not None:
+      attention.PagedWriteOperation(k, None if self.shared_kv else v, paged,
+                                    params.num_heads)
+      context.record_new_states([paged])
+    elif context.mode == transformer.FIRST_PART:
       name = context.length_dim.name       # states carry "memory_length"
       context.record_new_states(
           [mtf.rename_dimension(t, name, "memory_length")

@@ -160,3 +160,39 @@ def test_attention_refusals(lib):
   if need:
     _refused(lib, with_(_20=1 << 20, _23=need - 1), -1, "workspace")
     _refused(lib, with_(_20=1 << 20, _22=None), -1, "workspace")
+
+
+def test_paged_states_of_layers():
+  """What a layer takes for its state, and where it looks for it."""
+  import mesh_amd as mtf
+  from mesh_amd.transformer import attention
+  from mesh_amd.transformer import transformer
+  cache = cache_hip.PagedCache.empty(6, 8, 2, 16, device="cpu")
+  state = attention.PagedState(cache, torch.zeros(3, 2, dtype=torch.int32))
+  state.check(32, 2, [3], False)
+  for args in ((64, 2, [3], False), (32, 4, [3], False), (32, 2, [3], True),
+               (32, 2, [2], False), (32, 2, [3, 1], False)):
+    with pytest.raises(ValueError):
+      state.check(*args)
+  graph = mtf.Graph()
+  mesh = mtf.Mesh(graph, "mesh")
+  batch, channels = mtf.Dimension("batch", 3), mtf.Dimension("heads", 32)
+  t = lambda *dims, **kw: mtf.import_tf_tensor(
+      mesh, torch.zeros([d.size for d in dims], **kw), mtf.Shape(list(dims)))
+  q, other = t(batch, channels), t(batch, mtf.Dimension("heads", 16))
+  position = t(batch, dtype=torch.int32)
+  op = attention.PagedDecodeOperation(q, q, q, position, state, 2)
+  assert op.outputs[0].shape == q.shape
+  for args in ((q, other, q, position, state, 2), (q, q, q, other, state, 2),
+               (q, q, q, position, state, 4), (q, q, None, position, state, 2)):
+    with pytest.raises(ValueError):
+      attention.PagedDecodeOperation(*args)
+  model = transformer.Unitransformer(None, d_model=16)
+  context = transformer.Context(
+      model, mesh, [batch], mtf.Dimension("length", 8), mtf.VariableDType(torch.float32),
+      mode="incremental", position=position, states=[q, q, state])
+  assert context.paged_state() is None
+  context.record_new_states(context.get_states(2))
+  assert context.paged_state() is state
+  context.record_new_states([state])
+  assert context.paged_state() is None
