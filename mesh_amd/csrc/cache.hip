@@ -1090,10 +1090,16 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
         for (int r = 0; r < 4; ++r) {
           // (row 4 j + r of the product is what lane c = 4 j + r read)
           const int at = p * 16 * VE + (4 * j + r) * VE;
-          const int from = PADDED ? min(at, D - VE) : at;
+          if (!PADDED || D % VE == 0) {
+            if (!PADDED || at < D)
 #pragma unroll
-          for (int u = 0; u < VE; ++u)
-            if (!PADDED || (from + u >= at && at < D)) to[from + u] = o[p * VE + u][r];
+              for (int u = 0; u < VE; ++u) to[at + u] = o[p * VE + u][r];
+          } else {
+            const int from = min(at, D - VE);
+#pragma unroll
+            for (int u = 0; u < VE; ++u)
+              if (from + u >= at && at < D) to[from + u] = o[p * VE + u][r];
+          }
         }
     }
     __syncthreads();
