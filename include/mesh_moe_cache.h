@@ -17,7 +17,8 @@
  *                      128 rounded up (a row's last block may be shorter), or both NULL.
  *                      Value i of a row stands for page[i] * 2^(scale[i / 128] - 127);
  *                      exponents, roundings and blocks that are not finite as in
- *                      mesh_moe_fp8.h.  Bytes from 10 on are taken, as the calls make them.
+ *                      mesh_moe_fp8.h.  Bytes from 10 to 254 are taken; the calls make
+ *                      these.
  * (v_pages NULL: keys and values are the same tensor, mesh_tensorflow/transformer/
  * attention.py:499-515; v_scales is NULL then, too.)  Where a sequence's rows lie is told
  * by
@@ -27,9 +28,9 @@
  * sequences may share pages that they only read; what a call leaves in a row that it is
  * told to write twice is unspecified.
  *
- * Limits: D up to 256, HK up to 65536, P * S up to 2^30, and what 2^24 workgroups cover.
- * Tensors lie on their elements' size; on 16 bytes, D a multiple of 16, the calls are
- * fastest.
+ * Limits: D up to 256, HK up to 65536, T and P * S up to 2^30, and what 2^24 workgroups
+ * cover.  Tensors lie on their elements' size; the calls are fastest on 16 bytes, with D of
+ * 64, 128 or 256 and pages of 16 rows and more.
  *
  * The reference keeps recurrent states as whole tensors (mesh_tensorflow/transformer/
  * transformer_layers.py:231-254); these calls are a form of what it does with them.

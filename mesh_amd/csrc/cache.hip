@@ -11,6 +11,7 @@ namespace mesh_moe {
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int MAX_WIDTH = 256;                  // D
+constexpr int TILES_FROM = 16;                  // D of the kernels on matrix cores
 constexpr int MAX_HEADS = 1 << 16;              // HK
 constexpr int MAX_POSITIONS = 1 << 30;          // P * S
 constexpr int64_t MAX_BLOCKS = MAX_THREADS / 256;   // of 256 threads
@@ -626,16 +627,17 @@ __device__ __forceinline__ bool parts_of(const Attention& a, const Shares& s, in
 }
 
 // What a wavefront has of NS x 16 positions: words of keys and values as the products take
-// them, their scale bytes, and which of the pages are there.  SMALL: pages of fewer than 16
-// rows, whose rows are looked up one by one.
-template <typename T, bool EIGHT, int DP, bool SMALL>
+// them, their scale bytes, and which of the pages are there.  SMALL: 0 for pages of
+// 16 rows and more, 1 of 4 or 8, 2 of 1 or 2.
+template <typename T, bool EIGHT, int DP, int SMALL>
 struct Group {
   typedef TileOf<T, EIGHT, DP> Tile;
   static constexpr int NS = Tile::NS, BLOCKS = DP == 256 ? 2 : 1;
   uint32_t k[NS][Tile::KC][4], v[NS][4][Tile::VP][Tile::VB / 4];
   uint32_t k_units[NS];                      // a byte for each block of the lane's key
-  uint32_t v_units[NS][BLOCKS];              // [4 rows][blocks] bytes
-  bool there[NS];                            // the values' page
+  static constexpr int PAGES = SMALL == 2 ? 4 : 1;   // of a lane's values
+  uint32_t v_units[NS][SMALL == 2 ? 4 : BLOCKS];     // [4 rows][blocks] bytes, of each row
+  bool there[NS][PAGES];                     // the values' pages
 };
 
 // What a scale byte (bits 8 n .. of the word) stands for.
@@ -644,7 +646,7 @@ __device__ __forceinline__ float unit_in(uint32_t word, int n) {
 }
 
 // PADDED: rows of fewer than DP values, or on any address.
-template <typename T, bool EIGHT, int DP, bool PADDED, bool SMALL>
+template <typename T, bool EIGHT, int DP, bool PADDED, int SMALL>
 __global__ __launch_bounds__(256, (TileOf<T, EIGHT, DP>::template at_once<PADDED>()))
 void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
   typedef TileOf<T, EIGHT, DP> Tile;
@@ -652,6 +654,7 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
   constexpr int NS = Tile::NS, KC = Tile::KC, KV = Tile::KV, SIZE = Tile::SIZE;
   constexpr int VD = Tile::VD, VP = Tile::VP, VE = Tile::VE, VB = Tile::VB;
   constexpr int VW = VB / 4;                         // words of a value's piece
+  constexpr int PAGES = Group::PAGES, PER_PAGE = 4 / PAGES;
   extern __shared__ __attribute__((aligned(16))) float joined[];
   __shared__ __attribute__((aligned(16))) uint8_t fresh_rows[2][DP * SIZE];
   __shared__ uint8_t fresh_units[2][2];
@@ -702,16 +705,18 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
 
     // The pages of the 16 positions from t0 + 16 s on, SMALL: of the lane's key and values;
     // behind the end, that of the last one.
-    struct Looked { int k, v; };
+    struct Looked { int k, v[PAGES]; };
     auto look_up = [&](int t0, Looked (&page)[NS]) {
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         const int t = t0 + 16 * s, most = max(end - 1, 0);
         if constexpr (SMALL) {
           page[s].k = table[min(t + c, most) >> a.pages.shift];
-          page[s].v = table[min(t + 4 * j, most) >> a.pages.shift];
+#pragma unroll
+          for (int n = 0; n < PAGES; ++n)
+            page[s].v[n] = table[min(t + 4 * j + n, most) >> a.pages.shift];
         } else {
-          page[s].k = page[s].v = scalar_load(table + (min(t, most) >> a.pages.shift));
+          page[s].k = page[s].v[0] = scalar_load(table + (min(t, most) >> a.pages.shift));
         }
       }
     };
@@ -741,21 +746,28 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
       }
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        const int64_t row =
-            row_in(page[s].v, SMALL ? t0 + 16 * s + 4 * j : min(t0 + 16 * s, end - 1) & ~15);
-        const uint8_t* from = v_pages + row * D * SIZE;
-        g.there[s] = (unsigned)page[s].v < (unsigned)a.pages.N;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+        for (int n = 0; n < PAGES; ++n) {
+          const int64_t row = row_in(page[s].v[n], SMALL ? t0 + 16 * s + 4 * j + n
+                                                         : min(t0 + 16 * s, end - 1) & ~15);
+          const uint8_t* from = v_pages + row * D * SIZE;
+          g.there[s][n] = (unsigned)page[s].v[n] < (unsigned)a.pages.N;
 #pragma unroll
-          for (int p = 0; p < VP; ++p)
-            if (!PADDED || v_extra[p] < VE)
-              load_words<VB>(from + r * D * SIZE +
-                                 (uint32_t)(((SMALL ? 0 : 4 * j * D) + v_at[p]) * SIZE),
-                             g.v[s][r][p]);
-        if constexpr (EIGHT)
-          load_words<4 * Group::BLOCKS>(
-              a.v_scales + row * DB + (SMALL ? 0 : 4 * j * DB), g.v_units[s]);
+          for (int r = 0; r < PER_PAGE; ++r)
+#pragma unroll
+            for (int p = 0; p < VP; ++p)
+              if (!PADDED || v_extra[p] < VE)
+                load_words<VB>(from + r * D * SIZE +
+                                   (uint32_t)(((SMALL ? 0 : 4 * j * D) + v_at[p]) * SIZE),
+                               g.v[s][n + r][p]);
+          if constexpr (EIGHT && SMALL == 2) {
+            const uint8_t* units = a.v_scales + row * DB;
+            g.v_units[s][n] = DB == 2 ? units[0] | (uint32_t)units[1] << 8 : units[0];
+          } else if constexpr (EIGHT) {
+            load_words<4 * Group::BLOCKS>(
+                a.v_scales + row * DB + (SMALL ? 0 : 4 * j * DB), g.v_units[s]);
+          }
+        }
       }
     };
 
@@ -855,10 +867,14 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
                 load_words<VB>(fresh_rows[1] + v_at[p] * SIZE, g.v[s][r][p]);
             if (EIGHT) {
               const uint32_t units = fresh_units[1][0] | (uint32_t)fresh_units[1][1] << 8;
-              const int bits = 8 * DB * (r % (4 / DB));
-              uint32_t& word = g.v_units[s][r * DB / 4];
-              word = (word & ~((DB == 2 ? 0xffffu : 0xffu) << bits)) |
-                     (DB == 2 ? units : units & 0xffu) << bits;
+              if constexpr (SMALL == 2) {
+                g.v_units[s][r] = units;
+              } else {
+                const int bits = 8 * DB * (r % (4 / DB));
+                uint32_t& word = g.v_units[s][r * DB / 4];
+                word = (word & ~((DB == 2 ? 0xffffu : 0xffu) << bits)) |
+                       (DB == 2 ? units : units & 0xffu) << bits;
+              }
             }
           }
         }
@@ -944,13 +960,15 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
       }
       bool whole = t0 + 16 * NS <= end;
 #pragma unroll
-      for (int s = 0; s < NS; ++s) whole = whole && g.there[s];
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int n = 0; n < PAGES; ++n) whole = whole && g.there[s][n];
       if (SMALL ? !__all(whole) : !whole) {
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            if (g.there[s] && t0 + 16 * s + 4 * j + r < end) continue;
+            if (g.there[s][r / PER_PAGE] && t0 + 16 * s + 4 * j + r < end) continue;
             x[s][r] = -INFINITY;
 #pragma unroll
             for (int p = 0; p < VP; ++p)
@@ -993,6 +1011,8 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
       // -- sums of values
       auto v_unit = [&](int s, int r) {
         if constexpr (!EIGHT) return 1.f;
+        else if constexpr (SMALL == 2)
+          return DB == 2 && c >= 8 ? unit_in(g.v_units[s][r], 1) : unit_in(g.v_units[s][r], 0);
         else if constexpr (DB == 2)
           return c >= 8 ? unit_in(g.v_units[s][r / 2], r % 2 * 2 + 1)
                         : unit_in(g.v_units[s][r / 2], r % 2 * 2);
@@ -1338,7 +1358,7 @@ static Division divide(int B, int H, int HK, int D, int S, int P, int dtype, boo
   return v;
 }
 
-template <typename T, bool EIGHT, int DP, bool PADDED, bool SMALL>
+template <typename T, bool EIGHT, int DP, bool PADDED, int SMALL>
 static int run_tiles(const Attention& a, const Division& v, char* workspace,
                      hipStream_t st) {
   auto kern = cache_attention_tiles_kernel<T, EIGHT, DP, PADDED, SMALL>;
@@ -1365,9 +1385,7 @@ static int run_tiles(const Attention& a, const Division& v, char* workspace,
   return 0;
 }
 
-// what the tiles' kernel takes
-static bool takes_tiles(int D, int S) { return D >= 16 && S >= 4; }
-// whether it is its PADDED form
+// whether the tiles' kernel takes its PADDED form
 static bool rows_padded(const Attention& a) {
   const int D = a.pages.D;
   return a.pages.shift < 4 || (D != 64 && D != 128 && D != 256) ||
@@ -1378,16 +1396,17 @@ template <typename T, bool EIGHT>
 static int run_attention(const Attention& a, const Division& v, bool padded,
                          char* workspace, hipStream_t st) {
   const int D = a.pages.D;
-  if (!takes_tiles(D, 1 << a.pages.shift)) {
+  if (D < TILES_FROM) {
     cache_attention_kernel<T, EIGHT><<<(unsigned)((int64_t)a.B * a.H), 256, 0, st>>>(a);
     MOE_CHECK_LAUNCH("cache_attention");
     return 0;
   }
-  const bool small = a.pages.shift < 4;
+  const int small = a.pages.shift >= 4 ? 0 : a.pages.shift >= 2 ? 1 : 2;
 #define TILES(dp)                                                                     \
-  (small    ? run_tiles<T, EIGHT, dp, true, true>                                     \
-   : padded ? run_tiles<T, EIGHT, dp, true, false>                                    \
-            : run_tiles<T, EIGHT, dp, false, false>)
+  (small == 2   ? run_tiles<T, EIGHT, dp, true, 2>                                    \
+   : small == 1 ? run_tiles<T, EIGHT, dp, true, 1>                                    \
+   : padded     ? run_tiles<T, EIGHT, dp, true, 0>                                    \
+                : run_tiles<T, EIGHT, dp, false, 0>)
   auto run = D <= 64 ? TILES(64) : D <= 128 ? TILES(128) : TILES(256);
 #undef TILES
   return run(a, v, workspace, st);
@@ -1418,6 +1437,7 @@ extern "C" int mesh_moe_cache_write(const void* k, const void* v, const int32_t*
   RowsOf r = {};
   if (int rc = pages_of("cache_write", table, B, HK, D, N, S, P, &r.pages)) return rc;
   MOE_REQUIRE(T >= 1, MESH_MOE_E_ARG, "cache_write: bad sizes T=%d", T);
+  MOE_REQUIRE(T <= MAX_POSITIONS, MESH_MOE_E_UNSUPPORTED, "cache_write: %d rows, up to 2^30", T);
   r.position = position;
   r.count = count;
   r.B = B;
@@ -1442,6 +1462,7 @@ extern "C" int mesh_moe_cache_read(const void* k_pages, const void* v_pages,
   RowsOf r = {};
   if (int rc = pages_of("cache_read", table, B, HK, D, N, S, P, &r.pages)) return rc;
   MOE_REQUIRE(T >= 1, MESH_MOE_E_ARG, "cache_read: bad sizes T=%d", T);
+  MOE_REQUIRE(T <= MAX_POSITIONS, MESH_MOE_E_UNSUPPORTED, "cache_read: %d rows, up to 2^30", T);
   r.position = position;
   r.count = count;
   r.B = B;
@@ -1459,7 +1480,7 @@ extern "C" int mesh_moe_cache_read(const void* k_pages, const void* v_pages,
 extern "C" size_t mesh_moe_cache_attention_workspace_bytes(int B, int H, int HK, int D,
                                                            int S, int P, int dtype,
                                                            int eight_bit) {
-  if (B < 1 || H < 1 || HK < 1 || H % HK || !takes_tiles(D, S) || D > MAX_WIDTH || P < 1 ||
+  if (B < 1 || H < 1 || HK < 1 || H % HK || D < TILES_FROM || D > MAX_WIDTH || S < 1 || P < 1 ||
       !valid_dtype(dtype))
     return 0;
   // (the form with more blocks, wherever the operands lie)
@@ -1488,7 +1509,7 @@ extern "C" int mesh_moe_cache_attention(
   a.v_pages = v_pages ? v_pages : k_pages;
   a.k_scales = k_scales;
   a.v_scales = v_pages ? v_scales : k_scales;
-  const bool tiles = takes_tiles(D, S);
+  const bool tiles = D >= TILES_FROM;
   a.k_new = tiles ? k_new : nullptr;
   a.v_new = tiles ? v_new : nullptr;
   a.position = position;
@@ -1501,7 +1522,7 @@ extern "C" int mesh_moe_cache_attention(
   a.H = H;
   a.G = H / HK;
   const bool padded = rows_padded(a);
-  const Division v = divide(B, H, HK, std::max(D, 16), S, P, dtype, k_scales != nullptr,
+  const Division v = divide(B, H, HK, std::max(D, TILES_FROM), S, P, dtype, k_scales != nullptr,
                             padded);
   MOE_REQUIRE(v.fits && (tiles || (int64_t)B * H <= MAX_BLOCKS), MESH_MOE_E_UNSUPPORTED,
               "cache_attention: %d sequences of %d heads and %d pages are more than a "

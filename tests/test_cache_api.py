@@ -115,6 +115,7 @@ def test_write_refusals(lib):
   _refused(lib, with_(_12=257), -2, "256")
   _refused(lib, with_(_11=65537), -2, "65536")
   _refused(lib, with_(_14=1 << 16, _15=1 << 15), -2, "2^30")
+  _refused(lib, with_(_10=(1 << 30) + 1), -2, "2^30")
 
 
 def test_read_refusals(lib):
@@ -131,6 +132,7 @@ def test_read_refusals(lib):
     _refused(lib, with_(**{"_%d" % at: -1}), -1, "sizes")
   _refused(lib, with_(_16=2), -1, "dtype")
   _refused(lib, with_(_14=3), -2, "power of two")
+  _refused(lib, with_(_10=(1 << 30) + 1), -2, "2^30")
 
 
 def test_attention_refusals(lib):
