@@ -211,7 +211,9 @@ def _check(got, q, held, table, position, page, name, relative=None):
     (2, 2, 36, 16, False), (20, 1, 64, 64, True), (6, 3, 256, 16, False),
     (1, 1, 1, 1, False), (5, 5, 100, 4, True), (34, 2, 32, 128, False),
     (2, 1, 192, 2, True), (3, 3, 112, 16, False), (2, 2, 13, 32, True),
-    (16, 1, 96, 256, False), (1, 1, 48, 16, True)],
+    (16, 1, 96, 256, False), (1, 1, 48, 16, True), (3, 1, 17, 16, False),
+    (4, 2, 33, 8, True), (2, 1, 131, 16, False), (17, 1, 255, 4, False),
+    (2, 2, 16, 1, False), (5, 5, 64, 2, True)],
     ids=lambda c: "x".join(map(str, c)))
 def test_attention(case, store):
   """Lengths from none to several hundred, pages that end anywhere and some that are not
@@ -283,7 +285,9 @@ def test_step(case, store, shared):
 @pytest.mark.parametrize("case", [
     # lengths, query heads, key / value heads, width, page
     ([20011], 2, 1, 128, 64), ([9000, 3, 4096, 1], 2, 2, 64, 16),
-    ([2500] * 3, 1, 1, 40, 32)], ids=["one", "uneven", "odd"])
+    ([2500] * 3, 1, 1, 40, 32), ([6000, 700], 20, 1, 64, 32), ([5000], 2, 1, 256, 16),
+    ([3000, 40], 3, 1, 128, 1), ([4100], 1, 1, 72, 8)],
+    ids=["one", "uneven", "odd", "tiles", "wide", "rows", "small"])
 def test_long_sequences(case, store):
   lengths, heads, kv, width, page = case
   name, eight = store
@@ -313,6 +317,67 @@ def test_many_sequences(name):
   position = lengths - 1
   got = cache_hip.attention(q, cache, _int32(table), _int32(position))
   _check(got, q, held, table, position, 16, name)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_more_than_the_grid_has(eight):
+  """More rows of a sequence, and more sequences, than a launch has blocks for at once."""
+  gen = _gen(21)
+  t, page, width = 300001, 1024, 16
+  cache, (before, _) = _cache(gen, 295, page, 1, width, torch.bfloat16, eight, shared=True)
+  table = np.arange(294, dtype=np.int32)[::-1].copy()[None]
+  k = _rows(gen, (1, t, width), torch.bfloat16)
+  cache_hip.write(cache, k, None, _int32(table), _int32([5]))
+  got = cache_hip.read(cache, _int32(table), _int32([5]), t)[0]
+  stored = C.stored(_np(k).reshape(1, t, 1, width), eight)
+  there = min(t, 294 * page - 5)
+  want = np.zeros((t, width))
+  want[:there] = stored[0, :there, 0]
+  np.testing.assert_array_equal(_np(got)[0], want)
+  np.testing.assert_array_equal(_held(cache)[0][294], before[294])
+  b = 17001
+  cache, _ = _cache(gen, b, 2, 1, width, torch.bfloat16, eight)
+  table = np.random.default_rng(21).permutation(b).astype(np.int32)[:, None]
+  rows = [_rows(gen, (b, width), torch.bfloat16) for _ in range(2)]
+  at = np.arange(b) % 3 - 1
+  cache_hip.write(cache, rows[0], rows[1], _int32(table), _int32(at))
+  for got, x in zip(cache_hip.read(cache, _int32(table), _int32(at), 1), rows):
+    want = C.stored(_np(x), eight) * (at >= 0)[:, None]
+    np.testing.assert_array_equal(_np(got)[:, 0], want)
+  held = _held(cache)
+  q = _rows(gen, (b, 2 * width), torch.float32).mul(0.3).bfloat16()
+  got = cache_hip.attention(q, cache, _int32(table), _int32(at))
+  _check(got, q, held, table, at, 2, "bf16")
+
+
+def test_shared_pages():
+  """Sequences that begin with the same pages, and one that has a page twice."""
+  rng, gen = np.random.default_rng(22), _gen(22)
+  page = 16
+  cache, held = _cache(gen, 9, page, 2, 64, torch.bfloat16, False)
+  table = np.array([[3, 7, 1, 0], [3, 7, 2, 8], [5, 5, 5, -1]], np.int32)
+  position = np.array([60, 49, 47])
+  q = _rows(gen, (3, 4 * 64), torch.float32).mul(0.1).bfloat16()
+  got = cache_hip.attention(q, cache, _int32(table), _int32(position))
+  _check(got, q, held, table, position, page, "bf16")
+  k, _ = cache_hip.read(cache, _int32(table), _int32([0, 3, 1]), 30)
+  np.testing.assert_array_equal(
+      _np(k).reshape(3, 30, 2, 64), C.read(held[0], table, [0, 3, 1], 30, None, page))
+  del rng
+
+
+def test_buckets_that_there_are_not():
+  """Bucket numbers out of range read nothing out of bounds: they count as the nearest."""
+  gen = _gen(23)
+  table = np.arange(5, dtype=np.int32)[None]
+  cache, held = _cache(gen, 5, 16, 2, 64, torch.bfloat16, False)
+  q = _rows(gen, (1, 128), torch.float32).mul(0.1).bfloat16()
+  values = torch.randn((2, 4), generator=gen, device="cuda").bfloat16()
+  bucket = np.full(39, 1 << 30, np.int32)
+  bucket[::2] = -1 << 30
+  got = cache_hip.attention(q, cache, _int32(table), _int32([79]),
+                            relative_bias=(values, _gpu(bucket)))
+  _check(got, q, held, table, np.array([79]), 16, "bf16", (values, np.clip(bucket, 0, 3)))
 
 
 def test_positions_behind_the_table():
@@ -421,7 +486,7 @@ def test_recorded_steps(store):
   q = q * 0.2
   step = lambda c: cache_hip.attention(q, c, tables, position, k_new=k, v_new=v)
   stream = torch.cuda.Stream()
-  graphs, outs, pool = [], [], None
+  graphs, outs, reads, pool = [], [], [], None
   torch.cuda.synchronize()
   with torch.cuda.stream(stream):
     step(cache)
@@ -431,6 +496,7 @@ def test_recorded_steps(store):
       graph = torch.cuda.CUDAGraph()
       with torch.cuda.graph(graph, pool=pool, stream=stream):
         outs.append(step(cache))
+        reads.append(cache_hip.read(cache, tables, position, 2, dtype=dtype))
       pool = graph.pool()
       graphs.append(graph)
   torch.cuda.synchronize()
@@ -442,9 +508,33 @@ def test_recorded_steps(store):
     want = step(other)
     torch.cuda.synchronize()
     assert torch.equal(outs[i % 2], want), i
+    for a, c in zip(reads[i % 2], cache_hip.read(other, tables, position, 2, dtype=dtype)):
+      assert torch.equal(a[:, 0], c[:, 0])
     for a, c in ((cache.k_pages, other.k_pages), (cache.v_pages, other.v_pages)):
       assert torch.equal(_bits(a), _bits(c))
     torch.empty(1 << 20, device="cuda").normal_()
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_recorded_with_wide_tiles(eight):
+  """16 heads of 256 a tile: the launches that ask for more than 64 KB of LDS."""
+  rng, gen = np.random.default_rng(24), _gen(24)
+  lengths = np.array([700, 90])
+  table, pages = _table(rng, lengths, 16)
+  cache, held = _cache(gen, pages, 16, 1, 256, torch.bfloat16, eight)
+  tables, position = _int32(table), _int32(lengths - 1)
+  q = _rows(gen, (2, 16 * 256), torch.float32).mul(0.05).bfloat16()
+  stream = torch.cuda.Stream()
+  torch.cuda.synchronize()
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph, stream=stream):
+    out = cache_hip.attention(q, cache, tables, position)
+  for shift in (0, 13, 40):
+    position.copy_(_int32(lengths - 1 - shift))
+    graph.replay()
+    torch.cuda.synchronize()
+    _check(out, q, held, table, lengths - 1 - shift, 16, "bf16")
+    assert torch.equal(out, cache_hip.attention(q, cache, tables, position))
 
 
 def test_two_streams():
