@@ -24,9 +24,10 @@
  * by
  *   table [B,P] int32  position p of sequence b is row p % S of page table[b][p / S]
  * Entries outside 0 .. N - 1 are pages that are not there, and so are all positions from P
- * * S on: rows for them are not written, read as zeros, and are not attended to.  Two
- * sequences may share pages that they only read; what a call leaves in a row that it is
- * told to write twice is unspecified.
+ * * S on: rows for them are not written, read as zeros, and are not attended to.  A page may
+ * be named several times, by sequences or by one, where the rows that they have of it are
+ * only read; what a call leaves in a row that it is told to write twice, or reads of a row
+ * that it writes for another place of the table, is unspecified.
  *
  * Limits: D up to 256, HK up to 65536, T and P * S up to 2^30, and what 2^24 workgroups
  * cover.  Tensors lie on their elements' size; the calls are fastest on 16 bytes, with D of

@@ -107,6 +107,9 @@ __device__ __forceinline__ void store_eight(uint8_t* row, int at, int D, uint32_
 // once; with one row a sequence the wavefronts of a block share it.  A lane has 8 values of
 // each, and a head's lanes are a power of two (16 for each block of 128 where it has more
 // than one), so that a block's largest magnitude is found by DPP steps among neighbours.
+// Nothing is used twice: bound by the memory.  16 sequences of up to 4096 rows of 1024
+// bfloat16 keys and values into 8 bits move 278 MB in 46 us (6.0 TB/s, some of it to the
+// last level's cache; a copy of 1 GiB reaches 5.15), 4 x 16384 rows back 406 MB in 61.
 // ---------------------------------------------------------------------------
 struct RowsOf {
   Pages pages;
@@ -269,8 +272,12 @@ __global__ __launch_bounds__(256) void cache_read_kernel(
 // turn them into
 //   m' = max(m, x)   l' = l e^(m - m') + e^(x - m')   o' = o e^(m - m') + e^(x - m') v
 // and two such triples of different positions are joined the same way; o / l is the
-// result.  A block has a query head of a sequence, its four wavefronts every fourth
-// position each.
+// result.
+//
+// The kernel for rows of fewer than 16 values, whose pieces the matrix cores' tiles (below)
+// do not have: a block has a query head of a sequence, its four wavefronts every fourth
+// position each.  Bound by the latency of one position after the other; with 16 values a
+// row is a quarter of a wavefront's load.
 // ---------------------------------------------------------------------------
 struct Attention {
   Pages pages;
@@ -398,14 +405,19 @@ __global__ __launch_bounds__(256) void cache_attention_kernel(Attention a) {
 // Bound by the memory: a position costs 2 D values of traffic for 4 D operations a head,
 // and the products of 16 columns take a twentieth of the matrix cores' time.  Four
 // wavefronts take turns with groups of NS x 16 positions, without barriers; what they have
-// in flight at once is what hides the memory's latency.
+// in flight at once is what hides the memory's latency.  One sequence of 131072 positions,
+// 8 key / value heads of 128, 8 bits: 42 us, 6.4 TB/s; 128 of up to 16384 in bfloat16: 714
+// us, 6.1 TB/s (a kernel that only reads reaches 6.3).  A wavefront's next group is not loaded
+// ahead of the one in use: the registers for it cost the second block of a CU, and two
+// blocks take turns as well (64 sequences of up to 8192: 121 us with, 118 without; rows of
+// 256, 87 and 71).
 //
 // The work is dealt out evenly to as many blocks as the chip holds at once, by what the
 // sequences' lengths turn out to be on the device (run_of).  Where a unit's positions fall
 // to several blocks, their triples go to the workspace, and cache_attention_join_kernel
 // puts them together.  (In the same launch, by the block of a unit that is done last, a
-// join costs its block three or four round trips to a memory that is busy with the others'
-// streams: 64 sequences of up to 8192, 129 us instead of 98.)
+// join costs its block round trips to a memory that is busy with the others' streams: 64
+// sequences of up to 8192, 130 us instead of 125.)
 // ---------------------------------------------------------------------------
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
@@ -440,12 +452,16 @@ struct TileOf {
   static constexpr int VP = VD * SIZE / VB;
   static constexpr int VE = VB / SIZE;                         // values of a piece
   static constexpr bool WIDE = sizeof(T) == 4;                 // float32 products
-  // groups of 16 positions that a wavefront has in registers at once
+  // Groups of 16 positions that a wavefront has in registers at once: as many as leave the
+  // blocks below their registers.  (8 bits, 128 values, 64 sequences of up to 8192: 125 us
+  // by 2, 115 by 4; bfloat16, 64 values, by 4 with two blocks 18.5, by 2 with three 17.4.)
   static constexpr int NS =
       WIDE ? (EIGHT ? (DP == 256 ? 1 : 2) : (DP == 64 ? 2 : 1))
            : (EIGHT && DP < 256 ? 4 : 2);
   static constexpr int GRAIN = 4 * 16 * NS;                    // positions of four wavefronts
-  // blocks that a CU holds
+  // Blocks that a CU holds, by their registers.  (Rows of 256, 16 sequences of 16384, 8 bits:
+  // 79 us by one, 72 by two; bfloat16, where two do not have the registers for it, 100 and
+  // 125.)
   template <bool PADDED>
   static constexpr int at_once() {
     return DP == 256 && !(EIGHT && !PADDED) ? 1 : DP == 64 && !EIGHT && !WIDE ? 3 : 2;
@@ -463,7 +479,8 @@ struct Shares {
   int blocks;                     // at most; 0: a block for every unit
 };
 // A unit's first positions take their block about as long to begin with and to put away as
-// a grain of them to go through: units count as that much longer.
+// a grain of them to go through: units count as that much longer.  (64 sequences of up to
+// 8192: 125 us without it, 115 with one grain, 118 with two.)
 constexpr int AHEAD = 1;
 
 // grains of a unit, those ahead of the first included
@@ -693,7 +710,7 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
     const int from_grain = max(run.grain - AHEAD, 0), to_grain = run.grain + taken - AHEAD;
     const bool begins = from_grain == 0, ends = run.grain + taken == run.of_unit;
     left -= taken;
-    if (to_grain <= 0) break;                        // (only what is ahead: the run's end)
+    if (to_grain <= 0 || b >= a.B) break;            // (only what is ahead: the run's end)
     const int kv_head = unit / tiles, head0 = (unit - kv_head * tiles) * HEADS;
     const int heads = min(a.G - head0, HEADS);       // columns in use
     const int64_t first_head = (int64_t)kv_head * a.G + head0;
@@ -771,6 +788,15 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
       }
     };
 
+    // zeros for the first bytes of a piece: another's values do not count twice
+    auto without_first = [](int bytes, uint32_t (&w)[4]) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int bits = min(max(bytes * 8 - 32 * e, 0), 32);
+        w[e] &= bits == 32 ? 0u : ~0u << bits;
+      }
+    };
+
     // ---- the queries, as the second operand of the first product; 0 where there is no head
     Looked page[NS];
     look_up(start, page);
@@ -789,6 +815,7 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
           uint32_t w[4] = {0, 0, 0, 0};
           if (there)
             load_words<16>(reinterpret_cast<const uint8_t*>(row + k_at[i] + u * PER), w);
+          if constexpr (PADDED) without_first((k_extra[i] - u * PER) * (int)sizeof(T), w);
           if constexpr (Tile::WIDE) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) q[i * KV + u * 4 + e] = __uint_as_float(w[e]);
@@ -887,14 +914,7 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
 #pragma unroll
         for (int i = 0; i < KC; ++i) {
           uint32_t* w = g.k[s][i];
-          if constexpr (PADDED) {
-            // (another piece's values do not count twice)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int bits = min(max(k_extra[i] * SIZE * 8 - 32 * e, 0), 32);
-              w[e] &= bits == 32 ? 0u : ~0u << bits;
-            }
-          }
+          if constexpr (PADDED) without_first(k_extra[i] * SIZE, g.k[s][i]);
           if constexpr (EIGHT) {
             const float unit = unit_in(g.k_units[s], DP == 256 ? i / 2 : 0);
 #pragma unroll

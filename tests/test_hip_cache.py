@@ -442,6 +442,27 @@ def test_what_is_not_finite_stays_in_its_head():
   assert torch.equal(got[1, 2:][:, keep], clean[1, 2:][:, keep])
 
 
+@pytest.mark.parametrize("store", STORES, ids=STORE_IDS)
+@pytest.mark.parametrize("width,at", [(17, 10), (33, 27), (72, 64), (131, 127), (200, 199)])
+def test_queries_that_are_infinite(width, at, store):
+  """Every value of a query counts once, also where the pieces of a row overlap: an infinite
+  one with keys below zero there makes all logits -infinity, and the output 0."""
+  dtype, eight = DTYPES[store[0]], store[1]
+  gen = _gen(width + at)
+  cache = cache_hip.PagedCache.empty(3, 16, 1, width, E4M3 if eight else dtype)
+  k = torch.rand((1, 40, width), generator=gen, device="cuda").sub(0.5).to(dtype)
+  k[..., at] = -0.25
+  v = _rows(gen, (1, 40, width), dtype)
+  table = _int32([[2, 0, 1]])
+  cache_hip.write(cache, k, v, table, _int32([0]))
+  q = torch.ones((1, 2 * width), dtype=dtype, device="cuda")
+  q[0, at] = float("inf")
+  out = cache_hip.attention(q, cache, table, _int32([39]))
+  assert torch.equal(out[0, :width], torch.zeros_like(out[0, :width]))
+  want, _ = cache_hip.attention(torch.ones_like(q), cache, table, _int32([39])).split(width, 1)
+  assert torch.equal(out[:, width:], want)
+
+
 @pytest.mark.parametrize("eight", [False, True])
 def test_pages_beyond_32_bits(eight):
   """Pages whose offsets pass 2^32 elements."""
