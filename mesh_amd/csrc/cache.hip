@@ -417,7 +417,8 @@ __global__ __launch_bounds__(256) void cache_attention_kernel(Attention a) {
 // to several blocks, their triples go to the workspace, and cache_attention_join_kernel
 // puts them together.  (In the same launch, by the block of a unit that is done last, a
 // join costs its block round trips to a memory that is busy with the others' streams: 64
-// sequences of up to 8192, 130 us instead of 125.)
+// sequences of up to 8192, 130 us instead of 125.)  Where there are many units and all are
+// short, every wavefront has units of its own.
 // ---------------------------------------------------------------------------
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
@@ -441,6 +442,27 @@ __device__ __forceinline__ void four_floats(uint32_t word, float unit, float (&f
 }
 
 constexpr int HEADS = 16;                          // columns of a tile
+
+// N values (a multiple of 4) to neighbouring places, but for the first `skip`.
+template <typename T, int N>
+__device__ __forceinline__ void store_some(T* to, const float (&f)[N], int skip) {
+  if (skip != 0) {
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+      if (u >= skip) store_f32<T>(to + u, f[u]);
+    return;
+  }
+#pragma unroll
+  for (int u = 0; u < N; u += 4) {
+    if constexpr (sizeof(T) == 2)
+      *reinterpret_cast<Words<8>::type*>(to + u) = Words<8>::type{
+          f32x2_to_bf16x2(f[u], f[u + 1]), f32x2_to_bf16x2(f[u + 2], f[u + 3])};
+    else
+      *reinterpret_cast<Words<16>::type*>(to + u) =
+          Words<16>::type{__float_as_uint(f[u]), __float_as_uint(f[u + 1]),
+                          __float_as_uint(f[u + 2]), __float_as_uint(f[u + 3])};
+  }
+}
 
 template <typename T, bool EIGHT, int DP>
 struct TileOf {
@@ -468,6 +490,8 @@ struct TileOf {
   }
   // grains that are not divided among blocks (see divide)
   static constexpr int WHOLE = DP == 64 && !EIGHT && !WIDE ? 8 : 4;
+  // positions of a wavefront's own units (see divide): eight turns
+  static constexpr int ALONE = 8 * 16 * NS;
 };
 
 // How the work is divided.  A unit is a key / value head of a sequence with a tile of its
@@ -477,6 +501,9 @@ struct Shares {
   int units;                      // of a sequence
   int grain;
   int blocks;                     // at most; 0: a block for every unit
+  // Where no sequence has more than `alone` positions, every wavefront takes units of its
+  // own instead; blocks = 0: whether that is so (not 0) is known from the table's size.
+  int alone;
 };
 // A unit's first positions take their block about as long to begin with and to put away as
 // a grain of them to go through: units count as that much longer.  (64 sequences of up to
@@ -524,10 +551,14 @@ struct Runs {
   }
 };
 
-// false for a block without work.  The same for all lanes of a wavefront.
+// false for a block without work; *alone: every wavefront takes units of its own, and there
+// is no run.  The same for all lanes of a wavefront.
 __device__ __forceinline__ bool run_of(const Attention& a, const Shares& s, int block,
-                                       Run* run) {
+                                       Run* run, bool* alone) {
   const int lane = threadIdx.x & 63;
+  run->count = 0;
+  *alone = s.blocks == 0 && s.alone != 0;
+  if (*alone) return true;
   if (s.blocks == 0) {
     run->b = block / s.units;
     run->unit = block - run->b * s.units;
@@ -535,11 +566,18 @@ __device__ __forceinline__ bool run_of(const Attention& a, const Shares& s, int 
     run->count = run->of_unit = grains_of(seen_of(a, run->b), s.grain);
     return true;
   }
-  auto grains = [&](int b) { return b < a.B ? grains_of(seen_of(a, b), s.grain) : 0; };
+  bool longer = false;
+  auto grains = [&](int b) {
+    const int seen = b < a.B ? seen_of(a, b) : 0;
+    longer = longer || seen > s.alone;
+    return b < a.B ? grains_of(seen, s.grain) : 0;
+  };
   const int of_lane = grains(lane);
   int up_to = sums_up_to(of_lane), all = __builtin_amdgcn_readlane(up_to, 63);
   for (int b = 64; b < a.B; b += 64)
     all += __builtin_amdgcn_readlane(sums_up_to(grains(b + lane)), 63);
+  *alone = s.alone != 0 && !__any(longer);
+  if (*alone) return true;
   const Runs runs(s, all * s.units);
   if (block >= runs.blocks) return false;
   run->first = runs.first(block);
@@ -626,9 +664,11 @@ __device__ __forceinline__ bool parts_of(const Attention& a, const Shares& s, in
   *b = id / s.units;
   *unit = id - *b * s.units;
   int before = 0, all = 0, own = 0;                  // grains of units of one kind
+  bool longer = s.alone == 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int grains =
-        b0 + lane < a.B ? grains_of(seen_of(a, b0 + lane), s.grain) : 0;
+    const int seen = b0 + lane < a.B ? seen_of(a, b0 + lane) : 0;
+    const int grains = b0 + lane < a.B ? grains_of(seen, s.grain) : 0;
+    longer = longer || seen > s.alone;
     const int up_to = sums_up_to(grains);
     if (*b >= b0 && *b < b0 + 64) {
       own = __builtin_amdgcn_readlane(grains, *b - b0);
@@ -636,6 +676,7 @@ __device__ __forceinline__ bool parts_of(const Attention& a, const Shares& s, in
     }
     all += __builtin_amdgcn_readlane(up_to, 63);
   }
+  if (!__any(longer)) return false;                  // (wavefronts had whole ones)
   const Runs runs(s, all * s.units);
   const int first = before * s.units + *unit * own;
   *from = runs.block_of(first + AHEAD);
@@ -673,12 +714,15 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
   constexpr int VW = VB / 4;                         // words of a value's piece
   constexpr int PAGES = Group::PAGES, PER_PAGE = 4 / PAGES;
   extern __shared__ __attribute__((aligned(16))) float joined[];
-  __shared__ __attribute__((aligned(16))) uint8_t fresh_rows[2][DP * SIZE];
-  __shared__ uint8_t fresh_units[2][2];
+  __shared__ __attribute__((aligned(16))) uint8_t fresh_of[4][2][DP * SIZE];
+  __shared__ uint8_t fresh_units_of[4][2][2];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Run run;
-  if (!run_of(a, shares, (int)blockIdx.x, &run)) return;
+  bool alone;
+  if (!run_of(a, shares, (int)blockIdx.x, &run, &alone)) return;
+  auto& fresh_rows = fresh_of[alone ? wave : 0];
+  auto& fresh_units = fresh_units_of[alone ? wave : 0];
   const int c = lane & 15, j = lane >> 4;
   const int D = PADDED ? a.pages.D : DP, S = 1 << a.pages.shift;
   const int DB = DP == 256 ? 2 : 1;
@@ -702,8 +746,16 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
     v_extra[p] = at - v_at[p];
   }
 
-  for (int left = run.count; left > 0;) {
+  int left = run.count, id = (int)blockIdx.x * 4 + wave;   // (id: of the unit of this wavefront)
+  while (alone ? id < a.B * shares.units : left > 0) {
     // ---- the next unit, or what of it falls to this block
+    if (alone) {
+      run.b = id / shares.units;
+      run.unit = id - run.b * shares.units;
+      run.grain = 0;
+      run.of_unit = left = 1 << 30;                  // (all of it)
+      id += (int)gridDim.x * 4;
+    }
     const int b = __builtin_amdgcn_readfirstlane(run.b);
     const int unit = __builtin_amdgcn_readfirstlane(run.unit);
     const int taken = min(left, run.of_unit - run.grain);
@@ -718,7 +770,8 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
     const int first = from_grain * Tile::GRAIN;
     const int end = (int)min((int64_t)to_grain * Tile::GRAIN, (int64_t)seen);
     const int32_t* table = a.pages.table + (int64_t)b * a.pages.P;
-    const int step = Tile::GRAIN, start = first + wave * (16 * NS);
+    const int step = alone ? 16 * NS : Tile::GRAIN;
+    const int start = alone ? 0 : first + wave * (16 * NS);
 
     // The pages of the 16 positions from t0 + 16 s on, SMALL: of the lane's key and values;
     // behind the end, that of the last one.
@@ -834,11 +887,16 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
       const int64_t to = a.pages.row(b, last);
       fresh = to >= 0;
       if (fresh) {
-        __syncthreads();                             // (the unit before is done with them)
-        if (wave < 2)
-          keep_row<T, EIGHT>(a, wave, b, kv_head, a.pages.head(to, kv_head), head0 == 0,
-                             fresh_rows[wave], fresh_units[wave]);
-        __syncthreads();
+        auto wait = [&] {
+          if (alone) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          else __syncthreads();
+        };
+        wait();                                      // (the unit before is done with them)
+#pragma unroll 1
+        for (int of = alone ? 0 : wave; of < 2; of += alone ? 1 : 2)
+          keep_row<T, EIGHT>(a, of, b, kv_head, a.pages.head(to, kv_head), head0 == 0,
+                             fresh_rows[of], fresh_units[of]);
+        wait();
       }
     }
 
@@ -1111,9 +1169,34 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
       use(t0, g);
     }
 
-    // ---- the four wavefronts' triples
+    // ---- the result, or the four wavefronts' triples
+    // (known again only now, so that the places below are not computed ahead of the
+    // positions and held in registers meanwhile)
+    int column = c, rows = 4 * j;
+    asm volatile("" : "+v"(column), "+v"(rows));
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
+    T* out = static_cast<T*>(a.out) + ((int64_t)b * a.H + first_head) * D;
+    if (alone) {
+      if (column < heads) {
+        const float of_all = 1.f / l;
+#pragma unroll
+        for (int p = 0; p < VP; ++p)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            // (row 4 j + r of the product is what lane c = 4 j + r read)
+            const int at = p * 16 * VE + (rows + r) * VE;
+            if (PADDED && at >= D) continue;
+            const int from = PADDED ? min(at, D - VE) : at;
+            float f[VE];
+#pragma unroll
+            for (int u = 0; u < VE; ++u)             // (nothing seen: 0)
+              f[u] = l == 0.f ? 0.f : o[p * VE + u][r] * of_all;
+            store_some<T, VE>(out + (int64_t)column * D + from, f, at - from);
+          }
+      }
+      continue;
+    }
     float* ms = joined;                              // [4][HEADS]
     float* ls = ms + 4 * HEADS;                      // [4][HEADS]
     float* os = ls + 4 * HEADS;                      // [4][heads][D]
@@ -1122,14 +1205,14 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
       ms[wave * HEADS + lane] = m;
       ls[wave * HEADS + lane] = l;
     }
-    if (c < heads) {
-      float* to = os + (wave * heads + c) * D;
+    if (column < heads) {
+      float* to = os + (wave * heads + column) * D;
 #pragma unroll
       for (int p = 0; p < VP; ++p)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           // (row 4 j + r of the product is what lane c = 4 j + r read)
-          const int at = p * 16 * VE + (4 * j + r) * VE;
+          const int at = p * 16 * VE + (rows + r) * VE;
           if (!PADDED || D % VE == 0) {
             if (!PADDED || at < D)
 #pragma unroll
@@ -1145,7 +1228,6 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
     __syncthreads();
     const bool whole_unit = begins && ends;
     const int64_t place = 2 * (int64_t)blockIdx.x + (begins ? 1 : 0);
-    T* out = static_cast<T*>(a.out) + ((int64_t)b * a.H + first_head) * D;
     // (two values a thread, as they go to the workspace)
     const int halves = (D + 1) / 2;
     for (int i = threadIdx.x; i < heads * halves; i += 256) {
@@ -1338,7 +1420,8 @@ static Shares shares_of(bool padded, int* whole) {
   *whole = Tile::WHOLE;
   return Shares{0, Tile::GRAIN,
                 CUS * (padded ? Tile::template at_once<true>()
-                              : Tile::template at_once<false>())};
+                              : Tile::template at_once<false>()),
+                Tile::ALONE};
 }
 template <typename T, bool EIGHT>
 static Shares shares_of(int D, bool padded, int* whole) {
@@ -1368,8 +1451,18 @@ static Division divide(int B, int H, int HK, int D, int S, int P, int dtype, boo
   // of 2001, 1 head of 128 in 8 bits (8 grains) 19 whole, 12 divided; one of 700, 16 heads
   // of 64 (6 grains) 8.4 whole, 10.3 divided.
   v.joins = most > (units * B >= CUS ? 2 * whole : whole);
+  // Of many short units each is a wavefront's, from beginning to end: no barriers, no sums
+  // of four, and four times as many units under way.  256 sequences of 20, 8 heads of 128
+  // in a table of 8192: 22 us by blocks, 15 alone; of 250 60 and 56, in 8 bits 36 and 31;
+  // 512 of 500 in 8 bits (8 turns) 137 and 114.  Of 500 in bfloat16 (16 turns), lengths
+  // differing, 192 sequences take 54 us by blocks, 61 alone, and with no more units than
+  // blocks (64 sequences of 250, 8 bits) it is 14 and 16.
+  if (2 * units * B < 3 * v.shares.blocks || (!v.joins && (int64_t)P * S > v.shares.alone))
+    v.shares.alone = 0;
   if (!v.joins) v.shares.blocks = 0;
-  v.blocks = v.joins ? std::min<int64_t>(v.shares.blocks, units * each * B) : units * B;
+  v.blocks = v.joins          ? std::min<int64_t>(v.shares.blocks, units * each * B)
+             : v.shares.alone ? (units * B + 3) / 4
+                              : units * B;
   if (v.joins) {
     const size_t rows = 2 * (size_t)v.blocks * std::min(G, HEADS);
     v.sums = sizeof(float2) * rows;
@@ -1383,7 +1476,9 @@ static int run_tiles(const Attention& a, const Division& v, char* workspace,
                      hipStream_t st) {
   auto kern = cache_attention_tiles_kernel<T, EIGHT, DP, PADDED, SMALL>;
   const int heads = std::min(a.G, HEADS);
-  const size_t lds = sizeof(float) * 4 * (2 * HEADS + (size_t)heads * a.pages.D);
+  const size_t lds = v.shares.blocks == 0 && v.shares.alone
+                         ? 0
+                         : sizeof(float) * 4 * (2 * HEADS + (size_t)heads * a.pages.D);
   MOE_ALLOW_LDS(kern, lds);
   Joins joins = {};
   joins.tops = reinterpret_cast<float2*>(workspace);
@@ -1408,7 +1503,7 @@ static int run_tiles(const Attention& a, const Division& v, char* workspace,
 // whether the tiles' kernel takes its PADDED form
 static bool rows_padded(const Attention& a) {
   const int D = a.pages.D;
-  return a.pages.shift < 4 || (D != 64 && D != 128 && D != 256) ||
+  return a.pages.shift < 2 || (D != 64 && D != 128 && D != 256) ||
          !on_16_bytes({a.q, a.k_pages, a.v_pages});
 }
 
@@ -1424,7 +1519,8 @@ static int run_attention(const Attention& a, const Division& v, bool padded,
   const int small = a.pages.shift >= 4 ? 0 : a.pages.shift >= 2 ? 1 : 2;
 #define TILES(dp)                                                                     \
   (small == 2   ? run_tiles<T, EIGHT, dp, true, 2>                                    \
-   : small == 1 ? run_tiles<T, EIGHT, dp, true, 1>                                    \
+   : small == 1 ? (padded ? run_tiles<T, EIGHT, dp, true, 1>                          \
+                          : run_tiles<T, EIGHT, dp, false, 1>)                        \
    : padded     ? run_tiles<T, EIGHT, dp, true, 0>                                    \
                 : run_tiles<T, EIGHT, dp, false, 0>)
   auto run = D <= 64 ? TILES(64) : D <= 128 ? TILES(128) : TILES(256);

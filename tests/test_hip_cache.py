@@ -319,6 +319,44 @@ def test_many_sequences(name):
   _check(got, q, held, table, position, 16, name)
 
 
+@pytest.mark.parametrize("store", STORES, ids=STORE_IDS)
+@pytest.mark.parametrize("case", [
+    # sequences, query heads, key / value heads, width, page, longest, columns more
+    (160, 8, 8, 64, 16, 100, 0), (160, 8, 8, 64, 16, 120, 500), (70, 32, 16, 128, 16, 90, 300),
+    (400, 19, 1, 80, 8, 60, 700), (400, 3, 3, 33, 2, 60, 0), (800, 1, 1, 256, 1, 30, 9),
+    (790, 2, 1, 256, 32, 70, 0), (300, 4, 4, 100, 4, 50, 600), (130, 6, 6, 128, 8, 100, 800)],
+    ids=lambda c: "x".join(map(str, c)))
+@pytest.mark.parametrize("longer", [False, True], ids=["short", "one-longer"])
+def test_many_short_sequences(case, store, longer):
+  """More heads of short sequences than there are blocks, with and without a longer
+  sequence among them: over what is there, and as a step with a bias."""
+  b, heads, kv, width, page, longest, more = case
+  name, eight = store
+  dtype = DTYPES[name]
+  rng, gen = np.random.default_rng(b), _gen(b)
+  lengths = rng.integers(0, longest + 1, b)
+  lengths[:4] = longest, 0, 1, 17
+  if longer:
+    lengths[b // 2] = 1500
+  table, pages = _table(rng, lengths, page, extra=more)
+  table[5, 0] = -1                          # (a sequence without its first page)
+  cache, held = _cache(gen, pages, page, kv, width, dtype, eight)
+  q = (torch.randn((b, heads * width), generator=gen, device="cuda")
+       * 2 * width ** -0.5).to(dtype)
+  position = lengths - 1
+  got = cache_hip.attention(q, cache, _int32(table), _int32(position))
+  _check(got, q, held, table, position, page, name)
+  k, v = (_rows(gen, (b, kv * width), dtype) for _ in range(2))
+  relative = _relative(gen, rng, heads, dtype, 40)
+  got = cache_hip.attention(q, cache, _int32(table), _int32(position), k_new=k, v_new=v,
+                            relative_bias=(relative[0], _gpu(relative[1])))
+  want = [C.write(was, C.stored(_np(x).reshape(b, 1, kv, width), eight), table, position,
+                  None, page) for was, x in zip(held, (k, v))]
+  for a, x in zip(_held(cache), want):
+    np.testing.assert_array_equal(a, x)
+  _check(got, q, want, table, position, page, name, relative)
+
+
 @pytest.mark.parametrize("eight", [False, True])
 def test_more_than_the_grid_has(eight):
   """More rows of a sequence, and more sequences, than a launch has blocks for at once."""
@@ -555,6 +593,28 @@ def test_recorded_with_wide_tiles(eight):
     graph.replay()
     torch.cuda.synchronize()
     _check(out, q, held, table, lengths - 1 - shift, 16, "bf16")
+    assert torch.equal(out, cache_hip.attention(q, cache, tables, position))
+
+
+def test_recorded_while_lengths_grow():
+  """A recorded call whose sequences are all short in one replay, and not in the next."""
+  rng, gen = np.random.default_rng(25), _gen(25)
+  lengths = np.full(100, 200)
+  lengths[37] = 1200
+  table, pages = _table(rng, lengths, 16, extra=10)
+  cache, held = _cache(gen, pages, 16, 8, 128, torch.bfloat16, False)
+  tables, position = _int32(table), _int32(lengths * 0)
+  q = _rows(gen, (100, 16 * 128), torch.float32).mul(0.1).bfloat16()
+  stream = torch.cuda.Stream()
+  torch.cuda.synchronize()
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph, stream=stream):
+    out = cache_hip.attention(q, cache, tables, position)
+  for at in (lengths * 0 - 1, np.minimum(lengths - 1, 180), lengths - 1, lengths * 0 + 5):
+    position.copy_(_int32(at))
+    graph.replay()
+    torch.cuda.synchronize()
+    _check(out, q, held, table, at, 16, "bf16")
     assert torch.equal(out, cache_hip.attention(q, cache, tables, position))
 
 
