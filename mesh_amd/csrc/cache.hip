@@ -569,14 +569,20 @@ __device__ __forceinline__ bool run_of(const Attention& a, const Shares& s, int 
   }
   bool longer = false;
   auto grains = [&](int b) {
-    const int seen = b < a.B ? seen_of(a, b) : 0;
+    const int seen = seen_of(a, min(b, a.B - 1));    // (no branch around the load)
     longer = longer || seen > s.alone;
     return b < a.B ? grains_of(seen, s.grain) : 0;
   };
   const int of_lane = grains(lane);
   int up_to = sums_up_to(of_lane), all = __builtin_amdgcn_readlane(up_to, 63);
-  for (int b = 64; b < a.B; b += 64)
-    all += __builtin_amdgcn_readlane(sums_up_to(grains(b + lane)), 63);
+  if (a.B > 64) {
+    int rest = 0;
+    for (int b = 64; b < a.B; b += 256) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rest += grains(b + 64 * i + lane);
+    }
+    all += __builtin_amdgcn_readlane(sums_up_to(rest), 63);
+  }
   *alone = s.alone != 0 && !__any(longer);
   if (*alone) return true;
   run->of_all = all * s.units;
@@ -650,40 +656,20 @@ __device__ __forceinline__ void keep_row(const Attention& a, int of, int b, int 
 
 // Units that fall to several blocks.  A block has a place in the workspace for the triple
 // of the unit it begins with (if that began before) and one for the unit it ends with.
+struct Part {                     // a unit's parts are those of blocks from, from + 1, ..
+  int b, unit, from, parts;       // (1: it is whole, 0: there is none)
+};
 struct Joins {
   float2* tops;                   // [places][columns]: largest logit, sum of weights
   float2* sums;                   // [places][columns][(D + 1) / 2]: two values each
+  // For the launch that joins them, null if there is none: of every unit, or (where blocks
+  // are fewer) of every block the unit that others go on with.
+  Part* parts;
+  bool of_units;
 };
 // the place of part `part` of a unit whose first block is `from`
 __device__ __forceinline__ int64_t place_of(int from, int part) {
   return 2 * (int64_t)(from + part) + (part == 0 ? 1 : 0);
-}
-
-// The parts of unit `id` (of all units): false where it is whole.  The same for all lanes.
-__device__ __forceinline__ bool parts_of(const Attention& a, const Shares& s, int id,
-                                         int* b, int* unit, int* from, int* parts) {
-  const int lane = threadIdx.x & 63;
-  *b = id / s.units;
-  *unit = id - *b * s.units;
-  int before = 0, all = 0, own = 0;                  // grains of units of one kind
-  bool longer = s.alone == 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int seen = b0 + lane < a.B ? seen_of(a, b0 + lane) : 0;
-    const int grains = b0 + lane < a.B ? grains_of(seen, s.grain) : 0;
-    longer = longer || seen > s.alone;
-    const int up_to = sums_up_to(grains);
-    if (*b >= b0 && *b < b0 + 64) {
-      own = __builtin_amdgcn_readlane(grains, *b - b0);
-      before = all + __builtin_amdgcn_readlane(up_to, *b - b0) - own;
-    }
-    all += __builtin_amdgcn_readlane(up_to, 63);
-  }
-  if (!__any(longer)) return false;                  // (wavefronts had whole ones)
-  const Runs runs(s, all * s.units);
-  const int first = before * s.units + *unit * own;
-  *from = runs.block_of(first + AHEAD);
-  *parts = runs.block_of(first + own - 1) - *from + 1;
-  return *parts > 1;
 }
 
 // What a wavefront has of NS x 16 positions: words of keys and values as the products take
@@ -720,6 +706,8 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
   __shared__ uint8_t fresh_units_of[4][2][2];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (joins.parts && !joins.of_units && threadIdx.x == 0)
+    joins.parts[blockIdx.x] = Part{0, 0, 0, 0};
   Run run;
   bool alone;
   if (!run_of(a, shares, (int)blockIdx.x, &run, &alone)) return;
@@ -1230,6 +1218,13 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
     __syncthreads();
     const bool whole_unit = begins && ends;
     const int64_t place = 2 * (int64_t)blockIdx.x + (begins ? 1 : 0);
+    if (joins.parts && begins && (!ends || joins.of_units) && threadIdx.x == 0) {
+      // (the unit's last grain, of all)
+      const int to = run.first + run.count - left - taken - run.grain + run.of_unit - 1;
+      const int from = (int)blockIdx.x;
+      joins.parts[joins.of_units ? b * shares.units + unit : from] =
+          Part{b, unit, from, ends ? 1 : Runs(shares, run.of_all).block_of(to) - from + 1};
+    }
     // (two values a thread, as they go to the workspace)
     const int halves = (D + 1) / 2;
     for (int i = threadIdx.x; i < heads * halves; i += 256) {
@@ -1267,31 +1262,18 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
   }
 }
 
-// Puts the parts of a unit together.  Block (x, y): unit x, or (BY_RUNS) the unit in which
-// run x ends, if that is the first to end there; `per` (a power of two) of its heads' pairs of
-// values; 256 / per groups of threads take every so many-th part.  (Where there are more units
-// than runs most are whole, and the blocks that find that out take the time: 512 sequences of
-// 1000, 8 heads, 18 us by units, @ by runs.)
-template <typename T, bool BY_RUNS>
-__global__ __launch_bounds__(256) void cache_attention_join_kernel(
-    Attention a, Shares shares, Joins joins, int per) {
+// Puts the parts of a unit together.  Block (x, y): the unit of joins.parts[x], `per` (a power
+// of two) of its heads' pairs of values; 256 / per groups of threads take every so many-th
+// part.
+template <typename T>
+__global__ __launch_bounds__(256) void cache_attention_join_kernel(Attention a, Joins joins,
+                                                                   int per) {
   constexpr int IN_FLIGHT = 16;
   __shared__ float tops[256], alls[256], sums[2][256];
-  int b, unit, from, parts;
-  if constexpr (BY_RUNS) {
-    Run run;
-    bool alone;
-    if (!run_of(a, shares, (int)blockIdx.x + 1, &run, &alone) || alone) return;
-    const Runs runs(shares, run.of_all);
-    const int first = run.first - run.grain;         // grain of the unit
-    from = runs.block_of(first + AHEAD);
-    if (run.grain <= AHEAD || from != (int)blockIdx.x) return;
-    parts = runs.block_of(first + run.of_unit - 1) - from + 1;
-    b = run.b;
-    unit = run.unit;
-  } else {
-    if (!parts_of(a, shares, (int)blockIdx.x, &b, &unit, &from, &parts)) return;
-  }
+  const int32_t* part = reinterpret_cast<const int32_t*>(joins.parts + blockIdx.x);
+  const int b = scalar_load(part), unit = scalar_load(part + 1);
+  const int from = scalar_load(part + 2), parts = scalar_load(part + 3);
+  if (parts <= 1) return;
   const int D = a.pages.D, halves = (D + 1) / 2;
   const int tiles = (a.G + HEADS - 1) / HEADS, columns = min(a.G, HEADS);
   const int kv_head = unit / tiles, head0 = (unit - kv_head * tiles) * HEADS;
@@ -1428,7 +1410,7 @@ struct Division {
   Shares shares;
   int64_t blocks;
   bool joins;                     // whether a unit can fall to several blocks
-  size_t sums, bytes;             // of the workspace: tops, sums
+  size_t sums, parts, bytes;      // of the workspace: tops, sums, parts
   bool fits;                      // all grains can be counted
 };
 
@@ -1484,7 +1466,8 @@ static Division divide(int B, int H, int HK, int D, int S, int P, int dtype, boo
   if (v.joins) {
     const size_t rows = 2 * (size_t)v.blocks * std::min(G, HEADS);
     v.sums = sizeof(float2) * rows;
-    v.bytes = v.sums + sizeof(float2) * rows * ((D + 1) / 2) + 8;
+    v.parts = v.sums + sizeof(float2) * rows * ((D + 1) / 2);
+    v.bytes = v.parts + sizeof(Part) * v.blocks + 8;
   }
   return v;
 }
@@ -1501,20 +1484,19 @@ static int run_tiles(const Attention& a, const Division& v, char* workspace,
   Joins joins = {};
   joins.tops = reinterpret_cast<float2*>(workspace);
   joins.sums = reinterpret_cast<float2*>(workspace + v.sums);
+  joins.parts = v.joins ? reinterpret_cast<Part*>(workspace + v.parts) : nullptr;
+  joins.of_units = (int64_t)a.B * v.shares.units <= v.blocks;
   kern<<<(unsigned)v.blocks, 256, lds, st>>>(a, v.shares, joins);
   MOE_CHECK_LAUNCH("cache_attention");
   if (v.joins) {
     // (blocks for every CU twice, as far as there are pairs of values)
-    const bool by_runs = (int64_t)a.B * v.shares.units > v.blocks;
-    const int64_t units = by_runs ? v.blocks - 1 : (int64_t)a.B * v.shares.units;
+    const int64_t units = joins.of_units ? (int64_t)a.B * v.shares.units : v.blocks;
     const int items = heads * ((a.pages.D + 1) / 2);
     int per = 256;
     while (per > 32 && (per >= 2 * items || units * ((items + per - 1) / per) < 2 * CUS))
       per /= 2;
-    auto join = by_runs ? cache_attention_join_kernel<T, true>
-                        : cache_attention_join_kernel<T, false>;
-    join<<<dim3((unsigned)units, (items + per - 1) / per), 256, 0, st>>>(a, v.shares, joins,
-                                                                       per);
+    cache_attention_join_kernel<T>
+        <<<dim3((unsigned)units, (items + per - 1) / per), 256, 0, st>>>(a, joins, per);
     MOE_CHECK_LAUNCH("cache_attention");
   }
   return 0;
