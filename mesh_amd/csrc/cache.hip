@@ -553,12 +553,13 @@ struct Runs {
 };
 
 // false for a block without work; *alone: every wavefront takes units of its own, and there
-// is no run.  The same for all lanes of a wavefront.
+// is no run (MANY: s.alone may be set).  The same for all lanes of a wavefront.
+template <bool MANY>
 __device__ __forceinline__ bool run_of(const Attention& a, const Shares& s, int block,
                                        Run* run, bool* alone) {
   const int lane = threadIdx.x & 63;
   run->count = 0;
-  *alone = s.blocks == 0 && s.alone != 0;
+  *alone = MANY && s.blocks == 0 && s.alone != 0;
   if (*alone) return true;
   if (s.blocks == 0) {
     run->b = block / s.units;
@@ -583,7 +584,7 @@ __device__ __forceinline__ bool run_of(const Attention& a, const Shares& s, int 
     }
     all += __builtin_amdgcn_readlane(sums_up_to(rest), 63);
   }
-  *alone = s.alone != 0 && !__any(longer);
+  *alone = MANY && s.alone != 0 && !__any(longer);
   if (*alone) return true;
   run->of_all = all * s.units;
   const Runs runs(s, run->of_all);
@@ -691,8 +692,10 @@ __device__ __forceinline__ float unit_in(uint32_t word, int n) {
   return __uint_as_float((n < 3 ? word << (23 - 8 * n) : word >> 1) & 0x7f800000u);
 }
 
-// PADDED: rows of fewer than DP values, or on any address.
-template <typename T, bool EIGHT, int DP, bool PADDED, int SMALL>
+// PADDED: rows of fewer than DP values, or on any address.  MANY: wavefronts may take units
+// of their own; without it there is less code, which every block of a short launch waits for
+// (one sequence of 1600, 8 heads of 128: 10.2 us with, 9.8 without).
+template <typename T, bool EIGHT, int DP, bool PADDED, int SMALL, bool MANY>
 __global__ __launch_bounds__(256, (TileOf<T, EIGHT, DP>::template at_once<PADDED>()))
 void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
   typedef TileOf<T, EIGHT, DP> Tile;
@@ -710,7 +713,7 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
     joins.parts[blockIdx.x] = Part{0, 0, 0, 0};
   Run run;
   bool alone;
-  if (!run_of(a, shares, (int)blockIdx.x, &run, &alone)) return;
+  if (!run_of<MANY>(a, shares, (int)blockIdx.x, &run, &alone)) return;
   auto& fresh_rows = fresh_of[alone ? wave : 0];
   auto& fresh_units = fresh_units_of[alone ? wave : 0];
   const int c = lane & 15, j = lane >> 4;
@@ -1452,11 +1455,10 @@ static Division divide(int B, int H, int HK, int D, int S, int P, int dtype, boo
   // of 64 (6 grains) 8.4 whole, 10.3 divided.
   v.joins = most > (units * B >= CUS ? 2 * whole : whole);
   // Of many short units each is a wavefront's, from beginning to end: no barriers, no sums
-  // of four, and four times as many units under way.  256 sequences of 20, 8 heads of 128
-  // in a table of 8192: 22 us by blocks, 15 alone; of 250 60 and 56, in 8 bits 36 and 31;
-  // 512 of 500 in 8 bits (8 turns) 137 and 114.  Of 500 in bfloat16 (16 turns), lengths
-  // differing, 192 sequences take 54 us by blocks, 61 alone, and with no more units than
-  // blocks (64 sequences of 250, 8 bits) it is 14 and 16.
+  // of four, and four times as many units under way.  512 sequences of 20, 8 heads of 128
+  // in tables of 8192: 35 us by blocks, 19 alone; of up to 250 77 and 72; of up to 500 in 8
+  // bits (8 turns) 88 and 78.  192 of up to 500 in bfloat16 (16 turns) take 52 us by blocks,
+  // 60 alone, and with no more units than blocks (64 of 250, 8 bits) it is 14 and 16.
   if (2 * units * B < 3 * v.shares.blocks || (!v.joins && (int64_t)P * S > v.shares.alone))
     v.shares.alone = 0;
   if (!v.joins) v.shares.blocks = 0;
@@ -1472,10 +1474,10 @@ static Division divide(int B, int H, int HK, int D, int S, int P, int dtype, boo
   return v;
 }
 
-template <typename T, bool EIGHT, int DP, bool PADDED, int SMALL>
+template <typename T, bool EIGHT, int DP, bool PADDED, int SMALL, bool MANY>
 static int run_tiles(const Attention& a, const Division& v, char* workspace,
                      hipStream_t st) {
-  auto kern = cache_attention_tiles_kernel<T, EIGHT, DP, PADDED, SMALL>;
+  auto kern = cache_attention_tiles_kernel<T, EIGHT, DP, PADDED, SMALL, MANY>;
   const int heads = std::min(a.G, HEADS);
   const size_t lds = v.shares.blocks == 0 && v.shares.alone
                          ? 0
@@ -1519,13 +1521,16 @@ static int run_attention(const Attention& a, const Division& v, bool padded,
     return 0;
   }
   const int small = a.pages.shift >= 4 ? 0 : a.pages.shift >= 2 ? 1 : 2;
-#define TILES(dp)                                                                     \
-  (small == 2   ? run_tiles<T, EIGHT, dp, true, 2>                                    \
-   : small == 1 ? (padded ? run_tiles<T, EIGHT, dp, true, 1>                          \
-                          : run_tiles<T, EIGHT, dp, false, 1>)                        \
-   : padded     ? run_tiles<T, EIGHT, dp, true, 0>                                    \
-                : run_tiles<T, EIGHT, dp, false, 0>)
-  auto run = D <= 64 ? TILES(64) : D <= 128 ? TILES(128) : TILES(256);
+#define TILES(dp, padded)                                                             \
+  (v.shares.alone ? run_tiles<T, EIGHT, dp, padded, 0, true>                          \
+                  : run_tiles<T, EIGHT, dp, padded, 0, false>)
+#define TILES_OF(dp)                                                                  \
+  (small == 2   ? run_tiles<T, EIGHT, dp, true, 2, true>                              \
+   : small == 1 ? (padded ? run_tiles<T, EIGHT, dp, true, 1, true>                    \
+                          : run_tiles<T, EIGHT, dp, false, 1, true>)                  \
+                : (padded ? TILES(dp, true) : TILES(dp, false)))
+  auto run = D <= 64 ? TILES_OF(64) : D <= 128 ? TILES_OF(128) : TILES_OF(256);
+#undef TILES_OF
 #undef TILES
   return run(a, v, workspace, st);
 }
