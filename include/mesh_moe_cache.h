@@ -85,6 +85,8 @@ int mesh_moe_cache_read(const void* k_pages, const void* v_pages,
  * The logits, the softmax and its sums are float32; with bfloat16 the weights are rounded
  * to it, unnormalised, and the sum of those that were multiplied divides the result.
  * out[h] is 0 where nothing is seen (position[b] < 0) or all logits are -infinity.
+ * Calls with the same sizes and positions give the same bits; a sequence's last bits may
+ * depend on the others' lengths, by which its sums are divided.
  *   q, out [B,H*D] dtype
  *   k_new, v_new [B,HK*D] dtype or NULL: the step's own row, written to position[b] first
  *     (mesh_moe_cache_write with T = 1); v_new is NULL also where v_pages is

@@ -86,35 +86,38 @@ class PagedCache(object):
   __slots__ = ("_k", "_v", "_k_scales", "_v_scales", "_shape", "_device")
 
   def __init__(self, k_pages, v_pages=None, k_scales=None, v_scales=None):
-    shape = k_pages.shape
-    eight = k_pages.dtype is _E4M3
-    pairs = [(k_pages, k_scales)] + ([] if v_pages is None else [(v_pages, v_scales)])
-    if (len(shape) != 4 or min(shape) < 1 or
-        (v_pages is None and v_scales is not None)):
+    shape, dtype = k_pages.shape, k_pages.dtype
+    eight = dtype is _E4M3
+    if len(shape) != 4 or 0 in shape or (v_pages is None and v_scales is not None):
       raise ValueError("pages %s: expected [pages, heads, page_size, d_kv]"
                        % (tuple(shape),))
     if shape[2] & (shape[2] - 1):
       raise ValueError("pages of %d rows, not a power of two" % shape[2])
     if not eight:
-      moe_hip.dtype_code(k_pages.dtype)
-    for values, scales in pairs:
-      if (values.dtype is not k_pages.dtype or values.shape != shape or
-          (scales is not None) != eight):
-        raise ValueError("pages of keys %s and of values %s differ, or are without "
-                         "their scales" % (tuple(shape), tuple(values.shape)))
-      if eight and (scales.dtype is not torch.uint8 or scales.shape != shape[:-1] + (
-          scale_blocks(shape[3]),)):
-        raise ValueError("scales %s of %s do not go with pages %s"
-                         % (tuple(scales.shape), scales.dtype, tuple(shape)))
+      moe_hip.dtype_code(dtype)
+    if (v_pages is not None and (
+        v_pages.dtype is not dtype or v_pages.shape != shape or
+        (v_scales is not None) != eight)) or (k_scales is not None) != eight:
+      raise ValueError("pages of keys %s and of values %s differ, or are without their "
+                       "scales" % (tuple(shape), None if v_pages is None else
+                                   tuple(v_pages.shape)))
+    if eight:
+      blocks = shape[:-1] + (scale_blocks(shape[3]),)
+      for scales in (k_scales, v_scales):
+        if scales is not None and (scales.dtype is not torch.uint8 or
+                                   scales.shape != blocks):
+          raise ValueError("scales %s of %s do not go with pages %s"
+                           % (tuple(scales.shape), scales.dtype, tuple(shape)))
     self._k, self._v = k_pages, v_pages
     self._k_scales, self._v_scales = k_scales, v_scales
-    self._shape = tuple(shape)
+    self._shape = shape
     # the device of all buffers, where they are what the library takes
     self._device = None
     if k_pages.is_cuda:
       device = k_pages.get_device()
-      if all(x is None or (x.is_cuda and x.get_device() == device and x.is_contiguous())
-             for x in (k_pages, v_pages, k_scales, v_scales)):
+      if k_pages.is_contiguous() and all(
+          x is None or (x.is_cuda and x.get_device() == device and x.is_contiguous())
+          for x in ((v_pages, k_scales, v_scales) if eight else (v_pages,))):
         self._device = device
 
   @classmethod
@@ -145,7 +148,7 @@ class PagedCache(object):
 
   def __repr__(self):
     return "PagedCache(pages=%d, heads=%d, page_size=%d, d_kv=%d, dtype=%s)" % (
-        self._shape + (self.dtype,))
+        tuple(self._shape) + (self.dtype,))
 
 
 def _pointers(cache):
