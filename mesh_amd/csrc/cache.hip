@@ -907,6 +907,18 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
     for (int t = 0; t < VD; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
 
+    // the scale bytes of the values of a lane's row r
+    auto set_units = [&](Group& g, int s, int r, uint32_t units) {
+      if constexpr (SMALL == 2) {
+        g.v_units[s][r] = units;
+      } else {
+        const int bits = 8 * DB * (r % (4 / DB));
+        uint32_t& word = g.v_units[s][r * DB / 4];
+        word = (word & ~((DB == 2 ? 0xffffu : 0xffu) << bits)) |
+               (DB == 2 ? units : units & 0xffu) << bits;
+      }
+    };
+
     // ---- a group's positions into m, l and o
     auto use = [&](int t0, Group& g) {
       if (PADDED) {
@@ -943,17 +955,8 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
             for (int p = 0; p < VP; ++p)
               if (!PADDED || v_extra[p] < VE)
                 load_words<VB>(fresh_rows[1] + v_at[p] * SIZE, g.v[s][r][p]);
-            if (EIGHT) {
-              const uint32_t units = fresh_units[1][0] | (uint32_t)fresh_units[1][1] << 8;
-              if constexpr (SMALL == 2) {
-                g.v_units[s][r] = units;
-              } else {
-                const int bits = 8 * DB * (r % (4 / DB));
-                uint32_t& word = g.v_units[s][r * DB / 4];
-                word = (word & ~((DB == 2 ? 0xffffu : 0xffu) << bits)) |
-                       (DB == 2 ? units : units & 0xffu) << bits;
-              }
-            }
+            if constexpr (EIGHT)
+              set_units(g, s, r, fresh_units[1][0] | (uint32_t)fresh_units[1][1] << 8);
           }
         }
       }
@@ -1045,6 +1048,7 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
             for (int p = 0; p < VP; ++p)
 #pragma unroll
               for (int w = 0; w < VW; ++w) g.v[s][r][p][w] = 0;
+            if constexpr (EIGHT) set_units(g, s, r, 0);   // (255 times 0 is NaN)
           }
       }
       // -- weights

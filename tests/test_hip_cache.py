@@ -283,6 +283,39 @@ def test_step(case, store, shared):
 
 @pytest.mark.parametrize("store", STORES, ids=STORE_IDS)
 @pytest.mark.parametrize("case", [
+    # sequences, longest, query heads, key / value heads, width, page, columns more
+    (5, 70, 2, 2, 64, 16, 0), (3, 90, 3, 1, 128, 32, 200), (4, 40, 2, 1, 256, 64, 0),
+    (3, 60, 2, 2, 80, 8, 0), (4, 30, 1, 1, 40, 2, 0), (3, 20, 2, 1, 200, 16, 0),
+    (3, 20, 2, 1, 8, 16, 0), (800, 25, 2, 2, 64, 32, 0), (800, 25, 1, 1, 128, 8, 500)],
+    ids=lambda c: "x".join(map(str, c)))
+@pytest.mark.parametrize("byte", [0xff, 0x00])
+def test_rows_that_nothing_was_written_to(case, store, byte):
+  """Whatever bytes pages and scales have where nothing was written, it does not matter."""
+  b, longest, heads, kv, width, page, more = case
+  name, eight = store
+  dtype = DTYPES[name]
+  rng, gen = np.random.default_rng(b + width), _gen(b + width)
+  lengths = rng.integers(0, longest + 1, b)
+  lengths[:3] = longest, 1, 0
+  table, pages = _table(rng, lengths, page, extra=more)
+  table[0, table.shape[1] // 2] = -1
+  cache, _ = _cache(gen, pages, page, kv, width, dtype, eight)
+  for x in (cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales):
+    if x is not None:
+      x.view(torch.uint8).fill_(byte)
+  rows = [_rows(gen, (b, longest, kv * width), dtype) for _ in range(2)]
+  cache_hip.write(cache, *rows, _int32(table), _int32([0] * b), count=_int32(lengths))
+  held = [C.write(np.zeros((pages, kv, page, width)),
+                  C.stored(_np(x).reshape(b, longest, kv, width), eight), table, [0] * b,
+                  lengths, page) for x in rows]
+  q = (torch.randn((b, heads * width), generator=gen, device="cuda")
+       * 2 * width ** -0.5).to(dtype)
+  got = cache_hip.attention(q, cache, _int32(table), _int32(lengths - 1))
+  _check(got, q, held, table, lengths - 1, page, name)
+
+
+@pytest.mark.parametrize("store", STORES, ids=STORE_IDS)
+@pytest.mark.parametrize("case", [
     # lengths, query heads, key / value heads, width, page
     ([20011], 2, 1, 128, 64), ([9000, 3, 4096, 1], 2, 2, 64, 16),
     ([2500] * 3, 1, 1, 40, 32), ([6000, 700], 20, 1, 64, 32), ([5000], 2, 1, 256, 16),
