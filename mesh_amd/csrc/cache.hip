@@ -274,10 +274,11 @@ __global__ __launch_bounds__(256) void cache_read_kernel(
 // and two such triples of different positions are joined the same way; o / l is the
 // result.
 //
-// The kernel for rows of fewer than 16 values, whose pieces the matrix cores' tiles (below)
-// do not have: a block has a query head of a sequence, its four wavefronts every fourth
-// position each.  Bound by the latency of one position after the other; with 16 values a
-// row is a quarter of a wavefront's load.
+// The kernel for rows of fewer than 16 values, which the matrix cores' tiles (below) do not
+// take: a block has a query head of a sequence, and a lane every 256th position, with sums
+// of its own.  Bound by the latency of one turn after the other; a long sequence has no
+// more blocks than a short one (1 sequence of 16384, 8 heads of 8, bfloat16: @ us; a
+// wavefront for a position took @).
 // ---------------------------------------------------------------------------
 struct Attention {
   Pages pages;
@@ -314,45 +315,50 @@ __device__ __forceinline__ float weight_of(float x, float m) {
                         : __builtin_amdgcn_exp2f((x - m) * 1.4426950408889634f);
 }
 
+// a row's values, 0 from D on
 template <typename T, bool EIGHT>
-__device__ __forceinline__ float page_value(const void* pages, const uint8_t* scales,
-                                            int64_t row, int d, int D, int DB) {
-  if constexpr (EIGHT) {
-    const uint32_t byte = static_cast<const uint8_t*>(pages)[row * D + d];
-    return __builtin_amdgcn_cvt_f32_fp8((int)byte, 0) *
-           unit_of(scales[row * DB + d / FP8_BLOCK]);
-  } else {
-    return load_f32<T>(static_cast<const T*>(pages) + row * D + d);
+__device__ __forceinline__ void few_values(const void* pages, const uint8_t* scales,
+                                           int64_t row, int D, float (&f)[TILES_FROM]) {
+  uint32_t code[TILES_FROM];
+  float unit = 1.f;
+  if constexpr (EIGHT) unit = unit_of(scales[row]);
+#pragma unroll
+  for (int d = 0; d < TILES_FROM; ++d) {
+    f[d] = 0.f;
+    if (d >= D) continue;
+    if constexpr (EIGHT) code[d] = static_cast<const uint8_t*>(pages)[row * D + d];
+    else f[d] = load_f32<T>(static_cast<const T*>(pages) + row * D + d);
   }
+  if constexpr (EIGHT)
+#pragma unroll
+    for (int d = 0; d < TILES_FROM; ++d)
+      if (d < D) f[d] = __builtin_amdgcn_cvt_f32_fp8((int)code[d], 0) * unit;
 }
 
 template <typename T, bool EIGHT>
 __global__ __launch_bounds__(256) void cache_attention_kernel(Attention a) {
-  constexpr int NI = MAX_WIDTH / 64;            // values of a row per lane
-  __shared__ float part_o[4][MAX_WIDTH], part_m[4], part_l[4];
+  __shared__ float part_o[4][TILES_FROM], part_m[4], part_l[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int b = (int)(blockIdx.x / a.H), h = (int)(blockIdx.x - (int64_t)b * a.H);
-  const int D = a.pages.D, seen = seen_of(a, b), last = a.position[b];
+  const int D = a.pages.D, last = scalar_load(a.position + b), seen = seen_from(a, last);
   const int64_t at = ((int64_t)b * a.H + h) * D;
-  float q[NI], o[NI], m = -INFINITY, l = 0.f;
+  float q[TILES_FROM], o[TILES_FROM], m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    const int d = lane + 64 * i;
-    q[i] = d < D ? load_f32<T>(static_cast<const T*>(a.q) + at + d) : 0.f;
-    o[i] = 0.f;
+  for (int d = 0; d < TILES_FROM; ++d) {
+    q[d] = d < D ? load_f32<T>(static_cast<const T*>(a.q) + at + d) : 0.f;
+    o[d] = 0.f;
   }
-  for (int j = wave; j < seen; j += 4) {
+  for (int j = threadIdx.x; j < seen; j += 256) {
     int64_t row = a.pages.row(b, j);
     if (row < 0) continue;
     row = a.pages.head(row, h / a.G);
+    float k[TILES_FROM], v[TILES_FROM];
+    few_values<T, EIGHT>(a.k_pages, a.k_scales, row, D, k);
+    few_values<T, EIGHT>(a.v_pages, a.v_scales, row, D, v);
     float x = 0.f;
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
-      if (lane + 64 * i < D)
-        x = fmaf(q[i], page_value<T, EIGHT>(a.k_pages, a.k_scales, row, lane + 64 * i, D,
-                                            a.pages.DB), x);
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+    for (int d = 0; d < TILES_FROM; ++d)
+      if (d < D) x = fmaf(q[d], k[d], x);
     if (a.rel_values)
       x += load_f32<T>(static_cast<const T*>(a.rel_values) + (int64_t)h * a.NB +
                        bucket_of(a, j - last));
@@ -361,30 +367,42 @@ __global__ __launch_bounds__(256) void cache_attention_kernel(Attention a) {
     m = top;
     l = l * was + w;
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
-      if (lane + 64 * i < D)
-        o[i] = fmaf(w, page_value<T, EIGHT>(a.v_pages, a.v_scales, row, lane + 64 * i, D,
-                                            a.pages.DB), o[i] * was);
+    for (int d = 0; d < TILES_FROM; ++d)
+      if (d < D) o[d] = fmaf(w, v[d], o[d] * was);
   }
+  // ---- the lanes' triples, then the wavefronts'
+  float top = m;
 #pragma unroll
-  for (int i = 0; i < NI; ++i) part_o[wave][lane + 64 * i] = o[i];
+  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  const float factor = weight_of(m, top);
+  l *= factor;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off, 64);
+#pragma unroll
+  for (int d = 0; d < TILES_FROM; ++d) {
+    if (d >= D) continue;
+    o[d] *= factor;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) o[d] += __shfl_xor(o[d], off, 64);
+    if (lane == 0) part_o[wave][d] = o[d];
+  }
   if (lane == 0) {
-    part_m[wave] = m;
+    part_m[wave] = top;
     part_l[wave] = l;
   }
   __syncthreads();
-  float top = part_m[0];
+  if ((int)threadIdx.x >= D) return;
+  const int d = threadIdx.x;
+  top = part_m[0];
   for (int w = 1; w < 4; ++w) top = fmaxf(top, part_m[w]);
-  for (int d = threadIdx.x; d < D; d += 256) {
-    float sum = 0.f, all = 0.f;
-    for (int w = 0; w < 4; ++w) {
-      const float factor = weight_of(part_m[w], top);
-      sum += part_o[w][d] * factor;
-      all += part_l[w] * factor;
-    }
-    // (nothing seen: 0)
-    store_f32<T>(static_cast<T*>(a.out) + at + d, all == 0.f ? 0.f : sum / all);
+  float sum = 0.f, all = 0.f;
+  for (int w = 0; w < 4; ++w) {
+    const float of_wave = weight_of(part_m[w], top);
+    sum += part_o[w][d] * of_wave;
+    all += part_l[w] * of_wave;
   }
+  // (nothing seen: 0)
+  store_f32<T>(static_cast<T*>(a.out) + at + d, all == 0.f ? 0.f : sum / all);
 }
 
 // ---------------------------------------------------------------------------

@@ -282,6 +282,31 @@ def test_step(case, store, shared):
 
 
 @pytest.mark.parametrize("store", STORES, ids=STORE_IDS)
+@pytest.mark.parametrize("width", [1, 5, 8, 15])
+def test_narrow_rows(width, store):
+  name, eight = store
+  dtype = DTYPES[name]
+  rng, gen = np.random.default_rng(width), _gen(width)
+  lengths = np.array([1, 64, 255, 256, 257, 1500, 3, 40])
+  table, pages = _table(rng, lengths, 8)
+  table[7, 1:3] = -1
+  cache, held = _cache(gen, pages, 8, 2, width, dtype, eight)
+  q = (torch.randn((8, 6 * width), generator=gen, device="cuda") * 2).to(dtype)
+  position = lengths - 1
+  position[6] = -1
+  relative = _relative(gen, rng, 6, dtype, 300)
+  for bias in (None, relative):
+    got = cache_hip.attention(q, cache, _int32(table), _int32(position),
+                              relative_bias=bias and (bias[0], _gpu(bias[1])))
+    _check(got, q, held, table, position, 8, name, bias)
+  k, v = (_rows(gen, (8, 2 * width), dtype) for _ in range(2))
+  got = cache_hip.attention(q, cache, _int32(table), _int32(position), k_new=k, v_new=v)
+  held = [C.write(was, C.stored(_np(x).reshape(8, 1, 2, width), eight), table, position,
+                  None, 8) for was, x in zip(held, (k, v))]
+  _check(got, q, held, table, position, 8, name)
+
+
+@pytest.mark.parametrize("store", STORES, ids=STORE_IDS)
 @pytest.mark.parametrize("case", [
     # sequences, longest, query heads, key / value heads, width, page, columns more
     (5, 70, 2, 2, 64, 16, 0), (3, 90, 3, 1, 128, 32, 200), (4, 40, 2, 1, 256, 64, 0),
