@@ -276,9 +276,9 @@ __global__ __launch_bounds__(256) void cache_read_kernel(
 //
 // The kernel for rows of fewer than 16 values, which the matrix cores' tiles (below) do not
 // take: a block has a query head of a sequence, and a lane every 256th position, with sums
-// of its own.  Bound by the latency of one turn after the other; a long sequence has no
-// more blocks than a short one (1 sequence of 16384, 8 heads of 8, bfloat16: @ us; a
-// wavefront for a position took @).
+// of its own.  Bound by the latency of one turn after the other, as a long sequence has no
+// more blocks than a short one: 1 sequence of 16384, 8 heads of 8, bfloat16 takes 122 us
+// (2863 with a wavefront for a position), 64 of 500 take 10.
 // ---------------------------------------------------------------------------
 struct Attention {
   Pages pages;
