@@ -120,10 +120,15 @@ class Context(object):
     """The next recurrent state, where it is kept in pages (attention.PagedState), else
     None."""
     from mesh_amd.transformer import attention
-    states = self.states[len(self.new_states):len(self.new_states) + 1]
-    if states and isinstance(states[0], attention.PagedState):
-      return states[0]
-    return None
+    states = self.states[:len(self.new_states) + 1]
+    if len(states) <= len(self.new_states) or not isinstance(
+        states[-1], attention.PagedState):
+      return None
+    state = states.pop()
+    if any(isinstance(s, attention.PagedState) and s.cache is state.cache
+           for s in states):
+      raise ValueError("two layers were given the same pages")
+    return state
 
   def record_new_states(self, new_states):
     """transformer.py:263-271."""

@@ -198,3 +198,11 @@ def test_paged_states_of_layers():
   assert context.paged_state() is state
   context.record_new_states([state])
   assert context.paged_state() is None
+  # pages that an earlier layer has already
+  context = transformer.Context(
+      model, mesh, [batch], mtf.Dimension("length", 8), mtf.VariableDType(torch.float32),
+      mode="incremental", position=position,
+      states=[state, attention.PagedState(cache, state.table)])
+  context.record_new_states([context.paged_state()])
+  with pytest.raises(ValueError, match="the same pages"):
+    context.paged_state()
