@@ -104,9 +104,9 @@ __device__ __forceinline__ void store_eight(uint8_t* row, int at, int D, uint32_
 // ---------------------------------------------------------------------------
 // Rows into pages and back.  A wavefront has R rows of keys or of values (blockIdx.z) that
 // follow each other in a sequence (blockIdx.y), so that loads of R rows are on their way at
-// once; with one row a sequence the wavefronts of a block share it.  A lane has 8 values of
-// each, and a head's lanes are a power of two (16 for each block of 128 where it has more
-// than one), so that a block's largest magnitude is found by DPP steps among neighbours.
+// once; wide rows are shared by two or four wavefronts.  A lane has 8 values of each, and a
+// head's lanes are a power of two (16 for each block of 128 where it has more than one), so
+// that a block's largest magnitude is found by DPP steps among neighbours.
 // Nothing is used twice: bound by the memory.  16 sequences of up to 4096 rows of 1024
 // bfloat16 keys and values into 8 bits move 278 MB in 46 us (6.0 TB/s, some of it to the
 // last level's cache; a copy of 1 GiB reaches 5.15), 4 x 16384 rows back 406 MB in 61.
@@ -117,11 +117,12 @@ struct RowsOf {
   const int32_t* count;           // [B] or null
   int B, T;
   int lanes;                      // of a head, log2
+  int sharing;                    // wavefronts that share a row (1, 2 or 4), log2
 };
-// Rows of a wavefront, where a sequence has several: 4 x 16384 rows of 1024 values out of
-// an 8-bit cache take 84 us by one, 82 by two, 69 by four; 23 x 1000 of 480 out of a
-// bfloat16 one 24 by one, 17 by two, 21 by four.
-template <bool EIGHT> constexpr int ROWS = EIGHT ? 4 : 2;
+// Rows of a wavefront, where there are many: 4 x 16384 rows of 1024 values out of an 8-bit
+// cache take 84 us by one, 82 by two, 70 by four; 23 x 1000 of 480 out of a bfloat16 one 24
+// by one, 18 by two, 21 by four.
+template <typename T, bool EIGHT> constexpr int ROWS = EIGHT && sizeof(T) == 2 ? 4 : 2;
 
 // Where piece `piece` of a head's row begins: a piece that would end behind the row begins as
 // much earlier, if that is in its block of 128 (EIGHT) or row, and the values that two lanes
@@ -145,8 +146,8 @@ __device__ __forceinline__ void for_rows(const RowsOf& r, F f) {
     const int count = r.count ? min(max(scalar_load(r.count + b), 0), r.T) : r.T;
     const int position = scalar_load(r.position + b);
     const int32_t* table = r.pages.table + (int64_t)b * r.pages.P;
-    for (int64_t g = R == 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
-         g < groups; g += R == 1 ? (int64_t)gridDim.x : (int64_t)gridDim.x * 4) {
+    for (int64_t g = ((int64_t)blockIdx.x * 4 + wave) >> r.sharing; g < groups;
+         g += (int64_t)gridDim.x * 4 >> r.sharing) {
       const int t0 = (int)g * R;
       int64_t rows[R];
 #pragma unroll
@@ -159,8 +160,8 @@ __device__ __forceinline__ void for_rows(const RowsOf& r, F f) {
           rows[i] = (((int64_t)page * r.pages.HK) << r.pages.shift) +
                     (p & ((1 << r.pages.shift) - 1));
       }
-      f(b, t0, min(r.T - t0, R), rows, R == 1 ? (int)threadIdx.x : lane,
-        R == 1 ? 256 : 64);
+      f(b, t0, min(r.T - t0, R), rows, (wave & (1 << r.sharing) - 1) * 64 + lane,
+        64 << r.sharing);
     }
   }
 }
@@ -1393,39 +1394,55 @@ static int lanes_of(int D) {
   return n;
 }
 
-// the grid of the kernels that have rows
+// Sets the wavefronts that share a row; true if a wavefront is to have one row at a time.
+// Few rows: as many wavefronts as there can be (writing 2 x 400 rows of 2048 values in 8
+// bits and reading them 22 us with rows by four and a wavefront each, 9 so; at 4000 rows
+// they are even).  Many: rows that fill four wavefronts to three quarters, or two (16 x 1000
+// rows of 2048 in 8 bits 41 us and 31, of 480 in bfloat16 18 and 20).  Float32 rows of a
+// wavefront and more take their registers one by one, too (16 x 1000 of 1024 116 us by two,
+// 103; of 64 values 15 and 19).
+static bool few_rows(RowsOf& r, bool wide_type) {
+  const int64_t pieces = (int64_t)r.pages.HK << r.lanes;
+  const bool few = r.T == 1 || (int64_t)r.B * r.T <= 2048;
+  if (few) r.sharing = pieces <= 64 ? 0 : pieces <= 128 ? 1 : 2;
+  else r.sharing = pieces < 128 ? 0 : pieces < 192 ? 1 : 2;
+  return few || (wide_type && pieces >= 64);
+}
+
+// the grid of the kernels that have rows, of `rows` a wavefront
 static dim3 row_grid(const RowsOf& r, int rows, bool v) {
-  const int64_t groups = rows == 1 ? r.T : ((int64_t)r.T + 4 * rows - 1) / (4 * rows);
-  return dim3((unsigned)std::min<int64_t>(groups, 1 << 14),
+  const int64_t groups = ((int64_t)r.T + rows - 1) / rows;
+  const int of_block = 4 >> r.sharing;
+  return dim3((unsigned)std::min<int64_t>((groups + of_block - 1) / of_block, 1 << 14),
               (unsigned)std::min(r.B, 1 << 14), v ? 2 : 1);
 }
 
 template <typename T, bool EIGHT>
-static void run_write(const RowsOf& r, const void* k, const void* v, void* k_pages,
+static void run_write(RowsOf r, const void* k, const void* v, void* k_pages,
                       void* v_pages, uint8_t* k_scales, uint8_t* v_scales,
                       hipStream_t st) {
   const bool aligned = r.pages.D % 8 == 0 && on_16_bytes({k, v, k_pages, v_pages});
-  const bool one = r.T == 1;
+  const bool one = few_rows(r, sizeof(T) == 4);
   auto kern = aligned ? (one ? cache_write_kernel<T, EIGHT, true, 1>
-                             : cache_write_kernel<T, EIGHT, true, ROWS<EIGHT>>)
+                             : cache_write_kernel<T, EIGHT, true, ROWS<T, EIGHT>>)
                       : (one ? cache_write_kernel<T, EIGHT, false, 1>
-                             : cache_write_kernel<T, EIGHT, false, ROWS<EIGHT>>);
-  kern<<<row_grid(r, one ? 1 : ROWS<EIGHT>, v != nullptr), 256, 0, st>>>(
+                             : cache_write_kernel<T, EIGHT, false, ROWS<T, EIGHT>>);
+  kern<<<row_grid(r, one ? 1 : ROWS<T, EIGHT>, v != nullptr), 256, 0, st>>>(
       r, static_cast<const T*>(k), static_cast<const T*>(v), k_pages, v_pages, k_scales,
       v_scales);
 }
 
 template <typename T, bool EIGHT>
-static void run_read(const RowsOf& r, const void* k_pages, const void* v_pages,
+static void run_read(RowsOf r, const void* k_pages, const void* v_pages,
                      const uint8_t* k_scales, const uint8_t* v_scales, void* k, void* v,
                      hipStream_t st) {
   const bool aligned = r.pages.D % 8 == 0 && on_16_bytes({k, v, k_pages, v_pages});
-  const bool one = r.T == 1;
+  const bool one = few_rows(r, sizeof(T) == 4);
   auto kern = aligned ? (one ? cache_read_kernel<T, EIGHT, true, 1>
-                             : cache_read_kernel<T, EIGHT, true, ROWS<EIGHT>>)
+                             : cache_read_kernel<T, EIGHT, true, ROWS<T, EIGHT>>)
                       : (one ? cache_read_kernel<T, EIGHT, false, 1>
-                             : cache_read_kernel<T, EIGHT, false, ROWS<EIGHT>>);
-  kern<<<row_grid(r, one ? 1 : ROWS<EIGHT>, v != nullptr), 256, 0, st>>>(
+                             : cache_read_kernel<T, EIGHT, false, ROWS<T, EIGHT>>);
+  kern<<<row_grid(r, one ? 1 : ROWS<T, EIGHT>, v != nullptr), 256, 0, st>>>(
       r, k_pages, v_pages, k_scales, v_scales, static_cast<T*>(k), static_cast<T*>(v));
 }
 

@@ -143,6 +143,36 @@ def test_write_and_read(case, store):
           C.read(held, table, start, t, counted, page))
 
 
+@pytest.mark.parametrize("store", STORES, ids=STORE_IDS)
+@pytest.mark.parametrize("case", [
+    # sequences, rows, heads, width, page
+    (3, 903, 1, 36, 16), (3, 901, 4, 40, 4), (2, 1101, 8, 128, 32), (2, 1101, 5, 256, 16),
+    (2, 1101, 24, 64, 16), (1, 2099, 16, 80, 8), (2, 1102, 20, 131, 64), (4, 701, 2, 17, 1)],
+    ids=lambda c: "x".join(map(str, c)))
+def test_many_rows(case, store):
+  """Rows in twos and fours, shared by one, two and four wavefronts."""
+  b, t, heads, width, page = case
+  dtype, eight = DTYPES[store[0]], store[1]
+  rng, gen = np.random.default_rng(sum(case)), _gen(sum(case))
+  start = np.array([3, -2, 0, page + 1])[:b]
+  count = np.array([t, t - 3, t // 2 + 1, 0])[:b]
+  table, pages = _table(rng, [max(s, 0) + t for s in start], page, extra=1)
+  table[0, 2] = -1
+  cache, before = _cache(gen, pages, page, heads, width, dtype, eight)
+  rows = [_rows(gen, (b, t, heads * width), dtype) for _ in range(2)]
+  cache_hip.write(cache, *rows, _int32(table), _int32(start), count=_int32(count))
+  held = [C.write(was, C.stored(_np(x).reshape(b, t, heads, width), eight), table, start,
+                  count, page) for was, x in zip(before, rows)]
+  for got, want in zip(_held(cache), held):
+    np.testing.assert_array_equal(got, want)
+  for counted in (count, None):
+    got = cache_hip.read(cache, _int32(table), _int32(start), t, dtype=dtype,
+                         count=None if counted is None else _int32(counted))
+    for x, was in zip(got, held):
+      np.testing.assert_array_equal(_np(x).reshape(b, t, heads, width),
+                                    C.read(was, table, start, t, counted, page))
+
+
 @pytest.mark.parametrize("store", STORES[:2], ids=STORE_IDS[:2])
 def test_rows_at_any_address_and_shared_keys(store):
   """Dense tensors off 16 bytes; a cache whose keys are its values; one row a sequence."""
