@@ -108,8 +108,8 @@ __device__ __forceinline__ void store_eight(uint8_t* row, int at, int D, uint32_
 // head's lanes are a power of two (16 for each block of 128 where it has more than one), so
 // that a block's largest magnitude is found by DPP steps among neighbours.
 // Nothing is used twice: bound by the memory.  16 sequences of up to 4096 rows of 1024
-// bfloat16 keys and values into 8 bits move 278 MB in 46 us (6.0 TB/s, some of it to the
-// last level's cache; a copy of 1 GiB reaches 5.15), 4 x 16384 rows back 406 MB in 61.
+// bfloat16 keys and values into 8 bits move 278 MB in 48 us (5.8 TB/s, some of it to the
+// last level's cache; a copy of 1 GiB reaches 5.15), 4 x 16384 rows back 406 MB in 60.
 // ---------------------------------------------------------------------------
 struct RowsOf {
   Pages pages;
