@@ -234,6 +234,13 @@ def relative_position_bucket(relative_position, bidirectional=True,
   return ret + np.where(is_small, n, large)
 
 
+def last_bucket_from(bidirectional, num_buckets):
+  """The distance from which on everything farther back has one bucket, or None: where
+  distances up to MAX_DISTANCE and beyond have buckets of their own, there is none."""
+  exact = (num_buckets // 2 if bidirectional else num_buckets) // 2
+  return MAX_DISTANCE if exact < MAX_DISTANCE else None
+
+
 class SelfAttentionOperation(mtf.Operation):
   """attention.attention (attention.py:27-88) on combined-dim tensors
   q, k, v [batch..., length, heads * d_kv]: float32 logits, an optional
@@ -510,8 +517,10 @@ class PagedDecodeOperation(mtf.Operation):
       rel = None
       if has_rel:
         values = extra[-1].to(q.dtype).contiguous()
-        # (from MAX_DISTANCE on all positions are in one bucket)
-        reach = min(state.table.shape[-1] * state.cache.page_size, MAX_DISTANCE + 1)
+        reach = state.table.shape[-1] * state.cache.page_size
+        far = last_bucket_from(bidirectional, values.shape[-1])
+        if far is not None:
+          reach = min(reach, far + 1)
         rel = (values, relative_bucket_table(reach, bidirectional, values.shape[-1],
                                              values.device))
       return cache_hip.attention(

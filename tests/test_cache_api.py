@@ -4,6 +4,7 @@ what is refused before a launch."""
 import os
 import re
 
+import numpy as np
 import pytest
 import torch
 
@@ -206,3 +207,22 @@ def test_paged_states_of_layers():
   context.record_new_states([context.paged_state()])
   with pytest.raises(ValueError, match="the same pages"):
     context.paged_state()
+
+
+@pytest.mark.parametrize("bidirectional", [False, True])
+def test_distances_that_share_the_last_bucket(bidirectional):
+  """A bucket table that ends where the last bucket begins stands for all distances behind
+  it; where there is no last bucket, none is cut."""
+  from mesh_amd.transformer import attention
+  once = 2 if bidirectional else 1
+  for buckets in list(range(2, 70)) + list(range(250, 256)):
+    buckets *= once
+    far = attention.last_bucket_from(bidirectional, buckets)
+    assert far <= attention.MAX_DISTANCE
+    got = attention.relative_position_bucket(-np.arange(far, 5000), bidirectional, buckets)
+    assert (got == got[0]).all()
+  for buckets in (256, 257, 300, 1000):
+    assert attention.last_bucket_from(bidirectional, buckets * once) is None
+  # the distance at which a table of 129 positions was wrong
+  got = attention.relative_position_bucket(np.array([-128, -139]), bidirectional, 300 * once)
+  assert got.tolist() == [128, 139]

@@ -158,3 +158,49 @@ def test_operations_are_the_calls(kind, relative):
     recorded.replay(dict(zip(feeds, (q, k, v, position))))
     check(q, k, v, position)
     torch.empty(1 << 20, device="cuda").normal_()
+
+
+@pytest.mark.parametrize("buckets,bidirectional", [(300, False), (600, True), (320, False),
+                                                   (254, False)])
+@pytest.mark.parametrize("act_dtype", [torch.float32, torch.bfloat16])
+def test_biases_of_many_buckets(act_dtype, buckets, bidirectional):
+  """More buckets than the distances that usually differ: a position far back has the bias
+  that it has on whole states."""
+  b, memory = 3, 150
+  rng, gen = np.random.default_rng(6), torch.Generator(device="cuda").manual_seed(6)
+  mk = lambda *s: torch.randn(s, generator=gen, device="cuda").to(act_dtype)
+  state = _states(b, memory, act_dtype, False, 1)[0]
+  assert state.table.shape[-1] * PAGE > memory
+  old = [mk(b, memory, HEADS * WIDTH) for _ in range(2)]
+  cache_hip.write(state.cache, old[0], old[1], state.table,
+                  torch.zeros(b, dtype=torch.int32, device="cuda"))
+  q, k, v = (mk(b, HEADS * WIDTH) for _ in range(3))
+  q *= WIDTH ** -0.5
+  values = torch.from_numpy(rng.standard_normal((HEADS, buckets)).astype(np.float32)).cuda()
+  position = torch.tensor([149, 128, 139], dtype=torch.int32, device="cuda")
+  graph = mtf.Graph()
+  mesh = mtf.Mesh(graph, "mesh")
+  batch, length, chan = (mtf.Dimension("batch", b), mtf.Dimension("memory_length", memory),
+                         mtf.Dimension("heads", HEADS * WIDTH))
+  t = lambda a, *dims: mtf.import_tf_tensor(mesh, a, mtf.Shape(dims))
+  feeds = [t(q, batch, chan), t(k, batch, chan), t(v, batch, chan)]
+  states = [t(x, batch, length, chan) for x in old]
+  at = t(position, batch)
+  bias = dict(relative_values=t(values.to(act_dtype), mtf.Dimension("h", HEADS),
+                                mtf.Dimension("buckets", buckets)),
+              relative_bidirectional=bidirectional)
+  on_pages = attention.PagedDecodeOperation(*feeds, at, state, HEADS, **bias).outputs[0]
+  whole = attention.AttentionDecodeOperation(*feeds, *states, at, HEADS, **bias).outputs[0]
+  lowering = mtf.Lowering(graph, {mesh: mtf.HipMeshImpl()})
+  got, want = (lowering.export_to_tf_tensor(x).float() for x in (on_pages, whole))
+  # (bfloat16: weights and the result are rounded, each by half a step of 2^-8, and the sum of
+  # weights times |v| is below 2, so each is off by 2 * 2^-8 * 2 + 2^-8 |out| at most, which
+  # is 0.016 and 0.4 %, twice.  float32: logits below 16 and 150 terms, 2^-24 * 400 * 2.)
+  torch.testing.assert_close(
+      got, want, **(dict(rtol=2e-4, atol=2e-4) if act_dtype == torch.float32
+                    else dict(rtol=5e-2, atol=5e-2)))
+  # and the bits of the call with the whole table
+  table = attention.relative_bucket_table(memory + 1, bidirectional, buckets, values.device)
+  assert torch.equal(got, cache_hip.attention(
+      q, state.cache, state.table, position,
+      relative_bias=(values.to(act_dtype), table)).float())
