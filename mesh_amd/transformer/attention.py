@@ -325,7 +325,9 @@ _BUCKET_TABLES = {}
 
 def relative_bucket_table(length, bidirectional, num_buckets, device):
   """int32 [2 * length - 1] on `device`: entry d is the bucket of the distance
-  d - (length - 1)."""
+  d - (length - 1).  Kernels index with what is in it: where the formula leaves
+  [0, num_buckets) (half of them in single distances beyond MAX_DISTANCE), it is the
+  nearest bucket there is."""
   key = (int(length), bool(bidirectional), int(num_buckets), str(device))
   table = _BUCKET_TABLES.get(key)
   if table is None:
@@ -336,7 +338,8 @@ def relative_bucket_table(length, bidirectional, num_buckets, device):
           "recorded: run the step once before capturing it" % length)
     bucket = relative_position_bucket(
         np.arange(-(length - 1), length), bidirectional, num_buckets)
-    table = torch.from_numpy(bucket.astype(np.int32)).to(device)
+    bucket = np.clip(bucket.astype(np.int32), 0, num_buckets - 1)
+    table = torch.from_numpy(bucket).to(device)
     _BUCKET_TABLES[key] = table
   return table
 

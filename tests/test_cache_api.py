@@ -226,3 +226,20 @@ def test_distances_that_share_the_last_bucket(bidirectional):
   # the distance at which a table of 129 positions was wrong
   got = attention.relative_position_bucket(np.array([-128, -139]), bidirectional, 300 * once)
   assert got.tolist() == [128, 139]
+
+
+@pytest.mark.parametrize("bidirectional", [False, True])
+def test_bucket_tables_hold_buckets(bidirectional):
+  """Kernels index the bias with what a table holds, so all of it is in range, also where
+  the formula (which ends at MAX_DISTANCE) gives far positions negative numbers."""
+  from mesh_amd.transformer import attention
+  for buckets in (8, 32, 254, 256, 257, 258, 300, 512, 600, 1000):
+    for length in (1, 129, 150, 512, 3001):
+      table = attention.relative_bucket_table(length, bidirectional, buckets, "cpu")
+      assert table.dtype == torch.int32 and table.shape == (2 * length - 1,)
+      assert 0 <= int(table.min()) and int(table.max()) < buckets, (buckets, length)
+  # (what the formula has in range stays as it is)
+  got = attention.relative_bucket_table(512, bidirectional, 300, "cpu").numpy()
+  formula = attention.relative_position_bucket(np.arange(-511, 512), bidirectional, 300)
+  inside = (formula >= 0) & (formula < 300)
+  np.testing.assert_array_equal(got[inside], formula[inside])
