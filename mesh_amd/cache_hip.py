@@ -146,6 +146,15 @@ class PagedCache(object):
   eight_bit = property(lambda self: self._k_scales is not None)
   shared_kv = property(lambda self: self._v is None)
 
+  def overlaps(self, other):
+    """Whether some of this cache's buffers and of the other's are the same memory."""
+    def spans(cache):
+      return [(t.device, t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
+              for t in (cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales)
+              if t is not None]
+    return any(a[0] == b[0] and a[1] < b[2] and b[1] < a[2]
+               for a in spans(self) for b in spans(other))
+
   def __repr__(self):
     return "PagedCache(pages=%d, heads=%d, page_size=%d, d_kv=%d, dtype=%s)" % (
         tuple(self._shape) + (self.dtype,))

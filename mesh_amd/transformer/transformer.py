@@ -125,7 +125,7 @@ class Context(object):
         states[-1], attention.PagedState):
       return None
     state = states.pop()
-    if any(isinstance(s, attention.PagedState) and s.cache is state.cache
+    if any(isinstance(s, attention.PagedState) and s.cache.overlaps(state.cache)
            for s in states):
       raise ValueError("two layers were given the same pages")
     return state

@@ -243,3 +243,49 @@ def test_bucket_tables_hold_buckets(bidirectional):
   formula = attention.relative_position_bucket(np.arange(-511, 512), bidirectional, 300)
   inside = (formula >= 0) & (formula < 300)
   np.testing.assert_array_equal(got[inside], formula[inside])
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_layers_with_the_same_buffers(eight):
+  """Two layers' caches are two objects, but one memory: refused; parts of one buffer that
+  do not meet are taken."""
+  import mesh_amd as mtf
+  from mesh_amd.transformer import attention
+  from mesh_amd.transformer import transformer
+  mesh = mtf.Mesh(mtf.Graph(), "mesh")
+  batch = mtf.Dimension("batch", 3)
+  position = mtf.import_tf_tensor(mesh, torch.zeros(3, dtype=torch.int32),
+                                  mtf.Shape([batch]))
+  table = torch.zeros(3, 2, dtype=torch.int32)
+  kind = E4M3 if eight else torch.bfloat16
+
+  def caches(first, second):
+    """Of pages `first` and `second` (keys, values) of one buffer."""
+    pages = torch.empty((6, 4, 2, 8, 16), dtype=kind)
+    scales = [torch.empty((6, 4, 2, 8, 1), dtype=torch.uint8) if eight else None] * 2
+    return [cache_hip.PagedCache(pages[k], None if v is None else pages[v], *(
+        None if x is None or at is None else x[at] for x, at in zip(scales, (k, v))))
+            for k, v in (first, second)]
+
+  def second_state(one, two):
+    context = transformer.Context(
+        transformer.Unitransformer(None, d_model=16), mesh, [batch],
+        mtf.Dimension("length", 8), mtf.VariableDType(torch.float32), mode="incremental",
+        position=position, states=[attention.PagedState(c, table) for c in (one, two)])
+    context.record_new_states([context.paged_state()])
+    return context.paged_state()
+
+  for pair in (((0, 1), (0, 1)), ((0, 1), (2, 1)), ((0, 1), (1, 0)), ((0, None), (1, 0)),
+               ((3, None), (3, None))):
+    with pytest.raises(ValueError, match="the same pages"):
+      second_state(*caches(*pair))
+  for pair in (((0, 1), (2, 3)), ((5, 0), (1, 4)), ((0, None), (1, None))):
+    one, two = caches(*pair)
+    assert second_state(one, two).cache is two
+  # buffers that meet in a part only
+  flat = torch.empty(6 * 2 * 8 * 16, dtype=torch.float32)
+  size = 4 * 2 * 8 * 16
+  one, two = (cache_hip.PagedCache(flat[at:at + size].view(4, 2, 8, 16))
+              for at in (0, flat.numel() - size))
+  with pytest.raises(ValueError, match="the same pages"):
+    second_state(one, two)
