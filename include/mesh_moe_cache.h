@@ -29,8 +29,10 @@
  * only read; what a call leaves in a row that it is told to write twice, or reads of a row
  * that it writes for another place of the table, is unspecified.
  *
- * Limits: D up to 256, HK up to 65536, T and P * S up to 2^30, and what 2^24 workgroups
- * cover.  Tensors lie on their elements' size; the calls are fastest on 16 bytes, with D of
+ * Limits: D up to 256, HK up to 65536, T and P * S up to 2^30.  Attention of H query heads
+ * takes B * H up to 2^24 - 1 with D below 16.  From 16 on it takes U = B * HK * (H / HK / 16
+ * rounded up) up to that, and U * (P * S / R + 1, rounded up) up to 2^31 - 1; R is 256 for
+ * 8-bit pages with bfloat16 queries and D up to 128, and 64 or 128 otherwise.  Tensors lie on their elements' size; the calls are fastest on 16 bytes, with D of
  * 64, 128 or 256 and pages of 16 rows and more.
  *
  * The reference keeps recurrent states as whole tensors (mesh_tensorflow/transformer/
@@ -46,7 +48,7 @@ extern "C" {
 #endif
 
 /* (counted up with every change of a declaration, and of what a call accepts) */
-#define MESH_MOE_CACHE_ABI_VERSION 1
+#define MESH_MOE_CACHE_ABI_VERSION 2
 
 int mesh_moe_cache_abi_version(void);
 
@@ -93,7 +95,8 @@ int mesh_moe_cache_read(const void* k_pages, const void* v_pages,
  *   rel_values [H,num_buckets] dtype and rel_bucket [2*reach-1] int32, or both NULL: a
  *     relative attention bias as in mesh_moe_attention_decode; positions farther than
  *     reach - 1 back have the bias of that distance
- *   workspace: mesh_moe_cache_attention_workspace_bytes bytes, which may be 0
+ *   workspace: mesh_moe_cache_attention_workspace_bytes bytes, which may be 0 (and are for
+ *     sizes that the call refuses)
  */
 size_t mesh_moe_cache_attention_workspace_bytes(int B, int H, int HK, int D, int S,
                                                 int P, int dtype, int eight_bit);

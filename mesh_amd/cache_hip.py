@@ -26,7 +26,7 @@ from mesh_amd import fp8_hip
 from mesh_amd import moe_hip
 from mesh_amd.moe_hip import MoeHipError
 
-ABI_VERSION = 1
+ABI_VERSION = 2
 BLOCK = fp8_hip.BLOCK
 _E4M3 = torch.float8_e4m3fn
 

@@ -1684,9 +1684,9 @@ extern "C" int mesh_moe_cache_attention(
   a.H = H;
   a.G = H / HK;
   const bool padded = rows_padded(a);
-  const Division v = divide(B, H, HK, std::max(D, TILES_FROM), S, P, dtype, k_scales != nullptr,
-                            padded);
-  MOE_REQUIRE(v.fits && (tiles || (int64_t)B * H <= MAX_BLOCKS), MESH_MOE_E_UNSUPPORTED,
+  const Division v = tiles ? divide(B, H, HK, D, S, P, dtype, k_scales != nullptr, padded)
+                           : Division{};
+  MOE_REQUIRE(tiles ? v.fits : (int64_t)B * H <= MAX_BLOCKS, MESH_MOE_E_UNSUPPORTED,
               "cache_attention: %d sequences of %d heads and %d pages are more than a "
               "launch has", B, H, P);
   MOE_REQUIRE(!tiles || v.bytes == 0 || (workspace && workspace_bytes >= v.bytes),

@@ -289,3 +289,28 @@ def test_layers_with_the_same_buffers(eight):
               for at in (0, flat.numel() - size))
   with pytest.raises(ValueError, match="the same pages"):
     second_state(one, two)
+
+
+@pytest.mark.parametrize("d,dtype,eight,rows", [
+    (64, 1, True, 256), (128, 1, True, 256), (256, 1, True, 128), (64, 1, False, 128),
+    (256, 1, False, 128), (64, 0, True, 128), (256, 0, True, 64), (64, 0, False, 128),
+    (128, 0, False, 64), (16, 0, False, 128)])
+def test_limits_of_attention(lib, d, dtype, eight, rows):
+  """The header's bound on heads times positions, from both sides: within it a call goes
+  on, up to its missing workspace."""
+  scales = dict() if eight else dict(_5=None, _6=None)
+  with_ = _changed(lib.mesh_moe_cache_attention,
+                   [AT] * 9 + [None, None, 0, 0, AT, 1, 34, 2, d, 5, 1 << 10, 1 << 20,
+                               dtype, None, 0, None])
+  units = 2 * 2                                 # (17 heads in tiles of 16, twice)
+  most = ((1 << 31) - 1) // ((1 << 30) // rows + 1) // units
+  _refused(lib, with_(_14=most, **scales), -1, "workspace")
+  _refused(lib, with_(_14=most + 1, **scales), -2, "more than a launch")
+  assert lib.mesh_moe_cache_attention_workspace_bytes(
+      most, 34, 2, d, 1 << 10, 1 << 20, dtype, int(eight)) > 0
+  assert lib.mesh_moe_cache_attention_workspace_bytes(
+      most + 1, 34, 2, d, 1 << 10, 1 << 20, dtype, int(eight)) == 0
+  # more heads than workgroups, however short the table, also with narrow rows
+  _refused(lib, with_(_14=1 << 22, _19=1, _20=1, **scales), -2, "more than a launch")
+  _refused(lib, with_(_14=(1 << 24) // 34 + 1, _17=8, _19=1, _20=1, **scales), -2,
+           "more than a launch")

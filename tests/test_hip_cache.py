@@ -337,6 +337,27 @@ def test_narrow_rows(width, store):
 
 
 @pytest.mark.parametrize("store", STORES, ids=STORE_IDS)
+def test_narrow_rows_in_a_wide_table(store):
+  """Rows of fewer than 16 values under a table of 2^30 positions: their kernel does not
+  divide them, so that the bound on what is divided is not theirs."""
+  name, eight = store
+  dtype = DTYPES[name]
+  b, kv, heads, page, columns = 4, 64, 128, 1 << 16, 1 << 14
+  gen = _gen(30)
+  cache = cache_hip.PagedCache.empty(b, page, kv, 1, E4M3 if eight else dtype)
+  lengths = np.array([300, 1, 0, 257])
+  table = np.full((b, columns), -1, np.int32)
+  table[:, 0] = np.arange(b)[::-1]
+  rows = [_rows(gen, (b, 300, kv), dtype) for _ in range(2)]
+  cache_hip.write(cache, *rows, _int32(table), _int32([0] * b), count=_int32(lengths))
+  q = torch.randn((b, heads), generator=gen, device="cuda").to(dtype)
+  got = cache_hip.attention(q, cache, _int32(table), _int32(lengths - 1))
+  held = [C.stored(_np(x).reshape(b, 300, kv, 1), eight).transpose(0, 2, 1, 3)[::-1]
+          for x in rows]
+  _check(got, q, held, np.arange(b)[::-1][:, None], lengths - 1, 300, name)
+
+
+@pytest.mark.parametrize("store", STORES, ids=STORE_IDS)
 @pytest.mark.parametrize("case", [
     # sequences, longest, query heads, key / value heads, width, page, columns more
     (5, 70, 2, 2, 64, 16, 0), (3, 90, 3, 1, 128, 32, 200), (4, 40, 2, 1, 256, 64, 0),
