@@ -291,6 +291,30 @@ def test_layers_with_the_same_buffers(eight):
     second_state(one, two)
 
 
+def test_workspaces_that_are_too_small(lib):
+  """A table of 2^24 positions is divided among blocks, which takes a workspace; one that
+  is short, or of narrow rows, is not."""
+  # (arguments as above)
+  with_ = _changed(lib.mesh_moe_cache_attention,
+                   [AT] * 9 + [None, None, 0, 0, AT, 2, 8, 4, 64, 5, 16, 1 << 20, 1, AT,
+                               1 << 40, None])
+  for dtype in (0, 1):
+    for eight in (0, 1):
+      for d in (16, 64, 128, 200, 256):
+        need = lib.mesh_moe_cache_attention_workspace_bytes(2, 8, 4, d, 16, 1 << 20, dtype,
+                                                            eight)
+        assert need > 0
+        pages = dict() if eight else dict(_5=None, _6=None)
+        # (rows of other widths may do with fewer blocks)
+        short = need - 1 if d in (64, 128, 256) else need // 4
+        _refused(lib, with_(_17=d, _21=dtype, _23=short, **pages), -1, "workspace")
+        _refused(lib, with_(_17=d, _21=dtype, _22=None, **pages), -1, "workspace")
+        assert lib.mesh_moe_cache_attention_workspace_bytes(2, 8, 4, d, 16, 4, dtype,
+                                                            eight) == 0
+      assert lib.mesh_moe_cache_attention_workspace_bytes(2, 8, 4, 15, 16, 1 << 20, dtype,
+                                                          eight) == 0
+
+
 @pytest.mark.parametrize("d,dtype,eight,rows", [
     (64, 1, True, 256), (128, 1, True, 256), (256, 1, True, 128), (64, 1, False, 128),
     (256, 1, False, 128), (64, 0, True, 128), (256, 0, True, 64), (64, 0, False, 128),
