@@ -4,8 +4,8 @@ or in 8 bits, and attention of one new token over them.
 
 The calls follow those of moe_hip, whose attention_decode keeps its states as whole
 tensors: GPU tensors that are contiguous, checked on the host; launched on the current
-stream; nothing kept between calls, so that each can be recorded into a HIP graph.  All
-tensors of a call have to lie on the current device.
+stream; nothing kept between calls but how large a workspace of some sizes is, so that each
+can be recorded into a HIP graph.  All tensors of a call have to lie on the current device.
 
 A decoding program keeps a PagedCache for each layer and one table for all of them:
 
@@ -189,7 +189,7 @@ def _table(table, batch):
   return _dev(table, "table", torch.int32, (batch, columns)), columns
 
 
-@functools.lru_cache(maxsize=None)
+@functools.lru_cache(maxsize=1024)
 def _workspace_bytes(*sizes):
   return load_library().mesh_moe_cache_attention_workspace_bytes(*sizes)
 

@@ -338,3 +338,13 @@ def test_limits_of_attention(lib, d, dtype, eight, rows):
   _refused(lib, with_(_14=1 << 22, _19=1, _20=1, **scales), -2, "more than a launch")
   _refused(lib, with_(_14=(1 << 24) // 34 + 1, _17=8, _19=1, _20=1, **scales), -2,
            "more than a launch")
+
+
+def test_sizes_that_are_kept_are_bounded(lib):
+  """A server's batches and tables change without end; what is kept of them does not."""
+  del lib
+  most = cache_hip._workspace_bytes.cache_info().maxsize
+  assert most is not None
+  for columns in range(1, most + 50):
+    cache_hip._workspace_bytes(2, 8, 4, 64, 16, columns, 1, False)
+  assert cache_hip._workspace_bytes.cache_info().currsize <= most
