@@ -431,7 +431,12 @@ class PagedState(object):
   which page has every page_size positions of a batch entry (-1: none yet).  Passed as the
   layer's one state in "first_part" and "incremental" mode, and recorded as its new one;
   the cache itself is updated in place, and the program gives sequences pages by writing
-  into `table`, also between the replays of a recorded step."""
+  into `table`, also between the replays of a recorded step.  No two layers' caches have
+  memory in common.
+
+  A page that several sequences share is named once in the table of a "first_part", which
+  writes every position that has a page, and by all of them from the first step on, whose
+  rows go to pages of their own."""
 
   def __init__(self, cache, table):
     self.cache, self.table = cache, table

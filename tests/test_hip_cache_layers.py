@@ -204,3 +204,52 @@ def test_biases_of_many_buckets(act_dtype, buckets, bidirectional):
   assert torch.equal(got, cache_hip.attention(
       q, state.cache, state.table, position,
       relative_bias=(values.to(act_dtype), table)).float())
+
+
+@pytest.mark.parametrize("act_dtype", [torch.float32, torch.bfloat16])
+def test_decoding_with_pages_shared_by_sequences(act_dtype):
+  """Three sequences of which two begin with the same 16 tokens: the first part's table names
+  their two pages for one of them, the steps' table for both."""
+  b, length, first, shared = 3, 27, 19, 2 * PAGE
+  rng = np.random.default_rng(8)
+  x = torch.from_numpy(rng.standard_normal((b, length, MODEL)).astype(np.float32)).to(
+      act_dtype)
+  x[2, :shared] = x[0, :shared]
+  graph = mtf.Graph()
+  mesh = mtf.Mesh(graph, "mesh")
+  batch, len_dim, model_dim = (mtf.Dimension("batch", b), mtf.Dimension("length", length),
+                               mtf.Dimension("d_model", MODEL))
+  vdt = mtf.VariableDType(torch.float32, torch.float32, act_dtype)
+  model = _model(mesh, False, "bias")
+  t = lambda a: mtf.import_tf_tensor(mesh, a, mtf.Shape([batch, len_dim, model_dim]))
+  y_full, _ = model.call_layers(t(x), vdt, mode="eval")
+  known = x.clone()
+  known[:, first:] = 0
+  begin = _states(b, length, act_dtype, False)
+  spare = begin[0].table[2, :2].clone()
+  steps_table = begin[0].table.clone()
+  steps_table[2, :2] = steps_table[0, :2]
+  begin[0].table[2, :2] = -1                 # (one tensor for both layers)
+  going_on = [attention.PagedState(s.cache, steps_table) for s in begin]
+  model.call_layers(t(known), vdt, mode="first_part", states=begin, reuse=True)
+  steps = []
+  for p in range(first, length):
+    token = mtf.import_tf_tensor(mesh, x[:, p].contiguous(),
+                                 mtf.Shape([batch, model_dim]))
+    position = mtf.import_tf_tensor(mesh, torch.full((b,), p, dtype=torch.int32),
+                                    mtf.Shape([batch]))
+    steps.append(model.call_layers(token, vdt, mode="incremental", position=position,
+                                   states=going_on, length_dim=len_dim)[0])
+  for s in begin:                            # (nobody's pages any more)
+    s.cache.k_pages[spare.long()] = s.cache.v_pages[spare.long()] = float("nan")
+  lowering = mtf.Lowering(graph, {mesh: mtf.HipMeshImpl()},
+                          initial_values=_initial_values(graph, rng))
+  # (the tolerances of decoding above)
+  tol = (dict(rtol=2e-4, atol=2e-4) if act_dtype == torch.float32
+         else dict(rtol=5e-2, atol=5e-2))
+  want = lowering.export_to_tf_tensor(y_full).float()
+  for p, step in zip(range(first, length), steps):
+    torch.testing.assert_close(lowering.export_to_tf_tensor(step).float(), want[:, p],
+                               **tol)
+  for s in begin:
+    assert torch.isnan(s.cache.k_pages[spare.long()].float()).all()
