@@ -312,6 +312,49 @@ def test_step(case, store, shared):
 
 
 @pytest.mark.parametrize("store", STORES, ids=STORE_IDS)
+@pytest.mark.parametrize("case", [(4, 4, 64, 16), (8, 2, 128, 32), (6, 1, 256, 64),
+                                  (2, 2, 64, 4), (2, 1, 128, 1), (3, 1, 80, 8),
+                                  (2, 2, 8, 16)],
+                         ids=lambda c: "x".join(map(str, c)))
+@pytest.mark.parametrize("off", ["query", "keys", "values", "row", "all"])
+def test_attention_at_any_address(case, store, off):
+  """Operands that lie on their elements' size and not on 16 bytes: the results against
+  float64, and the pages' bytes."""
+  heads, kv, width, page = case
+  name, eight = store
+  dtype = DTYPES[name]
+  rng, gen = np.random.default_rng(sum(case)), _gen(sum(case))
+  lengths = np.array([1, 17, 64, 130, 700, 33])
+  table, pages = _table(rng, lengths, page)
+  table[3, 0] = -1
+  made, held = _cache(gen, pages, page, kv, width, dtype, eight)
+  position = lengths - 1
+
+  def moved(x, name):
+    if x is None or off not in (name, "all"):
+      return x
+    buffer = torch.empty(x.numel() + 1, dtype=x.dtype, device="cuda")
+    out = buffer[1:].view(x.shape)
+    out.copy_(x)
+    assert out.data_ptr() % 16
+    return out
+  cache = cache_hip.PagedCache(moved(made.k_pages, "keys"), moved(made.v_pages, "values"),
+                               moved(made.k_scales, "keys"), moved(made.v_scales, "values"))
+  b = len(lengths)
+  q = moved((torch.randn((b, heads * width), generator=gen, device="cuda")
+             * 2 * width ** -0.5).to(dtype), "query")
+  k, v = (moved(_rows(gen, (b, kv * width), dtype), "row") for _ in range(2))
+  got = cache_hip.attention(q, cache, _int32(table), _int32(position))
+  _check(got, q, held, table, position, page, name)
+  got = cache_hip.attention(q, cache, _int32(table), _int32(position), k_new=k, v_new=v)
+  held = [C.write(was, C.stored(_np(x).reshape(b, 1, kv, width), eight), table, position,
+                  None, page) for was, x in zip(held, (k, v))]
+  for a, x in zip(_held(cache), held):
+    np.testing.assert_array_equal(a, x)
+  _check(got, q, held, table, position, page, name)
+
+
+@pytest.mark.parametrize("store", STORES, ids=STORE_IDS)
 @pytest.mark.parametrize("width", [1, 5, 8, 15])
 def test_narrow_rows(width, store):
   name, eight = store
