@@ -107,9 +107,13 @@ __device__ __forceinline__ void store_eight(uint8_t* row, int at, int D, uint32_
 // once; wide rows are shared by two or four wavefronts.  A lane has 8 values of each, and a
 // head's lanes are a power of two (16 for each block of 128 where it has more than one), so
 // that a block's largest magnitude is found by DPP steps among neighbours.
-// Nothing is used twice: bound by the memory.  16 sequences of up to 4096 rows of 1024
-// bfloat16 keys and values into 8 bits move 278 MB in 48 us (5.8 TB/s, some of it to the
-// last level's cache; a copy of 1 GiB reaches 5.15), 4 x 16384 rows back 406 MB in 60.
+// Nothing is used twice: bound by the memory, but for writes of narrow heads.  16 sequences
+// of up to 4096 rows of 16 x 64 bfloat16 keys and values into 8 bits move 215 MB in 48 us,
+// 4.4 TB/s where a copy of 1 GiB reaches 5.2 (probably: a row of 64 bytes is half a line, a
+// wavefront's store goes to all heads' pages, and scale bytes are stored one by one).  The way
+// back moves 341 MB in 46, 7.5 TB/s, as the pages are in the last level's cache still (of the
+// 268 MB that it stores, 5.9 where a fill reaches 6.7); 4 x 16384 rows 404 MB in 60 when
+// repeated on the same pages, 75 on others (5.4 TB/s).
 // ---------------------------------------------------------------------------
 struct RowsOf {
   Pages pages;
@@ -120,8 +124,8 @@ struct RowsOf {
   int sharing;                    // wavefronts that share a row (1, 2 or 4), log2
 };
 // Rows of a wavefront, where there are many: 4 x 16384 rows of 1024 values out of an 8-bit
-// cache take 84 us by one, 82 by two, 70 by four; 23 x 1000 of 480 out of a bfloat16 one 24
-// by one, 18 by two, 21 by four.
+// cache take 84 us by one, 82 by two, 70 by four (recorded calls); 23 x 1000 of 480 out of a
+// bfloat16 one 24 by one, 18 by two, 21 by four.
 template <typename T, bool EIGHT> constexpr int ROWS = EIGHT && sizeof(T) == 2 ? 4 : 2;
 
 // Where piece `piece` of a head's row begins: a piece that would end behind the row begins as
@@ -425,14 +429,14 @@ __global__ __launch_bounds__(256) void cache_attention_kernel(Attention a) {
 // and the products of 16 columns take a twentieth of the matrix cores' time.  Four
 // wavefronts take turns with groups of NS x 16 positions, without barriers; what they have
 // in flight at once is what hides the memory's latency.  One sequence of 131072 positions,
-// 8 key / value heads of 128, 8 bits: 42 us, 6.4 TB/s; 128 of up to 16384 in bfloat16: 714
-// us, 6.1 TB/s (a kernel that only reads reaches 6.3).  A wavefront's next group is not loaded
-// ahead of the one in use: the registers for it cost the second block of a CU, and two
-// blocks take turns as well (64 sequences of up to 8192: 121 us with, 118 without; rows of
-// 256, 87 and 71).
+// 8 key / value heads of 128, 8 bits: 42 us, 6.4 TB/s when repeated, as some of the 270 MB
+// stay in the last level's cache; 128 of up to 16384 in bfloat16: 715 us, 6.05 TB/s (a kernel
+// that only reads reaches 6.3).  A wavefront's next group is not loaded ahead of the one in
+// use: the registers for it cost the second block of a CU, and two blocks take turns as well
+// (64 sequences of up to 8192: 121 us with, 118 without; rows of 256, 87 and 71).
 //
-// The work is dealt out evenly to as many blocks as the chip holds at once, by what the
-// sequences' lengths turn out to be on the device (run_of).  Where a unit's positions fall
+// The work is dealt out evenly to one to three blocks a CU (at_once), by what the sequences'
+// lengths turn out to be on the device (run_of).  Where a unit's positions fall
 // to several blocks, their triples go to the workspace, and cache_attention_join_kernel
 // puts them together.  (In the same launch, by the block of a unit that is done last, a
 // join costs its block round trips to a memory that is busy with the others' streams: 64
@@ -495,14 +499,20 @@ struct TileOf {
   static constexpr bool WIDE = sizeof(T) == 4;                 // float32 products
   // Groups of 16 positions that a wavefront has in registers at once: as many as leave the
   // blocks below their registers.  (8 bits, 128 values, 64 sequences of up to 8192: 125 us
-  // by 2, 115 by 4; bfloat16, 64 values, by 4 with two blocks 18.5, by 2 with three 17.4.)
+  // by 2, 115 by 4; bfloat16, 64 values, by 4 with two blocks 18.5, by 2 with three 17.4.
+  // Padded 8-bit rows of 65 to 127 values do not have the registers for 4 in pages of 4 and 8
+  // rows, where 28 bytes a lane go to scratch memory, and of 1 and 2, where it is 84; 2 has
+  // not been timed there.)
   static constexpr int NS =
       WIDE ? (EIGHT ? (DP == 256 ? 1 : 2) : (DP == 64 ? 2 : 1))
            : (EIGHT && DP < 256 ? 4 : 2);
   static constexpr int GRAIN = 4 * 16 * NS;                    // positions of four wavefronts
-  // Blocks that a CU holds, by their registers.  (Rows of 256, 16 sequences of 16384, 8 bits:
-  // 79 us by one, 72 by two; bfloat16, where two do not have the registers for it, 100 and
-  // 125.)
+  // Blocks that divided work counts on in a CU, and that the registers are kept below for.
+  // (Rows of 256, 16 sequences of 16384, 8 bits: 79 us by one, 72 by two; bfloat16, where two
+  // do not have the registers for it, 100 and 125.)  Some kernels without padding come out
+  // with registers for more, which has not been timed: 8-bit rows of 64 (153 of them) and
+  // float32 ones (155) for three, 8-bit ones under float32 for four (119; of 128, 157, for
+  // three), bfloat16 ones of 64 (117) for four.
   template <bool PADDED>
   static constexpr int at_once() {
     return DP == 256 && !(EIGHT && !PADDED) ? 1 : DP == 64 && !EIGHT && !WIDE ? 3 : 2;
@@ -1093,7 +1103,10 @@ void cache_attention_tiles_kernel(Attention a, Shares shares, Joins joins) {
         if constexpr (!Tile::WIDE) {
           pairs[s][0] = f32x2_to_bf16x2(x[s][0], x[s][1]);
           pairs[s][1] = f32x2_to_bf16x2(x[s][2], x[s][3]);
-          // (the sum of what is multiplied, so that weights add up to 1)
+          // (Rounded, as the products of bfloat16 values on the matrix cores take them; the
+          // sum is of what is multiplied, so that weights add up to 1.  Against 64 bits, 128
+          // sequences of up to 16384 are off by 0.0017 of the result's norm, with weights
+          // in float32 by 0.0016: the result's own rounding is most of both.)
 #pragma unroll
           for (int e = 0; e < 2; ++e)
             l += __uint_as_float(pairs[s][e] << 16) +
@@ -1400,7 +1413,11 @@ static int lanes_of(int D) {
 // they are even).  Many: rows that fill four wavefronts to three quarters, or two (16 x 1000
 // rows of 2048 in 8 bits 41 us and 31, of 480 in bfloat16 18 and 20).  Float32 rows of a
 // wavefront and more take their registers one by one, too (16 x 1000 of 1024 116 us by two,
-// 103; of 64 values 15 and 19).
+// 103; of 64 values 15 and 19).  One shape lost by it: 3 x 1000 rows of 4096 8-bit values
+// back into float32, whose results stay in the last level's cache, took 30 us by two and
+// unshared and take 36 (4 x 1000 53 and 48, 16 x 1000 238 and 198).  Float32 rows that come
+// out of 8 bits are stored at 2.6 to 3.1 TB/s: a lane's eight values are two stores of 16
+// bytes, each of them every other piece of a line.
 static bool few_rows(RowsOf& r, bool wide_type) {
   const int64_t pieces = (int64_t)r.pages.HK << r.lanes;
   const bool few = r.T == 1 || (int64_t)r.B * r.T <= 2048;
