@@ -32,8 +32,9 @@
  * Limits: D up to 256, HK up to 65536, T and P * S up to 2^30.  Attention of H query heads
  * takes B * H up to 2^24 - 1 with D below 16.  From 16 on it takes U = B * HK * (H / HK / 16
  * rounded up) up to that, and U * (P * S / R + 1, rounded up) up to 2^31 - 1; R is 256 for
- * 8-bit pages with bfloat16 queries and D up to 128, and 64 or 128 otherwise.  Tensors lie on their elements' size; the calls are fastest on 16 bytes, with D of
- * 64, 128 or 256 and pages of 16 rows and more.
+ * 8-bit pages with bfloat16 queries and D up to 128, and 64 or 128 otherwise.  The buffers
+ * of a cache do not overlap each other.  Tensors lie on their elements' size; the calls are
+ * fastest on 16 bytes, with D of 64, 128 or 256 and pages of 16 rows and more.
  *
  * The reference keeps recurrent states as whole tensors (mesh_tensorflow/transformer/
  * transformer_layers.py:231-254); these calls are a form of what it does with them.
